@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/lmp_hip.h.
+"""ctypes binding of the C ABI in include/lmp_hip.h and include/lmp_hip_transformer.h.
 
 This is the thinnest possible caller of liblmp_hip.so: kernel-level parity
 tests and the benchmark drive the backend through it, exactly as a Lamp3
@@ -59,6 +59,16 @@ class PoolStats(C.Structure):
                 ("device_mallocs", C.c_uint64)]
 
 
+ADAMW_BLOCK = 256  # values that share one scale of an 8-bit state
+ATTENTION_MAX_DIM = 256
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
+                ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("n", C.c_uint64),
+                ("decay", C.c_double)]
+
+
 _vp, _sz, _i, _d = C.c_void_p, C.c_size_t, C.c_int, C.c_double
 
 # name -> (restype, argtypes); every entry point declared in lmp_hip.h
@@ -115,6 +125,20 @@ SIGNATURES = {
     "lmp_jit_disk_loaded_count": (_i, [C.POINTER(C.c_uint64)]),
 }
 
+# name -> (restype, argtypes); every entry point declared in lmp_hip_transformer.h
+TRANSFORMER_SIGNATURES = {
+    "lmp_k_layer_norm": (_i, [_i, _sz, _sz, _vp, _sz, _vp, _vp, _d, _vp, _sz, _vp, _vp]),
+    "lmp_k_layer_norm_backward": (_i, [_i, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz,
+                                       _vp, _vp]),
+    "lmp_k_adamw_f32": (_i, [_i, _sz, _vp, _d, _d, _d, _d, C.c_uint64, _vp]),
+    "lmp_k_adamw_decode": (_i, [_i, _vp, _vp, _sz, _vp]),
+    "lmp_k_attention_plan_create": (_i, [C.POINTER(_vp), _sz, _vp, _vp, _sz, _sz, _sz, _i]),
+    "lmp_k_attention_plan_destroy": (_i, [_vp]),
+    "lmp_k_attention_f32": (_i, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _d, _vp, _sz, _vp]),
+    "lmp_k_attention_backward_f32": (_i, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _d, _vp, _sz, _vp,
+                                          _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz]),
+}
+
 _lib = None
 
 
@@ -126,7 +150,7 @@ def lib() -> C.CDLL:
             raise RuntimeError(
                 f"{LIB_PATH} is missing: build it with `python rushlite_amd/build.py hip`")
         handle = C.CDLL(str(LIB_PATH), mode=os.RTLD_NOW | C.RTLD_GLOBAL)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **TRANSFORMER_SIGNATURES}.items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
@@ -305,3 +329,37 @@ class Timer:
         ms = C.c_float()
         check(lib().lmp_rt_event_elapsed_ms(self.start, self.stop, C.byref(ms)))
         return ms.value
+
+
+class AttentionPlan:
+    """The work lists of a packed batch (lmp_k_attention_plan_create); `handle` is the plan the
+    attention entry points take.  Keep it while calls, or graphs that recorded them, use it."""
+
+    handle = None
+
+    def __init__(self, q_lengths, k_lengths=None, *, heads, kv_heads=None, head_dim, causal=True):
+        q = np.ascontiguousarray(q_lengths, np.int64)
+        k = q if k_lengths is None else np.ascontiguousarray(k_lengths, np.int64)
+        if q.ndim != 1 or q.shape != k.shape:
+            raise ValueError("attention plan: one query length and one key length per sequence")
+        self.heads, self.kv_heads = int(heads), int(heads if kv_heads is None else kv_heads)
+        self.head_dim, self.causal = int(head_dim), bool(causal)
+        if min(self.heads, self.kv_heads, self.head_dim) < 0:
+            raise ValueError("attention plan: negative heads or head_dim")
+        self.queries, self.keys = int(q.sum()), int(k.sum())
+        p = C.c_void_p()
+        check(lib().lmp_k_attention_plan_create(C.byref(p), len(q), q.ctypes.data, k.ctypes.data,
+                                                self.heads, self.kv_heads, self.head_dim,
+                                                int(self.causal)))
+        self.handle = p.value
+
+    def free(self) -> None:
+        if self.handle:
+            handle, self.handle = self.handle, None
+            check(lib().lmp_k_attention_plan_destroy(handle))
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass

@@ -1,0 +1,408 @@
+// One AdamW step over many tensors, its states in 32 or in 8 bits.
+//
+//   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+//   p = p (1 - lr decay) - lr m^ / (sqrt(v^) + eps),  m^, v^ corrected by 1 - beta^t
+//
+// Bound by memory: 28 bytes a parameter with states of 32 bits (p, m, v read and
+// written, g read), 16 with states of 8.  All tensors share a launch: their
+// pointers ride in the kernel's arguments (kTensors of them), so nothing is
+// copied to the device per step and a recorded step replays; a workgroup finds
+// its tensor by bisection of the running workgroup counts.  The step count
+// lives on the device, and every workgroup forms the two bias corrections from it
+// in float64 while its loads are on their way.
+//
+// States of 8 bits: a wave owns a block of 256 values, four a lane, so the
+// block's scale is a maximum over the wave and a state costs one 4-byte access
+// per lane.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+#include <vector>
+
+#include "common.hpp"
+#include "lmp_hip_transformer.h"
+
+namespace lmp_hip {
+namespace {
+
+#define LMP_WAVE_SWAP_SRC(...) __VA_ARGS__
+#include "wave_swap.inc"
+#undef LMP_WAVE_SWAP_SRC
+
+constexpr int kTensors = 48;  // a launch's list: 48 x 60 bytes, inside the 4 KiB of arguments
+constexpr int kThreads = 256;
+constexpr int kUnits = 4;  // units of four values per lane and workgroup
+constexpr int kPerGroup = kThreads * 4 * kUnits;
+// Launches of at most this many workgroups count themselves done and the last
+// one advances the step; above, that costs more than a launch of its own.
+constexpr int kSelfCounted = 256;
+
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u1_any __attribute__((aligned(1)));
+
+struct AdamWList {
+  float* p[kTensors];
+  const float* g[kTensors];
+  void* m[kTensors];
+  void* v[kTensors];
+  float* m_scale[kTensors];
+  float* v_scale[kTensors];
+  int64_t n[kTensors];
+  float keep[kTensors];       // 1 - lr decay
+  uint32_t first[kTensors];   // the tensor's first workgroup
+};
+
+struct AdamWArgs {
+  AdamWList list;
+  int count;
+  uint32_t place;  // of the list's first tensor among all of the step's
+  float beta1, rest1, beta2, rest2, eps;
+  double lr, beta1_d, beta2_d;
+  uint32_t seed;
+  int64_t* step;
+  int advance;  // the last workgroup to finish advances the step
+};
+
+__device__ __forceinline__ double power(double base, int64_t t) {
+  double r = 1;
+  for (; t > 0; t >>= 1) {
+    if (t & 1) r *= base;
+    base *= base;
+  }
+  return r;
+}
+
+__device__ __forceinline__ uint32_t mixed(uint32_t x) {  // MurmurHash3's 32-bit finalizer
+  x ^= x >> 16;
+  x *= 0x85EBCA6Bu;
+  x ^= x >> 13;
+  x *= 0xC2B2AE35u;
+  return x ^ (x >> 16);
+}
+
+// One value.  Each operation rounds once (no contraction), so that a state in 8
+// bits is a function of its inputs alone.
+__device__ __forceinline__ void step_one(const AdamWArgs& a, float keep, float size, float root,
+                                         float g, float& p, float& m, float& v) {
+  m = m * a.beta1 + g * a.rest1;
+  v = v * a.beta2 + (g * g) * a.rest2;
+  p = p * keep - size * (m / (sqrtf(v) * root + a.eps));
+}
+
+// Codes of a block's four values in this lane.  x scaled to [0, Q^2] has code c
+// with c^2 <= t < (c + 1)^2, and moves up to c + 1 with probability
+// (t - c^2) / (2 c + 1), the random 16 bits u being below it.
+template <int Q>
+__device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (&r)[4],
+                                           float* scale, bool first_lane) {
+  float top = 0;
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    top = fmaxf(top, fabsf(x[j]));
+    nan = nan || x[j] != x[j];
+  }
+  top = nan ? __builtin_inff() : top;
+  top = fmaxf(top, lmp_swap<1>(top));
+  top = fmaxf(top, lmp_swap<2>(top));
+  top = fmaxf(top, lmp_swap<4>(top));
+  top = fmaxf(top, lmp_swap<8>(top));
+  top = fmaxf(top, lmp_swap<16>(top));
+  top = fmaxf(top, lmp_swap<32>(top));
+  const bool live = top >= 1e-30f && top < __builtin_inff();
+  if (first_lane) *scale = live ? top : top < 1e-30f ? 0.0f : __builtin_nanf("");
+  if (!live) return 0;
+  const float inv = (1.0f / top) * float(Q * Q);
+  uint32_t packed = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float t = fminf(fabsf(x[j]) * inv, float(Q * Q));
+    float c = floorf(sqrtf(t));
+    c = c * c > t ? c - 1 : c;
+    c = (c + 1) * (c + 1) <= t ? c + 1 : c;
+    c = float(r[j]) * (1.0f / 65536) * (2 * c + 1) < t - c * c ? c + 1 : c;
+    if (Q == 255) c = c == 0 && t > 0 ? 1.0f : c;
+    c = fminf(c, float(Q));
+    const int code = x[j] < 0 ? -int(c) : int(c);
+    packed |= uint32_t(code & 255) << (8 * j);
+  }
+  return packed;
+}
+
+template <bool SIGNED>
+__device__ __forceinline__ float decoded(uint32_t packed, int j, float unit) {
+  const uint32_t byte = (packed >> (8 * j)) & 255;
+  const float c = SIGNED ? float(int(int8_t(byte))) : float(byte);
+  return (c * fabsf(c)) * unit;
+}
+constexpr float kUnitM = float(1.0 / (127 * 127)), kUnitV = float(1.0 / (255 * 255));
+
+template <int BITS>
+__global__ __launch_bounds__(kThreads) void adamw_step(AdamWArgs a) {
+  __shared__ float factors[2];
+  __shared__ uint32_t key_of_step;
+  if (threadIdx.x == 0) {
+    const int64_t t = a.step[0] + 1;
+    factors[0] = float(a.lr / (1.0 - power(a.beta1_d, t)));
+    factors[1] = float(1.0 / sqrt(1.0 - power(a.beta2_d, t)));
+    key_of_step = mixed(uint32_t(t) ^ a.seed);
+  }
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (blockIdx.x >= a.list.first[mid]) lo = mid;
+    else hi = mid - 1;
+  }
+  const int i = lo;
+  const int64_t n = a.list.n[i];
+  float* p = a.list.p[i];
+  const float* g = a.list.g[i];
+  const float keep = a.list.keep[i];
+  const int64_t begin = int64_t(blockIdx.x - a.list.first[i]) * kPerGroup;
+  float pv[kUnits][4], gv[kUnits][4];
+  const auto at_of = [&](int u) { return begin + (int64_t(u) * kThreads + threadIdx.x) * 4; };
+  const auto load4 = [&](const float* from, int64_t at, float (&v)[4]) {
+    if (at + 4 <= n) {
+      const f4 x = *reinterpret_cast<const f4*>(from + at);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = x[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = at + j < n ? from[at + j] : 0.0f;
+    }
+  };
+  const auto store4 = [&](float* to, int64_t at, const float (&v)[4]) {
+    if (at + 4 <= n) {
+      *reinterpret_cast<f4*>(to + at) = f4{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (at + j < n) to[at + j] = v[j];
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    load4(p, at_of(u), pv[u]);
+    load4(g, at_of(u), gv[u]);
+  }
+  if constexpr (BITS == 32) {
+    float* m = static_cast<float*>(a.list.m[i]);
+    float* v = static_cast<float*>(a.list.v[i]);
+    float mv[kUnits][4], vv[kUnits][4];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      load4(m, at_of(u), mv[u]);
+      load4(v, at_of(u), vv[u]);
+    }
+    __syncthreads();
+    const float size = factors[0], root = factors[1];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        step_one(a, keep, size, root, gv[u][j], pv[u][j], mv[u][j], vv[u][j]);
+      store4(p, at_of(u), pv[u]);
+      store4(m, at_of(u), mv[u]);
+      store4(v, at_of(u), vv[u]);
+    }
+  } else {
+    uint8_t* m = static_cast<uint8_t*>(a.list.m[i]);
+    uint8_t* v = static_cast<uint8_t*>(a.list.v[i]);
+    uint32_t mc[kUnits], vc[kUnits];
+    float ms[kUnits], vs[kUnits];
+    const auto codes = [&](const uint8_t* from, int64_t at) -> uint32_t {
+      if (at + 4 <= n) return *reinterpret_cast<const u1_any*>(from + at);
+      uint32_t c = 0;
+      for (int j = 0; j < 4; ++j)
+        if (at + j < n) c |= uint32_t(from[at + j]) << (8 * j);
+      return c;
+    };
+    const auto put = [&](uint8_t* to, int64_t at, uint32_t c) {
+      if (at + 4 <= n) {
+        *reinterpret_cast<u1_any*>(to + at) = c;
+      } else {
+        for (int j = 0; j < 4; ++j)
+          if (at + j < n) to[at + j] = uint8_t(c >> (8 * j));
+      }
+    };
+    // A wave's 64 lanes x 4 values of one unit are one block.
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int64_t block = at_of(u) / LMP_ADAMW_BLOCK;
+      const bool there = block * LMP_ADAMW_BLOCK < n;
+      mc[u] = codes(m, at_of(u));
+      vc[u] = codes(v, at_of(u));
+      ms[u] = there ? a.list.m_scale[i][block] : 0.0f;
+      vs[u] = there ? a.list.v_scale[i][block] : 0.0f;
+    }
+    __syncthreads();
+    const float size = factors[0], root = factors[1];
+    const uint32_t key = mixed(key_of_step + 0x9E3779B9u * (a.place + uint32_t(i) + 1));
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int64_t at = at_of(u), block = at / LMP_ADAMW_BLOCK;
+      if (block * LMP_ADAMW_BLOCK >= n) continue;  // the whole wave
+      float mv[4], vv[4];
+      uint32_t lo16[4], hi16[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        mv[j] = decoded<true>(mc[u], j, ms[u] * kUnitM);
+        vv[j] = decoded<false>(vc[u], j, vs[u] * kUnitV);
+        step_one(a, keep, size, root, gv[u][j], pv[u][j], mv[j], vv[j]);
+        if (at + j >= n) mv[j] = vv[j] = 0.0f;
+        const uint64_t place = uint64_t(at + j);
+        const uint32_t r = mixed(uint32_t(place) ^ key ^ uint32_t((place >> 32) * 0x85EBCA6Bu));
+        lo16[j] = r & 0xFFFF;
+        hi16[j] = r >> 16;
+      }
+      const bool first_lane = (threadIdx.x & 63) == 0;
+      const uint32_t m2 = encode<127>(mv, lo16, a.list.m_scale[i] + block, first_lane);
+      const uint32_t v2 = encode<255>(vv, hi16, a.list.v_scale[i] + block, first_lane);
+      store4(p, at, pv[u]);
+      put(m, at, m2);
+      put(v, at, v2);
+    }
+  }
+  if (a.advance && threadIdx.x == 0) {
+    // This workgroup read the step before its barrier; the last to come here
+    // finds that all have, and the next launch finds the counter at 0.
+    unsigned long long* done = reinterpret_cast<unsigned long long*>(a.step + 1);
+    if (atomicAdd(done, 1ull) == gridDim.x - 1) {
+      *done = 0;
+      a.step[0] += 1;
+    }
+  }
+}
+
+__global__ void adamw_advance(int64_t* step) { step[0] += 1; }
+
+template <bool SIGNED>
+__global__ __launch_bounds__(kThreads) void adamw_values(const uint8_t* codes, const float* scales,
+                                                         int64_t n, float* out) {
+  constexpr float unit = SIGNED ? kUnitM : kUnitV;
+  const int64_t stride = int64_t(gridDim.x) * kThreads * 4;
+  for (int64_t at = (int64_t(blockIdx.x) * kThreads + threadIdx.x) * 4; at < n; at += stride) {
+    const float s = scales[at / LMP_ADAMW_BLOCK] * unit;
+    if (at + 4 <= n) {
+      const uint32_t c = *reinterpret_cast<const u1_any*>(codes + at);
+      *reinterpret_cast<f4*>(out + at) = f4{decoded<SIGNED>(c, 0, s), decoded<SIGNED>(c, 1, s),
+                                            decoded<SIGNED>(c, 2, s), decoded<SIGNED>(c, 3, s)};
+    } else {
+      for (int j = 0; at + j < n; ++j) out[at + j] = decoded<SIGNED>(codes[at + j], 0, s);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace lmp_hip
+
+using namespace lmp_hip;
+
+extern "C" int lmp_k_adamw_f32(int bits, size_t count, const lmp_adamw_tensor* tensors, double lr,
+                               double beta1, double beta2, double eps, uint64_t seed,
+                               int64_t* step) {
+  const char* name = "lmp_k_adamw_f32: ";
+  if (bits != 32 && bits != 8)
+    return fail(LMP_ERR_INVALID, std::string(name) + "states have 32 or 8 bits, not " +
+                                     std::to_string(bits));
+  if (!step) return fail(LMP_ERR_INVALID, std::string(name) + "null step");
+  if (count && !tensors) return fail(LMP_ERR_INVALID, std::string(name) + "null list of tensors");
+  if (!std::isfinite(lr)) return fail(LMP_ERR_INVALID, std::string(name) + "lr is not finite");
+  if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1))
+    return fail(LMP_ERR_INVALID, std::string(name) + "beta1 and beta2 lie in [0, 1)");
+  if (!(eps >= 0) || std::isinf(eps))
+    return fail(LMP_ERR_INVALID, std::string(name) + "eps is negative or not finite");
+  if (count > (size_t(1) << 31))
+    return fail(LMP_ERR_UNSUPPORTED, std::string(name) + "more than 2^31 tensors");
+  for (size_t i = 0; i < count; ++i) {
+    const lmp_adamw_tensor& t = tensors[i];
+    const std::string which = std::string(name) + "tensor " + std::to_string(i) + ": ";
+    if (!std::isfinite(t.decay)) return fail(LMP_ERR_INVALID, which + "decay is not finite");
+    if (t.n == 0) continue;
+    if (!t.p || !t.g || !t.m || !t.v) return fail(LMP_ERR_INVALID, which + "null buffer");
+    if (bits == 8 && (!t.m_scale || !t.v_scale))
+      return fail(LMP_ERR_INVALID, which + "states of 8 bits need their scales");
+    if (t.n > (uint64_t(1) << 35))
+      return fail(LMP_ERR_UNSUPPORTED, which + "more than 2^35 values");
+  }
+  LMP_RUNTIME_OR_FAIL(rt);
+  AdamWArgs a{};
+  a.beta1 = float(beta1);
+  a.rest1 = float(1 - beta1);
+  a.beta2 = float(beta2);
+  a.rest2 = float(1 - beta2);
+  a.eps = float(eps);
+  a.lr = lr;
+  a.beta1_d = beta1;
+  a.beta2_d = beta2;
+  a.seed = uint32_t(seed);
+  a.step = step;
+  uint64_t groups = 0;
+  bool advanced = false;
+  const auto launch = [&]() -> int {
+    if (bits == 32)
+      adamw_step<32><<<dim3(uint32_t(groups)), dim3(kThreads), 0, rt->stream>>>(a);
+    else
+      adamw_step<8><<<dim3(uint32_t(groups)), dim3(kThreads), 0, rt->stream>>>(a);
+    LMP_LAUNCH_CHECK("adamw_step");
+    return LMP_OK;
+  };
+  // A launch takes tensors until its list is full or its grid would pass 2^23
+  // workgroups (2^31 threads).
+  constexpr uint64_t kMostGroups = uint64_t(1) << 23;
+  for (size_t i = 0; i < count; ++i) {
+    const lmp_adamw_tensor& t = tensors[i];
+    const uint64_t need = (t.n + kPerGroup - 1) / kPerGroup;
+    if (need == 0 && a.count == 0) continue;
+    if (a.count == kTensors || (a.count && groups + need > kMostGroups)) {
+      if (int s = launch()) return s;
+      a.count = 0;
+      groups = 0;
+      if (need == 0) continue;
+    }
+    if (a.count == 0) a.place = uint32_t(i);
+    // A tensor without values keeps its place, and no workgroup.
+    const int k = a.count++;
+    a.list.p[k] = t.p;
+    a.list.g[k] = t.g;
+    a.list.m[k] = t.m;
+    a.list.v[k] = t.v;
+    a.list.m_scale[k] = t.m_scale;
+    a.list.v_scale[k] = t.v_scale;
+    a.list.n[k] = int64_t(t.n);
+    a.list.keep[k] = float(1 - lr * t.decay);
+    a.list.first[k] = uint32_t(groups);
+    groups += need;
+  }
+  if (groups) {
+    a.advance = advanced = groups <= kSelfCounted;
+    if (int s = launch()) return s;
+  }
+  if (!advanced) {
+    adamw_advance<<<dim3(1), dim3(1), 0, rt->stream>>>(step);
+    LMP_LAUNCH_CHECK("adamw_advance");
+  }
+  return LMP_OK;
+}
+
+extern "C" int lmp_k_adamw_decode(int signed_codes, const void* codes, const float* scales,
+                                  size_t n, float* out) {
+  if (n == 0) return LMP_OK;
+  if (!codes || !scales || !out) return fail(LMP_ERR_INVALID, "lmp_k_adamw_decode: null buffer");
+  if (n > (size_t(1) << 40)) return fail(LMP_ERR_UNSUPPORTED, "lmp_k_adamw_decode: too many values");
+  LMP_RUNTIME_OR_FAIL(rt);
+  const size_t groups = std::min<size_t>((n + kThreads * 4 - 1) / (kThreads * 4),
+                                         size_t(rt->cu_count) * 256);
+  const uint8_t* c = static_cast<const uint8_t*>(codes);
+  if (signed_codes)
+    adamw_values<true><<<dim3(uint32_t(groups)), dim3(kThreads), 0, rt->stream>>>(c, scales,
+                                                                                   int64_t(n), out);
+  else
+    adamw_values<false><<<dim3(uint32_t(groups)), dim3(kThreads), 0, rt->stream>>>(c, scales,
+                                                                                    int64_t(n), out);
+  LMP_LAUNCH_CHECK("adamw_decode");
+  return LMP_OK;
+}

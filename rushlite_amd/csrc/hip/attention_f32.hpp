@@ -1,0 +1,518 @@
+// Packed attention on the fp32 matrix cores: right for every case, and the
+// kernels of short batches, single tokens and operands that the split-fp16
+// kernels leave out.
+//
+//   S = c Q K^T (c = scale log2 e), P = 2^(S - lse2), O = P V
+//   D = rowsum(dO O), dS = P (dO V^T - D), dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO
+//
+// A wave works on 16 packed rows (the query heads that share a key head lie side
+// by side, so one read of a key serves all of them) and 16 keys at a time with
+// v_mfma_f32_16x16x4_f32.  Its operands come from memory straight into their
+// registers: an operand whose rows are contracted over d is read 4 values of d a
+// lane ("along"), one contracted over its rows 4 columns a lane ("across"); both
+// are 16-byte loads, since the order of a contraction is free.  Scores are formed
+// transposed, S^T = K Q^T: a lane then holds 4 keys of one query, which is the
+// layout in which P is the next product's operand, and a query's running maximum
+// and sum stay in its own lanes.  The four waves of a workgroup take every fourth
+// step of the keys (or rows) and join at the end, in a fixed order.
+//
+// Masked places.  A masked score becomes -inf (P exactly 0) whatever it was, and
+// where a step holds masked places the operand that P multiplies may hold an
+// infinity or NaN that its row must not see (0 inf = NaN): such values are taken
+// out of the product and added to the rows that see them.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "attention_plan.hpp"
+
+namespace lmp_hip {
+namespace {
+
+typedef float a4 __attribute__((ext_vector_type(4)));
+typedef float a4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef float a2_any __attribute__((ext_vector_type(2), aligned(4)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ a4 mfma_16(float a, float b, a4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ bool finite(float x) {
+  return (__builtin_bit_cast(uint32_t, x) & 0x7fffffffu) < 0x7f800000u;
+}
+// Over the four lanes that share a column of a 16 x 16 block.
+__device__ __forceinline__ float column_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float column_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+struct AttnArgs {
+  const AttnItem* items;
+  int count, kv_heads, group, dim;
+  bool causal;
+  const float *q, *k, *v, *g;
+  int64_t q_ld, k_ld, v_ld, g_ld;
+  float scale;
+  const float* lse_in;
+  const float* delta;  // [query][head]
+  float *o, *lse, *dk;  // o: forward's output or dq; dk with o as dv
+  int64_t o_ld, dk_ld;
+  float *part, *part_ml;  // [part][kv head][16 rows][dim], [...][16][2]
+  // Only the (sequence, key head)s that the split kernels leave out, or all.
+  const int16_t *q_exp, *k_exp, *v_exp, *g_exp;
+};
+
+// W values at p, zero from column `end` on.
+template <int W>
+__device__ __forceinline__ void load_cols(const float* p, int col, int end, float* out) {
+  if (col + W <= end) {
+    if constexpr (W == 4) {
+      const a4_any x = *reinterpret_cast<const a4_any*>(p + col);
+      out[0] = x[0]; out[1] = x[1]; out[2] = x[2]; out[3] = x[3];
+    } else if constexpr (W == 2) {
+      const a2_any x = *reinterpret_cast<const a2_any*>(p + col);
+      out[0] = x[0]; out[1] = x[1];
+    } else {
+      out[0] = p[col];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j) out[j] = col + j < end ? p[col + j] : 0.0f;
+  }
+}
+
+// ND: blocks of 16 columns.  Across: column j * 16 .. of chunk j / 4 is held
+// interleaved, `width` neighbouring columns a lane.
+template <int ND>
+struct Cols {
+  static constexpr int width(int j) { return j / 4 < ND / 4 ? 4 : ND % 4; }
+  static __device__ __forceinline__ int at(int j, int m) {
+    return 64 * (j / 4) + width(j) * m + j % 4;
+  }
+};
+
+// 16 columns x ND of one row, 4 a lane group: the operand contracted over d.
+template <int ND>
+__device__ __forceinline__ void load_along(const float* row, int g, int dim, float (&f)[ND][4]) {
+#pragma unroll
+  for (int b = 0; b < ND; ++b) load_cols<4>(row, 16 * b + 4 * g, dim, f[b]);
+}
+// One row as the operand contracted over its rows: lane m holds columns at(j, m).
+template <int ND>
+__device__ __forceinline__ void load_across(const float* row, int m, int dim, float (&f)[ND]) {
+#pragma unroll
+  for (int c = 0; c < ND / 4; ++c) load_cols<4>(row, 64 * c + 4 * m, dim, f + 4 * c);
+  constexpr int rest = ND % 4;
+  if constexpr (rest != 0)
+    load_cols<rest>(row, 64 * (ND / 4) + rest * m, dim, f + ND / 4 * 4);
+}
+
+template <int ND>
+__device__ __forceinline__ a4 product_along(const float (&a)[ND][4], const float (&b)[ND][4]) {
+  a4 s = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = mfma_16(a[i][j], b[i][j], s);
+  return s;
+}
+
+// acc += rows^T p over 16 rows, p the lane's 4 of them (4 g + r) for its column.
+// With `masked`, infinities and NaN of the rows reach only the columns that see
+// them: sees(row in 0..15) for the lane's column; row_at(row) is its address.
+template <int ND, class Sees, class RowAt>
+__device__ __forceinline__ void accumulate(a4 (&acc)[ND], float (&f)[4][ND], const float (&p)[4],
+                                           int dim, bool masked, Sees&& sees, RowAt&& row_at) {
+  bool odd = false;
+  if (masked) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+        if (!finite(f[r][j])) {
+          odd = true;
+          f[r][j] = 0.0f;
+        }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int j = 0; j < ND; ++j) acc[j] = mfma_16(f[r][j], p[r], acc[j]);
+  if (masked && __any(odd)) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    for (int kk = 0; kk < 16; ++kk) {
+      float pk = 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = __shfl(p[r], (kk >> 2) * 16 + n);
+        pk = (kk & 3) == r ? x : pk;
+      }
+      const bool s = sees(kk);
+      const float* row = row_at(kk);
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int c = Cols<ND>::at(j, 4 * g + r);
+          const float x = c < dim ? row[c] : 0.0f;
+          if (s && !finite(x)) acc[j][r] += pk * x;
+        }
+    }
+  }
+}
+
+// The four waves' blocks [column of 16][d], summed in order and handed out:
+// put(row, column, 4 values) by every lane.
+template <int ND, class Put>
+__device__ __forceinline__ void join_waves(const a4 (&acc)[ND], float* lds, Put&& put) {
+  constexpr int PITCH = ND * 16 + 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < ND; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      lds[(wave * 16 + n) * PITCH + Cols<ND>::at(j, 4 * g + r)] = acc[j][r];
+  __syncthreads();
+  const int row = threadIdx.x >> 4;
+  for (int c = (threadIdx.x & 15) * 4; c < ND * 16; c += 64) {
+    a4 s = *reinterpret_cast<const a4*>(lds + row * PITCH + c);
+#pragma unroll
+    for (int w = 1; w < 4; ++w) s += *reinterpret_cast<const a4*>(lds + (w * 16 + row) * PITCH + c);
+    put(row, c, s);
+  }
+}
+__device__ __forceinline__ void store_cols(float* row, int col, int end, a4 x) {
+  if (col + 4 <= end) {
+    *reinterpret_cast<a4_any*>(row + col) = x;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < end) row[col + j] = x[j];
+  }
+}
+
+// Whether a (sequence, key head) is left to the fp32 kernels: one of its tiles
+// holds what the split cannot (see attention_split.hpp).  All threads call it.
+constexpr int16_t kIrregular = 0x7fff;
+__device__ __forceinline__ bool left_out(const AttnItem& it, const int16_t* q_exp,
+                                         const int16_t* k_exp, const int16_t* v_exp,
+                                         const int16_t* g_exp, int kv_heads, int group, int kv) {
+  const int qt = (it.lq + kAttnTile - 1) / kAttnTile, kt = (it.lk + kAttnTile - 1) / kAttnTile;
+  bool odd = false;
+  for (int t = threadIdx.x; t < kt; t += blockDim.x) {
+    const int64_t at = int64_t(it.kt0 + t) * kv_heads + kv;
+    odd = odd || k_exp[at] == kIrregular || v_exp[at] == kIrregular;
+  }
+  for (int t = threadIdx.x; t < qt * group; t += blockDim.x) {
+    const int64_t at = int64_t(it.qt0 + t / group) * kv_heads * group + kv * group + t % group;
+    odd = odd || q_exp[at] == kIrregular || (g_exp && g_exp[at] == kIrregular);
+  }
+  return __syncthreads_or(odd);
+}
+__device__ __forceinline__ bool skipped(const AttnArgs& a, const AttnItem& it, int kv) {
+  return a.k_exp &&
+         !left_out(it, a.q_exp, a.k_exp, a.v_exp, a.g_exp, a.kv_heads, a.group, kv);
+}
+
+template <int ND>
+__global__ __launch_bounds__(256) void attention_rows(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (ND * 16 + 4)];
+  __shared__ float ml[2][4][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+  for (int64_t w = blockIdx.x; w < int64_t(a.count) * a.kv_heads; w += gridDim.x) {
+    const int kv = int(w % a.kv_heads);
+    const AttnItem it = a.items[w / a.kv_heads];
+    if (skipped(a, it, kv)) continue;
+    const int rows = min(kAttnRows, it.lq * a.group - it.first);
+    const int packed = it.first + min(n, rows - 1);
+    const int query = packed / a.group, head = kv * a.group + packed % a.group;
+    const int limit = min(it.key_end, a.causal ? max(0, query + 1 + it.lk - it.lq) : it.lk);
+    float q[ND][4];
+    load_along<ND>(a.q + int64_t(it.q0 + query) * a.q_ld + int64_t(head) * a.dim, g, a.dim, q);
+    const float c = a.scale * kLog2e;
+    const float* k0 = a.k + int64_t(it.k0) * a.k_ld + int64_t(kv) * a.dim;
+    const float* v0 = a.v + int64_t(it.k0) * a.v_ld + int64_t(kv) * a.dim;
+    a4 acc[ND];
+#pragma unroll
+    for (int j = 0; j < ND; ++j) acc[j] = a4{0, 0, 0, 0};
+    float top = -__builtin_inff(), sum = 0;
+    for (int kt = it.key_begin + wave * 16; kt < it.key_end; kt += 64) {
+      const auto key = [&](int i) { return min(kt + i, it.lk - 1); };
+      float k[ND][4], v[4][ND];
+      load_along<ND>(k0 + int64_t(key(n)) * a.k_ld, g, a.dim, k);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        load_across<ND>(v0 + int64_t(key(4 * g + r)) * a.v_ld, n, a.dim, v[r]);
+      const a4 s = product_along<ND>(k, q);
+      float p[4], best = top;
+      bool whole = true;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool seen = kt + 4 * g + r < limit;
+        whole = whole && seen;
+        p[r] = seen ? s[r] * c : -__builtin_inff();
+        best = fmaxf(best, p[r]);
+      }
+      best = column_max(best);
+      const float base = best > -__builtin_inff() ? best : 0.0f;
+      const float fade = exp2_of(top - base);  // 0 at the first keys
+      top = best;
+      sum *= fade;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[r] = exp2_of(p[r] - base);
+        sum += p[r];
+      }
+#pragma unroll
+      for (int j = 0; j < ND; ++j) acc[j] *= fade;
+      accumulate<ND>(acc, v, p, a.dim, __any(!whole), [&](int i) { return kt + i < limit; },
+                     [&](int i) { return v0 + int64_t(key(i)) * a.v_ld; });
+    }
+    sum = column_sum(sum);
+    if (g == 0) {
+      ml[0][wave][n] = top;
+      ml[1][wave][n] = sum;
+    }
+    __syncthreads();
+    float all = ml[0][0][n];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) all = fmaxf(all, ml[0][i][n]);
+    const float base = all > -__builtin_inff() ? all : 0.0f;
+    float total = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) total += ml[1][i][n] * exp2_of(ml[0][i][n] - base);
+    float mine = exp2_of(top - base);
+    if (it.part < 0) mine = total > 0 || total != total ? mine / total : 0.0f;
+#pragma unroll
+    for (int j = 0; j < ND; ++j) acc[j] *= mine;
+    const int64_t slot = int64_t(it.part) * a.kv_heads + kv;
+    if (wave == 0 && g == 0 && n < rows) {
+      if (it.part >= 0) {
+        a.part_ml[(slot * 16 + n) * 2] = all;
+        a.part_ml[(slot * 16 + n) * 2 + 1] = total;
+      } else if (a.lse) {
+        a.lse[int64_t(it.q0 + query) * (a.kv_heads * a.group) + head] =
+            (base + __builtin_amdgcn_logf(total)) * kLn2;
+      }
+    }
+    join_waves<ND>(acc, lds, [&](int row, int col, a4 x) {
+      if (row >= rows) return;
+      const int r = it.first + row;
+      float* to = it.part >= 0
+                      ? a.part + (slot * 16 + row) * a.dim
+                      : a.o + int64_t(it.q0 + r / a.group) * a.o_ld +
+                            int64_t(kv * a.group + r % a.group) * a.dim;
+      store_cols(to, col, a.dim, x);
+    });
+    __syncthreads();
+  }
+}
+
+// Joins the parts of packed rows: 16 lanes a row.
+__global__ __launch_bounds__(256) void attention_join(AttnArgs a, const AttnJoin* joins, int count) {
+  for (int64_t w = blockIdx.x; w < int64_t(count) * a.kv_heads; w += gridDim.x) {
+    const int kv = int(w % a.kv_heads);
+    const AttnJoin j = joins[w / a.kv_heads];
+    const int rows = min(kAttnRows, j.lq * a.group - j.first), row = threadIdx.x >> 4;
+    if (row >= rows) continue;
+    const auto slot = [&](int p) {
+      return ((int64_t(j.part) + p) * a.kv_heads + kv) * 16 + row;
+    };
+    float all = -__builtin_inff();
+    for (int p = 0; p < j.parts; ++p) all = fmaxf(all, a.part_ml[slot(p) * 2]);
+    const float base = all > -__builtin_inff() ? all : 0.0f;
+    float total = 0;
+    for (int p = 0; p < j.parts; ++p)
+      total += a.part_ml[slot(p) * 2 + 1] * exp2_of(a.part_ml[slot(p) * 2] - base);
+    const float one = total > 0 || total != total ? 1.0f / total : 0.0f;
+    const int r = j.first + row, query = r / a.group, head = kv * a.group + r % a.group;
+    float* to = a.o + int64_t(j.q0 + query) * a.o_ld + int64_t(head) * a.dim;
+    for (int c = (threadIdx.x & 15) * 4; c < a.dim; c += 64) {
+      a4 s = {0, 0, 0, 0};
+      for (int p = 0; p < j.parts; ++p) {
+        float x[4];
+        load_cols<4>(a.part + slot(p) * a.dim, c, a.dim, x);
+        const float f = exp2_of(a.part_ml[slot(p) * 2] - base);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] += f * x[i];
+      }
+      store_cols(to, c, a.dim, s * one);
+    }
+    if (a.lse && (threadIdx.x & 15) == 0)
+      a.lse[int64_t(j.q0 + query) * (a.kv_heads * a.group) + head] =
+          (base + __builtin_amdgcn_logf(total)) * kLn2;
+  }
+}
+
+// delta = rowsum(g o) of every query and head: 16 lanes each.
+__global__ __launch_bounds__(256) void attention_delta(int64_t queries, int heads, int dim,
+                                                       const float* o, int64_t o_ld, const float* g,
+                                                       int64_t g_ld, float* delta) {
+  const int64_t step = int64_t(gridDim.x) * 16, total = queries * heads;
+  for (int64_t first = int64_t(blockIdx.x) * 16; first < total; first += step) {
+    const int64_t i = min(first + (threadIdx.x >> 4), total - 1);
+    const int64_t row = i / heads, head = i % heads;
+    float s = 0;
+    for (int c = (threadIdx.x & 15) * 4; c < dim; c += 64) {
+      float x[4], y[4];
+      load_cols<4>(o + row * o_ld + head * dim, c, dim, x);
+      load_cols<4>(g + row * g_ld + head * dim, c, dim, y);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = fmaf(x[j], y[j], s);
+    }
+    s += __shfl_xor(s, 1);
+    s += __shfl_xor(s, 2);
+    s += __shfl_xor(s, 4);
+    s += __shfl_xor(s, 8);
+    if ((threadIdx.x & 15) == 0) delta[i] = s;
+  }
+}
+
+// A row's lse in base 2; +inf, which makes its P zero, where it sees nothing.
+__device__ __forceinline__ float lse2_of(float lse) {
+  return lse == -__builtin_inff() ? __builtin_inff() : lse * kLog2e;
+}
+
+template <int ND>
+__global__ __launch_bounds__(256) void attention_back_rows(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (ND * 16 + 4)];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+  const int heads = a.kv_heads * a.group;
+  for (int64_t w = blockIdx.x; w < int64_t(a.count) * a.kv_heads; w += gridDim.x) {
+    const int kv = int(w % a.kv_heads);
+    const AttnItem it = a.items[w / a.kv_heads];
+    if (it.part >= 0 && it.key_begin > 0) continue;  // a split row's first part takes all its keys
+    if (skipped(a, it, kv)) continue;
+    const int rows = min(kAttnRows, it.lq * a.group - it.first);
+    const int packed = it.first + min(n, rows - 1);
+    const int query = packed / a.group, head = kv * a.group + packed % a.group;
+    const int limit = a.causal ? max(0, query + 1 + it.lk - it.lq) : it.lk;
+    const int last = (it.first + rows - 1) / a.group;
+    const int key_end = a.causal ? max(0, min(it.lk, last + 1 + it.lk - it.lq)) : it.lk;
+    float q[ND][4], go[ND][4];
+    load_along<ND>(a.q + int64_t(it.q0 + query) * a.q_ld + int64_t(head) * a.dim, g, a.dim, q);
+    load_along<ND>(a.g + int64_t(it.q0 + query) * a.g_ld + int64_t(head) * a.dim, g, a.dim, go);
+    const float c = a.scale * kLog2e;
+    const float lse2 = lse2_of(a.lse_in[int64_t(it.q0 + query) * heads + head]);
+    const float delta = a.delta[int64_t(it.q0 + query) * heads + head];
+    const float* k0 = a.k + int64_t(it.k0) * a.k_ld + int64_t(kv) * a.dim;
+    const float* v0 = a.v + int64_t(it.k0) * a.v_ld + int64_t(kv) * a.dim;
+    a4 acc[ND];
+#pragma unroll
+    for (int j = 0; j < ND; ++j) acc[j] = a4{0, 0, 0, 0};
+    for (int kt = wave * 16; kt < key_end; kt += 64) {
+      const auto key = [&](int i) { return min(kt + i, it.lk - 1); };
+      float k[ND][4], v[ND][4], kc[4][ND];
+      load_along<ND>(k0 + int64_t(key(n)) * a.k_ld, g, a.dim, k);
+      load_along<ND>(v0 + int64_t(key(n)) * a.v_ld, g, a.dim, v);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        load_across<ND>(k0 + int64_t(key(4 * g + r)) * a.k_ld, n, a.dim, kc[r]);
+      const a4 s = product_along<ND>(k, q), dp = product_along<ND>(v, go);
+      float ds[4];
+      bool whole = true;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool seen = kt + 4 * g + r < limit;
+        whole = whole && seen;
+        ds[r] = seen ? exp2_of(s[r] * c - lse2) * (dp[r] - delta) : 0.0f;
+      }
+      accumulate<ND>(acc, kc, ds, a.dim, __any(!whole), [&](int i) { return kt + i < limit; },
+                     [&](int i) { return k0 + int64_t(key(i)) * a.k_ld; });
+    }
+    join_waves<ND>(acc, lds, [&](int row, int col, a4 x) {
+      if (row >= rows) return;
+      const int r = it.first + row;
+      store_cols(a.o + int64_t(it.q0 + r / a.group) * a.o_ld +
+                     int64_t(kv * a.group + r % a.group) * a.dim,
+                 col, a.dim, x * a.scale);
+    });
+    __syncthreads();
+  }
+}
+
+template <int ND>
+__global__ __launch_bounds__(256) void attention_back_keys(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (ND * 16 + 4)];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+  const int heads = a.kv_heads * a.group;
+  for (int64_t w = blockIdx.x; w < int64_t(a.count) * a.kv_heads; w += gridDim.x) {
+    const int kv = int(w % a.kv_heads);
+    const AttnItem it = a.items[w / a.kv_heads];
+    if (skipped(a, it, kv)) continue;
+    const int keys = min(kAttnRows, it.lk - it.first), key = it.first + min(n, keys - 1);
+    const int rows = it.lq * a.group, ahead = it.lk - it.lq;
+    // The first query that sees the first key here.
+    const int from = a.causal ? max(0, it.first - ahead) * a.group / 16 * 16 : 0;
+    float k[ND][4], v[ND][4];
+    load_along<ND>(a.k + int64_t(it.k0 + key) * a.k_ld + int64_t(kv) * a.dim, g, a.dim, k);
+    load_along<ND>(a.v + int64_t(it.k0 + key) * a.v_ld + int64_t(kv) * a.dim, g, a.dim, v);
+    const float c = a.scale * kLog2e;
+    a4 dk[ND], dv[ND];
+#pragma unroll
+    for (int j = 0; j < ND; ++j) dk[j] = dv[j] = a4{0, 0, 0, 0};
+    for (int rt = from + wave * 16; rt < rows; rt += 64) {
+      const auto packed = [&](int i) { return min(rt + i, rows - 1); };
+      const auto q_at = [&](int i) {
+        const int r = packed(i);
+        return a.q + int64_t(it.q0 + r / a.group) * a.q_ld +
+               int64_t(kv * a.group + r % a.group) * a.dim;
+      };
+      const auto g_at = [&](int i) {
+        const int r = packed(i);
+        return a.g + int64_t(it.q0 + r / a.group) * a.g_ld +
+               int64_t(kv * a.group + r % a.group) * a.dim;
+      };
+      const auto sees = [&](int i) {
+        return rt + i < rows && (!a.causal || key <= (rt + i) / a.group + ahead);
+      };
+      float q[ND][4], go[ND][4];
+      load_along<ND>(q_at(n), g, a.dim, q);
+      load_along<ND>(g_at(n), g, a.dim, go);
+      const a4 s = product_along<ND>(q, k), dp = product_along<ND>(go, v);
+      float p[4], ds[4];
+      bool whole = true;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 4 * g + r, at = packed(i);
+        const int64_t stat =
+            int64_t(it.q0 + at / a.group) * heads + kv * a.group + at % a.group;
+        const bool seen = sees(i);
+        whole = whole && seen;
+        p[r] = seen ? exp2_of(s[r] * c - lse2_of(a.lse_in[stat])) : 0.0f;
+        ds[r] = seen ? p[r] * (dp[r] - a.delta[stat]) : 0.0f;
+      }
+      const bool masked = __any(!whole);
+      float f[4][ND];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) load_across<ND>(g_at(4 * g + r), n, a.dim, f[r]);
+      accumulate<ND>(dv, f, p, a.dim, masked, sees, g_at);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) load_across<ND>(q_at(4 * g + r), n, a.dim, f[r]);
+      accumulate<ND>(dk, f, ds, a.dim, masked, sees, q_at);
+    }
+    join_waves<ND>(dv, lds, [&](int row, int col, a4 x) {
+      if (row < keys)
+        store_cols(a.o + int64_t(it.k0 + it.first + row) * a.o_ld + int64_t(kv) * a.dim, col, a.dim,
+                   x);
+    });
+    join_waves<ND>(dk, lds, [&](int row, int col, a4 x) {
+      if (row < keys)
+        store_cols(a.dk + int64_t(it.k0 + it.first + row) * a.dk_ld + int64_t(kv) * a.dim, col,
+                   a.dim, x * a.scale);
+    });
+    __syncthreads();
+  }
+}
+
+}  // namespace
+}  // namespace lmp_hip
