@@ -153,18 +153,20 @@ void device_sync() {
 Variable s2v(const Variable& like, Scalar s) { return ag::scalar_var(like, s); }
 
 // One captured device graph (lmp_rt_graph_*): the library stream's work
-// between begin() and end(), replayed by launch().  Scalars the capture reads
-// are kept here for the graph's lifetime.
+// between begin() and end(), replayed by launch().  Scalars the capture reads,
+// and the plans and optimizer states it uses, are kept here for the graph's
+// lifetime.
 struct HipGraph {
   void* handle = nullptr;
   bool open = false;
   std::vector<Tensor> keep;
+  std::vector<std::shared_ptr<const void>> held;
 
   void begin() {
     LMP_CHECK(!open && !handle) << "graph: already captured (make a new Graph)";
     lmp::hip_ok(lmp_rt_graph_begin(), "lmp_rt_graph_begin");
     open = true;
-    lmp::tensor::set_graph_keep_alive(&keep);
+    lmp::tensor::set_graph_keep_alive(&keep, &held);
   }
   void end() {
     LMP_CHECK(open) << "graph: no capture is open";
@@ -189,6 +191,8 @@ struct HipGraph {
 };
 
 }  // namespace
+
+void bind_transformer(py::module_& m);  // transformer.cpp
 
 PYBIND11_MODULE(_C, m) {
   m.doc() = "Lamp3 on AMD Instinct MI355X: HIP device backend + host framework";
@@ -405,6 +409,8 @@ PYBIND11_MODULE(_C, m) {
         py::arg("requires_grad") = false, py::arg("device") = lmp::tensor::DEFAULT_DEVICE,
         py::arg("dtype") = lmp::tensor::DEFAULT_DTYPE);
   m.def("manual_seed", &ag::manual_seed, py::arg("seed"));
+
+  bind_transformer(m);
 
   m.def("set_capture_enabled", &lmp::tensor::lazy::set_capture_enabled);
   m.def("is_capture_enabled", &lmp::tensor::lazy::is_capture_enabled);

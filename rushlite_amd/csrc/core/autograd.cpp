@@ -209,6 +209,15 @@ bool Variable::incr_grad_linear(Variable& w, Variable& b, const Tensor& x, const
   return true;
 }
 
+void Variable::incr_grad_owned(const Tensor& g) {
+  LMP_CHECK(requires_grad()) << "Cannot access grad() if requires_grad = false";
+  if (impl_->grad.defined()) return incr_grad(g);
+  LMP_INTERNAL_ASSERT(g.shape() == impl_->data.shape())
+      << "There should be no broadcasting in incr_grad";
+  impl_->grad = g;
+  impl_->grad_pass = t_backward_pass;
+}
+
 void Variable::set_grad_fn(std::shared_ptr<Function> fn) {
   LMP_CHECK(requires_grad()) << "Cannot access grad() if requires_grad = false";
   impl_->grad_fn = std::move(fn);

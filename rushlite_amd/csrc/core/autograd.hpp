@@ -74,6 +74,9 @@ class Variable {
   // in one launch where the products are small.
   static bool incr_grad_linear(Variable& w, Variable& b, const Tensor& x, const Tensor& g,
                                const Tensor* relu_out = nullptr, Variable* xv = nullptr);
+  // grad += g for a tensor a backward kernel has just made, which nothing else
+  // holds: the first term becomes the gradient as it is.
+  void incr_grad_owned(const Tensor& g);
   void set_grad_fn(std::shared_ptr<Function> fn);
   void copy(const Variable& other);
   void fill(Scalar value);

@@ -295,11 +295,19 @@ Tensor zeros_like(const Tensor& t) { return full_like(t, 0); }
 namespace {
 std::mutex g_scalar_mu;
 std::vector<Tensor>* g_graph_keep = nullptr;
+std::vector<std::shared_ptr<const void>>* g_graph_held = nullptr;
 }  // namespace
 
-void set_graph_keep_alive(std::vector<Tensor>* keep) {
+void set_graph_keep_alive(std::vector<Tensor>* keep,
+                          std::vector<std::shared_ptr<const void>>* held) {
   std::lock_guard<std::mutex> lock(g_scalar_mu);
   g_graph_keep = keep;
+  g_graph_held = held;
+}
+
+void keep_for_graph(std::shared_ptr<const void> what) {
+  std::lock_guard<std::mutex> lock(g_scalar_mu);
+  if (g_graph_held) g_graph_held->push_back(std::move(what));
 }
 
 Tensor scalar_like(const Tensor& t, Scalar s) {
