@@ -1,5 +1,5 @@
 // Packed attention: plans, checks and launches.  The kernels and their
-// mathematics: attention_f32.hpp.
+// mathematics: attention_f32.hpp and attention_split.hpp.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -12,20 +12,28 @@
 #include "common.hpp"
 #include "lmp_hip_transformer.h"
 
-#include "attention_f32.hpp"
+#include "attention_split.hpp"
 
 namespace lmp_hip {
 namespace {
 
+// A list on the device.
+template <class T>
+struct List {
+  const T* at = nullptr;
+  int count = 0;
+};
+
 struct AttentionPlan {
   int64_t heads, kv_heads, dim;
   bool causal;
-  int64_t queries, keys, parts;
+  int64_t queries, keys, parts, q_parts, k_parts;
   double pairs;
-  int rows_count, keys_count, joins_count;
   char* device = nullptr;  // the lists, one after another
-  const AttnItem *rows, *key_items;
-  const AttnJoin* joins;
+  List<AttnItem> rows, key_items, q_blocks, k_blocks;
+  List<AttnJoin> joins, q_joins, k_joins;
+  List<AttnTile> q_tiles, k_tiles;
+  List<AttnSeq> seqs;
 };
 
 // Calls f with the ND blocks of 16 columns that hold `dim`.
@@ -61,58 +69,285 @@ AttnArgs common_args(const AttentionPlan& plan, double scale) {
   return a;
 }
 
-int forward(Runtime* rt, const AttentionPlan& plan, AttnArgs a) {
-  if (plan.queries == 0) return LMP_OK;
-  Scratch part;
-  const size_t slots = size_t(plan.parts) * size_t(plan.kv_heads) * kAttnRows;
-  if (!part.get(slots * size_t(plan.dim + 2) * sizeof(float))) return LMP_ERR_OOM;
-  a.part_ml = static_cast<float*>(part.p);
-  a.part = a.part_ml + slots * 2;
-  a.items = plan.rows;
-  a.count = plan.rows_count;
-  const uint32_t grid = grid_of(int64_t(a.count) * plan.kv_heads);
+// Batches of at least this many multiplications per product (pairs, heads and
+// columns) take the split-fp16 kernels.
+constexpr double kSplitWork = 1;
+
+// Whether the split-fp16 kernels run a batch.
+bool split_form(const AttentionPlan& plan, double scale) {
+  const int64_t grid = int64_t(plan.q_blocks.count) * plan.heads +
+                       int64_t(plan.k_blocks.count) * plan.kv_heads +
+                       int64_t(plan.q_tiles.count) * 2 * plan.heads +
+                       int64_t(plan.k_tiles.count) * 2 * plan.kv_heads;
+  return plan.dim <= 128 && scale != 0 && grid < (int64_t(1) << 23) &&
+         plan.pairs * double(plan.heads) * double(plan.dim) >= kSplitWork;
+}
+
+// Calls f with the ND of the split kernels that hold `dim` (at most 128).
+template <class F>
+void with_split_dim(int64_t dim, F&& f) {
+  using std::integral_constant;
+  const int64_t nd = (dim + 15) / 16;
+  if (nd <= 2) f(integral_constant<int, 2>{});
+  else if (nd <= 4) f(integral_constant<int, 4>{});
+  else if (nd <= 5) f(integral_constant<int, 5>{});
+  else if (nd <= 6) f(integral_constant<int, 6>{});
+  else f(integral_constant<int, 8>{});
+}
+
+// The operands' fragments, exponents and marks in one allocation.
+struct SplitOperands {
+  Scratch memory;
+  SplitAttnArgs args{};
+  float* stats = nullptr;
+  int32_t* any_mark = nullptr;
+};
+
+// Splits q, k, v (and g) for the forward or the backward kernels.  LMP_ERR_OOM
+// leaves nothing launched.
+int split_operands(Runtime* rt, const AttentionPlan& plan, const AttnArgs& a, double scale,
+                   bool back, SplitOperands& out) {
+  const int64_t qn = int64_t(plan.q_tiles.count) * plan.heads,
+                kn = int64_t(plan.k_tiles.count) * plan.kv_heads;
+  int status = LMP_OK;
+  with_split_dim(plan.dim, [&](auto nd) {
+    using F = Frag<nd>;
+    size_t bytes = 0;
+    const auto place = [&](size_t n) {
+      const size_t at = bytes;
+      bytes += (n + 255) / 256 * 256;
+      return at;
+    };
+    const size_t q_along = place(qn * F::ALONG), k_along = place(kn * F::ALONG);
+    const size_t v_across = place(back ? 0 : kn * F::ACROSS), v_along = place(back ? kn * F::ALONG : 0);
+    const size_t g_along = place(back ? qn * F::ALONG : 0);
+    const size_t q_across = place(back ? qn * F::ACROSS : 0), g_across = place(back ? qn * F::ACROSS : 0);
+    const size_t k_across = place(back ? kn * F::ACROSS : 0);
+    const size_t exps = place((2 * qn + 2 * kn) * 4), marks = place((plan.seqs.count * plan.kv_heads + 1) * 4);
+    const size_t stats = place(back ? qn * 256 : 0);
+    if (!out.memory.get(bytes)) {
+      status = LMP_ERR_OOM;
+      return;
+    }
+    char* m = static_cast<char*>(out.memory.p);
+    int32_t* e = reinterpret_cast<int32_t*>(m + exps);
+    SplitAttnArgs& s = out.args;
+    s.kv_heads = int(plan.kv_heads);
+    s.group = int(plan.heads / plan.kv_heads);
+    s.dim = int(plan.dim);
+    s.causal = plan.causal;
+    s.scale = float(scale);
+    s.scale_log2e = std::fabs(float(scale)) * kLog2e;
+    s.q_along = m + q_along;
+    s.k_along = m + k_along;
+    s.v_along = m + v_along;
+    s.v_across = m + v_across;
+    s.g_along = m + g_along;
+    s.q_across = m + q_across;
+    s.g_across = m + g_across;
+    s.k_across = m + k_across;
+    s.q_exp = e;
+    s.k_exp = e + qn;
+    s.v_exp = e + qn + kn;
+    s.g_exp = back ? e + qn + 2 * kn : nullptr;
+    s.marks = reinterpret_cast<const int32_t*>(m + marks);
+    out.any_mark = reinterpret_cast<int32_t*>(m + marks) + plan.seqs.count * plan.kv_heads;
+    out.stats = reinterpret_cast<float*>(m + stats);
+    s.stats = out.stats;
+    SplitArgs p{};
+    p.dim = int(plan.dim);
+    p.any_mark = out.any_mark;
+    const auto add = [&](const float* x, int64_t ld, bool queries, float sign, char* along,
+                         char* across, const int32_t* exponent) {
+      const auto& tiles = queries ? plan.q_tiles : plan.k_tiles;
+      if (tiles.count)
+        p.op[p.count++] = {x, ld, tiles.at, tiles.count, int(queries ? plan.heads : plan.kv_heads),
+                           sign, along, across, const_cast<int32_t*>(exponent)};
+    };
+    add(a.q, a.q_ld, true, scale < 0 ? -1.0f : 1.0f, m + q_along, back ? m + q_across : nullptr, s.q_exp);
+    add(a.k, a.k_ld, false, 1.0f, m + k_along, back ? m + k_across : nullptr, s.k_exp);
+    add(a.v, a.v_ld, false, 1.0f, back ? m + v_along : nullptr, back ? nullptr : m + v_across, s.v_exp);
+    if (back) add(a.g, a.g_ld, true, 1.0f, m + g_along, m + g_across, s.g_exp);
+    attention_split<nd><<<dim3(uint32_t(qn + 2 * kn + (back ? qn : 0))), dim3(256), 0, rt->stream>>>(p);
+    status = [&]() -> int {
+      LMP_LAUNCH_CHECK("attention_split");
+      attention_marks<<<dim3(uint32_t(plan.seqs.count * plan.kv_heads)), dim3(256), 0, rt->stream>>>(
+          plan.seqs.at, s.kv_heads, s.group, s.q_exp, s.k_exp, s.v_exp, s.g_exp,
+          const_cast<int32_t*>(s.marks), out.any_mark);
+      LMP_LAUNCH_CHECK("attention_marks");
+      return LMP_OK;
+    }();
+  });
+  return status;
+}
+
+// Launches a split kernel with its stages of LDS, which pass 64 KiB.
+template <class Kernel>
+int launch_split(Runtime* rt, const char* name, Kernel kernel, int64_t grid, int lds,
+                 const SplitAttnArgs& s) {
+  LMP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  kernel<<<dim3(uint32_t(grid)), dim3(256), size_t(lds), rt->stream>>>(s);
+  LMP_LAUNCH_CHECK(name);
+  return LMP_OK;
+}
+
+// The fp32 kernels, over all rows or over the marked ones only (none as a rule:
+// a small grid finds that out).
+uint32_t f32_grid(const AttnArgs& a) {
+  const int64_t work = int64_t(a.count) * a.kv_heads;
+  return grid_of(a.marks ? std::min<int64_t>(work, 1024) : work);
+}
+int forward_f32(Runtime* rt, const AttentionPlan& plan, AttnArgs a) {
+  a.items = plan.rows.at;
+  a.count = plan.rows.count;
   with_dim(plan.dim, [&](auto nd) {
-    attention_rows<nd><<<dim3(grid), dim3(256), 0, rt->stream>>>(a);
+    attention_rows<nd><<<dim3(f32_grid(a)), dim3(256), 0, rt->stream>>>(a);
   });
   LMP_LAUNCH_CHECK("attention_rows");
-  if (plan.joins_count) {
-    attention_join<<<dim3(grid_of(int64_t(plan.joins_count) * plan.kv_heads)), dim3(256), 0,
-                     rt->stream>>>(a, plan.joins, plan.joins_count);
+  return LMP_OK;
+}
+
+int forward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale) {
+  if (plan.queries == 0) return LMP_OK;
+  SplitOperands split;
+  Scratch part;
+  const auto parts = [&](int64_t n, int64_t heads, int64_t rows) {
+    const size_t slots = size_t(n) * size_t(heads) * size_t(rows);
+    if (!part.get(slots * size_t(plan.dim + 2) * sizeof(float))) return false;
+    a.part_ml = static_cast<float*>(part.p);
+    a.part = a.part_ml + slots * 2;
+    return true;
+  };
+  if (split_form(plan, scale)) {
+    if (!parts(plan.q_parts, plan.heads, kAttnSplitRows)) return LMP_ERR_OOM;
+    if (int s = split_operands(rt, plan, a, scale, false, split)) return s;
+    SplitAttnArgs& s = split.args;
+    s.items = plan.q_blocks.at;
+    s.count = plan.q_blocks.count;
+    s.o = a.o;
+    s.o_ld = a.o_ld;
+    s.lse = a.lse;
+    s.part = a.part;
+    s.part_ml = a.part_ml;
+    int status = LMP_OK;
+    with_split_dim(plan.dim, [&](auto nd) {
+      status = launch_split(rt, "attention_split_rows", attention_split_rows<nd>,
+                            int64_t(s.count) * plan.heads,
+                            2 * (Frag<nd>::ALONG + Frag<nd>::ACROSS), s);
+    });
+    if (status) return status;
+    if (plan.q_joins.count) {
+      AttnArgs j = a;  // every head's rows by themselves
+      j.kv_heads = int(plan.heads);
+      j.group = 1;
+      attention_join<kAttnSplitRows>
+          <<<dim3(grid_of(int64_t(plan.q_joins.count) * plan.heads * (kAttnSplitRows / 16))),
+             dim3(256), 0, rt->stream>>>(j, plan.q_joins.at, plan.q_joins.count);
+      LMP_LAUNCH_CHECK("attention_join");
+    }
+    a.marks = s.marks;
+    a.any_mark = split.any_mark;
+    return forward_f32(rt, plan, a);
+  }
+  if (!parts(plan.parts, plan.kv_heads, kAttnRows)) return LMP_ERR_OOM;
+  if (int s = forward_f32(rt, plan, a)) return s;
+  if (plan.joins.count) {
+    attention_join<kAttnRows>
+        <<<dim3(grid_of(int64_t(plan.joins.count) * plan.kv_heads)), dim3(256), 0, rt->stream>>>(
+            a, plan.joins.at, plan.joins.count);
     LMP_LAUNCH_CHECK("attention_join");
   }
   return LMP_OK;
 }
 
-int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, const float* o, int64_t o_ld,
-             float* dq, int64_t dq_ld, float* dk, int64_t dk_ld, float* dv, int64_t dv_ld) {
+int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, const float* o,
+             int64_t o_ld, float* dq, int64_t dq_ld, float* dk, int64_t dk_ld, float* dv,
+             int64_t dv_ld) {
   Scratch delta;
+  SplitOperands split;
   if (!delta.get(size_t(plan.queries) * size_t(plan.heads) * sizeof(float))) return LMP_ERR_OOM;
-  if (plan.queries) {
+  if (split_form(plan, scale)) {
+    if (int s = split_operands(rt, plan, a, scale, true, split)) return s;
+    SplitAttnArgs& s = split.args;
+    attention_split_stats<<<dim3(uint32_t(int64_t(plan.q_tiles.count) * plan.heads)), dim3(256), 0,
+                            rt->stream>>>(plan.q_tiles.at, int(plan.heads), int(plan.dim), o, o_ld,
+                                          a.g, a.g_ld, a.lse_in, split.stats,
+                                          static_cast<float*>(delta.p));
+    LMP_LAUNCH_CHECK("attention_split_stats");
+    // Rows first, then keys; each one's parts are summed before the next needs the
+    // memory.
+    const size_t slot = size_t(kAttnSplitRows) * size_t(plan.dim) * sizeof(float);
+    const size_t q_bytes = size_t(plan.q_parts) * size_t(plan.heads) * slot,
+                 k_bytes = size_t(plan.k_parts) * size_t(plan.kv_heads) * slot;
+    Scratch part;
+    if (!part.get(std::max(q_bytes, 2 * k_bytes))) return LMP_ERR_OOM;
+    s.part = static_cast<float*>(part.p);
+    s.part_dk = int64_t(k_bytes / sizeof(float));
+    const auto sum = [&](const List<AttnJoin>& joins, int64_t heads, const float* from, float* to,
+                         int64_t ld) -> int {
+      if (!joins.count) return LMP_OK;
+      attention_sum<<<dim3(grid_of(int64_t(joins.count) * heads * (kAttnSplitRows / 16))),
+                      dim3(256), 0, rt->stream>>>(
+          SumArgs{joins.at, joins.count, int(heads), int(plan.dim), from, to, ld});
+      LMP_LAUNCH_CHECK("attention_sum");
+      return LMP_OK;
+    };
+    int status = LMP_OK;
+    with_split_dim(plan.dim, [&](auto nd) {
+      using F = Frag<nd>;
+      SplitAttnArgs r = s;
+      r.items = plan.q_blocks.at;
+      r.count = plan.q_blocks.count;
+      r.o = dq;
+      r.o_ld = dq_ld;
+      status = launch_split(rt, "attention_split_back_rows", attention_split_back_rows<nd>,
+                            int64_t(r.count) * plan.heads, 2 * (2 * F::ALONG + F::ACROSS), r);
+      if (!status) status = sum(plan.q_joins, plan.heads, r.part, dq, dq_ld);
+      if (status || !plan.keys) return;
+      SplitAttnArgs k = s;
+      k.items = plan.k_blocks.at;
+      k.count = plan.k_blocks.count;
+      k.scale = std::fabs(s.scale);  // q's parts carry its sign
+      k.o = dv;
+      k.o_ld = dv_ld;
+      k.dk = dk;
+      k.dk_ld = dk_ld;
+      status = launch_split(rt, "attention_split_back_keys", attention_split_back_keys<nd>,
+                            int64_t(k.count) * plan.kv_heads,
+                            2 * (2 * F::ALONG + 2 * F::ACROSS + 1024), k);
+      if (!status) status = sum(plan.k_joins, plan.kv_heads, k.part, dv, dv_ld);
+      if (!status) status = sum(plan.k_joins, plan.kv_heads, k.part + k.part_dk, dk, dk_ld);
+    });
+    if (status) return status;
+    a.marks = s.marks;
+    a.any_mark = split.any_mark;
+  } else if (plan.queries) {
     attention_delta<<<dim3(grid_of((plan.queries * plan.heads + 15) / 16)), dim3(256), 0,
                       rt->stream>>>(plan.queries, int(plan.heads), int(plan.dim), o, o_ld, a.g,
                                     a.g_ld, static_cast<float*>(delta.p));
     LMP_LAUNCH_CHECK("attention_delta");
+  }
+  if (plan.queries) {
     a.delta = static_cast<const float*>(delta.p);
-    a.items = plan.rows;
-    a.count = plan.rows_count;
+    a.items = plan.rows.at;
+    a.count = plan.rows.count;
     a.o = dq;
     a.o_ld = dq_ld;
-    const uint32_t grid = grid_of(int64_t(a.count) * plan.kv_heads);
     with_dim(plan.dim, [&](auto nd) {
-      attention_back_rows<nd><<<dim3(grid), dim3(256), 0, rt->stream>>>(a);
+      attention_back_rows<nd><<<dim3(f32_grid(a)), dim3(256), 0, rt->stream>>>(a);
     });
     LMP_LAUNCH_CHECK("attention_back_rows");
   }
   if (plan.keys) {
-    a.items = plan.key_items;
-    a.count = plan.keys_count;
+    a.items = plan.key_items.at;
+    a.count = plan.key_items.count;
     a.o = dv;
     a.o_ld = dv_ld;
     a.dk = dk;
     a.dk_ld = dk_ld;
-    const uint32_t grid = grid_of(int64_t(a.count) * plan.kv_heads);
     with_dim(plan.dim, [&](auto nd) {
-      attention_back_keys<nd><<<dim3(grid), dim3(256), 0, rt->stream>>>(a);
+      attention_back_keys<nd><<<dim3(f32_grid(a)), dim3(256), 0, rt->stream>>>(a);
     });
     LMP_LAUNCH_CHECK("attention_back_keys");
   }
@@ -156,7 +391,7 @@ extern "C" int lmp_k_attention_plan_create(void** out, size_t sequences, const i
   // Host memory can run out here; no exception crosses the C boundary.
   try {
     AttnLists lists = attn_lists(sequences, q_lengths, k_lengths, int64_t(heads),
-                                 int64_t(kv_heads), causal != 0, int64_t(rt->cu_count) * 4);
+                                 int64_t(kv_heads), causal != 0, int64_t(rt->cu_count));
     auto plan = std::make_unique<AttentionPlan>();
     plan->heads = int64_t(heads);
     plan->kv_heads = int64_t(kv_heads);
@@ -166,17 +401,30 @@ extern "C" int lmp_k_attention_plan_create(void** out, size_t sequences, const i
     plan->keys = lists.key_rows;
     plan->parts = lists.parts;
     plan->pairs = lists.pairs;
-    plan->rows_count = int(lists.rows.size());
-    plan->keys_count = int(lists.keys.size());
-    plan->joins_count = int(lists.joins.size());
+    plan->q_parts = lists.q_parts;
+    plan->k_parts = lists.k_parts;
     std::string bytes;
-    const auto add = [&](const auto& v) {
-      const size_t at = bytes.size();
-      bytes.append(reinterpret_cast<const char*>(v.data()), v.size() * sizeof(v[0]));
+    // Appends a list; its place is an offset until the memory is there.
+    const auto add = [&](const auto& v, auto& list) {
+      using T = std::remove_cv_t<std::remove_pointer_t<decltype(list.at)>>;
+      list.at = reinterpret_cast<const T*>(bytes.size());
+      list.count = int(v.size());
+      bytes.append(reinterpret_cast<const char*>(v.data()), v.size() * sizeof(T));
       bytes.resize((bytes.size() + 255) / 256 * 256);
-      return at;
     };
-    const size_t rows = add(lists.rows), key_items = add(lists.keys), joins = add(lists.joins);
+    const auto each = [&](auto&& f) {
+      f(lists.rows, plan->rows);
+      f(lists.keys, plan->key_items);
+      f(lists.q_blocks, plan->q_blocks);
+      f(lists.k_blocks, plan->k_blocks);
+      f(lists.joins, plan->joins);
+      f(lists.q_joins, plan->q_joins);
+      f(lists.k_joins, plan->k_joins);
+      f(lists.q_tiles, plan->q_tiles);
+      f(lists.k_tiles, plan->k_tiles);
+      f(lists.seqs, plan->seqs);
+    };
+    each(add);
     if (!bytes.empty()) {
       void* p = nullptr;
       if (int s = lmp_rt_malloc(&p, bytes.size())) return s;
@@ -186,9 +434,10 @@ extern "C" int lmp_k_attention_plan_create(void** out, size_t sequences, const i
       }
       plan->device = static_cast<char*>(p);
     }
-    plan->rows = reinterpret_cast<const AttnItem*>(plan->device + rows);
-    plan->key_items = reinterpret_cast<const AttnItem*>(plan->device + key_items);
-    plan->joins = reinterpret_cast<const AttnJoin*>(plan->device + joins);
+    each([&](const auto&, auto& list) {
+      using T = std::remove_cv_t<std::remove_pointer_t<decltype(list.at)>>;
+      list.at = reinterpret_cast<const T*>(plan->device + reinterpret_cast<size_t>(list.at));
+    });
     *out = plan.release();
   } catch (const std::exception& e) {
     return fail(LMP_ERR_OOM, name + e.what());
@@ -237,7 +486,7 @@ extern "C" int lmp_k_attention_f32(const void* handle, const float* q, size_t q_
   a.o = o;
   a.o_ld = int64_t(o_ld);
   a.lse = lse;
-  return forward(rt, *plan, a);
+  return forward(rt, *plan, a, scale);
 }
 
 extern "C" int lmp_k_attention_backward_f32(const void* handle, const float* q, size_t q_ld,
@@ -265,6 +514,6 @@ extern "C" int lmp_k_attention_backward_f32(const void* handle, const float* q, 
   a.g = g;
   a.g_ld = int64_t(g_ld);
   a.lse_in = lse;
-  return backward(rt, *plan, a, o, int64_t(o_ld), dq, int64_t(dq_ld), dk, int64_t(dk_ld), dv,
+  return backward(rt, *plan, a, scale, o, int64_t(o_ld), dq, int64_t(dq_ld), dk, int64_t(dk_ld), dv,
                   int64_t(dv_ld));
 }

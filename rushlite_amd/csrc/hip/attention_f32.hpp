@@ -66,8 +66,10 @@ struct AttnArgs {
   float *o, *lse, *dk;  // o: forward's output or dq; dk with o as dv
   int64_t o_ld, dk_ld;
   float *part, *part_ml;  // [part][kv head][16 rows][dim], [...][16][2]
-  // Only the (sequence, key head)s that the split kernels leave out, or all.
-  const int16_t *q_exp, *k_exp, *v_exp, *g_exp;
+  // [sequence][key head]: not 0 where the split kernels leave the work to these
+  // (attention_split.hpp); null where all of it is theirs.
+  const int32_t* marks;
+  const int32_t* any_mark;
 };
 
 // W values at p, zero from column `end` on.
@@ -200,39 +202,28 @@ __device__ __forceinline__ void store_cols(float* row, int col, int end, a4 x) {
   }
 }
 
-// Whether a (sequence, key head) is left to the fp32 kernels: one of its tiles
-// holds what the split cannot (see attention_split.hpp).  All threads call it.
-constexpr int16_t kIrregular = 0x7fff;
-__device__ __forceinline__ bool left_out(const AttnItem& it, const int16_t* q_exp,
-                                         const int16_t* k_exp, const int16_t* v_exp,
-                                         const int16_t* g_exp, int kv_heads, int group, int kv) {
-  const int qt = (it.lq + kAttnTile - 1) / kAttnTile, kt = (it.lk + kAttnTile - 1) / kAttnTile;
-  bool odd = false;
-  for (int t = threadIdx.x; t < kt; t += blockDim.x) {
-    const int64_t at = int64_t(it.kt0 + t) * kv_heads + kv;
-    odd = odd || k_exp[at] == kIrregular || v_exp[at] == kIrregular;
-  }
-  for (int t = threadIdx.x; t < qt * group; t += blockDim.x) {
-    const int64_t at = int64_t(it.qt0 + t / group) * kv_heads * group + kv * group + t % group;
-    odd = odd || q_exp[at] == kIrregular || (g_exp && g_exp[at] == kIrregular);
-  }
-  return __syncthreads_or(odd);
-}
+// Whether a (sequence, key head) is another set of kernels' work.
 __device__ __forceinline__ bool skipped(const AttnArgs& a, const AttnItem& it, int kv) {
-  return a.k_exp &&
-         !left_out(it, a.q_exp, a.k_exp, a.v_exp, a.g_exp, a.kv_heads, a.group, kv);
+  return a.marks && !a.marks[int64_t(it.seq) * a.kv_heads + kv];
 }
 
 template <int ND>
 __global__ __launch_bounds__(256) void attention_rows(AttnArgs a) {
+  if (a.marks && !*a.any_mark) return;
   __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (ND * 16 + 4)];
   __shared__ float ml[2][4][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   for (int64_t w = blockIdx.x; w < int64_t(a.count) * a.kv_heads; w += gridDim.x) {
     const int kv = int(w % a.kv_heads);
-    const AttnItem it = a.items[w / a.kv_heads];
+    AttnItem it = a.items[w / a.kv_heads];
     if (skipped(a, it, kv)) continue;
     const int rows = min(kAttnRows, it.lq * a.group - it.first);
+    if (a.marks && it.part >= 0) {  // no join follows: a split row's first part takes all its keys
+      if (it.key_begin > 0) continue;
+      const int last = (it.first + rows - 1) / a.group;
+      it.part = -1;
+      it.key_end = a.causal ? max(0, min(it.lk, last + 1 + it.lk - it.lq)) : it.lk;
+    }
     const int packed = it.first + min(n, rows - 1);
     const int query = packed / a.group, head = kv * a.group + packed % a.group;
     const int limit = min(it.key_end, a.causal ? max(0, query + 1 + it.lk - it.lq) : it.lk);
@@ -317,15 +308,19 @@ __global__ __launch_bounds__(256) void attention_rows(AttnArgs a) {
   }
 }
 
-// Joins the parts of packed rows: 16 lanes a row.
+// Joins the parts of ROWS packed rows: 16 lanes a row, 16 rows a workgroup.
+template <int ROWS>
 __global__ __launch_bounds__(256) void attention_join(AttnArgs a, const AttnJoin* joins, int count) {
-  for (int64_t w = blockIdx.x; w < int64_t(count) * a.kv_heads; w += gridDim.x) {
-    const int kv = int(w % a.kv_heads);
-    const AttnJoin j = joins[w / a.kv_heads];
-    const int rows = min(kAttnRows, j.lq * a.group - j.first), row = threadIdx.x >> 4;
+  const int64_t work = int64_t(count) * a.kv_heads * (ROWS / 16);
+  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const int64_t item = w / (ROWS / 16);
+    const int kv = int(item % a.kv_heads);
+    const AttnJoin j = joins[item / a.kv_heads];
+    const int rows = min(ROWS, j.lq * a.group - j.first);
+    const int row = int(w % (ROWS / 16)) * 16 + (threadIdx.x >> 4);
     if (row >= rows) continue;
     const auto slot = [&](int p) {
-      return ((int64_t(j.part) + p) * a.kv_heads + kv) * 16 + row;
+      return ((int64_t(j.part) + p) * a.kv_heads + kv) * ROWS + row;
     };
     float all = -__builtin_inff();
     for (int p = 0; p < j.parts; ++p) all = fmaxf(all, a.part_ml[slot(p) * 2]);
@@ -384,6 +379,7 @@ __device__ __forceinline__ float lse2_of(float lse) {
 
 template <int ND>
 __global__ __launch_bounds__(256) void attention_back_rows(AttnArgs a) {
+  if (a.marks && !*a.any_mark) return;
   __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (ND * 16 + 4)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   const int heads = a.kv_heads * a.group;
@@ -442,6 +438,7 @@ __global__ __launch_bounds__(256) void attention_back_rows(AttnArgs a) {
 
 template <int ND>
 __global__ __launch_bounds__(256) void attention_back_keys(AttnArgs a) {
+  if (a.marks && !*a.any_mark) return;
   __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (ND * 16 + 4)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   const int heads = a.kv_heads * a.group;

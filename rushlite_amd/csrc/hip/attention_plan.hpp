@@ -3,7 +3,6 @@
 
 #include <algorithm>
 #include <cstdint>
-#include <stdexcept>
 #include <vector>
 
 namespace lmp_hip {
@@ -20,14 +19,22 @@ struct AttnItem {
   int32_t q0, k0;      // the sequence's first query and key in the packed rows
   int32_t lq, lk;
   int32_t first;       // first packed row, query or key
-  int32_t key_begin, key_end;  // of the forward pass
+  // Keys of packed rows and of queries; of the split kernels' keys, steps over the
+  // queries that may see them (attn_key_steps).
+  int32_t key_begin, key_end;
   int32_t part;        // place of its partial result, or -1 where it is the whole
   int32_t qt0, kt0;    // the sequence's first tile of queries and of keys
+  int32_t seq;
 };
 
 // Packed rows whose partial results are joined.
 struct AttnJoin {
   int32_t q0, lq, first, part, parts;
+};
+
+// A sequence's tiles of queries and of keys.
+struct AttnSeq {
+  int32_t qt0, q_tiles, kt0, k_tiles;
 };
 
 // A tile of the split-fp16 operands: rows at .. at + rows - 1 of the packed rows.
@@ -40,9 +47,12 @@ struct AttnLists {
   std::vector<AttnItem> keys;      // keys, fp32 kernels
   std::vector<AttnJoin> joins;
   std::vector<AttnItem> q_blocks;  // queries, split kernels
+  std::vector<AttnJoin> q_joins;
   std::vector<AttnItem> k_blocks;  // keys, split kernels
+  std::vector<AttnJoin> k_joins;   // q0 and lq are those of the keys
+  std::vector<AttnSeq> seqs;
   std::vector<AttnTile> q_tiles, k_tiles;
-  int64_t queries = 0, key_rows = 0, parts = 0;
+  int64_t queries = 0, key_rows = 0, parts = 0, q_parts = 0, k_parts = 0;
   double pairs = 0;  // (query, key) pairs the mask leaves, of one head
 };
 
@@ -51,58 +61,89 @@ inline int64_t attn_seen(int64_t i, int64_t lq, int64_t lk, bool causal) {
   return causal ? std::clamp<int64_t>(i + 1 + lk - lq, 0, lk) : lk;
 }
 
-// `workgroups`: how many fill the chip well.  The keys of packed rows are split
-// over several workgroups where the rows alone are too few, in parts of at least
-// kLeastPart keys.
-constexpr int64_t kLeastPart = 128;
+// The steps of the split kernels' keys from `first` on: a tile of queries of one
+// of the group's heads each, the last tile first, the heads of a tile in turn.
+inline int64_t attn_key_steps(int64_t first, int64_t lq, int64_t lk, bool causal, int64_t group) {
+  const int64_t tiles = (lq + kAttnTile - 1) / kAttnTile;
+  const int64_t from = causal ? std::min(tiles, std::max<int64_t>(0, first - (lk - lq)) / kAttnTile) : 0;
+  return (tiles - from) * group;
+}
+
+// Rows whose keys are split take parts of nearly equal length, at multiples of
+// `step` keys: emit(begin, end, part) for each.
+template <class Emit>
+inline void attn_parts(int64_t seen, int64_t part_keys, int64_t step, int64_t* next_part,
+                       Emit&& emit) {
+  const int64_t parts = seen <= part_keys ? 1 : (seen + part_keys - 1) / part_keys;
+  if (parts == 1) return emit(0, seen, int64_t(-1));
+  const int64_t steps = (seen + step - 1) / step;
+  for (int64_t p = 0; p < parts; ++p)
+    emit(steps * p / parts * step, std::min(seen, steps * (p + 1) / parts * step), (*next_part)++);
+}
+
+// The length of a part that gives about `workgroups` of them, `least` at least;
+// no split where the rows alone are as many.
+inline int64_t attn_part_keys(double work, int64_t rows, int64_t workgroups, int64_t least) {
+  if (rows >= workgroups) return INT64_MAX;
+  return std::max(least, int64_t(work / double(workgroups)) / 64 * 64 + 64);
+}
+
+// `compute_units` of the chip.  The fp32 kernels hold two workgroups on each and
+// are split for twice that, the split kernels' forward two.
+constexpr int64_t kLeastPart = 128, kLeastSplitPart = 512, kLeastSteps = 16;
 
 inline AttnLists attn_lists(size_t sequences, const int64_t* ql, const int64_t* kl, int64_t heads,
-                            int64_t kv_heads, bool causal, int64_t workgroups) {
+                            int64_t kv_heads, bool causal, int64_t compute_units) {
   AttnLists a;
   const int64_t group = heads / kv_heads;
-  // The keys of all row tiles, for the length of a part.
-  double work = 0;
-  int64_t tiles = 0;
+  // The keys of all rows, for the length of a part.
+  double work = 0, block_work = 0, steps = 0;
+  int64_t tiles = 0, blocks = 0;
   for (size_t s = 0; s < sequences; ++s) {
     const int64_t lq = ql[s], lk = kl[s], rows = lq * group;
-    for (int64_t r = 0; r < rows; r += kAttnRows) {
-      const int64_t last = std::min(rows, r + kAttnRows) - 1;
-      work += double(attn_seen(last / group, lq, lk, causal));
-      ++tiles;
-    }
-    for (int64_t i = 0; i < lq; ++i) a.pairs += double(attn_seen(i, lq, lk, causal));
+    for (int64_t r = 0; r < rows; r += kAttnRows, ++tiles)
+      work += double(attn_seen((std::min(rows, r + kAttnRows) - 1) / group, lq, lk, causal));
+    for (int64_t q = 0; q < lq; q += kAttnSplitRows, ++blocks)
+      block_work += double(attn_seen(std::min(lq, q + kAttnSplitRows) - 1, lq, lk, causal));
+    for (int64_t k = 0; k < lk; k += kAttnSplitRows)
+      steps += double(attn_key_steps(k, lq, lk, causal, group));
+    // Queries that see `first` keys or more: one more each, up to lk.
+    const int64_t blind = causal ? std::clamp<int64_t>(lq - lk, 0, lq) : 0, sees = lq - blind;
+    a.pairs += causal ? double(sees) * double(attn_seen(blind, lq, lk, causal) + lk) / 2
+                      : double(lq) * double(lk);
   }
-  int64_t part_keys = INT64_MAX;
-  if (tiles * kv_heads < workgroups) {
-    part_keys = int64_t(work * double(kv_heads) / double(workgroups));
-    part_keys = std::max(kLeastPart, (part_keys + 63) / 64 * 64);
-  }
+  const int64_t part_keys = attn_part_keys(work * double(kv_heads), tiles * kv_heads,
+                                           compute_units * 4, kLeastPart);
+  const int64_t block_keys = attn_part_keys(block_work * double(heads), blocks * heads,
+                                            compute_units * 2, kLeastSplitPart);
+  // The key kernel holds one workgroup on a unit; four parts for each even out the
+  // causal mask's long and short ones.
+  const int64_t part_steps =
+      std::max(kLeastSteps, int64_t(steps * double(kv_heads) / double(compute_units * 4)) + 1);
   for (size_t s = 0; s < sequences; ++s) {
     const int64_t lq = ql[s], lk = kl[s], rows = lq * group;
     AttnItem it{int32_t(a.queries), int32_t(a.key_rows), int32_t(lq), int32_t(lk), 0, 0, 0, -1,
-                int32_t(a.q_tiles.size()), int32_t(a.k_tiles.size())};
-    for (int64_t r = 0; r < rows; r += kAttnRows) {
-      const int64_t last = std::min(rows, r + kAttnRows) - 1;
-      const int64_t seen = attn_seen(last / group, lq, lk, causal);
-      const int64_t parts = std::max<int64_t>(1, part_keys == INT64_MAX ? 1 : (seen + part_keys - 1) / part_keys);
-      it.first = int32_t(r);
-      if (parts > 1) {
-        a.joins.push_back({it.q0, it.lq, it.first, int32_t(a.parts), int32_t(parts)});
-        // Parts of nearly equal length, at multiples of 16 keys.
-        const int64_t steps = (seen + 15) / 16;
-        for (int64_t p = 0; p < parts; ++p) {
-          it.key_begin = int32_t(steps * p / parts * 16);
-          it.key_end = int32_t(std::min(seen, steps * (p + 1) / parts * 16));
-          it.part = int32_t(a.parts++);
-          a.rows.push_back(it);
-        }
-      } else {
-        it.key_begin = 0;
-        it.key_end = int32_t(seen);
-        it.part = -1;
-        a.rows.push_back(it);
-      }
-    }
+                int32_t(a.q_tiles.size()), int32_t(a.k_tiles.size()), int32_t(s)};
+    const auto split = [&](int64_t first, int64_t seen, int64_t keys, int64_t step,
+                           int64_t* next_part, std::vector<AttnItem>& items,
+                           std::vector<AttnJoin>& joins) {
+      it.first = int32_t(first);
+      const int64_t before = *next_part;
+      attn_parts(seen, keys, step, next_part, [&](int64_t begin, int64_t end, int64_t part) {
+        it.key_begin = int32_t(begin);
+        it.key_end = int32_t(end);
+        it.part = int32_t(part);
+        items.push_back(it);
+      });
+      if (*next_part > before)
+        joins.push_back({it.q0, it.lq, it.first, int32_t(before), int32_t(*next_part - before)});
+    };
+    for (int64_t r = 0; r < rows; r += kAttnRows)
+      split(r, attn_seen((std::min(rows, r + kAttnRows) - 1) / group, lq, lk, causal), part_keys,
+            16, &a.parts, a.rows, a.joins);
+    for (int64_t q = 0; q < lq; q += kAttnSplitRows)
+      split(q, attn_seen(std::min(lq, q + kAttnSplitRows) - 1, lq, lk, causal), block_keys,
+            kAttnTile, &a.q_parts, a.q_blocks, a.q_joins);
     it.part = -1;
     it.key_begin = 0;
     it.key_end = it.lk;
@@ -110,20 +151,25 @@ inline AttnLists attn_lists(size_t sequences, const int64_t* ql, const int64_t* 
       it.first = int32_t(k);
       a.keys.push_back(it);
     }
-    for (int64_t q = 0; q < lq; q += kAttnSplitRows) {
-      it.first = int32_t(q);
-      it.key_end = int32_t(attn_seen(std::min(lq, q + kAttnSplitRows) - 1, lq, lk, causal));
-      a.q_blocks.push_back(it);
-    }
-    it.key_end = it.lk;
     for (int64_t k = 0; k < lk; k += kAttnSplitRows) {
       it.first = int32_t(k);
-      a.k_blocks.push_back(it);
+      const int64_t before = a.k_parts;
+      attn_parts(attn_key_steps(k, lq, lk, causal, group), part_steps, 1, &a.k_parts,
+                 [&](int64_t begin, int64_t end, int64_t part) {
+                   it.key_begin = int32_t(begin);
+                   it.key_end = int32_t(end);
+                   it.part = int32_t(part);
+                   a.k_blocks.push_back(it);
+                 });
+      if (a.k_parts > before)
+        a.k_joins.push_back({it.k0, it.lk, it.first, int32_t(before), int32_t(a.k_parts - before)});
     }
     for (int64_t q = 0; q < lq; q += kAttnTile)
       a.q_tiles.push_back({int32_t(a.queries + q), int32_t(std::min<int64_t>(kAttnTile, lq - q))});
     for (int64_t k = 0; k < lk; k += kAttnTile)
       a.k_tiles.push_back({int32_t(a.key_rows + k), int32_t(std::min<int64_t>(kAttnTile, lk - k))});
+    a.seqs.push_back({it.qt0, int32_t(a.q_tiles.size()) - it.qt0, it.kt0,
+                      int32_t(a.k_tiles.size()) - it.kt0});
     a.queries += lq;
     a.key_rows += lk;
   }
@@ -137,7 +183,7 @@ inline AttnLists attn_lists(size_t sequences, const int64_t* ql, const int64_t* 
   };
   const auto more = [&](const AttnItem& x, const AttnItem& y) { return queries_of(x) > queries_of(y); };
   std::stable_sort(a.keys.begin(), a.keys.end(), more);
-  std::stable_sort(a.k_blocks.begin(), a.k_blocks.end(), more);
+  std::stable_sort(a.k_blocks.begin(), a.k_blocks.end(), longer);
   return a;
 }
 
