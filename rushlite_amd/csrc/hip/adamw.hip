@@ -28,17 +28,13 @@
 namespace lmp_hip {
 namespace {
 
-#define LMP_WAVE_SWAP_SRC(...) __VA_ARGS__
-#include "wave_swap.inc"
-#undef LMP_WAVE_SWAP_SRC
-
 constexpr int kTensors = 48;  // a launch's list: 48 x 60 bytes, inside the 4 KiB of arguments
 constexpr int kThreads = 256;
 constexpr int kUnits = 4;  // units of four values per lane and workgroup
 constexpr int kPerGroup = kThreads * 4 * kUnits;
 // Launches of at most this many workgroups count themselves done and the last
 // one advances the step; above, that costs more than a launch of its own.
-constexpr int kSelfCounted = 256;
+constexpr int kSelfCounted = 1 << 23;
 
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u1_any __attribute__((aligned(1)));
@@ -83,35 +79,49 @@ __device__ __forceinline__ uint32_t mixed(uint32_t x) {  // MurmurHash3's 32-bit
   return x ^ (x >> 16);
 }
 
-// One value.  Each operation rounds once (no contraction), so that a state in 8
-// bits is a function of its inputs alone.
+// One value.  Each operation on the moments rounds once (no contraction), so that a
+// state in 8 bits is a function of its inputs alone.  FAST: the parameter's root and
+// quotient to a unit in their last places, where the arithmetic is what bounds the
+// kernel.
+template <bool FAST>
 __device__ __forceinline__ void step_one(const AdamWArgs& a, float keep, float size, float root,
                                          float g, float& p, float& m, float& v) {
   m = m * a.beta1 + g * a.rest1;
   v = v * a.beta2 + (g * g) * a.rest2;
-  p = p * keep - size * (m / (sqrtf(v) * root + a.eps));
+  if constexpr (FAST)
+    p = p * keep - size * (m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * root + a.eps));
+  else
+    p = p * keep - size * (m / (sqrtf(v) * root + a.eps));
+}
+
+// Largest of the wave's values, which are not negative as integers: DPP within
+// rows of 16 lanes, then the rows' broadcasts to the next, and lane 63 has it.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#define LMP_STEP(ctrl, rows) \
+  x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), ctrl, rows, 0xF, false)))
+  LMP_STEP(0xB1, 0xF);
+  LMP_STEP(0x4E, 0xF);
+  LMP_STEP(0x141, 0xF);
+  LMP_STEP(0x140, 0xF);
+  LMP_STEP(0x142, 0xA);
+  LMP_STEP(0x143, 0xC);
+#undef LMP_STEP
+  return uint32_t(__builtin_amdgcn_readlane(int(x), 63));
 }
 
 // Codes of a block's four values in this lane.  x scaled to [0, Q^2] has code c
 // with c^2 <= t < (c + 1)^2, and moves up to c + 1 with probability
-// (t - c^2) / (2 c + 1), the random 16 bits u being below it.
+// (t - c^2) / (2 c + 1), the random 16 bits u being below it.  The root may be off
+// by a unit in its last place: the two comparisons that follow settle c.
 template <int Q>
 __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (&r)[4],
                                            float* scale, bool first_lane) {
-  float top = 0;
-  bool nan = false;
+  // As integers, magnitudes order as they do as floats, and NaN is above all.
+  uint32_t bits = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    top = fmaxf(top, fabsf(x[j]));
-    nan = nan || x[j] != x[j];
-  }
-  top = nan ? __builtin_inff() : top;
-  top = fmaxf(top, lmp_swap<1>(top));
-  top = fmaxf(top, lmp_swap<2>(top));
-  top = fmaxf(top, lmp_swap<4>(top));
-  top = fmaxf(top, lmp_swap<8>(top));
-  top = fmaxf(top, lmp_swap<16>(top));
-  top = fmaxf(top, lmp_swap<32>(top));
+  for (int j = 0; j < 4; ++j)
+    bits = max(bits, __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu);
+  const float top = __builtin_bit_cast(float, wave_max(bits));
   const bool live = top >= 1e-30f && top < __builtin_inff();
   if (first_lane) *scale = live ? top : top < 1e-30f ? 0.0f : __builtin_nanf("");
   if (!live) return 0;
@@ -120,7 +130,7 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float t = fminf(fabsf(x[j]) * inv, float(Q * Q));
-    float c = floorf(sqrtf(t));
+    float c = floorf(__builtin_amdgcn_sqrtf(t));
     c = c * c > t ? c - 1 : c;
     c = (c + 1) * (c + 1) <= t ? c + 1 : c;
     c = float(r[j]) * (1.0f / 65536) * (2 * c + 1) < t - c * c ? c + 1 : c;
@@ -203,7 +213,7 @@ __global__ __launch_bounds__(kThreads) void adamw_step(AdamWArgs a) {
     for (int u = 0; u < kUnits; ++u) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        step_one(a, keep, size, root, gv[u][j], pv[u][j], mv[u][j], vv[u][j]);
+        step_one<false>(a, keep, size, root, gv[u][j], pv[u][j], mv[u][j], vv[u][j]);
       store4(p, at_of(u), pv[u]);
       store4(m, at_of(u), mv[u]);
       store4(v, at_of(u), vv[u]);
@@ -245,16 +255,16 @@ __global__ __launch_bounds__(kThreads) void adamw_step(AdamWArgs a) {
     for (int u = 0; u < kUnits; ++u) {
       const int64_t at = at_of(u), block = at / LMP_ADAMW_BLOCK;
       if (block * LMP_ADAMW_BLOCK >= n) continue;  // the whole wave
+      const uint32_t key_here = key ^ (uint32_t(uint64_t(at) >> 32) * 0x85EBCA6Bu);
       float mv[4], vv[4];
       uint32_t lo16[4], hi16[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         mv[j] = decoded<true>(mc[u], j, ms[u] * kUnitM);
         vv[j] = decoded<false>(vc[u], j, vs[u] * kUnitV);
-        step_one(a, keep, size, root, gv[u][j], pv[u][j], mv[j], vv[j]);
+        step_one<true>(a, keep, size, root, gv[u][j], pv[u][j], mv[j], vv[j]);
         if (at + j >= n) mv[j] = vv[j] = 0.0f;
-        const uint64_t place = uint64_t(at + j);
-        const uint32_t r = mixed(uint32_t(place) ^ key ^ uint32_t((place >> 32) * 0x85EBCA6Bu));
+        const uint32_t r = mixed(uint32_t(at + j) ^ key_here);
         lo16[j] = r & 0xFFFF;
         hi16[j] = r >> 16;
       }
@@ -283,15 +293,36 @@ template <bool SIGNED>
 __global__ __launch_bounds__(kThreads) void adamw_values(const uint8_t* codes, const float* scales,
                                                          int64_t n, float* out) {
   constexpr float unit = SIGNED ? kUnitM : kUnitV;
-  const int64_t stride = int64_t(gridDim.x) * kThreads * 4;
-  for (int64_t at = (int64_t(blockIdx.x) * kThreads + threadIdx.x) * 4; at < n; at += stride) {
-    const float s = scales[at / LMP_ADAMW_BLOCK] * unit;
-    if (at + 4 <= n) {
-      const uint32_t c = *reinterpret_cast<const u1_any*>(codes + at);
-      *reinterpret_cast<f4*>(out + at) = f4{decoded<SIGNED>(c, 0, s), decoded<SIGNED>(c, 1, s),
-                                            decoded<SIGNED>(c, 2, s), decoded<SIGNED>(c, 3, s)};
-    } else {
-      for (int j = 0; at + j < n; ++j) out[at + j] = decoded<SIGNED>(codes[at + j], 0, s);
+  for (int64_t begin = int64_t(blockIdx.x) * kPerGroup; begin < n;
+       begin += int64_t(gridDim.x) * kPerGroup) {
+    uint32_t c[kUnits];
+    float s[kUnits];
+    const auto at_of = [&](int u) { return begin + (int64_t(u) * kThreads + threadIdx.x) * 4; };
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int64_t at = at_of(u);
+      c[u] = 0;
+      s[u] = at < n ? scales[at / LMP_ADAMW_BLOCK] * unit : 0.0f;
+      if (at + 4 <= n) {
+        c[u] = *reinterpret_cast<const u1_any*>(codes + at);
+      } else {
+        for (int j = 0; j < 4; ++j)
+          if (at + j < n) c[u] |= uint32_t(codes[at + j]) << (8 * j);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int64_t at = at_of(u);
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = decoded<SIGNED>(c[u], j, s[u]);
+      if (at + 4 <= n) {
+        *reinterpret_cast<f4*>(out + at) = f4{v[0], v[1], v[2], v[3]};
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (at + j < n) out[at + j] = v[j];
+      }
     }
   }
 }
@@ -394,8 +425,7 @@ extern "C" int lmp_k_adamw_decode(int signed_codes, const void* codes, const flo
   if (!codes || !scales || !out) return fail(LMP_ERR_INVALID, "lmp_k_adamw_decode: null buffer");
   if (n > (size_t(1) << 40)) return fail(LMP_ERR_UNSUPPORTED, "lmp_k_adamw_decode: too many values");
   LMP_RUNTIME_OR_FAIL(rt);
-  const size_t groups = std::min<size_t>((n + kThreads * 4 - 1) / (kThreads * 4),
-                                         size_t(rt->cu_count) * 256);
+  const size_t groups = std::min<size_t>((n + kPerGroup - 1) / kPerGroup, size_t(rt->cu_count) * 256);
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   if (signed_codes)
     adamw_values<true><<<dim3(uint32_t(groups)), dim3(kThreads), 0, rt->stream>>>(c, scales,

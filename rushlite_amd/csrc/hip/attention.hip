@@ -28,7 +28,7 @@ struct AttentionPlan {
   int64_t heads, kv_heads, dim;
   bool causal;
   int64_t queries, keys, parts, q_parts, k_parts;
-  double pairs;
+  double row_work, block_work;  // AttnLists'
   char* device = nullptr;  // the lists, one after another
   List<AttnItem> rows, key_items, q_blocks, k_blocks;
   List<AttnJoin> joins, q_joins, k_joins;
@@ -69,18 +69,30 @@ AttnArgs common_args(const AttentionPlan& plan, double scale) {
   return a;
 }
 
-// Batches of at least this many multiplications per product (pairs, heads and
-// columns) take the split-fp16 kernels.
-constexpr double kSplitWork = 1;
-
-// Whether the split-fp16 kernels run a batch.
-bool split_form(const AttentionPlan& plan, double scale) {
-  const int64_t grid = int64_t(plan.q_blocks.count) * plan.heads +
-                       int64_t(plan.k_blocks.count) * plan.kv_heads +
-                       int64_t(plan.q_tiles.count) * 2 * plan.heads +
-                       int64_t(plan.k_tiles.count) * 2 * plan.kv_heads;
-  return plan.dim <= 128 && scale != 0 && grid < (int64_t(1) << 23) &&
-         plan.pairs * double(plan.heads) * double(plan.dim) >= kSplitWork;
+// Whether the split-fp16 kernels run a pass: where they are the faster ones by
+// what both forms have to do (attention_plan.hpp counts it), at rates measured
+// on this card.  The fp32 kernels take `start` and multiply at `rate` in their
+// 16 x 16 steps, mask and empty rows included; the split ones launch more, write
+// and read their fragments (8 bytes a value, at 3 TB/s) and multiply at theirs.
+// Forward, fp32 | split in us: one sequence of 1024, 4 heads of 128, 42 | 47; 16
+// heads, 80 | 52; 8 x 64 queries against 8192 keys, 8 heads of 128, 273 | 335;
+// 32 heads on 4 key heads, 894 | 398; 1 query against 8 x 8192 keys, 32 on 4
+// heads, 88 | 342.
+bool split_form(const AttentionPlan& plan, double scale, bool back) {
+  const double grid = double(plan.q_blocks.count) * double(plan.heads) +
+                      double(plan.k_blocks.count) * double(plan.kv_heads) +
+                      double(plan.q_tiles.count) * 2 * double(plan.heads) +
+                      double(plan.k_tiles.count) * 2 * double(plan.kv_heads);
+  // Grids stay below 2^32 threads; a scale of 0 leaves no power of two to divide.
+  if (plan.dim > 128 || scale == 0 || grid >= double(1 << 23)) return false;
+  const double dim = double(plan.dim), tile = 32 * dim * 8;  // bytes of a tile's fragments
+  const double q_bytes = double(plan.q_tiles.count) * double(plan.heads) * tile,
+               k_bytes = double(plan.k_tiles.count) * double(plan.kv_heads) * tile;
+  const double f32 = plan.row_work * double(plan.kv_heads) * dim, split = plan.block_work * double(plan.heads) * dim;
+  // Microseconds; a product is two operations, of which forward has two, backward
+  // seven.
+  return back ? 25 + f32 * 14 / 40e6 > 60 + (3 * q_bytes + 4 * k_bytes) / 3e6 + split * 14 / 150e6
+              : 8 + f32 * 4 / 75e6 > 25 + (q_bytes + 2 * k_bytes) / 3e6 + split * 4 / 250e6;
 }
 
 // Calls f with the ND of the split kernels that hold `dim` (at most 128).
@@ -219,7 +231,7 @@ int forward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale) {
     a.part = a.part_ml + slots * 2;
     return true;
   };
-  if (split_form(plan, scale)) {
+  if (split_form(plan, scale, false)) {
     if (!parts(plan.q_parts, plan.heads, kAttnSplitRows)) return LMP_ERR_OOM;
     if (int s = split_operands(rt, plan, a, scale, false, split)) return s;
     SplitAttnArgs& s = split.args;
@@ -267,7 +279,7 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
   Scratch delta;
   SplitOperands split;
   if (!delta.get(size_t(plan.queries) * size_t(plan.heads) * sizeof(float))) return LMP_ERR_OOM;
-  if (split_form(plan, scale)) {
+  if (split_form(plan, scale, true)) {
     if (int s = split_operands(rt, plan, a, scale, true, split)) return s;
     SplitAttnArgs& s = split.args;
     attention_split_stats<<<dim3(uint32_t(int64_t(plan.q_tiles.count) * plan.heads)), dim3(256), 0,
@@ -400,7 +412,8 @@ extern "C" int lmp_k_attention_plan_create(void** out, size_t sequences, const i
     plan->queries = lists.queries;
     plan->keys = lists.key_rows;
     plan->parts = lists.parts;
-    plan->pairs = lists.pairs;
+    plan->row_work = lists.row_work;
+    plan->block_work = lists.block_work;
     plan->q_parts = lists.q_parts;
     plan->k_parts = lists.k_parts;
     std::string bytes;

@@ -322,23 +322,34 @@ __global__ __launch_bounds__(256) void attention_join(AttnArgs a, const AttnJoin
     const auto slot = [&](int p) {
       return ((int64_t(j.part) + p) * a.kv_heads + kv) * ROWS + row;
     };
+    // The row's 16 lanes look at its parts side by side, then take its columns.
+    const int lane = threadIdx.x & 15;
+    const auto over_lanes = [](float x, auto&& f) {
+      x = f(x, __shfl_xor(x, 1));
+      x = f(x, __shfl_xor(x, 2));
+      x = f(x, __shfl_xor(x, 4));
+      return f(x, __shfl_xor(x, 8));
+    };
     float all = -__builtin_inff();
-    for (int p = 0; p < j.parts; ++p) all = fmaxf(all, a.part_ml[slot(p) * 2]);
+    for (int p = lane; p < j.parts; p += 16) all = fmaxf(all, a.part_ml[slot(p) * 2]);
+    all = over_lanes(all, [](float x, float y) { return fmaxf(x, y); });
     const float base = all > -__builtin_inff() ? all : 0.0f;
     float total = 0;
-    for (int p = 0; p < j.parts; ++p)
+    for (int p = lane; p < j.parts; p += 16)
       total += a.part_ml[slot(p) * 2 + 1] * exp2_of(a.part_ml[slot(p) * 2] - base);
+    total = over_lanes(total, [](float x, float y) { return x + y; });
     const float one = total > 0 || total != total ? 1.0f / total : 0.0f;
     const int r = j.first + row, query = r / a.group, head = kv * a.group + r % a.group;
     float* to = a.o + int64_t(j.q0 + query) * a.o_ld + int64_t(head) * a.dim;
-    for (int c = (threadIdx.x & 15) * 4; c < a.dim; c += 64) {
+    for (int c = lane * 4; c < a.dim; c += 64) {
       a4 s = {0, 0, 0, 0};
+#pragma unroll 8
       for (int p = 0; p < j.parts; ++p) {
         float x[4];
         load_cols<4>(a.part + slot(p) * a.dim, c, a.dim, x);
         const float f = exp2_of(a.part_ml[slot(p) * 2] - base);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] += f * x[i];
+        for (int i = 0; i < 4; ++i) s[i] = fmaf(f, x[i], s[i]);
       }
       store_cols(to, c, a.dim, s * one);
     }

@@ -53,7 +53,9 @@ struct AttnLists {
   std::vector<AttnSeq> seqs;
   std::vector<AttnTile> q_tiles, k_tiles;
   int64_t queries = 0, key_rows = 0, parts = 0, q_parts = 0, k_parts = 0;
-  double pairs = 0;  // (query, key) pairs the mask leaves, of one head
+  // (row, key) pairs of one head that the kernels go through: of 16 packed rows up
+  // to the last one's last key, and of 128 queries.
+  double row_work = 0, block_work = 0;
 };
 
 // Keys that query i of a sequence sees: [0, seen).
@@ -97,24 +99,20 @@ inline AttnLists attn_lists(size_t sequences, const int64_t* ql, const int64_t* 
   AttnLists a;
   const int64_t group = heads / kv_heads;
   // The keys of all rows, for the length of a part.
-  double work = 0, block_work = 0, steps = 0;
+  double steps = 0;
   int64_t tiles = 0, blocks = 0;
   for (size_t s = 0; s < sequences; ++s) {
     const int64_t lq = ql[s], lk = kl[s], rows = lq * group;
     for (int64_t r = 0; r < rows; r += kAttnRows, ++tiles)
-      work += double(attn_seen((std::min(rows, r + kAttnRows) - 1) / group, lq, lk, causal));
+      a.row_work += kAttnRows * double(attn_seen((std::min(rows, r + kAttnRows) - 1) / group, lq, lk, causal));
     for (int64_t q = 0; q < lq; q += kAttnSplitRows, ++blocks)
-      block_work += double(attn_seen(std::min(lq, q + kAttnSplitRows) - 1, lq, lk, causal));
+      a.block_work += kAttnSplitRows * double(attn_seen(std::min(lq, q + kAttnSplitRows) - 1, lq, lk, causal));
     for (int64_t k = 0; k < lk; k += kAttnSplitRows)
       steps += double(attn_key_steps(k, lq, lk, causal, group));
-    // Queries that see `first` keys or more: one more each, up to lk.
-    const int64_t blind = causal ? std::clamp<int64_t>(lq - lk, 0, lq) : 0, sees = lq - blind;
-    a.pairs += causal ? double(sees) * double(attn_seen(blind, lq, lk, causal) + lk) / 2
-                      : double(lq) * double(lk);
   }
-  const int64_t part_keys = attn_part_keys(work * double(kv_heads), tiles * kv_heads,
+  const int64_t part_keys = attn_part_keys(a.row_work / kAttnRows * double(kv_heads), tiles * kv_heads,
                                            compute_units * 4, kLeastPart);
-  const int64_t block_keys = attn_part_keys(block_work * double(heads), blocks * heads,
+  const int64_t block_keys = attn_part_keys(a.block_work / kAttnSplitRows * double(heads), blocks * heads,
                                             compute_units * 2, kLeastSplitPart);
   // The key kernel holds one workgroup on a unit; four parts for each even out the
   // causal mask's long and short ones.

@@ -69,8 +69,9 @@ __device__ __forceinline__ T row_sum(T v, T* lds) {
   return v;
 }
 
-// The lane's U units of a row of n values; zeros past its end.
-template <typename T, int L, int U>
+// The lane's U units of a row of n values; zeros past its end.  STREAM: with the
+// nontemporal hint (kStreamBytes).
+template <typename T, int L, int U, bool STREAM = false>
 __device__ __forceinline__ void load_row(const T* p, int lane, int n,
                                          T (&v)[U * Unit<T>::W]) {
   constexpr int W = Unit<T>::W;
@@ -78,7 +79,8 @@ __device__ __forceinline__ void load_row(const T* p, int lane, int n,
   for (int u = 0; u < U; ++u) {
     const int c = (u * L + lane) * W;
     if (c + W <= n) {
-      const typename Unit<T>::V x = *reinterpret_cast<const typename Unit<T>::V*>(p + c);
+      const auto* q = reinterpret_cast<const typename Unit<T>::V*>(p + c);
+      const typename Unit<T>::V x = STREAM ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
       for (int j = 0; j < W; ++j) v[u * W + j] = x[j];
     } else {
@@ -87,7 +89,7 @@ __device__ __forceinline__ void load_row(const T* p, int lane, int n,
     }
   }
 }
-template <typename T, int L, int U>
+template <typename T, int L, int U, bool STREAM = false>
 __device__ __forceinline__ void store_row(T* p, int lane, int n,
                                           const T (&v)[U * Unit<T>::W]) {
   constexpr int W = Unit<T>::W;
@@ -98,7 +100,9 @@ __device__ __forceinline__ void store_row(T* p, int lane, int n,
       typename Unit<T>::V x;
 #pragma unroll
       for (int j = 0; j < W; ++j) x[j] = v[u * W + j];
-      *reinterpret_cast<typename Unit<T>::V*>(p + c) = x;
+      auto* q = reinterpret_cast<typename Unit<T>::V*>(p + c);
+      if constexpr (STREAM) __builtin_nontemporal_store(x, q);
+      else *q = x;
     } else {
 #pragma unroll
       for (int j = 0; j < W; ++j)
@@ -118,6 +122,7 @@ struct NormArgs {
   T* y;
   int64_t ldy;
   T *mean, *rstd;
+  bool stream_in, stream_out;
 };
 
 template <typename T>
@@ -142,11 +147,20 @@ __global__ __launch_bounds__(threads_of(L)) void norm_rows(NormArgs<T> a) {
   __shared__ T meet[2][16];
   const int lane = threadIdx.x % L, sub = threadIdx.x / L;
   const T inv_n = T(1) / T(a.n);
+  T w[U * W], b[U * W];
+#pragma unroll
+  for (int i = 0; i < U * W; ++i) {
+    w[i] = T(1);
+    b[i] = T(0);
+  }
+  if (a.w) load_row<T, L, U>(a.w, lane, a.n, w);
+  if (a.b) load_row<T, L, U>(a.b, lane, a.n, b);
   for (int64_t first = int64_t(blockIdx.x) * R; first < a.rows; first += int64_t(gridDim.x) * R) {
     const bool live = first + sub < a.rows;
     const int64_t row = live ? first + sub : a.rows - 1;  // every lane takes part in the sums
     T v[U * W];
-    load_row<T, L, U>(a.x + row * a.ldx, lane, a.n, v);
+    if (a.stream_in) load_row<T, L, U, true>(a.x + row * a.ldx, lane, a.n, v);
+    else load_row<T, L, U>(a.x + row * a.ldx, lane, a.n, v);
     T s = 0;
 #pragma unroll
     for (int i = 0; i < U * W; ++i) s += v[i];
@@ -159,17 +173,11 @@ __global__ __launch_bounds__(threads_of(L)) void norm_rows(NormArgs<T> a) {
       q = c < a.n ? fma_of(v[i], v[i], q) : q;
     }
     const T rstd = T(1) / root_of(row_sum<L>(q, meet[1]) * inv_n + a.eps);
-    T w[U * W];
-    if (a.w) load_row<T, L, U>(a.w, lane, a.n, w);
 #pragma unroll
-    for (int i = 0; i < U * W; ++i) v[i] = v[i] * rstd * (a.w ? w[i] : T(1));
-    if (a.b) {
-      load_row<T, L, U>(a.b, lane, a.n, w);
-#pragma unroll
-      for (int i = 0; i < U * W; ++i) v[i] += w[i];
-    }
+    for (int i = 0; i < U * W; ++i) v[i] = v[i] * rstd * w[i] + b[i];
     if (!live) continue;  // only rows of 64 lanes or fewer, which share no barrier
-    store_row<T, L, U>(a.y + row * a.ldy, lane, a.n, v);
+    if (a.stream_out) store_row<T, L, U, true>(a.y + row * a.ldy, lane, a.n, v);
+    else store_row<T, L, U>(a.y + row * a.ldy, lane, a.n, v);
     if (lane == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
@@ -379,7 +387,9 @@ int layer_norm(Runtime* rt, const NormArgs<T>& a) {
   const int64_t cus = rt->cu_count;
   const bool held = with_variant<T>(a.n, [&](auto lanes, auto units) {
     constexpr int L = lanes, U = units, R = threads_of(L) / L;
-    const int64_t grid = capped((a.rows + R - 1) / R, cus * 1024);
+    // Workgroups that run together, each over several rows with w and b in its
+    // registers.
+    const int64_t grid = capped((a.rows + R - 1) / R, cus * (L > 256 ? 2 : L > 64 ? 4 : 8));
     norm_rows<T, L, U><<<dim3(uint32_t(grid)), dim3(threads_of(L)), 0, rt->stream>>>(a);
   });
   if (!held)
@@ -466,7 +476,8 @@ extern "C" int lmp_k_layer_norm(int dtype, size_t rows, size_t cols, const void*
     return layer_norm<T>(rt, {int64_t(rows), int(cols), static_cast<const T*>(x), int64_t(ldx),
                               static_cast<const T*>(w), static_cast<const T*>(b), T(eps),
                               static_cast<T*>(y), int64_t(ldy), static_cast<T*>(mean),
-                              static_cast<T*>(rstd)});
+                              static_cast<T*>(rstd), rows * cols * sizeof(T) >= kStreamBytes,
+                              rows * cols * sizeof(T) > kStreamStoreBytes});
   };
   return dtype == LMP_FLOAT64 ? go(double(0)) : go(float(0));
 }
