@@ -195,11 +195,11 @@ int split_operands(Runtime* rt, const AttentionPlan& plan, const AttnArgs& a, do
 
 // Launches a split kernel with its stages of LDS, which pass 64 KiB.
 template <class Kernel>
-int launch_split(Runtime* rt, const char* name, Kernel kernel, int64_t grid, int lds,
-                 const SplitAttnArgs& s) {
+int launch_split(Runtime* rt, const char* name, Kernel kernel, int64_t grid, int threads,
+                 int lds, const SplitAttnArgs& s) {
   LMP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  kernel<<<dim3(uint32_t(grid)), dim3(256), size_t(lds), rt->stream>>>(s);
+  kernel<<<dim3(uint32_t(grid)), dim3(threads), size_t(lds), rt->stream>>>(s);
   LMP_LAUNCH_CHECK(name);
   return LMP_OK;
 }
@@ -245,7 +245,7 @@ int forward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale) {
     int status = LMP_OK;
     with_split_dim(plan.dim, [&](auto nd) {
       status = launch_split(rt, "attention_split_rows", attention_split_rows<nd>,
-                            int64_t(s.count) * plan.heads,
+                            int64_t(s.count) * plan.heads, 256,
                             2 * (Frag<nd>::ALONG + Frag<nd>::ACROSS), s);
     });
     if (status) return status;
@@ -314,7 +314,8 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
       r.o = dq;
       r.o_ld = dq_ld;
       status = launch_split(rt, "attention_split_back_rows", attention_split_back_rows<nd>,
-                            int64_t(r.count) * plan.heads, 2 * (2 * F::ALONG + F::ACROSS), r);
+                            int64_t(r.count) * plan.heads, 512,
+                            4 * F::ALONG + 2 * F::ACROSS + 8 * 4096, r);
       if (!status) status = sum(plan.q_joins, plan.heads, r.part, dq, dq_ld);
       if (status || !plan.keys) return;
       SplitAttnArgs k = s;
@@ -326,8 +327,8 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
       k.dk = dk;
       k.dk_ld = dk_ld;
       status = launch_split(rt, "attention_split_back_keys", attention_split_back_keys<nd>,
-                            int64_t(k.count) * plan.kv_heads,
-                            2 * (2 * F::ALONG + 2 * F::ACROSS + 1024), k);
+                            int64_t(k.count) * plan.kv_heads, 512,
+                            4 * F::ALONG + 4 * F::ACROSS + 4 * 4096 + 512, k);
       if (!status) status = sum(plan.k_joins, plan.kv_heads, k.part, dv, dv_ld);
       if (!status) status = sum(plan.k_joins, plan.kv_heads, k.part + k.part_dk, dk, dk_ld);
     });

@@ -66,6 +66,18 @@ __device__ __forceinline__ void tiles_arrived() {
   __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
   asm volatile("s_barrier" ::: "memory");
 }
+// The same, and this wave's LDS accesses are done.
+__device__ __forceinline__ void step_begins() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(7 << 4);
+  asm volatile("s_barrier" ::: "memory");
+}
+// This wave's LDS accesses are done, and then the workgroup's.
+__device__ __forceinline__ void lds_settled() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (3 << 14));
+  asm volatile("s_barrier" ::: "memory");
+}
 __device__ __forceinline__ float times2(float x, int e) { return __builtin_ldexpf(x, e); }
 // The values of the two lanes (n and n + 32) that share a column, in both of
 // them.  An asm because the builtin of this instruction gives its first result
@@ -111,8 +123,8 @@ __device__ __forceinline__ Halves split_lane(const float (&x)[16]) {
   }
   return out;
 }
-// Row (of 32) of accumulator value r in this half of the wave.
-__device__ __forceinline__ int row_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+// Row (of 32) of accumulator value r in the wave's first half; 4 more in the other.
+constexpr int row_of(int r) { return 8 * (r >> 2) + (r & 3); }
 
 // ND: blocks of 16 columns; NT: of 32.  Bytes of one tile of one head.
 template <int ND>
@@ -252,6 +264,16 @@ struct SplitAttnArgs {
   int64_t part_dk;        // from dv's parts to dk's
 };
 
+// A tile's exponent, through the scalar cache: a vector load would wait for the
+// tiles that are on their way to LDS.
+__device__ __forceinline__ int exponent_at(const int32_t* exponents, int64_t at) {
+  typedef const int32_t __attribute__((address_space(4)))* scalar_ptr;
+  const uint32_t low = __builtin_amdgcn_readfirstlane(uint32_t(at));
+  const uint32_t high = __builtin_amdgcn_readfirstlane(uint32_t(uint64_t(at) >> 32));
+  return reinterpret_cast<scalar_ptr>(
+      reinterpret_cast<uintptr_t>(exponents))[int64_t((uint64_t(high) << 32) | low)];
+}
+
 // Heads that share keys, on one XCD (consecutive workgroups go round the eight).
 __device__ __forceinline__ int head_of(int slot, int heads) {
   return heads % 8 == 0 ? slot % 8 * (heads / 8) + slot / 8 : slot;
@@ -268,7 +290,16 @@ __device__ __forceinline__ void load_own(const char* tile, h8 (&h)[ND], h8 (&l)[
     l[s] = frag(tile, 2 * s + 1);
   }
 }
-// Rows (an LDS tile, along) times the wave's own rows.
+// Orders the instructions around it as `READS` LDS reads, then `MFMAS` products.
+template <int READS, int MFMAS>
+__device__ __forceinline__ void reads_then_products() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  __builtin_amdgcn_sched_group_barrier(0x008, MFMAS, 0);
+}
+// Rows (an LDS tile, along) times the wave's own rows.  The fragments of a step of
+// 16 columns are read two steps ahead; left to itself the compiler reads each one
+// when it is due and waits for it.  The small terms add up apart from the leading
+// ones.
 template <int ND>
 __device__ __forceinline__ void product(const char* lds, const h8 (&h)[ND], const h8 (&l)[ND],
                                         float (&out)[16]) {
@@ -280,20 +311,42 @@ __device__ __forceinline__ void product(const char* lds, const h8 (&h)[ND], cons
     lead = mfma_h(ah, h[s], lead);
     low = mfma_h(ah, l[s], low);
   }
+  reads_then_products<4, 0>();
+#pragma unroll
+  for (int s = 0; s < ND; ++s) reads_then_products<2, 3>();
 #pragma unroll
   for (int r = 0; r < 16; ++r) out[r] = lead[r] + low[r];
 }
-// acc += (an LDS tile, across) times the lane's 32 values.
+// acc += (an LDS tile, across) times the lane's 32 values: two blocks of columns at
+// a time, so that no product waits for the one before it, and their fragments
+// read one pair ahead.
 template <int NT>
 __device__ __forceinline__ void accumulate_tile(const char* lds, const Halves& p, s16 (&acc)[NT]) {
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int m = 0; m < NT; ++m) {
-      const h8 ah = frag(lds, (m * 2 + u) * 2), al = frag(lds, (m * 2 + u) * 2 + 1);
-      acc[m] = mfma_h(al, p.h[u], acc[m]);
-      acc[m] = mfma_h(ah, p.l[u], acc[m]);
-      acc[m] = mfma_h(ah, p.h[u], acc[m]);
+    for (int m = 0; m < NT; m += 2) {
+      constexpr int two = 2;
+      h8 ah[two], al[two];
+#pragma unroll
+      for (int i = 0; i < two && m + i < NT; ++i) {
+        ah[i] = frag(lds, ((m + i) * 2 + u) * 2);
+        al[i] = frag(lds, ((m + i) * 2 + u) * 2 + 1);
+      }
+#pragma unroll
+      for (int i = 0; i < two && m + i < NT; ++i) acc[m + i] = mfma_h(al[i], p.h[u], acc[m + i]);
+#pragma unroll
+      for (int i = 0; i < two && m + i < NT; ++i) acc[m + i] = mfma_h(ah[i], p.l[u], acc[m + i]);
+#pragma unroll
+      for (int i = 0; i < two && m + i < NT; ++i) acc[m + i] = mfma_h(ah[i], p.h[u], acc[m + i]);
+    }
+  reads_then_products<NT == 1 ? 2 : 4, 0>();
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int m = 0; m < NT; m += 2) {
+      if (m + 1 < NT) reads_then_products<4, 6>();
+      else reads_then_products<2, 3>();
     }
 }
 // A lane's column of the transposed result: `row` is its row in memory.
@@ -315,14 +368,22 @@ __device__ __forceinline__ void scale_acc(s16 (&acc)[NT], float f) {
   for (int m = 0; m < NT; ++m) acc[m] *= f;
 }
 
-// Copies `chunks` KiB to LDS, the four waves in turn.
-template <int CHUNKS>
+// The pointer in scalar registers (it is the same in every lane).
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t x = reinterpret_cast<uint64_t>(p);
+  const uint32_t low = __builtin_amdgcn_readfirstlane(uint32_t(x));
+  const uint32_t high = __builtin_amdgcn_readfirstlane(uint32_t(x >> 32));
+  return reinterpret_cast<const char*>((uint64_t(high) << 32) | low);
+}
+// Copies CHUNKS KiB to LDS, the WAVES waves in turn.
+template <int CHUNKS, int WAVES = 4>
 __device__ __forceinline__ void fetch(const char* src, char* lds, int wave) {
+  const char* from = uniform(src + wave * 1024);
+  const uint32_t lane = (threadIdx.x & 63) * 16;
 #pragma unroll
-  for (int i = 0; i < (CHUNKS + 3) / 4; ++i) {
-    const int c = i * 4 + wave;
-    if (CHUNKS % 4 == 0 || c < CHUNKS)
-      lds_load16(src + c * 1024 + (threadIdx.x & 63) * 16, lds + c * 1024);
+  for (int i = 0; i < (CHUNKS + WAVES - 1) / WAVES; ++i) {
+    if (CHUNKS % WAVES == 0 || i * WAVES + wave < CHUNKS)
+      lds_load16(from + i * WAVES * 1024 + lane, lds + (i * WAVES + wave) * 1024);
   }
 }
 
@@ -384,7 +445,7 @@ __global__ __launch_bounds__(256, 2) void attention_split_rows(SplitAttnArgs a) 
   int ref = kZeroTile;  // acc is O 2^(29 - ref)
   for (int t = 0; t < tiles; ++t) {
     const int64_t at = int64_t(it.kt0 + tile0 + t) * a.kv_heads + kv;
-    const int ek = a.k_exp[at], ev = a.v_exp[at];
+    const int ek = exponent_at(a.k_exp, at), ev = exponent_at(a.v_exp, at);
     tiles_arrived();
     if (t + 1 < tiles) fetch_tile(t + 1);
     const int key0 = (tile0 + t) * kAttnTile;
@@ -393,9 +454,9 @@ __global__ __launch_bounds__(256, 2) void attention_split_rows(SplitAttnArgs a) 
     float s[16];
     product<ND>(stage, qh, ql, s);
     if (key0 + 32 > whole) {
+      const int seen = limit - key0 - 4 * half;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        s[r] = key0 + row_of(r, half) < limit ? s[r] : -__builtin_inff();
+      for (int r = 0; r < 16; ++r) s[r] = row_of(r) < seen ? s[r] : -__builtin_inff();
     }
     float best = s[0];
 #pragma unroll
@@ -473,26 +534,53 @@ __global__ __launch_bounds__(256) void attention_split_stats(const AttnTile* til
   }
 }
 
-template <int ND>
-__global__ __launch_bounds__(256, 1) void attention_split_back_rows(SplitAttnArgs a) {
-  constexpr int NT = Frag<ND>::NT, ALONG = Frag<ND>::ALONG;
-  constexpr int STAGE = 2 * ALONG + Frag<ND>::ACROSS;
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
+// 16 values of a lane through LDS to the same lane of the wave's partner.
+__device__ __forceinline__ void give(char* lds, const float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<a4*>(lds + i * 1024 + (threadIdx.x & 63) * 16) =
+        a4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+}
+__device__ __forceinline__ void take(const char* lds, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const a4 v = *reinterpret_cast<const a4*>(lds + i * 1024 + (threadIdx.x & 63) * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j];
+  }
+}
+
+// The backward kernels pair two waves on a SIMD for 32 queries (or keys): one forms
+// the weights P, the other dP, and P goes over through LDS.  One wave for both
+// holds all of the SIMD's registers, and its exponentials and splits leave the
+// matrix cores idle (39% of the time in use, 1.45 ms for dq of 8192 positions, 16
+// heads of 128); paired, each has half, and one wave's arithmetic runs beside the
+// other's products.  A step's score products are formed a step ahead of its
+// gradient's, so a step has one barrier (dq) or two (dk and dv).
+template <int ND, bool WEIGHTS>
+__device__ __forceinline__ void split_back_rows_wave(const SplitAttnArgs& a, char* lds) {
+  constexpr int NT = Frag<ND>::NT, ALONG = Frag<ND>::ALONG, ACROSS = Frag<ND>::ACROSS;
+  // [2][K, V along], [2][K across], [2][pair][P]
+  char* const across = lds + 4 * ALONG;
+  char* const passed = across + 2 * ACROSS;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pair = wave & 3;
   const int half = lane >> 5, n = lane & 31, heads = a.kv_heads * a.group;
   const int head = head_of(int(blockIdx.x % heads), heads), kv = head / a.group;
   const AttnItem it = a.items[blockIdx.x / heads];
-  const int tile0 = it.key_begin / kAttnTile, tiles = (it.key_end - it.key_begin + 31) / kAttnTile;
-  const auto fetch_tile = [&](int t) {
-    const int64_t at = int64_t(it.kt0 + tile0 + t) * a.kv_heads + kv;
-    char* to = lds + (t & 1) * STAGE;
-    fetch<ND * 2>(a.k_along + at * ALONG, to, wave);
-    fetch<ND * 2>(a.v_along + at * ALONG, to + ALONG, wave);
-    fetch<NT * 4>(a.k_across + at * Frag<ND>::ACROSS, to + 2 * ALONG, wave);
-  };
   if (a.marks[int64_t(it.seq) * a.kv_heads + kv]) return;
-  if (tiles > 0) fetch_tile(0);
-  const int first = it.first + 32 * wave, own = min(first / 32, (it.lq - 1) / 32);
+  const int tile0 = it.key_begin / kAttnTile, tiles = (it.key_end - it.key_begin + 31) / kAttnTile;
+  const auto at_of = [&](int t) { return int64_t(it.kt0 + tile0 + t) * a.kv_heads + kv; };
+  const auto fetch_along = [&](int t) {
+    char* to = lds + (t & 1) * 2 * ALONG;
+    fetch<ND * 2, 8>(a.k_along + at_of(t) * ALONG, to, wave);
+    fetch<ND * 2, 8>(a.v_along + at_of(t) * ALONG, to + ALONG, wave);
+  };
+  const auto fetch_across = [&](int t) {
+    fetch<NT * 4, 8>(a.k_across + at_of(t) * ACROSS, across + (t & 1) * ACROSS, wave);
+  };
+  if (tiles > 0) fetch_along(0);
+  const int first = it.first + 32 * pair, own = min(first / 32, (it.lq - 1) / 32);
   const int query = min(first + n, it.lq - 1), last = min(first + 31, it.lq - 1);
   const auto seen_by = [&](int q) {
     return min(it.key_end, a.causal ? max(0, q + 1 + it.lk - it.lq) : it.lk);
@@ -500,57 +588,88 @@ __global__ __launch_bounds__(256, 1) void attention_split_back_rows(SplitAttnArg
   const int limit = seen_by(query), whole = seen_by(min(first, it.lq - 1));
   const int end = first < it.lq ? seen_by(last) : 0;
   const int64_t q_at = int64_t(it.qt0 + own) * heads + head;
-  h8 qh[ND], ql[ND], gh[ND], gl[ND];
-  load_own<ND>(a.q_along + q_at * ALONG, qh, ql);
-  load_own<ND>(a.g_along + q_at * ALONG, gh, gl);
-  const int eq = a.q_exp[q_at], eg = a.g_exp[q_at];
-  const float lse2 = a.stats[q_at * 64 + n], delta = a.stats[q_at * 64 + 32 + n];
+  h8 oh[ND], ol[ND];
+  load_own<ND>((WEIGHTS ? a.q_along : a.g_along) + q_at * ALONG, oh, ol);
+  const int e_own = WEIGHTS ? a.q_exp[q_at] : a.g_exp[q_at];
+  const float stat = a.stats[q_at * 64 + (WEIGHTS ? 0 : 32) + n];
   s16 acc[NT];
 #pragma unroll
   for (int m = 0; m < NT; ++m) acc[m] = s16(0.0f);
   Follower power;
-  for (int t = 0; t < tiles; ++t) {
-    const int64_t at = int64_t(it.kt0 + tile0 + t) * a.kv_heads + kv;
-    const int ek = a.k_exp[at], ev = a.v_exp[at];
-    tiles_arrived();
-    if (t + 1 < tiles) fetch_tile(t + 1);
+  float x[16];
+  // The wave's part of step t's scores: P, given to the partner, or dP - delta.
+  const auto scores = [&](int t) {
     const int key0 = (tile0 + t) * kAttnTile;
-    if (key0 >= end) continue;
-    const char* stage = lds + (t & 1) * STAGE;
-    float s[16], dp[16];
-    product<ND>(stage, qh, ql, s);
-    product<ND>(stage + ALONG, gh, gl, dp);
-    const float c = times2(a.scale_log2e, ek + eq - 28), cp = times2(1.0f, ev + eg - 28);
+    if (key0 >= end) return;
+    const char* stage = lds + (t & 1) * 2 * ALONG;
+    if constexpr (WEIGHTS) {
+      const float c = times2(a.scale_log2e, exponent_at(a.k_exp, at_of(t)) + e_own - 28);
+      product<ND>(stage, oh, ol, x);
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      s[r] = exp2_of(fmaf(s[r], c, -lse2)) * fmaf(dp[r], cp, -delta);
-    if (key0 + 32 > whole) {
+      for (int r = 0; r < 16; ++r) x[r] = exp2_of(fmaf(x[r], c, -stat));
+      if (key0 + 32 > whole) {
+        const int seen = limit - key0 - 4 * half;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = key0 + row_of(r, half) < limit ? s[r] : 0.0f;
+        for (int r = 0; r < 16; ++r) x[r] = row_of(r) < seen ? x[r] : 0.0f;
+      }
+      give(passed + ((t & 1) * 4 + pair) * 4096, x);
+    } else {
+      const float c = times2(1.0f, exponent_at(a.v_exp, at_of(t)) + e_own - 28);
+      product<ND>(stage + ALONG, oh, ol, x);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], c, -stat);
     }
-    const int up = power.follow(s, ek, acc);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = times2(s[r], up);
-    accumulate_tile<NT>(stage + 2 * ALONG, split_lane(s), acc);
+  };
+  if (tiles > 0) {
+    step_begins();
+    if (tiles > 1) fetch_along(1);
+    fetch_across(0);
+    scores(0);
   }
-  if (first + n >= it.lq) return;
+  for (int t = 0; t < tiles; ++t) {
+    step_begins();
+    if (t + 2 < tiles) fetch_along(t + 2);
+    if (t + 1 < tiles) fetch_across(t + 1);
+    if (!WEIGHTS && (tile0 + t) * kAttnTile < end) {
+      float p[16];
+      take(passed + ((t & 1) * 4 + pair) * 4096, p);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] *= p[r];
+      const int up = power.follow(x, exponent_at(a.k_exp, at_of(t)), acc);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = times2(x[r], up);
+      accumulate_tile<NT>(across + (t & 1) * ACROSS, split_lane(x), acc);
+    }
+    if (t + 1 < tiles) scores(t + 1);
+  }
+  if (WEIGHTS || first + n >= it.lq) return;
   float* to = it.part < 0 ? a.o + int64_t(it.q0 + query) * a.o_ld + int64_t(head) * a.dim
                           : a.part + ((int64_t(it.part) * heads + head) * kAttnSplitRows +
                                       (query - it.first)) * a.dim;
   store_lane<NT>(to, a.dim, half, acc, times2(a.scale, max(power.f, -200) - 14));
 }
-
 template <int ND>
-__global__ __launch_bounds__(256, 1) void attention_split_back_keys(SplitAttnArgs a) {
-  constexpr int NT = Frag<ND>::NT, ALONG = Frag<ND>::ALONG, ACROSS = Frag<ND>::ACROSS;
-  constexpr int STAGE = 2 * ALONG + 2 * ACROSS + 1024;
+__global__ __launch_bounds__(512, 2) void attention_split_back_rows(SplitAttnArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
+  // The first four waves form the weights, their partners the gradients of scores.
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < 4) split_back_rows_wave<ND, true>(a, lds);
+  else split_back_rows_wave<ND, false>(a, lds);
+}
+
+template <int ND, bool WEIGHTS>
+__device__ __forceinline__ void split_back_keys_wave(const SplitAttnArgs& a, char* lds) {
+  constexpr int NT = Frag<ND>::NT, ALONG = Frag<ND>::ALONG, ACROSS = Frag<ND>::ACROSS;
+  // [2][q, g along], [2][q, g across], [pair][P], [2][statistics]
+  char* const across = lds + 4 * ALONG;
+  char* const passed = across + 4 * ACROSS;
+  char* const stats = passed + 4 * 4096;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pair = wave & 3;
   const int half = lane >> 5, n = lane & 31, heads = a.kv_heads * a.group;
   const int kv = head_of(int(blockIdx.x % a.kv_heads), a.kv_heads);
   const AttnItem it = a.items[blockIdx.x / a.kv_heads];
-  const int ahead = it.lk - it.lq;
-  const int q_tiles = (it.lq + 31) / kAttnTile;
+  if (a.marks[int64_t(it.seq) * a.kv_heads + kv]) return;
+  const int ahead = it.lk - it.lq, q_tiles = (it.lq + 31) / kAttnTile;
   // From the last tile of queries back, the group's heads of a tile in turn: every
   // workgroup of a key head goes the same way, so those that run together read
   // the same tiles through the XCD's L2.
@@ -558,86 +677,120 @@ __global__ __launch_bounds__(256, 1) void attention_split_back_keys(SplitAttnArg
   const auto at_of = [&](int i) {
     return int64_t(it.qt0 + tile_of(i)) * heads + kv * a.group + i % a.group;
   };
-  const auto fetch_tile = [&](int i) {
+  const auto fetch_along = [&](int i) {
+    char* to = lds + (i & 1) * 2 * ALONG;
     const int64_t at = at_of(i);
-    char* to = lds + (i & 1) * STAGE;
-    fetch<ND * 2>(a.q_along + at * ALONG, to, wave);
-    fetch<ND * 2>(a.g_along + at * ALONG, to + ALONG, wave);
-    fetch<NT * 4>(a.q_across + at * ACROSS, to + 2 * ALONG, wave);
-    fetch<NT * 4>(a.g_across + at * ACROSS, to + 2 * ALONG + ACROSS, wave);
+    fetch<ND * 2, 8>(a.q_along + at * ALONG, to, wave);
+    fetch<ND * 2, 8>(a.g_along + at * ALONG, to + ALONG, wave);
     if (wave == 0)
-      lds_load4(reinterpret_cast<const char*>(a.stats + at * 64 + lane), to + 2 * ALONG + 2 * ACROSS);
+      lds_load4(reinterpret_cast<const char*>(a.stats + at * 64 + lane), stats + (i & 1) * 256);
   };
-  if (a.marks[int64_t(it.seq) * a.kv_heads + kv]) return;
-  if (it.key_begin < it.key_end) fetch_tile(it.key_begin);
-  const int first = it.first + 32 * wave, own = min(first / 32, (it.lk - 1) / 32);
+  const auto fetch_across = [&](int i) {
+    char* to = across + (i & 1) * 2 * ACROSS;
+    const int64_t at = at_of(i);
+    fetch<NT * 4, 8>(a.q_across + at * ACROSS, to, wave);
+    fetch<NT * 4, 8>(a.g_across + at * ACROSS, to + ACROSS, wave);
+  };
+  const int begin = it.key_begin, end = it.key_end;
+  if (begin < end) fetch_along(begin);
+  const int first = it.first + 32 * pair, own = min(first / 32, (it.lk - 1) / 32);
   const int key = first + n;
   const int64_t k_at = int64_t(it.kt0 + own) * a.kv_heads + kv;
-  h8 kh[ND], kl[ND], vh[ND], vl[ND];
-  load_own<ND>(a.k_along + k_at * ALONG, kh, kl);
-  load_own<ND>(a.v_along + k_at * ALONG, vh, vl);
-  const int ek = a.k_exp[k_at], ev = a.v_exp[k_at];
-  s16 dk[NT], dv[NT];
+  h8 oh[ND], ol[ND];
+  load_own<ND>((WEIGHTS ? a.k_along : a.v_along) + k_at * ALONG, oh, ol);
+  const int e_own = WEIGHTS ? a.k_exp[k_at] : a.v_exp[k_at];
+  s16 acc[NT];
 #pragma unroll
-  for (int m = 0; m < NT; ++m) dk[m] = dv[m] = s16(0.0f);
+  for (int m = 0; m < NT; ++m) acc[m] = s16(0.0f);
   Follower power;
-  int ref = kZeroTile;  // dv is dV 2^(29 - ref)
-  for (int i = it.key_begin; i < it.key_end; ++i) {
-    const int64_t at = at_of(i);
-    const int eq = a.q_exp[at], eg = a.g_exp[at];
-    tiles_arrived();
-    if (i + 1 < it.key_end) fetch_tile(i + 1);
+  int ref = kZeroTile;  // acc of dV is dV 2^(29 - ref)
+  float x[16];
+  // Whether a query of step i sees a key of the pair.
+  const auto seen = [&](int i) {
+    return first < it.lk && (!a.causal || tile_of(i) * kAttnTile + 31 + ahead >= first);
+  };
+  // The wave's part of step i's scores: P, given to the partner, or dP - delta.
+  const auto scores = [&](int i) {
+    if (!seen(i)) return;
+    const char* stage = lds + (i & 1) * 2 * ALONG;
+    const char* stat = stats + (i & 1) * 256 + (WEIGHTS ? 0 : 128) + half * 16;
     const int query0 = tile_of(i) * kAttnTile;
-    // Queries that see none of the wave's keys.
-    if (first >= it.lk || (a.causal && query0 + 31 + ahead < first)) continue;
-    const char* stage = lds + (i & 1) * STAGE;
-    const float* stats = reinterpret_cast<const float*>(stage + 2 * ALONG + 2 * ACROSS);
-    float p[16], dp[16];
-    product<ND>(stage, kh, kl, p);
-    product<ND>(stage + ALONG, vh, vl, dp);
-    const float c = times2(a.scale_log2e, ek + eq - 28), cp = times2(1.0f, ev + eg - 28);
-    if (eg > ref) {
-      scale_acc(dv, times2(1.0f, ref - eg));
-      ref = eg;
-    }
-    const float lift = times2(1.0f, 15 + eg - ref);
+    product<ND>(stage + (WEIGHTS ? 0 : ALONG), oh, ol, x);
+    const float c = WEIGHTS ? times2(a.scale_log2e, exponent_at(a.q_exp, at_of(i)) + e_own - 28)
+                            : times2(1.0f, exponent_at(a.g_exp, at_of(i)) + e_own - 28);
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const a4 lse2 = *reinterpret_cast<const a4*>(stats + 8 * b + 4 * half);
-      const a4 delta = *reinterpret_cast<const a4*>(stats + 32 + 8 * b + 4 * half);
+      const a4 v = *reinterpret_cast<const a4*>(stat + b * 32);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        p[4 * b + j] = exp2_of(fmaf(p[4 * b + j], c, -lse2[j]));
-        dp[4 * b + j] = fmaf(dp[4 * b + j], cp, -delta[j]);
-      }
+      for (int j = 0; j < 4; ++j) x[4 * b + j] = fmaf(x[4 * b + j], c, -v[j]);
     }
+    if constexpr (!WEIGHTS) return;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = exp2_of(x[r]);
     if (a.causal && query0 + ahead < first + 31) {
+      const int blind = key - query0 - ahead - 4 * half;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = key <= query0 + row_of(r, half) + ahead ? p[r] : 0.0f;
+      for (int r = 0; r < 16; ++r) x[r] = row_of(r) >= blind ? x[r] : 0.0f;
     }
+    give(passed + pair * 4096, x);
+  };
+  if (begin < end) {
+    step_begins();
+    if (begin + 1 < end) fetch_along(begin + 1);
+    fetch_across(begin);
+    scores(begin);
+  }
+  for (int i = begin; i < end; ++i) {
+    step_begins();
+    if (i + 2 < end) fetch_along(i + 2);
+    if (i + 1 < end) fetch_across(i + 1);
+    const char* stage = across + (i & 1) * 2 * ACROSS;
+    const bool here = seen(i);
+    if constexpr (WEIGHTS) {
+      if (here) {
+        const int eg = exponent_at(a.g_exp, at_of(i));
+        if (eg > ref) {
+          scale_acc(acc, times2(1.0f, ref - eg));
+          ref = eg;
+        }
+        const float lift = times2(1.0f, 15 + eg - ref);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      dp[r] *= p[r];
-      p[r] *= lift;
+        for (int r = 0; r < 16; ++r) x[r] *= lift;
+        accumulate_tile<NT>(stage + ACROSS, split_lane(x), acc);
+      }
+      lds_settled();  // the partner has taken P
+    } else {
+      if (here) {
+        float p[16];
+        take(passed + pair * 4096, p);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] *= p[r];
+        const int up = power.follow(x, exponent_at(a.q_exp, at_of(i)), acc);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = times2(x[r], up);
+      }
+      lds_settled();
+      if (here) accumulate_tile<NT>(stage, split_lane(x), acc);
     }
-    accumulate_tile<NT>(stage + 2 * ALONG + ACROSS, split_lane(p), dv);
-    const int up = power.follow(dp, eq, dk);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) dp[r] = times2(dp[r], up);
-    accumulate_tile<NT>(stage + 2 * ALONG, split_lane(dp), dk);
+    if (i + 1 < end) scores(i + 1);
   }
   if (key >= it.lk) return;
-  float *to_v, *to_k;
-  if (it.part < 0) {
-    to_v = a.o + int64_t(it.k0 + key) * a.o_ld + int64_t(kv) * a.dim;
-    to_k = a.dk + int64_t(it.k0 + key) * a.dk_ld + int64_t(kv) * a.dim;
-  } else {
-    to_v = a.part +
-           ((int64_t(it.part) * a.kv_heads + kv) * kAttnSplitRows + (key - it.first)) * a.dim;
-    to_k = to_v + a.part_dk;
-  }
-  store_lane<NT>(to_v, a.dim, half, dv, times2(1.0f, ref - 29));
-  store_lane<NT>(to_k, a.dim, half, dk, times2(a.scale, max(power.f, -200) - 14));
+  const float factor = WEIGHTS ? times2(1.0f, ref - 29) : times2(a.scale, max(power.f, -200) - 14);
+  float* to;
+  if (it.part < 0)
+    to = (WEIGHTS ? a.o + int64_t(it.k0 + key) * a.o_ld : a.dk + int64_t(it.k0 + key) * a.dk_ld) +
+         int64_t(kv) * a.dim;
+  else
+    to = a.part + (WEIGHTS ? 0 : a.part_dk) +
+         ((int64_t(it.part) * a.kv_heads + kv) * kAttnSplitRows + (key - it.first)) * a.dim;
+  store_lane<NT>(to, a.dim, half, acc, factor);
+}
+template <int ND>
+__global__ __launch_bounds__(512, 2) void attention_split_back_keys(SplitAttnArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  // The first four waves form the weights, their partners the gradients of scores.
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < 4) split_back_keys_wave<ND, true>(a, lds);
+  else split_back_keys_wave<ND, false>(a, lds);
 }
 
 // The sum of the parts of up to 128 rows of `heads` heads: 16 lanes a row.
