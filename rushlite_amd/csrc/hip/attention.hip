@@ -208,7 +208,7 @@ int launch_split(Runtime* rt, const char* name, Kernel kernel, int64_t grid, int
 // a small grid finds that out).
 uint32_t f32_grid(const AttnArgs& a) {
   const int64_t work = int64_t(a.count) * a.kv_heads;
-  return grid_of(a.marks ? std::min<int64_t>(work, 1024) : work);
+  return grid_of(a.marks ? std::min<int64_t>(work, 256) : work);
 }
 int forward_f32(Runtime* rt, const AttentionPlan& plan, AttnArgs a) {
   a.items = plan.rows.at;
@@ -296,12 +296,10 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
     if (!part.get(std::max(q_bytes, 2 * k_bytes))) return LMP_ERR_OOM;
     s.part = static_cast<float*>(part.p);
     s.part_dk = int64_t(k_bytes / sizeof(float));
-    const auto sum = [&](const List<AttnJoin>& joins, int64_t heads, const float* from, float* to,
-                         int64_t ld) -> int {
-      if (!joins.count) return LMP_OK;
-      attention_sum<<<dim3(grid_of(int64_t(joins.count) * heads * (kAttnSplitRows / 16))),
-                      dim3(256), 0, rt->stream>>>(
-          SumArgs{joins.at, joins.count, int(heads), int(plan.dim), from, to, ld});
+    const auto sum = [&](const SumArgs& p, int results) -> int {
+      if (!p.count) return LMP_OK;
+      const uint32_t grid = grid_of(int64_t(p.count) * p.heads * (kAttnSplitRows / 16));
+      attention_sum<<<dim3(grid, uint32_t(results)), dim3(256), 0, rt->stream>>>(p);
       LMP_LAUNCH_CHECK("attention_sum");
       return LMP_OK;
     };
@@ -316,7 +314,9 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
       status = launch_split(rt, "attention_split_back_rows", attention_split_back_rows<nd>,
                             int64_t(r.count) * plan.heads, 512,
                             4 * F::ALONG + 2 * F::ACROSS + 8 * 4096, r);
-      if (!status) status = sum(plan.q_joins, plan.heads, r.part, dq, dq_ld);
+      if (!status)
+        status = sum({plan.q_joins.at, plan.q_joins.count, int(plan.heads), int(plan.dim),
+                      {r.part}, {dq}, {dq_ld}}, 1);
       if (status || !plan.keys) return;
       SplitAttnArgs k = s;
       k.items = plan.k_blocks.at;
@@ -328,9 +328,10 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
       k.dk_ld = dk_ld;
       status = launch_split(rt, "attention_split_back_keys", attention_split_back_keys<nd>,
                             int64_t(k.count) * plan.kv_heads, 512,
-                            4 * F::ALONG + 4 * F::ACROSS + 4 * 4096 + 512, k);
-      if (!status) status = sum(plan.k_joins, plan.kv_heads, k.part, dv, dv_ld);
-      if (!status) status = sum(plan.k_joins, plan.kv_heads, k.part + k.part_dk, dk, dk_ld);
+                            4 * F::ALONG + 4 * F::ACROSS + 4 * 4096, k);
+      if (!status)
+        status = sum({plan.k_joins.at, plan.k_joins.count, int(plan.kv_heads), int(plan.dim),
+                      {k.part, k.part + k.part_dk}, {dv, dk}, {dv_ld, dk_ld}}, 2);
     });
     if (status) return status;
     a.marks = s.marks;

@@ -56,10 +56,6 @@ __device__ __forceinline__ void lds_load16(const char* src, char* lds) {
   __builtin_amdgcn_global_load_lds(reinterpret_cast<const float*>(src),
                                    reinterpret_cast<float*>(lds), 16, 0, 0);
 }
-__device__ __forceinline__ void lds_load4(const char* src, char* lds) {
-  __builtin_amdgcn_global_load_lds(reinterpret_cast<const float*>(src),
-                                   reinterpret_cast<float*>(lds), 4, 0, 0);
-}
 // This wave's loads have arrived, and then the workgroup's.
 __device__ __forceinline__ void tiles_arrived() {
   asm volatile("" ::: "memory");
@@ -649,7 +645,7 @@ __device__ __forceinline__ void split_back_rows_wave(const SplitAttnArgs& a, cha
   store_lane<NT>(to, a.dim, half, acc, times2(a.scale, max(power.f, -200) - 14));
 }
 template <int ND>
-__global__ __launch_bounds__(512, 2) void attention_split_back_rows(SplitAttnArgs a) {
+__global__ __launch_bounds__(512, ND <= 4 ? 4 : 2) void attention_split_back_rows(SplitAttnArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   // The first four waves form the weights, their partners the gradients of scores.
   if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < 4) split_back_rows_wave<ND, true>(a, lds);
@@ -659,10 +655,10 @@ __global__ __launch_bounds__(512, 2) void attention_split_back_rows(SplitAttnArg
 template <int ND, bool WEIGHTS>
 __device__ __forceinline__ void split_back_keys_wave(const SplitAttnArgs& a, char* lds) {
   constexpr int NT = Frag<ND>::NT, ALONG = Frag<ND>::ALONG, ACROSS = Frag<ND>::ACROSS;
-  // [2][q, g along], [2][q, g across], [pair][P], [2][statistics]
+  // [2][q, g along], [2][q, g across], [pair][P]: with heads of 64, half of the
+  // compute unit's LDS, so that two workgroups share it.
   char* const across = lds + 4 * ALONG;
   char* const passed = across + 4 * ACROSS;
-  char* const stats = passed + 4 * 4096;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pair = wave & 3;
   const int half = lane >> 5, n = lane & 31, heads = a.kv_heads * a.group;
@@ -682,9 +678,9 @@ __device__ __forceinline__ void split_back_keys_wave(const SplitAttnArgs& a, cha
     const int64_t at = at_of(i);
     fetch<ND * 2, 8>(a.q_along + at * ALONG, to, wave);
     fetch<ND * 2, 8>(a.g_along + at * ALONG, to + ALONG, wave);
-    if (wave == 0)
-      lds_load4(reinterpret_cast<const char*>(a.stats + at * 64 + lane), stats + (i & 1) * 256);
   };
+  // Lane n's statistic (lse2 or delta) of the step's query n.
+  const auto stats_of = [&](int i) { return a.stats[at_of(i) * 64 + (WEIGHTS ? 0 : 32) + n]; };
   const auto fetch_across = [&](int i) {
     char* to = across + (i & 1) * 2 * ACROSS;
     const int64_t at = at_of(i);
@@ -710,19 +706,18 @@ __device__ __forceinline__ void split_back_keys_wave(const SplitAttnArgs& a, cha
     return first < it.lk && (!a.causal || tile_of(i) * kAttnTile + 31 + ahead >= first);
   };
   // The wave's part of step i's scores: P, given to the partner, or dP - delta.
-  const auto scores = [&](int i) {
+  const auto scores = [&](int i, float stat) {
     if (!seen(i)) return;
     const char* stage = lds + (i & 1) * 2 * ALONG;
-    const char* stat = stats + (i & 1) * 256 + (WEIGHTS ? 0 : 128) + half * 16;
     const int query0 = tile_of(i) * kAttnTile;
     product<ND>(stage + (WEIGHTS ? 0 : ALONG), oh, ol, x);
     const float c = WEIGHTS ? times2(a.scale_log2e, exponent_at(a.q_exp, at_of(i)) + e_own - 28)
                             : times2(1.0f, exponent_at(a.g_exp, at_of(i)) + e_own - 28);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const a4 v = *reinterpret_cast<const a4*>(stat + b * 32);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * b + j] = fmaf(x[4 * b + j], c, -v[j]);
+    for (int r = 0; r < 16; ++r) {
+      const int v = __builtin_amdgcn_ds_bpermute(16 * half + 4 * row_of(r),
+                                                 __builtin_bit_cast(int, stat));
+      x[r] = fmaf(x[r], c, -__builtin_bit_cast(float, v));
     }
     if constexpr (!WEIGHTS) return;
 #pragma unroll
@@ -734,15 +729,25 @@ __device__ __forceinline__ void split_back_keys_wave(const SplitAttnArgs& a, cha
     }
     give(passed + pair * 4096, x);
   };
+  float stat = 0;  // of the step after this one
   if (begin < end) {
+    stat = stats_of(begin);
     step_begins();
-    if (begin + 1 < end) fetch_along(begin + 1);
+    const float now = stat;
+    if (begin + 1 < end) {
+      fetch_along(begin + 1);
+      stat = stats_of(begin + 1);
+    }
     fetch_across(begin);
-    scores(begin);
+    scores(begin, now);
   }
   for (int i = begin; i < end; ++i) {
     step_begins();
-    if (i + 2 < end) fetch_along(i + 2);
+    const float next = stat;
+    if (i + 2 < end) {
+      fetch_along(i + 2);
+      stat = stats_of(i + 2);
+    }
     if (i + 1 < end) fetch_across(i + 1);
     const char* stage = across + (i & 1) * 2 * ACROSS;
     const bool here = seen(i);
@@ -772,7 +777,7 @@ __device__ __forceinline__ void split_back_keys_wave(const SplitAttnArgs& a, cha
       lds_settled();
       if (here) accumulate_tile<NT>(stage, split_lane(x), acc);
     }
-    if (i + 1 < end) scores(i + 1);
+    if (i + 1 < end) scores(i + 1, next);
   }
   if (key >= it.lk) return;
   const float factor = WEIGHTS ? times2(1.0f, ref - 29) : times2(a.scale, max(power.f, -200) - 14);
@@ -786,7 +791,7 @@ __device__ __forceinline__ void split_back_keys_wave(const SplitAttnArgs& a, cha
   store_lane<NT>(to, a.dim, half, acc, factor);
 }
 template <int ND>
-__global__ __launch_bounds__(512, 2) void attention_split_back_keys(SplitAttnArgs a) {
+__global__ __launch_bounds__(512, ND <= 4 ? 4 : 2) void attention_split_back_keys(SplitAttnArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   // The first four waves form the weights, their partners the gradients of scores.
   if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < 4) split_back_keys_wave<ND, true>(a, lds);
@@ -797,12 +802,13 @@ __global__ __launch_bounds__(512, 2) void attention_split_back_keys(SplitAttnArg
 struct SumArgs {
   const AttnJoin* joins;
   int count, heads, dim;
-  const float* part;
-  float* out;
-  int64_t ld;
+  const float* part[2];
+  float* out[2];
+  int64_t ld[2];
 };
 __global__ __launch_bounds__(256) void attention_sum(SumArgs a) {
   const int64_t work = int64_t(a.count) * a.heads * (kAttnSplitRows / 16);
+  const int which = blockIdx.y;
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
     const int64_t item = w / (kAttnSplitRows / 16);
     const int head = int(item % a.heads);
@@ -814,11 +820,13 @@ __global__ __launch_bounds__(256) void attention_sum(SumArgs a) {
 #pragma unroll 4
       for (int p = 0; p < j.parts; ++p) {
         float x[4];
-        load_cols<4>(a.part + (((int64_t(j.part) + p) * a.heads + head) * kAttnSplitRows + row) * a.dim,
+        load_cols<4>(a.part[which] +
+                         (((int64_t(j.part) + p) * a.heads + head) * kAttnSplitRows + row) * a.dim,
                      c, a.dim, x);
         s += a4{x[0], x[1], x[2], x[3]};
       }
-      store_cols(a.out + int64_t(j.q0 + j.first + row) * a.ld + int64_t(head) * a.dim, c, a.dim, s);
+      store_cols(a.out[which] + int64_t(j.q0 + j.first + row) * a.ld[which] + int64_t(head) * a.dim,
+                 c, a.dim, s);
     }
   }
 }
