@@ -29,6 +29,10 @@ struct AttentionPlan {
   bool causal;
   int64_t queries, keys, parts, q_parts, k_parts;
   double row_work, block_work;  // AttnLists'
+  int64_t longest_q = 0, longest_k = 0;
+  // Each sequence has one item of packed rows, so that a pass reads every key once,
+  // and the keys and values pass the memory-side cache (kStreamBytes).
+  bool keys_once;
   char* device = nullptr;  // the lists, one after another
   List<AttnItem> rows, key_items, q_blocks, k_blocks;
   List<AttnJoin> joins, q_joins, k_joins;
@@ -69,30 +73,29 @@ AttnArgs common_args(const AttentionPlan& plan, double scale) {
   return a;
 }
 
-// Whether the split-fp16 kernels run a pass: where they are the faster ones by
-// what both forms have to do (attention_plan.hpp counts it), at rates measured
-// on this card.  The fp32 kernels take `start` and multiply at `rate` in their
-// 16 x 16 steps, mask and empty rows included; the split ones launch more, write
-// and read their fragments (8 bytes a value, at 3 TB/s) and multiply at theirs.
-// Forward, fp32 | split in us: one sequence of 1024, 4 heads of 128, 42 | 47; 16
-// heads, 80 | 52; 8 x 64 queries against 8192 keys, 8 heads of 128, 273 | 335;
-// 32 heads on 4 key heads, 894 | 398; 1 query against 8 x 8192 keys, 32 on 4
-// heads, 88 | 342.
+// Whether the split-fp16 kernels run a pass: where they take less time by what
+// both forms have to do.  The rates are a fit to 155 batches on this card (1 to
+// 2048 queries, 17 to 8192 keys, 1 to 32 heads of 32, 64 and 128): the form it
+// takes is 1% slower than the faster one on average, forward, and 2% backward.
+// Some of them, fp32 | split in us: forward, one sequence of 1024, 4 heads of 128,
+// 43 | 42; 16 heads, 89 | 52; one query against 8 x 8192 keys, 32 heads on 4, 88 |
+// 340; 64 queries, 900 | 400; backward, one sequence of 256, 4 heads of 64, 34 |
+// 41; of 1024, 16 heads of 64 on 4, 304 | 85.
 bool split_form(const AttentionPlan& plan, double scale, bool back) {
-  const double grid = double(plan.q_blocks.count) * double(plan.heads) +
-                      double(plan.k_blocks.count) * double(plan.kv_heads) +
-                      double(plan.q_tiles.count) * 2 * double(plan.heads) +
-                      double(plan.k_tiles.count) * 2 * double(plan.kv_heads);
+  const double q_tiles = double(plan.q_tiles.count) * double(plan.heads),
+               k_tiles = double(plan.k_tiles.count) * double(plan.kv_heads);
   // Grids stay below 2^32 threads; a scale of 0 leaves no power of two to divide.
-  if (plan.dim > 128 || scale == 0 || grid >= double(1 << 23)) return false;
-  const double dim = double(plan.dim), tile = 32 * dim * 8;  // bytes of a tile's fragments
-  const double q_bytes = double(plan.q_tiles.count) * double(plan.heads) * tile,
-               k_bytes = double(plan.k_tiles.count) * double(plan.kv_heads) * tile;
-  const double f32 = plan.row_work * double(plan.kv_heads) * dim, split = plan.block_work * double(plan.heads) * dim;
-  // Microseconds; a product is two operations, of which forward has two, backward
-  // seven.
-  return back ? 25 + f32 * 14 / 40e6 > 60 + (3 * q_bytes + 4 * k_bytes) / 3e6 + split * 14 / 150e6
-              : 8 + f32 * 4 / 75e6 > 25 + (q_bytes + 2 * k_bytes) / 3e6 + split * 4 / 250e6;
+  if (plan.dim > 128 || scale == 0 || 2 * (q_tiles + k_tiles) >= double(1 << 22)) return false;
+  // In millions: the multiplications of one product in each form's steps, and the
+  // bytes of a split operand's fragments.
+  const double dim = double(plan.dim), f32 = plan.row_work * double(plan.kv_heads) * dim / 1e6,
+               split = plan.block_work * double(plan.heads) * dim / 1e6,
+               q = q_tiles * dim * 256 / 1e6, k = k_tiles * dim * 256 / 1e6;
+  if (!back) return 10 + 0.077 * f32 > 20 + 0.011 * split + 0.22 * (q + 2 * k);
+  // The fp32 kernels do not share out the keys of a row or the rows of a key.
+  const double chain =
+      double(plan.longest_k + plan.longest_q * (plan.heads / plan.kv_heads)) * dim / 1e3;
+  return 15 + 0.26 * f32 + 0.61 * chain > 45 + 0.04 * split + 0.145 * (3 * q + 4 * k);
 }
 
 // Calls f with the ND of the split kernels that hold `dim` (at most 128).
@@ -214,7 +217,10 @@ int forward_f32(Runtime* rt, const AttentionPlan& plan, AttnArgs a) {
   a.items = plan.rows.at;
   a.count = plan.rows.count;
   with_dim(plan.dim, [&](auto nd) {
-    attention_rows<nd><<<dim3(f32_grid(a)), dim3(256), 0, rt->stream>>>(a);
+    if (plan.keys_once && !a.marks)
+      attention_rows<nd, true><<<dim3(f32_grid(a)), dim3(256), 0, rt->stream>>>(a);
+    else
+      attention_rows<nd, false><<<dim3(f32_grid(a)), dim3(256), 0, rt->stream>>>(a);
   });
   LMP_LAUNCH_CHECK("attention_rows");
   return LMP_OK;
@@ -415,6 +421,12 @@ extern "C" int lmp_k_attention_plan_create(void** out, size_t sequences, const i
     plan->keys = lists.key_rows;
     plan->parts = lists.parts;
     plan->row_work = lists.row_work;
+    plan->keys_once = uint64_t(lists.key_rows) * kv_heads * head_dim * 8 >= kStreamBytes;
+    for (size_t i = 0; i < sequences; ++i) {
+      plan->longest_q = std::max(plan->longest_q, q_lengths[i]);
+      plan->longest_k = std::max(plan->longest_k, k_lengths[i]);
+      plan->keys_once = plan->keys_once && q_lengths[i] * int64_t(heads / kv_heads) <= kAttnRows;
+    }
     plan->block_work = lists.block_work;
     plan->q_parts = lists.q_parts;
     plan->k_parts = lists.k_parts;

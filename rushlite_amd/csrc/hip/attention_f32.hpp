@@ -72,12 +72,13 @@ struct AttnArgs {
   const int32_t* any_mark;
 };
 
-// W values at p, zero from column `end` on.
-template <int W>
+// W values at p, zero from column `end` on.  STREAM: with the nontemporal hint.
+template <int W, bool STREAM = false>
 __device__ __forceinline__ void load_cols(const float* p, int col, int end, float* out) {
   if (col + W <= end) {
     if constexpr (W == 4) {
-      const a4_any x = *reinterpret_cast<const a4_any*>(p + col);
+      const auto* at = reinterpret_cast<const a4_any*>(p + col);
+      const a4_any x = STREAM ? __builtin_nontemporal_load(at) : *at;
       out[0] = x[0]; out[1] = x[1]; out[2] = x[2]; out[3] = x[3];
     } else if constexpr (W == 2) {
       const a2_any x = *reinterpret_cast<const a2_any*>(p + col);
@@ -102,19 +103,19 @@ struct Cols {
 };
 
 // 16 columns x ND of one row, 4 a lane group: the operand contracted over d.
-template <int ND>
+template <int ND, bool STREAM = false>
 __device__ __forceinline__ void load_along(const float* row, int g, int dim, float (&f)[ND][4]) {
 #pragma unroll
-  for (int b = 0; b < ND; ++b) load_cols<4>(row, 16 * b + 4 * g, dim, f[b]);
+  for (int b = 0; b < ND; ++b) load_cols<4, STREAM>(row, 16 * b + 4 * g, dim, f[b]);
 }
 // One row as the operand contracted over its rows: lane m holds columns at(j, m).
-template <int ND>
+template <int ND, bool STREAM = false>
 __device__ __forceinline__ void load_across(const float* row, int m, int dim, float (&f)[ND]) {
 #pragma unroll
-  for (int c = 0; c < ND / 4; ++c) load_cols<4>(row, 64 * c + 4 * m, dim, f + 4 * c);
+  for (int c = 0; c < ND / 4; ++c) load_cols<4, STREAM>(row, 64 * c + 4 * m, dim, f + 4 * c);
   constexpr int rest = ND % 4;
   if constexpr (rest != 0)
-    load_cols<rest>(row, 64 * (ND / 4) + rest * m, dim, f + ND / 4 * 4);
+    load_cols<rest, STREAM>(row, 64 * (ND / 4) + rest * m, dim, f + ND / 4 * 4);
 }
 
 template <int ND>
@@ -207,7 +208,9 @@ __device__ __forceinline__ bool skipped(const AttnArgs& a, const AttnItem& it, i
   return a.marks && !a.marks[int64_t(it.seq) * a.kv_heads + kv];
 }
 
-template <int ND>
+// The keys of a step are on their way while the step before it ends, its values
+// while its scores are formed.  STREAM: every key is read once.
+template <int ND, bool STREAM>
 __global__ __launch_bounds__(256) void attention_rows(AttnArgs a) {
   if (a.marks && !*a.any_mark) return;
   __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (ND * 16 + 4)];
@@ -236,14 +239,20 @@ __global__ __launch_bounds__(256) void attention_rows(AttnArgs a) {
 #pragma unroll
     for (int j = 0; j < ND; ++j) acc[j] = a4{0, 0, 0, 0};
     float top = -__builtin_inff(), sum = 0;
-    for (int kt = it.key_begin + wave * 16; kt < it.key_end; kt += 64) {
+    float k[ND][4];
+    const auto load_keys = [&](int kt) {
+      load_along<ND, STREAM>(k0 + int64_t(min(kt + n, it.lk - 1)) * a.k_ld, g, a.dim, k);
+    };
+    const int begin = it.key_begin + wave * 16;
+    if (begin < it.key_end) load_keys(begin);
+    for (int kt = begin; kt < it.key_end; kt += 64) {
       const auto key = [&](int i) { return min(kt + i, it.lk - 1); };
-      float k[ND][4], v[4][ND];
-      load_along<ND>(k0 + int64_t(key(n)) * a.k_ld, g, a.dim, k);
+      float v[4][ND];
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        load_across<ND>(v0 + int64_t(key(4 * g + r)) * a.v_ld, n, a.dim, v[r]);
+        load_across<ND, STREAM>(v0 + int64_t(key(4 * g + r)) * a.v_ld, n, a.dim, v[r]);
       const a4 s = product_along<ND>(k, q);
+      if (kt + 64 < it.key_end) load_keys(kt + 64);
       float p[4], best = top;
       bool whole = true;
 #pragma unroll

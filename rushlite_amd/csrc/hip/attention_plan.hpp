@@ -91,8 +91,8 @@ inline int64_t attn_part_keys(double work, int64_t rows, int64_t workgroups, int
 }
 
 // `compute_units` of the chip.  The fp32 kernels hold two workgroups on each and
-// are split for twice that, the split kernels' forward two.
-constexpr int64_t kLeastPart = 128, kLeastSplitPart = 512, kLeastSteps = 16;
+// are split for three times that, the split kernels' forward two.
+constexpr int64_t kLeastPart = 128, kLeastSplitPart = 256, kLeastSteps = 8;
 
 inline AttnLists attn_lists(size_t sequences, const int64_t* ql, const int64_t* kl, int64_t heads,
                             int64_t kv_heads, bool causal, int64_t compute_units) {
@@ -111,7 +111,7 @@ inline AttnLists attn_lists(size_t sequences, const int64_t* ql, const int64_t* 
       steps += double(attn_key_steps(k, lq, lk, causal, group));
   }
   const int64_t part_keys = attn_part_keys(a.row_work / kAttnRows * double(kv_heads), tiles * kv_heads,
-                                           compute_units * 4, kLeastPart);
+                                           compute_units * 6, kLeastPart);
   const int64_t block_keys = attn_part_keys(a.block_work / kAttnSplitRows * double(heads), blocks * heads,
                                             compute_units * 2, kLeastSplitPart);
   // The key kernel holds one workgroup on a unit; four parts for each even out the
