@@ -7,9 +7,9 @@
 // written, g read), 16 with states of 8.  All tensors share a launch: their
 // pointers ride in the kernel's arguments (kTensors of them), so nothing is
 // copied to the device per step and a recorded step replays; a workgroup finds
-// its tensor by bisection of the running workgroup counts.  The step count
+// a chunk's tensor by bisection of the running chunk counts.  The step count
 // lives on the device, and every workgroup forms the two bias corrections from it
-// in float64 while its loads are on their way.
+// in float64 while its first loads are on their way.
 //
 // States of 8 bits: a wave owns a block of 256 values, four a lane, so the
 // block's scale is a maximum over the wave and a state costs one 4-byte access
@@ -30,11 +30,14 @@ namespace {
 
 constexpr int kTensors = 48;  // a launch's list: 48 x 60 bytes, inside the 4 KiB of arguments
 constexpr int kThreads = 256;
-constexpr int kUnits = 4;  // units of four values per lane and workgroup
-constexpr int kPerGroup = kThreads * 4 * kUnits;
-// Launches of at most this many workgroups count themselves done and the last
-// one advances the step; above, that costs more than a launch of its own.
-constexpr int kSelfCounted = 1 << 23;
+// Chunks of UNITS units of four values a lane: four units, whose loads are all on
+// their way at once, or one where four would leave compute units idle (17 thousand
+// parameters: 8.5 us with four, 5.6 with one; 38 million: 250 us with two).
+constexpr int chunk_of(int units) { return kThreads * 4 * units; }
+// Workgroups per compute unit at most, each then over its share of the chunks: they
+// count themselves done on one counter, 3.4 ns each (38 million parameters, 9216
+// chunks: 185 us with 6 a unit, 180 with 18, 177 with 36).
+constexpr int kGroupsPerUnit = 36;
 
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u1_any __attribute__((aligned(1)));
@@ -48,12 +51,13 @@ struct AdamWList {
   float* v_scale[kTensors];
   int64_t n[kTensors];
   float keep[kTensors];       // 1 - lr decay
-  uint32_t first[kTensors];   // the tensor's first workgroup
+  uint32_t first[kTensors];   // the tensor's first chunk
 };
 
 struct AdamWArgs {
   AdamWList list;
   int count;
+  uint32_t chunks;
   uint32_t place;  // of the list's first tensor among all of the step's
   float beta1, rest1, beta2, rest2, eps;
   double lr, beta1_d, beta2_d;
@@ -150,130 +154,140 @@ __device__ __forceinline__ float decoded(uint32_t packed, int j, float unit) {
 }
 constexpr float kUnitM = float(1.0 / (127 * 127)), kUnitV = float(1.0 / (255 * 255));
 
-template <int BITS>
+// STREAM: accesses with the nontemporal hint (38 million parameters: 197 us without,
+// 177 with).
+template <int BITS, int kUnits, bool STREAM>
 __global__ __launch_bounds__(kThreads) void adamw_step(AdamWArgs a) {
   __shared__ float factors[2];
-  __shared__ uint32_t key_of_step;
-  if (threadIdx.x == 0) {
-    const int64_t t = a.step[0] + 1;
-    factors[0] = float(a.lr / (1.0 - power(a.beta1_d, t)));
-    factors[1] = float(1.0 / sqrt(1.0 - power(a.beta2_d, t)));
-    key_of_step = mixed(uint32_t(t) ^ a.seed);
-  }
-  int lo = 0, hi = a.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (blockIdx.x >= a.list.first[mid]) lo = mid;
-    else hi = mid - 1;
-  }
-  const int i = lo;
-  const int64_t n = a.list.n[i];
-  float* p = a.list.p[i];
-  const float* g = a.list.g[i];
-  const float keep = a.list.keep[i];
-  const int64_t begin = int64_t(blockIdx.x - a.list.first[i]) * kPerGroup;
-  float pv[kUnits][4], gv[kUnits][4];
-  const auto at_of = [&](int u) { return begin + (int64_t(u) * kThreads + threadIdx.x) * 4; };
-  const auto load4 = [&](const float* from, int64_t at, float (&v)[4]) {
-    if (at + 4 <= n) {
-      const f4 x = *reinterpret_cast<const f4*>(from + at);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = x[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = at + j < n ? from[at + j] : 0.0f;
-    }
-  };
-  const auto store4 = [&](float* to, int64_t at, const float (&v)[4]) {
-    if (at + 4 <= n) {
-      *reinterpret_cast<f4*>(to + at) = f4{v[0], v[1], v[2], v[3]};
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (at + j < n) to[at + j] = v[j];
-    }
-  };
-#pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
-    load4(p, at_of(u), pv[u]);
-    load4(g, at_of(u), gv[u]);
-  }
-  if constexpr (BITS == 32) {
-    float* m = static_cast<float*>(a.list.m[i]);
-    float* v = static_cast<float*>(a.list.v[i]);
-    float mv[kUnits][4], vv[kUnits][4];
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      load4(m, at_of(u), mv[u]);
-      load4(v, at_of(u), vv[u]);
+  const int64_t t = a.step[0] + 1;
+  // The factors, one in each of two lanes, while the first loads are on their way.
+  const auto corrections = [&] {
+    if (threadIdx.x < 2) {
+      const bool second = threadIdx.x == 1;
+      const double rest = 1.0 - power(second ? a.beta2_d : a.beta1_d, t);
+      factors[threadIdx.x] = float((second ? 1.0 : a.lr) / (second ? sqrt(rest) : rest));
     }
     __syncthreads();
-    const float size = factors[0], root = factors[1];
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        step_one<false>(a, keep, size, root, gv[u][j], pv[u][j], mv[u][j], vv[u][j]);
-      store4(p, at_of(u), pv[u]);
-      store4(m, at_of(u), mv[u]);
-      store4(v, at_of(u), vv[u]);
+  };
+  for (uint32_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    int lo = 0, hi = a.count - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (chunk >= a.list.first[mid]) lo = mid;
+      else hi = mid - 1;
     }
-  } else {
-    uint8_t* m = static_cast<uint8_t*>(a.list.m[i]);
-    uint8_t* v = static_cast<uint8_t*>(a.list.v[i]);
-    uint32_t mc[kUnits], vc[kUnits];
-    float ms[kUnits], vs[kUnits];
-    const auto codes = [&](const uint8_t* from, int64_t at) -> uint32_t {
-      if (at + 4 <= n) return *reinterpret_cast<const u1_any*>(from + at);
-      uint32_t c = 0;
-      for (int j = 0; j < 4; ++j)
-        if (at + j < n) c |= uint32_t(from[at + j]) << (8 * j);
-      return c;
-    };
-    const auto put = [&](uint8_t* to, int64_t at, uint32_t c) {
+    const int i = lo;
+    const int64_t n = a.list.n[i];
+    float* p = a.list.p[i];
+    const float* g = a.list.g[i];
+    const float keep = a.list.keep[i];
+    const int64_t begin = int64_t(chunk - a.list.first[i]) * chunk_of(kUnits);
+    float pv[kUnits][4], gv[kUnits][4];
+    const auto at_of = [&](int u) { return begin + (int64_t(u) * kThreads + threadIdx.x) * 4; };
+    const auto load4 = [&](const float* from, int64_t at, float (&v)[4]) {
       if (at + 4 <= n) {
-        *reinterpret_cast<u1_any*>(to + at) = c;
+        const auto* q = reinterpret_cast<const f4*>(from + at);
+        const f4 x = STREAM ? __builtin_nontemporal_load(q) : *q;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = x[j];
       } else {
-        for (int j = 0; j < 4; ++j)
-          if (at + j < n) to[at + j] = uint8_t(c >> (8 * j));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = at + j < n ? from[at + j] : 0.0f;
       }
     };
-    // A wave's 64 lanes x 4 values of one unit are one block.
+    const auto store4 = [&](float* to, int64_t at, const float (&v)[4]) {
+      if (at + 4 <= n) {
+        auto* q = reinterpret_cast<f4*>(to + at);
+        if constexpr (STREAM) __builtin_nontemporal_store(f4{v[0], v[1], v[2], v[3]}, q);
+        else *q = f4{v[0], v[1], v[2], v[3]};
+      } else {
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int64_t block = at_of(u) / LMP_ADAMW_BLOCK;
-      const bool there = block * LMP_ADAMW_BLOCK < n;
-      mc[u] = codes(m, at_of(u));
-      vc[u] = codes(v, at_of(u));
-      ms[u] = there ? a.list.m_scale[i][block] : 0.0f;
-      vs[u] = there ? a.list.v_scale[i][block] : 0.0f;
-    }
-    __syncthreads();
-    const float size = factors[0], root = factors[1];
-    const uint32_t key = mixed(key_of_step + 0x9E3779B9u * (a.place + uint32_t(i) + 1));
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int64_t at = at_of(u), block = at / LMP_ADAMW_BLOCK;
-      if (block * LMP_ADAMW_BLOCK >= n) continue;  // the whole wave
-      const uint32_t key_here = key ^ (uint32_t(uint64_t(at) >> 32) * 0x85EBCA6Bu);
-      float mv[4], vv[4];
-      uint32_t lo16[4], hi16[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        mv[j] = decoded<true>(mc[u], j, ms[u] * kUnitM);
-        vv[j] = decoded<false>(vc[u], j, vs[u] * kUnitV);
-        step_one<true>(a, keep, size, root, gv[u][j], pv[u][j], mv[j], vv[j]);
-        if (at + j >= n) mv[j] = vv[j] = 0.0f;
-        const uint32_t r = mixed(uint32_t(at + j) ^ key_here);
-        lo16[j] = r & 0xFFFF;
-        hi16[j] = r >> 16;
+        for (int j = 0; j < 4; ++j)
+          if (at + j < n) to[at + j] = v[j];
       }
-      const bool first_lane = (threadIdx.x & 63) == 0;
-      const uint32_t m2 = encode<127>(mv, lo16, a.list.m_scale[i] + block, first_lane);
-      const uint32_t v2 = encode<255>(vv, hi16, a.list.v_scale[i] + block, first_lane);
-      store4(p, at, pv[u]);
-      put(m, at, m2);
-      put(v, at, v2);
+    };
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      load4(p, at_of(u), pv[u]);
+      load4(g, at_of(u), gv[u]);
+    }
+    if constexpr (BITS == 32) {
+      float* m = static_cast<float*>(a.list.m[i]);
+      float* v = static_cast<float*>(a.list.v[i]);
+      float mv[kUnits][4], vv[kUnits][4];
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        load4(m, at_of(u), mv[u]);
+        load4(v, at_of(u), vv[u]);
+      }
+      if (chunk == blockIdx.x) corrections();
+      const float size = factors[0], root = factors[1];
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          step_one<false>(a, keep, size, root, gv[u][j], pv[u][j], mv[u][j], vv[u][j]);
+        store4(p, at_of(u), pv[u]);
+        store4(m, at_of(u), mv[u]);
+        store4(v, at_of(u), vv[u]);
+      }
+    } else {
+      uint8_t* m = static_cast<uint8_t*>(a.list.m[i]);
+      uint8_t* v = static_cast<uint8_t*>(a.list.v[i]);
+      uint32_t mc[kUnits], vc[kUnits];
+      float ms[kUnits], vs[kUnits];
+      const auto codes = [&](const uint8_t* from, int64_t at) -> uint32_t {
+        if (at + 4 <= n) return *reinterpret_cast<const u1_any*>(from + at);
+        uint32_t c = 0;
+        for (int j = 0; j < 4; ++j)
+          if (at + j < n) c |= uint32_t(from[at + j]) << (8 * j);
+        return c;
+      };
+      const auto put = [&](uint8_t* to, int64_t at, uint32_t c) {
+        if (at + 4 <= n) {
+          *reinterpret_cast<u1_any*>(to + at) = c;
+        } else {
+          for (int j = 0; j < 4; ++j)
+            if (at + j < n) to[at + j] = uint8_t(c >> (8 * j));
+        }
+      };
+      // A wave's 64 lanes x 4 values of one unit are one block.
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int64_t block = at_of(u) / LMP_ADAMW_BLOCK;
+        const bool there = block * LMP_ADAMW_BLOCK < n;
+        mc[u] = codes(m, at_of(u));
+        vc[u] = codes(v, at_of(u));
+        ms[u] = there ? a.list.m_scale[i][block] : 0.0f;
+        vs[u] = there ? a.list.v_scale[i][block] : 0.0f;
+      }
+      if (chunk == blockIdx.x) corrections();
+      const float size = factors[0], root = factors[1];
+      const uint32_t key = mixed(mixed(uint32_t(t) ^ a.seed) + 0x9E3779B9u * (a.place + uint32_t(i) + 1));
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int64_t at = at_of(u), block = at / LMP_ADAMW_BLOCK;
+        if (block * LMP_ADAMW_BLOCK >= n) continue;  // the whole wave
+        const uint32_t key_here = key ^ (uint32_t(uint64_t(at) >> 32) * 0x85EBCA6Bu);
+        float mv[4], vv[4];
+        uint32_t lo16[4], hi16[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          mv[j] = decoded<true>(mc[u], j, ms[u] * kUnitM);
+          vv[j] = decoded<false>(vc[u], j, vs[u] * kUnitV);
+          step_one<true>(a, keep, size, root, gv[u][j], pv[u][j], mv[j], vv[j]);
+          if (at + j >= n) mv[j] = vv[j] = 0.0f;
+          const uint32_t r = mixed(uint32_t(at + j) ^ key_here);
+          lo16[j] = r & 0xFFFF;
+          hi16[j] = r >> 16;
+        }
+        const bool first_lane = (threadIdx.x & 63) == 0;
+        const uint32_t m2 = encode<127>(mv, lo16, a.list.m_scale[i] + block, first_lane);
+        const uint32_t v2 = encode<255>(vv, hi16, a.list.v_scale[i] + block, first_lane);
+        store4(p, at, pv[u]);
+        put(m, at, m2);
+        put(v, at, v2);
+      }
     }
   }
   if (a.advance && threadIdx.x == 0) {
@@ -291,7 +305,8 @@ __global__ void adamw_advance(int64_t* step) { step[0] += 1; }
 
 template <bool SIGNED>
 __global__ __launch_bounds__(kThreads) void adamw_values(const uint8_t* codes, const float* scales,
-                                                         int64_t n, float* out) {
+                                                         int64_t n, float* out, bool stream) {
+  constexpr int kUnits = 4, kPerGroup = chunk_of(kUnits);
   constexpr float unit = SIGNED ? kUnitM : kUnitV;
   for (int64_t begin = int64_t(blockIdx.x) * kPerGroup; begin < n;
        begin += int64_t(gridDim.x) * kPerGroup) {
@@ -317,7 +332,9 @@ __global__ __launch_bounds__(kThreads) void adamw_values(const uint8_t* codes, c
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = decoded<SIGNED>(c[u], j, s[u]);
       if (at + 4 <= n) {
-        *reinterpret_cast<f4*>(out + at) = f4{v[0], v[1], v[2], v[3]};
+        auto* q = reinterpret_cast<f4*>(out + at);
+        if (stream) __builtin_nontemporal_store(f4{v[0], v[1], v[2], v[3]}, q);
+        else *q = f4{v[0], v[1], v[2], v[3]};
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -371,31 +388,38 @@ extern "C" int lmp_k_adamw_f32(int bits, size_t count, const lmp_adamw_tensor* t
   a.beta2_d = beta2;
   a.seed = uint32_t(seed);
   a.step = step;
-  uint64_t groups = 0;
+  uint64_t values = 0;
+  for (size_t i = 0; i < count; ++i) values += tensors[i].n;
+  // Bytes of all tensors against the memory-side cache (kStreamBytes).
+  const bool stream = values * (bits == 32 ? 16 : 10) >= kStreamBytes;
+  const bool few = values <= uint64_t(rt->cu_count) * chunk_of(4);
+  const int chunk = chunk_of(few ? 1 : 4);
+  uint64_t chunks = 0;
   bool advanced = false;
   const auto launch = [&]() -> int {
-    if (bits == 32)
-      adamw_step<32><<<dim3(uint32_t(groups)), dim3(kThreads), 0, rt->stream>>>(a);
-    else
-      adamw_step<8><<<dim3(uint32_t(groups)), dim3(kThreads), 0, rt->stream>>>(a);
+    a.chunks = uint32_t(chunks);
+    const dim3 grid(uint32_t(std::min<uint64_t>(chunks, uint64_t(rt->cu_count) * kGroupsPerUnit)));
+    const auto run = [&](auto kernel) { kernel<<<grid, dim3(kThreads), 0, rt->stream>>>(a); };
+    if (bits == 32) run(few ? adamw_step<32, 1, false> : stream ? adamw_step<32, 4, true> : adamw_step<32, 4, false>);
+    else run(few ? adamw_step<8, 1, false> : stream ? adamw_step<8, 4, true> : adamw_step<8, 4, false>);
     LMP_LAUNCH_CHECK("adamw_step");
     return LMP_OK;
   };
-  // A launch takes tensors until its list is full or its grid would pass 2^23
-  // workgroups (2^31 threads).
-  constexpr uint64_t kMostGroups = uint64_t(1) << 23;
+  // A launch takes tensors until its list is full or its chunks pass 32 bits (a
+  // tensor alone does not).
+  constexpr uint64_t kMostChunks = uint64_t(1) << 31;
   for (size_t i = 0; i < count; ++i) {
     const lmp_adamw_tensor& t = tensors[i];
-    const uint64_t need = (t.n + kPerGroup - 1) / kPerGroup;
+    const uint64_t need = (t.n + chunk - 1) / chunk;
     if (need == 0 && a.count == 0) continue;
-    if (a.count == kTensors || (a.count && groups + need > kMostGroups)) {
+    if (a.count == kTensors || (a.count && chunks + need > kMostChunks)) {
       if (int s = launch()) return s;
       a.count = 0;
-      groups = 0;
+      chunks = 0;
       if (need == 0) continue;
     }
     if (a.count == 0) a.place = uint32_t(i);
-    // A tensor without values keeps its place, and no workgroup.
+    // A tensor without values keeps its place, and no chunk.
     const int k = a.count++;
     a.list.p[k] = t.p;
     a.list.g[k] = t.g;
@@ -405,11 +429,12 @@ extern "C" int lmp_k_adamw_f32(int bits, size_t count, const lmp_adamw_tensor* t
     a.list.v_scale[k] = t.v_scale;
     a.list.n[k] = int64_t(t.n);
     a.list.keep[k] = float(1 - lr * t.decay);
-    a.list.first[k] = uint32_t(groups);
-    groups += need;
+    a.list.first[k] = uint32_t(chunks);
+    chunks += need;
   }
-  if (groups) {
-    a.advance = advanced = groups <= kSelfCounted;
+  if (chunks) {
+    a.advance = 1;  // the last launch's last workgroup
+    advanced = true;
     if (int s = launch()) return s;
   }
   if (!advanced) {
@@ -425,14 +450,15 @@ extern "C" int lmp_k_adamw_decode(int signed_codes, const void* codes, const flo
   if (!codes || !scales || !out) return fail(LMP_ERR_INVALID, "lmp_k_adamw_decode: null buffer");
   if (n > (size_t(1) << 40)) return fail(LMP_ERR_UNSUPPORTED, "lmp_k_adamw_decode: too many values");
   LMP_RUNTIME_OR_FAIL(rt);
-  const size_t groups = std::min<size_t>((n + kPerGroup - 1) / kPerGroup, size_t(rt->cu_count) * 256);
+  const size_t groups = std::min<size_t>((n + chunk_of(4) - 1) / chunk_of(4), size_t(rt->cu_count) * 256);
+  const bool stream = n * sizeof(float) > kStreamStoreBytes;
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   if (signed_codes)
     adamw_values<true><<<dim3(uint32_t(groups)), dim3(kThreads), 0, rt->stream>>>(c, scales,
-                                                                                   int64_t(n), out);
+                                                                                   int64_t(n), out, stream);
   else
     adamw_values<false><<<dim3(uint32_t(groups)), dim3(kThreads), 0, rt->stream>>>(c, scales,
-                                                                                    int64_t(n), out);
+                                                                                    int64_t(n), out, stream);
   LMP_LAUNCH_CHECK("adamw_decode");
   return LMP_OK;
 }

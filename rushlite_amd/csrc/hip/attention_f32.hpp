@@ -3,7 +3,7 @@
 // kernels leave out.
 //
 //   S = c Q K^T (c = scale log2 e), P = 2^(S - lse2), O = P V
-//   D = rowsum(dO O), dS = P (dO V^T - D), dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO
+//   D = rowsum(dO O), dS = scale P (dO V^T - D), dQ = dS K, dK = dS^T Q, dV = P^T dO
 //
 // A wave works on 16 packed rows (the query heads that share a key head lie side
 // by side, so one read of a key serves all of them) and 16 keys at a time with
@@ -440,7 +440,7 @@ __global__ __launch_bounds__(256) void attention_back_rows(AttnArgs a) {
       for (int r = 0; r < 4; ++r) {
         const bool seen = kt + 4 * g + r < limit;
         whole = whole && seen;
-        ds[r] = seen ? exp2_of(s[r] * c - lse2) * (dp[r] - delta) : 0.0f;
+        ds[r] = seen ? exp2_of(s[r] * c - lse2) * (dp[r] - delta) * a.scale : 0.0f;
       }
       accumulate<ND>(acc, kc, ds, a.dim, __any(!whole), [&](int i) { return kt + i < limit; },
                      [&](int i) { return k0 + int64_t(key(i)) * a.k_ld; });
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(256) void attention_back_rows(AttnArgs a) {
       const int r = it.first + row;
       store_cols(a.o + int64_t(it.q0 + r / a.group) * a.o_ld +
                      int64_t(kv * a.group + r % a.group) * a.dim,
-                 col, a.dim, x * a.scale);
+                 col, a.dim, x);
     });
     __syncthreads();
   }
@@ -506,7 +506,7 @@ __global__ __launch_bounds__(256) void attention_back_keys(AttnArgs a) {
         const bool seen = sees(i);
         whole = whole && seen;
         p[r] = seen ? exp2_of(s[r] * c - lse2_of(a.lse_in[stat])) : 0.0f;
-        ds[r] = seen ? p[r] * (dp[r] - a.delta[stat]) : 0.0f;
+        ds[r] = seen ? p[r] * (dp[r] - a.delta[stat]) * a.scale : 0.0f;
       }
       const bool masked = __any(!whole);
       float f[4][ND];
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(256) void attention_back_keys(AttnArgs a) {
     join_waves<ND>(dk, lds, [&](int row, int col, a4 x) {
       if (row < keys)
         store_cols(a.dk + int64_t(it.k0 + it.first + row) * a.dk_ld + int64_t(kv) * a.dim, col,
-                   a.dim, x * a.scale);
+                   a.dim, x);
     });
     __syncthreads();
   }

@@ -15,8 +15,9 @@
 // A tile with an infinity or a NaN, with a largest value outside [2^-60, 2^41) or
 // with rows more than 2^12 apart is marked, and the sequence's key head is left
 // to the fp32 kernels (attention_f32.hpp), which run over the marked ones only.
-// Weights P are at most 1 and take a fixed power of two; dS has no such bound and
-// takes one per query (dq) or key (dk) that follows its largest value so far.
+// The forward weights are at most 1 and take a fixed power of two; P and dS of the
+// backward pass take one per query (dq) or key (dk, dv) that follows its largest
+// value so far, so that a key that few see keeps its gradient's digits.
 //
 // Layout.  A first kernel writes the operands as MFMA fragments: the 16 bytes of
 // each lane, a fragment's 64 lanes one after another, so that a workgroup's
@@ -383,16 +384,16 @@ __device__ __forceinline__ void fetch(const char* src, char* lds, int wave) {
   }
 }
 
-// The power of two that takes a lane's dS (times 2^e) below 2^15, following its
+// The power of two that takes a lane's dS or P (times 2^e) below 2^15, following its
 // largest value so far; two bits are kept free so that it seldom moves.
 struct Follower {
   int f = -1000;
-  // Returns the power to apply to dS; `acc` follows when f moves.
+  // Returns the power to apply to x; `acc` follows when f moves.
   template <int NT>
-  __device__ __forceinline__ int follow(const float (&ds)[16], int e, s16 (&acc)[NT]) {
+  __device__ __forceinline__ int follow(const float (&x)[16], int e, s16 (&acc)[NT]) {
     float top = 0;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
     top = both_max(top);
     const int need = top > 0 ? __builtin_amdgcn_frexp_expf(top) + e - 15 : -1000;
     if (__any(need > f)) {
@@ -699,7 +700,6 @@ __device__ __forceinline__ void split_back_keys_wave(const SplitAttnArgs& a, cha
 #pragma unroll
   for (int m = 0; m < NT; ++m) acc[m] = s16(0.0f);
   Follower power;
-  int ref = kZeroTile;  // acc of dV is dV 2^(29 - ref)
   float x[16];
   // Whether a query of step i sees a key of the pair.
   const auto seen = [&](int i) {
@@ -753,14 +753,9 @@ __device__ __forceinline__ void split_back_keys_wave(const SplitAttnArgs& a, cha
     const bool here = seen(i);
     if constexpr (WEIGHTS) {
       if (here) {
-        const int eg = exponent_at(a.g_exp, at_of(i));
-        if (eg > ref) {
-          scale_acc(acc, times2(1.0f, ref - eg));
-          ref = eg;
-        }
-        const float lift = times2(1.0f, 15 + eg - ref);
+        const int up = power.follow(x, exponent_at(a.g_exp, at_of(i)), acc);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] *= lift;
+        for (int r = 0; r < 16; ++r) x[r] = times2(x[r], up);
         accumulate_tile<NT>(stage + ACROSS, split_lane(x), acc);
       }
       lds_settled();  // the partner has taken P
@@ -780,7 +775,7 @@ __device__ __forceinline__ void split_back_keys_wave(const SplitAttnArgs& a, cha
     if (i + 1 < end) scores(i + 1, next);
   }
   if (key >= it.lk) return;
-  const float factor = WEIGHTS ? times2(1.0f, ref - 29) : times2(a.scale, max(power.f, -200) - 14);
+  const float factor = times2(WEIGHTS ? 1.0f : a.scale, max(power.f, -200) - 14);
   float* to;
   if (it.part < 0)
     to = (WEIGHTS ? a.o + int64_t(it.k0 + key) * a.o_ld : a.dk + int64_t(it.k0 + key) * a.dk_ld) +

@@ -422,15 +422,15 @@ int layer_norm_backward(Runtime* rt, NormBackArgs<T> a, T* dw, T* db) {
       });
       LMP_LAUNCH_CHECK("layer_norm_backward");
     } else {
+      if (columns) {  // first: dx may be g or x
+        norm_back_columns<T><<<dim3(uint32_t((int64_t(a.n) + 255) / 256), uint32_t(parts)),
+                               dim3(256), 0, rt->stream>>>(a);
+        LMP_LAUNCH_CHECK("layer_norm_backward columns");
+      }
       if (a.dx) {
         norm_back_long_rows<T>
             <<<dim3(uint32_t(capped(a.rows, cus * 8))), dim3(1024), 0, rt->stream>>>(a);
         LMP_LAUNCH_CHECK("layer_norm_backward");
-      }
-      if (columns) {
-        norm_back_columns<T><<<dim3(uint32_t((int64_t(a.n) + 255) / 256), uint32_t(parts)),
-                               dim3(256), 0, rt->stream>>>(a);
-        LMP_LAUNCH_CHECK("layer_norm_backward columns");
       }
     }
     if (columns) {

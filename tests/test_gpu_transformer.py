@@ -102,13 +102,20 @@ def test_layer_norm_without_weights_in_place_and_parts_of_the_backward(hip):
             got = norm_back(hip, g, dx, n, None, mean, rstd, want=want)
             for a, f, t in zip(got, full, want):
                 assert not t or np.array_equal(a, f)
-        # y over x, statistics not asked for; dx over g
+        # y over x, statistics not asked for; dx over g, all gradients asked for
         hip.check(hip.lib().lmp_k_layer_norm(hip.FLOAT32, rows, n, dx.ptr, n, None, None, 0.0, dx.ptr, n, None, None))
         assert np.array_equal(dx.numpy(), y)
         dx, dg = up(hip, x), up(hip, g)
         hip.check(hip.lib().lmp_k_layer_norm_backward(hip.FLOAT32, rows, n, dg.ptr, n, dx.ptr, n, None, mean.ptr, rstd.ptr,
                                                       dg.ptr, n, None, None))
         assert np.array_equal(dg.numpy(), full[0])
+        dw, db = hip.DeviceBuffer((n,)), hip.DeviceBuffer((n,))
+        for over in (up(hip, x), up(hip, g)):
+            dx, dg = (over, up(hip, g)) if np.array_equal(over.numpy(), x) else (up(hip, x), over)
+            hip.check(hip.lib().lmp_k_layer_norm_backward(hip.FLOAT32, rows, n, dg.ptr, n, dx.ptr, n, None, mean.ptr,
+                                                          rstd.ptr, over.ptr, n, dw.ptr, db.ptr))
+            for a, f in zip((over, dw, db), full):
+                assert np.array_equal(a.numpy(), f)
 
 
 def test_layer_norm_constant_and_special_rows(hip):
@@ -449,16 +456,132 @@ def test_attention_special_values_in_sight(hip):
     assert np.abs(got[fine] - want[fine]).max() < 1e-5
 
 
-def test_attention_long_sequences_agree_with_64_bits(hip):
-    """Sizes of the large kernels, ragged: 64-bit scores by matrix products on the host."""
-    rng = np.random.default_rng(77)
-    for ql, heads, kv, d in (([700, 333], 4, 2, 64), ([513], 2, 1, 128), ([1000], 1, 1, 80)):
-        q, k, v, g = attention_inputs(rng, ql, ql, heads, kv, d)
-        got = attend(hip, ql, ql, heads, kv, d, True, q, k, v, d ** -0.5, g, pad=1)
-        want = T.attention(q, k, v, ql, ql, heads, kv, d ** -0.5, True, g)
-        bound = T.attention_bounds(q, k, v, ql, ql, heads, kv, d ** -0.5, True, g)
-        for a, w, b, what in zip(got, want, bound, ("o", "lse", "dq", "dk", "dv")):
-            close(a, w, b, what)
+def launches(hip):
+    n = C.c_uint64()
+    hip.check(hip.lib().lmp_rt_kernel_launch_count(C.byref(n)))
+    return n.value
+
+
+def check_split(hip, ql, kl, heads, kv, d, causal, q, k, v, g, scale, pad=0, split=True):
+    """Both passes against 64 bits; `split`: by the split-fp16 kernels, which launch more than the fp32 ones."""
+    before = launches(hip)
+    got = attend(hip, ql, kl, heads, kv, d, causal, q, k, v, scale, g, pad=pad)
+    assert (launches(hip) - before >= 10) == split
+    want = T.attention(q, k, v, ql, kl, heads, kv, scale, causal, g)
+    bound = T.attention_bounds(q, k, v, ql, kl, heads, kv, abs(scale), causal, g) if scale > 0 else \
+        T.attention_bounds(-q, k, v, ql, kl, heads, kv, -scale, causal, g)
+    empty = want[1] == -np.inf
+    assert np.array_equal(got[1][empty], want[1][empty])
+    got[1] = np.where(empty, 0, got[1])
+    for a, w, b, what in zip(got, (want[0], np.where(empty, 0, want[1]), *want[2:]), bound, ("o", "lse", "dq", "dk", "dv")):
+        close(a, w, b, what)
+    return got
+
+
+SPLIT = [
+    ([700, 333], [700, 333], 16, 4, 64, True), ([513], [513], 32, 8, 128, True), ([1000], [1000], 16, 2, 80, True),
+    ([600, 37, 0, 450], [600, 37, 5, 450], 12, 4, 96, True), ([640], [640], 16, 16, 33, False), ([777], [777], 16, 1, 100, True),
+    # the last query sees every key; the first see none
+    ([300, 1], [1200, 64], 16, 4, 128, True), ([900], [500], 16, 4, 64, True), ([257, 400], [90, 1100], 16, 8, 48, False),
+    # few blocks: keys and steps in parts that are joined
+    ([200], [3000], 8, 2, 128, True), ([1500], [1500], 2, 1, 128, True),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SPLIT)), ids=lambda i: str(SPLIT[i]).replace(" ", ""))
+def test_attention_of_long_batches(hip, case):
+    ql, kl, heads, kv, d, causal = SPLIT[case]
+    q, k, v, g = attention_inputs(np.random.default_rng(50 + case), ql, kl, heads, kv, d)
+    check_split(hip, ql, kl, heads, kv, d, causal, q, k, v, g, d ** -0.5, pad=case % 3)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1.0, 1e-6])
+def test_attention_of_long_batches_any_scale(hip, scale):
+    q, k, v, g = attention_inputs(np.random.default_rng(3), [640], [640], 16, 4, 64)
+    if scale == 0:  # every visible key weighs the same; the fp32 kernels run it
+        got = attend(hip, [640], [640], 16, 4, 64, True, q, k, v, 0.0, g)
+        mean = np.cumsum(v.astype(np.float64), 0) / np.arange(1, 641)[:, None]
+        want = np.repeat(mean.reshape(640, 4, 64), 4, 1).reshape(640, -1)
+        close(got[0], want, 700 * T.U32 * np.abs(v).max())
+        assert not got[2].any() and not got[3].any()
+        return
+    check_split(hip, [640], [640], 16, 4, 64, True, q, k, v, g, scale)
+
+
+@pytest.mark.parametrize("what", ["rows", "tiny", "huge", "columns", "zeros"])
+def test_attention_of_long_batches_ranges(hip, what):
+    """Operands of one power of two per tile: rows further apart than that carries, and largest values outside its range,
+    go to the fp32 kernels; columns apart and rows of zeros stay."""
+    n, heads, kv, d = 600, 16, 4, 64
+    q, k, v, g = attention_inputs(np.random.default_rng(4), [n], [n], heads, kv, d)
+    scale = d ** -0.5
+    if what == "rows":
+        for a in (q, k, v, g):
+            a[::7] *= np.float32(2.0 ** -16)
+            a[5] *= np.float32(8)
+    elif what == "tiny":
+        q *= np.float32(2.0 ** -70)
+        g *= np.float32(2.0 ** -70)
+        scale = float(2.0 ** 67)
+    elif what == "huge":
+        k *= np.float32(2.0 ** 45)
+        scale = float(2.0 ** -48)
+    elif what == "columns":
+        for a in (q, k):
+            a[:, 3::64] *= np.float32(64)
+        scale /= 512
+    else:
+        for a in (q, k, v, g):
+            a[64:128] = 0
+            a[200] = 0
+    check_split(hip, [n], [n], heads, kv, d, True, q, k, v, g, scale)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 3e38])
+def test_attention_of_long_batches_masked_places_reach_nothing(hip, bad):
+    """As above, at sizes of the split kernels: sequences and key heads without such a value stay bit for bit as they were,
+    those with one are as the fp32 kernels have them."""
+    ql, heads, kv, d = [500, 400], 16, 4, 64
+    q, k, v, g = attention_inputs(np.random.default_rng(12), ql, ql, heads, kv, d)
+    clean = check_split(hip, ql, ql, heads, kv, d, True, q, k, v, g, 0.125)
+    want = T.attention(q, k, v, ql, ql, heads, kv, 0.125, True, g)
+    bound = T.attention_bounds(q, k, v, ql, ql, heads, kv, 0.125, True, g)
+    at, width = 300, d * heads // kv  # in key head 1 of the first sequence
+    k2, v2 = k.copy(), v.copy()
+    k2[at, d + 3] = bad
+    v2[at, d:2 * d] = bad
+    got = attend(hip, ql, ql, heads, kv, d, True, q, k2, v2, 0.125, g)
+    hit = np.zeros((900, heads * d), bool)
+    hit[at:500, width:2 * width] = True
+    for i in (0, 2):
+        close(np.where(hit, 0, got[i]), np.where(hit, 0, want[i]), bound[i])
+        other = np.ones_like(hit)
+        other[:500, width:2 * width] = False
+        assert np.array_equal(got[i][other], clean[i][other])
+    q2, g2 = q.copy(), g.copy()
+    q2[at, width:width + 5] = bad
+    g2[at, width + 64:width + 70] = bad
+    got = attend(hip, ql, ql, heads, kv, d, True, q2, k, v, 0.125, g2)
+    for i in (3, 4):
+        seen = np.zeros((900, kv * d), bool)
+        seen[:at + 1, d:2 * d] = True
+        close(np.where(seen, 0, got[i]), np.where(seen, 0, want[i]), bound[i])
+        other = np.ones_like(seen)
+        other[:500, d:2 * d] = False
+        assert np.array_equal(got[i][other], clean[i][other])
+
+
+def test_attention_of_long_batches_special_values_in_sight(hip):
+    n, heads, kv, d = 600, 16, 4, 64
+    q, k, v, g = attention_inputs(np.random.default_rng(8), [n], [n], heads, kv, d)
+    v[200, 70], v[300, 5] = np.inf, np.nan
+    k[250, 2 * d] = -np.inf
+    q[:, 8 * d] = np.abs(q[:, 8 * d])
+    got = attend(hip, [n], [n], heads, kv, d, True, q, k, v, 0.125, g)[0]
+    want = T.attention(q, k, v, [n], [n], heads, kv, 0.125, True)[0]
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isposinf(got), np.isposinf(want))
+    fine = np.isfinite(want)
+    assert np.abs(got[fine] - want[fine]).max() < 1e-5
 
 
 def test_attention_plans_are_refused_inside_a_capture(hip):
@@ -519,10 +642,51 @@ def test_recorded_step_replays(hip):
     hip.check(L.lmp_rt_graph_destroy(graph))
 
 
+def test_recorded_long_attention_replays(hip):
+    """The split kernels, their workspaces and joins recorded once; replays with new operands in the same buffers, eager work
+    between them, one of them with a NaN that sends a key head to the fp32 kernels."""
+    L, ql, heads, kv, d = hip.lib(), [700, 350], 16, 4, 64
+    plan = hip.AttentionPlan(ql, heads=heads, kv_heads=kv, head_dim=d)
+    sizes = [heads * d, kv * d, kv * d, heads * d]
+    held = [hip.DeviceBuffer((1050, w)) for w in sizes]
+    outs = [hip.DeviceBuffer((1050, w)) for w in (heads * d, heads, heads * d, kv * d, kv * d)]
+
+    def step():
+        q, k, v, g = (b.ptr for b in held)
+        o, lse, dq, dk, dv = (b.ptr for b in outs)
+        qw, kw = heads * d, kv * d
+        hip.check(L.lmp_k_attention_f32(plan.handle, q, qw, k, kw, v, kw, 0.125, o, qw, lse))
+        hip.check(L.lmp_k_attention_backward_f32(plan.handle, q, qw, k, kw, v, kw, 0.125, o, qw, lse, g, qw, dq, qw, dk, kw,
+                                                 dv, kw))
+
+    graph = C.c_void_p()
+    hip.check(L.lmp_rt_graph_begin())
+    try:
+        step()
+    except BaseException:
+        hip.check(L.lmp_rt_graph_abort())
+        raise
+    hip.check(L.lmp_rt_graph_end(C.byref(graph)))
+    for i in range(4):
+        host = attention_inputs(np.random.default_rng(i), ql, ql, heads, kv, d)
+        if i == 2:
+            host[2][900, 70] = np.nan
+        for b, a in zip(held, host):
+            hip.check(L.lmp_rt_memcpy_h2d(b.ptr, a.ctypes.data, a.nbytes))
+        step()
+        want = [o.numpy() for o in outs]
+        for o in outs:
+            hip.check(L.lmp_k_fill(hip.FLOAT32, o.ptr, o.nbytes // 4, 7.0))
+        hip.check(L.lmp_rt_graph_launch(graph))
+        for o, w in zip(outs, want):
+            assert np.array_equal(o.numpy(), w, equal_nan=True), i
+    hip.check(L.lmp_rt_graph_destroy(graph))
+
+
 def test_calls_repeat_bit_for_bit(hip):
-    ql, kl, heads, kv, d = [1, 300, 40], [900, 300, 400], 4, 2, 64
-    q, k, v, g = attention_inputs(np.random.default_rng(6), ql, kl, heads, kv, d)
-    first = attend(hip, ql, kl, heads, kv, d, True, q, k, v, 0.125, g)
-    for _ in range(2):
-        for a, b in zip(attend(hip, ql, kl, heads, kv, d, True, q, k, v, 0.125, g), first):
-            assert np.array_equal(a, b)
+    for ql, kl, heads, kv, d in (([1, 300, 40], [900, 300, 400], 4, 2, 64), ([1000, 300], [1000, 300], 16, 2, 64)):
+        q, k, v, g = attention_inputs(np.random.default_rng(6), ql, kl, heads, kv, d)
+        first = attend(hip, ql, kl, heads, kv, d, True, q, k, v, 0.125, g)
+        for _ in range(3):
+            for a, b in zip(attend(hip, ql, kl, heads, kv, d, True, q, k, v, 0.125, g), first):
+                assert np.array_equal(a, b)
