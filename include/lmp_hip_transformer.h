@@ -105,8 +105,8 @@ int lmp_k_attention_plan_destroy(void* plan);
  * and dv may be slices of the same rows).
  * Short batches and single tokens run on the fp32 matrix cores.  Long ones run on
  * the fp16 matrix cores with every operand split into two fp16 parts that share a
- * power of two per 32 rows of one head: a product then errs by at most 2^-20.9 of
- * itself (2^-24 rms) and by 2^-40 of the largest one among its 32 rows; rows that
+ * power of two per 32 rows of one head: a product then errs by at most 2^-21 of
+ * itself (2^-23.5 rms) and by 2^-40 of the largest one among its 32 rows; rows that
  * lie further apart than 2^12, infinities, NaN and largest values outside
  * [2^-60, 2^41) send their sequence's key head to the fp32 kernels. */
 int lmp_k_attention_f32(const void* plan, const float* q, size_t q_ld, const float* k, size_t k_ld,

@@ -78,9 +78,9 @@ AttnArgs common_args(const AttentionPlan& plan, double scale) {
 // 2048 queries, 17 to 8192 keys, 1 to 32 heads of 32, 64 and 128): the form it
 // takes is 1% slower than the faster one on average, forward, and 2% backward.
 // Some of them, fp32 | split in us: forward, one sequence of 1024, 4 heads of 128,
-// 43 | 42; 16 heads, 89 | 52; one query against 8 x 8192 keys, 32 heads on 4, 88 |
-// 340; 64 queries, 900 | 400; backward, one sequence of 256, 4 heads of 64, 34 |
-// 41; of 1024, 16 heads of 64 on 4, 304 | 85.
+// 43 | 42; 16 heads, 89 | 52; 8 queries against 8 x 8192 keys, 32 heads on 4, 147 |
+// 302; 64 queries, 896 | 404; backward, one sequence of 256, 4 heads of 64, 28 |
+// 45; of 1024, 16 heads of 64 on 4, 244 | 91.
 bool split_form(const AttentionPlan& plan, double scale, bool back) {
   const double q_tiles = double(plan.q_tiles.count) * double(plan.heads),
                k_tiles = double(plan.k_tiles.count) * double(plan.kv_heads);
@@ -95,7 +95,7 @@ bool split_form(const AttentionPlan& plan, double scale, bool back) {
   // The fp32 kernels do not share out the keys of a row or the rows of a key.
   const double chain =
       double(plan.longest_k + plan.longest_q * (plan.heads / plan.kv_heads)) * dim / 1e3;
-  return 15 + 0.26 * f32 + 0.61 * chain > 45 + 0.04 * split + 0.145 * (3 * q + 4 * k);
+  return 13 + 0.27 * f32 + 0.46 * chain > 45 + 0.04 * split + 0.143 * (3 * q + 4 * k);
 }
 
 // Calls f with the ND of the split kernels that hold `dim` (at most 128).
@@ -213,6 +213,19 @@ uint32_t f32_grid(const AttnArgs& a) {
   const int64_t work = int64_t(a.count) * a.kv_heads;
   return grid_of(a.marks ? std::min<int64_t>(work, 256) : work);
 }
+// Calls f with the ND of the columns and the waves of a backward workgroup: eight
+// where two workgroups of four would leave compute units idle (columns past 128
+// have no registers for them).
+template <class F>
+void with_back_form(Runtime* rt, const AttnArgs& a, F&& f) {
+  using std::integral_constant;
+  const bool few = int64_t(a.count) * a.kv_heads <= int64_t(rt->cu_count) * 2;
+  with_dim(a.dim, [&](auto nd) {
+    constexpr int most = nd <= 8 ? 8 : 4;
+    if (few) f(nd, integral_constant<int, most>{});
+    else f(nd, integral_constant<int, 4>{});
+  });
+}
 int forward_f32(Runtime* rt, const AttentionPlan& plan, AttnArgs a) {
   a.items = plan.rows.at;
   a.count = plan.rows.count;
@@ -290,8 +303,7 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
     SplitAttnArgs& s = split.args;
     attention_split_stats<<<dim3(uint32_t(int64_t(plan.q_tiles.count) * plan.heads)), dim3(256), 0,
                             rt->stream>>>(plan.q_tiles.at, int(plan.heads), int(plan.dim), o, o_ld,
-                                          a.g, a.g_ld, a.lse_in, split.stats,
-                                          static_cast<float*>(delta.p));
+                                          a.g, a.g_ld, a.lse_in, split.stats);
     LMP_LAUNCH_CHECK("attention_split_stats");
     // Rows first, then keys; each one's parts are summed before the next needs the
     // memory.
@@ -342,20 +354,17 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
     if (status) return status;
     a.marks = s.marks;
     a.any_mark = split.any_mark;
-  } else if (plan.queries) {
-    attention_delta<<<dim3(grid_of((plan.queries * plan.heads + 15) / 16)), dim3(256), 0,
-                      rt->stream>>>(plan.queries, int(plan.heads), int(plan.dim), o, o_ld, a.g,
-                                    a.g_ld, static_cast<float*>(delta.p));
-    LMP_LAUNCH_CHECK("attention_delta");
   }
   if (plan.queries) {
-    a.delta = static_cast<const float*>(delta.p);
+    a.delta = static_cast<float*>(delta.p);
+    a.out = o;
+    a.out_ld = o_ld;
     a.items = plan.rows.at;
     a.count = plan.rows.count;
     a.o = dq;
     a.o_ld = dq_ld;
-    with_dim(plan.dim, [&](auto nd) {
-      attention_back_rows<nd><<<dim3(f32_grid(a)), dim3(256), 0, rt->stream>>>(a);
+    with_back_form(rt, a, [&](auto nd, auto waves) {
+      attention_back_rows<nd, waves><<<dim3(f32_grid(a)), dim3(waves * 64), 0, rt->stream>>>(a);
     });
     LMP_LAUNCH_CHECK("attention_back_rows");
   }
@@ -366,8 +375,8 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
     a.o_ld = dv_ld;
     a.dk = dk;
     a.dk_ld = dk_ld;
-    with_dim(plan.dim, [&](auto nd) {
-      attention_back_keys<nd><<<dim3(f32_grid(a)), dim3(256), 0, rt->stream>>>(a);
+    with_back_form(rt, a, [&](auto nd, auto waves) {
+      attention_back_keys<nd, waves><<<dim3(f32_grid(a)), dim3(waves * 64), 0, rt->stream>>>(a);
     });
     LMP_LAUNCH_CHECK("attention_back_keys");
   }

@@ -13,8 +13,8 @@
 // are 16-byte loads, since the order of a contraction is free.  Scores are formed
 // transposed, S^T = K Q^T: a lane then holds 4 keys of one query, which is the
 // layout in which P is the next product's operand, and a query's running maximum
-// and sum stay in its own lanes.  The four waves of a workgroup take every fourth
-// step of the keys (or rows) and join at the end, in a fixed order.
+// and sum stay in its own lanes.  The waves of a workgroup take the steps of the keys
+// (or rows) in turn and join at the end, in a fixed order.
 //
 // Masked places.  A masked score becomes -inf (P exactly 0) whatever it was, and
 // where a step holds masked places the operand that P multiplies may hold an
@@ -62,7 +62,9 @@ struct AttnArgs {
   int64_t q_ld, k_ld, v_ld, g_ld;
   float scale;
   const float* lse_in;
-  const float* delta;  // [query][head]
+  const float* out;    // forward's output
+  int64_t out_ld;
+  float* delta;        // [query][head]: rowsum(g o), which the rows leave for the keys
   float *o, *lse, *dk;  // o: forward's output or dq; dk with o as dv
   int64_t o_ld, dk_ld;
   float *part, *part_ml;  // [part][kv head][16 rows][dim], [...][16][2]
@@ -172,9 +174,9 @@ __device__ __forceinline__ void accumulate(a4 (&acc)[ND], float (&f)[4][ND], con
   }
 }
 
-// The four waves' blocks [column of 16][d], summed in order and handed out:
-// put(row, column, 4 values) by every lane.
-template <int ND, class Put>
+// The waves' blocks [column of 16][d], summed in order and handed out:
+// put(row, column, 4 values).
+template <int ND, int WAVES, class Put>
 __device__ __forceinline__ void join_waves(const a4 (&acc)[ND], float* lds, Put&& put) {
   constexpr int PITCH = ND * 16 + 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
@@ -185,11 +187,12 @@ __device__ __forceinline__ void join_waves(const a4 (&acc)[ND], float* lds, Put&
     for (int r = 0; r < 4; ++r)
       lds[(wave * 16 + n) * PITCH + Cols<ND>::at(j, 4 * g + r)] = acc[j][r];
   __syncthreads();
-  const int row = threadIdx.x >> 4;
-  for (int c = (threadIdx.x & 15) * 4; c < ND * 16; c += 64) {
+  constexpr int LANES = WAVES * 4;  // of a row
+  const int row = threadIdx.x / LANES;
+  for (int c = (threadIdx.x % LANES) * 4; c < ND * 16; c += LANES * 4) {
     a4 s = *reinterpret_cast<const a4*>(lds + row * PITCH + c);
 #pragma unroll
-    for (int w = 1; w < 4; ++w) s += *reinterpret_cast<const a4*>(lds + (w * 16 + row) * PITCH + c);
+    for (int w = 1; w < WAVES; ++w) s += *reinterpret_cast<const a4*>(lds + (w * 16 + row) * PITCH + c);
     put(row, c, s);
   }
 }
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(256) void attention_rows(AttnArgs a) {
             (base + __builtin_amdgcn_logf(total)) * kLn2;
       }
     }
-    join_waves<ND>(acc, lds, [&](int row, int col, a4 x) {
+    join_waves<ND, 4>(acc, lds, [&](int row, int col, a4 x) {
       if (row >= rows) return;
       const int r = it.first + row;
       float* to = it.part >= 0
@@ -368,39 +371,20 @@ __global__ __launch_bounds__(256) void attention_join(AttnArgs a, const AttnJoin
   }
 }
 
-// delta = rowsum(g o) of every query and head: 16 lanes each.
-__global__ __launch_bounds__(256) void attention_delta(int64_t queries, int heads, int dim,
-                                                       const float* o, int64_t o_ld, const float* g,
-                                                       int64_t g_ld, float* delta) {
-  const int64_t step = int64_t(gridDim.x) * 16, total = queries * heads;
-  for (int64_t first = int64_t(blockIdx.x) * 16; first < total; first += step) {
-    const int64_t i = min(first + (threadIdx.x >> 4), total - 1);
-    const int64_t row = i / heads, head = i % heads;
-    float s = 0;
-    for (int c = (threadIdx.x & 15) * 4; c < dim; c += 64) {
-      float x[4], y[4];
-      load_cols<4>(o + row * o_ld + head * dim, c, dim, x);
-      load_cols<4>(g + row * g_ld + head * dim, c, dim, y);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s = fmaf(x[j], y[j], s);
-    }
-    s += __shfl_xor(s, 1);
-    s += __shfl_xor(s, 2);
-    s += __shfl_xor(s, 4);
-    s += __shfl_xor(s, 8);
-    if ((threadIdx.x & 15) == 0) delta[i] = s;
-  }
-}
-
 // A row's lse in base 2; +inf, which makes its P zero, where it sees nothing.
 __device__ __forceinline__ float lse2_of(float lse) {
   return lse == -__builtin_inff() ? __builtin_inff() : lse * kLog2e;
 }
 
-template <int ND>
-__global__ __launch_bounds__(256) void attention_back_rows(AttnArgs a) {
+// The backward workgroups have four waves, or eight where there are few of them:
+// half as many steps in turn, at half the workgroups on a compute unit (one
+// sequence of 256, 4 heads of 64: 34 us with four, 28 with eight; 16 of 64, 16
+// heads of 64: 39 and 52).
+template <int ND, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attention_back_rows(AttnArgs a) {
   if (a.marks && !*a.any_mark) return;
-  __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (ND * 16 + 4)];
+  constexpr int STEP = WAVES * 16;
+  __shared__ __attribute__((aligned(16))) float lds[WAVES * 16 * (ND * 16 + 4)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   const int heads = a.kv_heads * a.group;
   for (int64_t w = blockIdx.x; w < int64_t(a.count) * a.kv_heads; w += gridDim.x) {
@@ -419,13 +403,23 @@ __global__ __launch_bounds__(256) void attention_back_rows(AttnArgs a) {
     load_along<ND>(a.g + int64_t(it.q0 + query) * a.g_ld + int64_t(head) * a.dim, g, a.dim, go);
     const float c = a.scale * kLog2e;
     const float lse2 = lse2_of(a.lse_in[int64_t(it.q0 + query) * heads + head]);
-    const float delta = a.delta[int64_t(it.q0 + query) * heads + head];
+    float delta = 0;
+#pragma unroll
+    for (int b = 0; b < ND; ++b) {
+      float o[4];
+      load_cols<4>(a.out + int64_t(it.q0 + query) * a.out_ld + int64_t(head) * a.dim, 16 * b + 4 * g,
+                   a.dim, o);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) delta = fmaf(go[b][j], o[j], delta);
+    }
+    delta = column_sum(delta);
+    if (wave == 0 && g == 0 && n < rows) a.delta[int64_t(it.q0 + query) * heads + head] = delta;
     const float* k0 = a.k + int64_t(it.k0) * a.k_ld + int64_t(kv) * a.dim;
     const float* v0 = a.v + int64_t(it.k0) * a.v_ld + int64_t(kv) * a.dim;
     a4 acc[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) acc[j] = a4{0, 0, 0, 0};
-    for (int kt = wave * 16; kt < key_end; kt += 64) {
+    for (int kt = wave * 16; kt < key_end; kt += STEP) {
       const auto key = [&](int i) { return min(kt + i, it.lk - 1); };
       float k[ND][4], v[ND][4], kc[4][ND];
       load_along<ND>(k0 + int64_t(key(n)) * a.k_ld, g, a.dim, k);
@@ -445,7 +439,7 @@ __global__ __launch_bounds__(256) void attention_back_rows(AttnArgs a) {
       accumulate<ND>(acc, kc, ds, a.dim, __any(!whole), [&](int i) { return kt + i < limit; },
                      [&](int i) { return k0 + int64_t(key(i)) * a.k_ld; });
     }
-    join_waves<ND>(acc, lds, [&](int row, int col, a4 x) {
+    join_waves<ND, WAVES>(acc, lds, [&](int row, int col, a4 x) {
       if (row >= rows) return;
       const int r = it.first + row;
       store_cols(a.o + int64_t(it.q0 + r / a.group) * a.o_ld +
@@ -456,10 +450,11 @@ __global__ __launch_bounds__(256) void attention_back_rows(AttnArgs a) {
   }
 }
 
-template <int ND>
-__global__ __launch_bounds__(256) void attention_back_keys(AttnArgs a) {
+template <int ND, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attention_back_keys(AttnArgs a) {
   if (a.marks && !*a.any_mark) return;
-  __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (ND * 16 + 4)];
+  constexpr int STEP = WAVES * 16;
+  __shared__ __attribute__((aligned(16))) float lds[WAVES * 16 * (ND * 16 + 4)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   const int heads = a.kv_heads * a.group;
   for (int64_t w = blockIdx.x; w < int64_t(a.count) * a.kv_heads; w += gridDim.x) {
@@ -477,7 +472,7 @@ __global__ __launch_bounds__(256) void attention_back_keys(AttnArgs a) {
     a4 dk[ND], dv[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) dk[j] = dv[j] = a4{0, 0, 0, 0};
-    for (int rt = from + wave * 16; rt < rows; rt += 64) {
+    for (int rt = from + wave * 16; rt < rows; rt += STEP) {
       const auto packed = [&](int i) { return min(rt + i, rows - 1); };
       const auto q_at = [&](int i) {
         const int r = packed(i);
@@ -517,12 +512,12 @@ __global__ __launch_bounds__(256) void attention_back_keys(AttnArgs a) {
       for (int r = 0; r < 4; ++r) load_across<ND>(q_at(4 * g + r), n, a.dim, f[r]);
       accumulate<ND>(dk, f, ds, a.dim, masked, sees, q_at);
     }
-    join_waves<ND>(dv, lds, [&](int row, int col, a4 x) {
+    join_waves<ND, WAVES>(dv, lds, [&](int row, int col, a4 x) {
       if (row < keys)
         store_cols(a.o + int64_t(it.k0 + it.first + row) * a.o_ld + int64_t(kv) * a.dim, col, a.dim,
                    x);
     });
-    join_waves<ND>(dk, lds, [&](int row, int col, a4 x) {
+    join_waves<ND, WAVES>(dk, lds, [&](int row, int col, a4 x) {
       if (row < keys)
         store_cols(a.dk + int64_t(it.k0 + it.first + row) * a.dk_ld + int64_t(kv) * a.dim, col,
                    a.dim, x);

@@ -507,8 +507,7 @@ __global__ __launch_bounds__(256, 2) void attention_split_rows(SplitAttnArgs a) 
 __global__ __launch_bounds__(256) void attention_split_stats(const AttnTile* tiles, int heads, int dim,
                                                              const float* o, int64_t o_ld,
                                                              const float* g, int64_t g_ld,
-                                                             const float* lse, float* stats,
-                                                             float* delta) {
+                                                             const float* lse, float* stats) {
   const int64_t w = blockIdx.x;
   const int head = int(w % heads), row = threadIdx.x >> 3;
   const AttnTile t = tiles[w / heads];
@@ -527,7 +526,6 @@ __global__ __launch_bounds__(256) void attention_split_stats(const AttnTile* til
   if ((threadIdx.x & 7) == 0) {
     stats[w * 64 + row] = row < t.rows ? lse2_of(lse[at * heads + head]) : __builtin_inff();
     stats[w * 64 + 32 + row] = row < t.rows ? s : 0.0f;
-    if (row < t.rows) delta[at * heads + head] = s;  // for the marked ones
   }
 }
 

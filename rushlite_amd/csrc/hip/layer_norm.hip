@@ -136,7 +136,8 @@ struct NormBackArgs {
   const T *w, *mean, *rstd;
   T* dx;
   int64_t lddx;
-  T* part;  // [workgroup][dw, db][n], or null
+  T* part;      // [workgroup][dw, db][n], or null
+  T *dw, *db;   // where one workgroup has all rows, and part is null
 };
 
 constexpr int threads_of(int lanes) { return lanes > 256 ? lanes : 256; }
@@ -258,11 +259,12 @@ __global__ __launch_bounds__(threads_of(L)) void norm_back_rows(NormBackArgs<T> 
     for (int i = 0; i < N; ++i) g[i] = rstd * (g[i] - c1 - x[i] * c2);
     if (live) store_row<T, L, U>(a.dx + row * a.lddx, lane, a.n, g);
   }
-  if (!a.part) return;
-  T* out = a.part + int64_t(blockIdx.x) * 2 * a.n;
+  T* to_w = a.part ? a.part + int64_t(blockIdx.x) * 2 * a.n : a.dw;
+  T* to_b = a.part ? to_w + a.n : a.db;
+  if (!to_w && !to_b) return;
   if constexpr (R == 1) {
-    store_row<T, L, U>(out, lane, a.n, dw);
-    store_row<T, L, U>(out + a.n, lane, a.n, db);
+    if (to_w) store_row<T, L, U>(to_w, lane, a.n, dw);
+    if (to_b) store_row<T, L, U>(to_b, lane, a.n, db);
   } else {
     __shared__ T sums[R][L * N];
     for (int which = 0; which < 2; ++which) {
@@ -275,7 +277,7 @@ __global__ __launch_bounds__(threads_of(L)) void norm_back_rows(NormBackArgs<T> 
         T s = sums[0][c];
 #pragma unroll
         for (int r = 1; r < R; ++r) s += sums[r][c];
-        out[int64_t(which) * a.n + c] = s;
+        if (T* to = which ? to_b : to_w) to[c] = s;
       }
     }
   }
@@ -402,14 +404,20 @@ template <typename T>
 int layer_norm_backward(Runtime* rt, NormBackArgs<T> a, T* dw, T* db) {
   const int64_t cus = rt->cu_count;
   const bool columns = dw || db;
-  // Workgroups over the rows: two waves' worth on every SIMD.
+  // Workgroups over the rows: two waves' worth on every SIMD.  Up to four groups of
+  // rows stay with one, which saves the launch that folds the partials.
   int64_t parts = 1;
   const bool held = with_variant<T>(a.n, [&](auto lanes, auto) {
     constexpr int L = lanes, R = threads_of(L) / L;
-    parts = capped((a.rows + R - 1) / R, L > 256 ? cus : cus * 2);
+    const int64_t groups = (a.rows + R - 1) / R;
+    parts = groups <= 4 ? 1 : std::min(groups, L > 256 ? cus : cus * 2);
   });
   if (!held) parts = capped(a.rows / 64, 64);
-  if (columns) {
+  const bool direct = held && parts == 1;
+  if (direct) {
+    a.dw = dw;
+    a.db = db;
+  } else if (columns) {
     a.part = static_cast<T*>(scratch_alloc(size_t(parts) * 2 * size_t(a.n) * sizeof(T)));
     if (!a.part) return LMP_ERR_OOM;
   }
@@ -433,7 +441,7 @@ int layer_norm_backward(Runtime* rt, NormBackArgs<T> a, T* dw, T* db) {
         LMP_LAUNCH_CHECK("layer_norm_backward");
       }
     }
-    if (columns) {
+    if (a.part) {
       norm_back_fold<T><<<dim3(uint32_t((2 * int64_t(a.n) + 31) / 32)), dim3(1024), 0,
                           rt->stream>>>(a.part, int(parts), a.n, dw, db);
       LMP_LAUNCH_CHECK("layer_norm_backward fold");
@@ -505,7 +513,7 @@ extern "C" int lmp_k_layer_norm_backward(int dtype, size_t rows, size_t cols, co
     NormBackArgs<T> a{int64_t(rows), int(cols), static_cast<const T*>(g), int64_t(ldg),
                       static_cast<const T*>(x), int64_t(ldx), static_cast<const T*>(w),
                       static_cast<const T*>(mean), static_cast<const T*>(rstd),
-                      static_cast<T*>(dx), int64_t(lddx), nullptr};
+                      static_cast<T*>(dx), int64_t(lddx), nullptr, nullptr, nullptr};
     return layer_norm_backward<T>(rt, a, static_cast<T*>(dw), static_cast<T*>(db));
   };
   return dtype == LMP_FLOAT64 ? go(double(0)) : go(float(0));
