@@ -71,16 +71,20 @@ inline int64_t attn_key_steps(int64_t first, int64_t lq, int64_t lk, bool causal
   return (tiles - from) * group;
 }
 
-// Rows whose keys are split take parts of nearly equal length, at multiples of
-// `step` keys: emit(begin, end, part) for each.
+// Rows whose keys are split take parts: emit(begin, end, part) for each.  With a
+// `step`, of nearly equal length, at multiples of it; without one, of part_keys but
+// for the last, so that the parts of different rows go over the same keys together.
 template <class Emit>
 inline void attn_parts(int64_t seen, int64_t part_keys, int64_t step, int64_t* next_part,
                        Emit&& emit) {
   const int64_t parts = seen <= part_keys ? 1 : (seen + part_keys - 1) / part_keys;
   if (parts == 1) return emit(0, seen, int64_t(-1));
-  const int64_t steps = (seen + step - 1) / step;
-  for (int64_t p = 0; p < parts; ++p)
-    emit(steps * p / parts * step, std::min(seen, steps * (p + 1) / parts * step), (*next_part)++);
+  const int64_t steps = step ? (seen + step - 1) / step : 0;
+  for (int64_t p = 0; p < parts; ++p) {
+    const int64_t begin = step ? steps * p / parts * step : p * part_keys;
+    const int64_t end = step ? steps * (p + 1) / parts * step : begin + part_keys;
+    emit(begin, std::min(seen, end), (*next_part)++);
+  }
 }
 
 // The length of a part that gives about `workgroups` of them, `least` at least;
@@ -141,7 +145,7 @@ inline AttnLists attn_lists(size_t sequences, const int64_t* ql, const int64_t* 
             16, &a.parts, a.rows, a.joins);
     for (int64_t q = 0; q < lq; q += kAttnSplitRows)
       split(q, attn_seen(std::min(lq, q + kAttnSplitRows) - 1, lq, lk, causal), block_keys,
-            kAttnTile, &a.q_parts, a.q_blocks, a.q_joins);
+            0, &a.q_parts, a.q_blocks, a.q_joins);
     it.part = -1;
     it.key_begin = 0;
     it.key_end = it.lk;
@@ -152,7 +156,7 @@ inline AttnLists attn_lists(size_t sequences, const int64_t* ql, const int64_t* 
     for (int64_t k = 0; k < lk; k += kAttnSplitRows) {
       it.first = int32_t(k);
       const int64_t before = a.k_parts;
-      attn_parts(attn_key_steps(k, lq, lk, causal, group), part_steps, 1, &a.k_parts,
+      attn_parts(attn_key_steps(k, lq, lk, causal, group), part_steps, 0, &a.k_parts,
                  [&](int64_t begin, int64_t end, int64_t part) {
                    it.key_begin = int32_t(begin);
                    it.key_end = int32_t(end);
@@ -173,7 +177,9 @@ inline AttnLists attn_lists(size_t sequences, const int64_t* ql, const int64_t* 
   }
   // Longest first: the last workgroups to start are short ones.
   const auto keys_of = [](const AttnItem& x) { return x.key_end - x.key_begin; };
-  const auto longer = [&](const AttnItem& x, const AttnItem& y) { return keys_of(x) > keys_of(y); };
+  const auto longer = [&](const AttnItem& x, const AttnItem& y) {
+    return keys_of(x) != keys_of(y) ? keys_of(x) > keys_of(y) : x.key_begin < y.key_begin;
+  };
   std::stable_sort(a.rows.begin(), a.rows.end(), longer);
   std::stable_sort(a.q_blocks.begin(), a.q_blocks.end(), longer);
   const auto queries_of = [&](const AttnItem& x) {
