@@ -13,7 +13,12 @@
 //
 // States of 8 bits: a wave owns a block of 256 values, four a lane, so the
 // block's scale is a maximum over the wave and a state costs one 4-byte access
-// per lane.
+// per lane.  What bounds that form is the arithmetic, two hashes' worth of integer
+// products and two roots a value, as much as the memory.
+//
+// Measured, 37.7 million parameters: 177 us = 6.0 TB/s with states of 32 bits; 143 us
+// = 4.2 TB/s with states of 8 (178 us with the compiler's exact root and quotient),
+// and 29 and 35 us to read them out.  17 thousand parameters in four tensors: 5.2 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

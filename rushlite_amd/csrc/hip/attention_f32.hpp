@@ -20,6 +20,12 @@
 // where a step holds masked places the operand that P multiplies may hold an
 // infinity or NaN that its row must not see (0 inf = NaN): such values are taken
 // out of the product and added to the rows that see them.
+//
+// Measured: one token of 32 requests, 32 heads of 128 on 8 key heads, up to 8192
+// keys (1.11 GB of keys and values): 187 us = 5.9 TB/s and 6 us for the join; with
+// ordinary loads, keys read when they are due and a third fewer parts 222 and 12.
+// One sequence of 32, 4 heads of 64: 5.6 us.  A batch of prompts multiplies at about
+// 77 TFLOP/s forward, half of what the fp32 matrix cores do.
 #pragma once
 
 #include <hip/hip_runtime.h>
