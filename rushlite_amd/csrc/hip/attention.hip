@@ -85,7 +85,7 @@ bool split_form(const AttentionPlan& plan, double scale, bool back) {
   const double q_tiles = double(plan.q_tiles.count) * double(plan.heads),
                k_tiles = double(plan.k_tiles.count) * double(plan.kv_heads);
   // Grids stay below 2^32 threads; a scale of 0 leaves no power of two to divide.
-  if (plan.dim > 128 || scale == 0 || 2 * (q_tiles + k_tiles) >= double(1 << 22)) return false;
+  if (plan.dim > 128 || scale == 0 || !plan.queries || !plan.keys || 2 * (q_tiles + k_tiles) >= double(1 << 22)) return false;
   // In millions: the multiplications of one product in each form's steps, and the
   // bytes of a split operand's fragments.
   const double dim = double(plan.dim), f32 = plan.row_work * double(plan.kv_heads) * dim / 1e6,
@@ -95,7 +95,7 @@ bool split_form(const AttentionPlan& plan, double scale, bool back) {
   // The fp32 kernels do not share out the keys of a row or the rows of a key.
   const double chain =
       double(plan.longest_k + plan.longest_q * (plan.heads / plan.kv_heads)) * dim / 1e3;
-  return 13 + 0.27 * f32 + 0.46 * chain > 45 + 0.04 * split + 0.143 * (3 * q + 4 * k);
+  return 13 + 0.27 * f32 + 0.46 * chain > 41 + 0.041 * split + 0.134 * (3 * q + 4 * k);
 }
 
 // Calls f with the ND of the split kernels that hold `dim` (at most 128).
@@ -177,12 +177,21 @@ int split_operands(Runtime* rt, const AttentionPlan& plan, const AttnArgs& a, do
       const auto& tiles = queries ? plan.q_tiles : plan.k_tiles;
       if (tiles.count)
         p.op[p.count++] = {x, ld, tiles.at, tiles.count, int(queries ? plan.heads : plan.kv_heads),
-                           sign, along, across, const_cast<int32_t*>(exponent)};
+                           sign, along, across, const_cast<int32_t*>(exponent),
+                           nullptr, 0, nullptr, nullptr, nullptr};
     };
     add(a.q, a.q_ld, true, scale < 0 ? -1.0f : 1.0f, m + q_along, back ? m + q_across : nullptr, s.q_exp);
     add(a.k, a.k_ld, false, 1.0f, m + k_along, back ? m + k_across : nullptr, s.k_exp);
     add(a.v, a.v_ld, false, 1.0f, back ? m + v_along : nullptr, back ? nullptr : m + v_across, s.v_exp);
-    if (back) add(a.g, a.g_ld, true, 1.0f, m + g_along, m + g_across, s.g_exp);
+    if (back && plan.queries) {
+      add(a.g, a.g_ld, true, 1.0f, m + g_along, m + g_across, s.g_exp);
+      SplitOperand& g = p.op[p.count - 1];
+      g.out = a.out;
+      g.out_ld = a.out_ld;
+      g.lse = a.lse_in;
+      g.stats = out.stats;
+      g.delta = a.delta;
+    }
     attention_split<nd><<<dim3(uint32_t(qn + 2 * kn + (back ? qn : 0))), dim3(256), 0, rt->stream>>>(p);
     status = [&]() -> int {
       LMP_LAUNCH_CHECK("attention_split");
@@ -298,13 +307,23 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
   Scratch delta;
   SplitOperands split;
   if (!delta.get(size_t(plan.queries) * size_t(plan.heads) * sizeof(float))) return LMP_ERR_OOM;
+  a.delta = static_cast<float*>(delta.p);
+  a.out = o;
+  a.out_ld = o_ld;
+  AttnArgs rows = a, keys = a;
+  rows.items = plan.rows.at;
+  rows.count = plan.rows.count;
+  rows.o = dq;
+  rows.o_ld = dq_ld;
+  keys.items = plan.key_items.at;
+  keys.count = plan.key_items.count;
+  keys.o = dv;
+  keys.o_ld = dv_ld;
+  keys.dk = dk;
+  keys.dk_ld = dk_ld;
   if (split_form(plan, scale, true)) {
     if (int s = split_operands(rt, plan, a, scale, true, split)) return s;
     SplitAttnArgs& s = split.args;
-    attention_split_stats<<<dim3(uint32_t(int64_t(plan.q_tiles.count) * plan.heads)), dim3(256), 0,
-                            rt->stream>>>(plan.q_tiles.at, int(plan.heads), int(plan.dim), o, o_ld,
-                                          a.g, a.g_ld, a.lse_in, split.stats);
-    LMP_LAUNCH_CHECK("attention_split_stats");
     // Rows first, then keys; each one's parts are summed before the next needs the
     // memory.
     const size_t slot = size_t(kAttnSplitRows) * size_t(plan.dim) * sizeof(float);
@@ -352,31 +371,26 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
                       {k.part, k.part + k.part_dk}, {dv, dk}, {dv_ld, dk_ld}}, 2);
     });
     if (status) return status;
-    a.marks = s.marks;
-    a.any_mark = split.any_mark;
+    for (AttnArgs* x : {&rows, &keys}) {
+      x->marks = s.marks;
+      x->any_mark = split.any_mark;
+    }
+    const uint32_t grid = std::max(f32_grid(rows), f32_grid(keys));
+    with_split_dim(plan.dim, [&](auto nd) {
+      attention_back_marked<nd><<<dim3(grid), dim3(256), 0, rt->stream>>>(rows, keys);
+    });
+    LMP_LAUNCH_CHECK("attention_back_marked");
+    return LMP_OK;
   }
   if (plan.queries) {
-    a.delta = static_cast<float*>(delta.p);
-    a.out = o;
-    a.out_ld = o_ld;
-    a.items = plan.rows.at;
-    a.count = plan.rows.count;
-    a.o = dq;
-    a.o_ld = dq_ld;
-    with_back_form(rt, a, [&](auto nd, auto waves) {
-      attention_back_rows<nd, waves><<<dim3(f32_grid(a)), dim3(waves * 64), 0, rt->stream>>>(a);
+    with_back_form(rt, rows, [&](auto nd, auto waves) {
+      attention_back_rows<nd, waves><<<dim3(f32_grid(rows)), dim3(waves * 64), 0, rt->stream>>>(rows);
     });
     LMP_LAUNCH_CHECK("attention_back_rows");
   }
   if (plan.keys) {
-    a.items = plan.key_items.at;
-    a.count = plan.key_items.count;
-    a.o = dv;
-    a.o_ld = dv_ld;
-    a.dk = dk;
-    a.dk_ld = dk_ld;
-    with_back_form(rt, a, [&](auto nd, auto waves) {
-      attention_back_keys<nd, waves><<<dim3(f32_grid(a)), dim3(waves * 64), 0, rt->stream>>>(a);
+    with_back_form(rt, keys, [&](auto nd, auto waves) {
+      attention_back_keys<nd, waves><<<dim3(f32_grid(keys)), dim3(waves * 64), 0, rt->stream>>>(keys);
     });
     LMP_LAUNCH_CHECK("attention_back_keys");
   }

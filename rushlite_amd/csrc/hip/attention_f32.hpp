@@ -387,10 +387,8 @@ __device__ __forceinline__ float lse2_of(float lse) {
 // sequence of 256, 4 heads of 64: 34 us with four, 28 with eight; 16 of 64, 16
 // heads of 64: 39 and 52).
 template <int ND, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void attention_back_rows(AttnArgs a) {
-  if (a.marks && !*a.any_mark) return;
+__device__ __forceinline__ void back_rows(const AttnArgs& a, float* lds) {
   constexpr int STEP = WAVES * 16;
-  __shared__ __attribute__((aligned(16))) float lds[WAVES * 16 * (ND * 16 + 4)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   const int heads = a.kv_heads * a.group;
   for (int64_t w = blockIdx.x; w < int64_t(a.count) * a.kv_heads; w += gridDim.x) {
@@ -410,16 +408,20 @@ __global__ __launch_bounds__(WAVES * 64) void attention_back_rows(AttnArgs a) {
     const float c = a.scale * kLog2e;
     const float lse2 = lse2_of(a.lse_in[int64_t(it.q0 + query) * heads + head]);
     float delta = 0;
+    if (a.marks) {  // the splitting kernel has left it
+      delta = a.delta[int64_t(it.q0 + query) * heads + head];
+    } else {
 #pragma unroll
-    for (int b = 0; b < ND; ++b) {
-      float o[4];
-      load_cols<4>(a.out + int64_t(it.q0 + query) * a.out_ld + int64_t(head) * a.dim, 16 * b + 4 * g,
-                   a.dim, o);
+      for (int b = 0; b < ND; ++b) {
+        float o[4];
+        load_cols<4>(a.out + int64_t(it.q0 + query) * a.out_ld + int64_t(head) * a.dim,
+                     16 * b + 4 * g, a.dim, o);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) delta = fmaf(go[b][j], o[j], delta);
+        for (int j = 0; j < 4; ++j) delta = fmaf(go[b][j], o[j], delta);
+      }
+      delta = column_sum(delta);
+      if (wave == 0 && g == 0 && n < rows) a.delta[int64_t(it.q0 + query) * heads + head] = delta;
     }
-    delta = column_sum(delta);
-    if (wave == 0 && g == 0 && n < rows) a.delta[int64_t(it.q0 + query) * heads + head] = delta;
     const float* k0 = a.k + int64_t(it.k0) * a.k_ld + int64_t(kv) * a.dim;
     const float* v0 = a.v + int64_t(it.k0) * a.v_ld + int64_t(kv) * a.dim;
     a4 acc[ND];
@@ -457,10 +459,8 @@ __global__ __launch_bounds__(WAVES * 64) void attention_back_rows(AttnArgs a) {
 }
 
 template <int ND, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void attention_back_keys(AttnArgs a) {
-  if (a.marks && !*a.any_mark) return;
+__device__ __forceinline__ void back_keys(const AttnArgs& a, float* lds) {
   constexpr int STEP = WAVES * 16;
-  __shared__ __attribute__((aligned(16))) float lds[WAVES * 16 * (ND * 16 + 4)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   const int heads = a.kv_heads * a.group;
   for (int64_t w = blockIdx.x; w < int64_t(a.count) * a.kv_heads; w += gridDim.x) {
@@ -530,6 +530,25 @@ __global__ __launch_bounds__(WAVES * 64) void attention_back_keys(AttnArgs a) {
     });
     __syncthreads();
   }
+}
+
+template <int ND, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attention_back_rows(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) float lds[WAVES * 16 * (ND * 16 + 4)];
+  back_rows<ND, WAVES>(a, lds);
+}
+template <int ND, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attention_back_keys(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) float lds[WAVES * 16 * (ND * 16 + 4)];
+  back_keys<ND, WAVES>(a, lds);
+}
+// Both over what the split kernels have left, in one launch: nothing as a rule.
+template <int ND>
+__global__ __launch_bounds__(256) void attention_back_marked(AttnArgs rows, AttnArgs keys) {
+  __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (ND * 16 + 4)];
+  if (!*rows.any_mark) return;
+  back_rows<ND, 4>(rows, lds);
+  back_keys<ND, 4>(keys, lds);
 }
 
 }  // namespace

@@ -145,6 +145,14 @@ struct SplitOperand {
   float sign;
   char *along, *across;  // fragments [tile][head], or null
   int32_t* exponent;     // [tile][head]
+  // With x the output gradient: the forward output and lse, for what the backward
+  // kernels read, lse in base 2 (+inf where a row sees nothing or is past its
+  // sequence) and delta = rowsum(x out), per tile and head one after another, and
+  // delta once more by query and head for the marked ones.  Else null.
+  const float* out;
+  int64_t out_ld;
+  const float* lse;
+  float *stats, *delta;
 };
 struct SplitArgs {
   SplitOperand op[4];
@@ -191,6 +199,28 @@ __global__ __launch_bounds__(256) void attention_split(SplitArgs a) {
   const bool marked = most >= 0x7f800000u ||
                       (most && (e < kLeastExponent || e > kMostExponent || e_least < e - kRowsApart));
   if (threadIdx.x == 0) op.exponent[w] = marked ? kIrregular : most ? e : kZeroTile;
+  if (op.out) {  // 8 lanes a row
+    const int row = threadIdx.x >> 3;
+    const int64_t at = int64_t(t.at) + min(row, t.rows - 1);
+    const float* out = op.out + at * op.out_ld + int64_t(head) * a.dim;
+    float s = 0;
+    for (int c = (threadIdx.x & 7) * 4; c < a.dim; c += 32) {
+      float y[4];
+      load_cols<4>(out, c, a.dim, y);
+      const a4 x = *reinterpret_cast<const a4*>(tile + row * PITCH + c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = fmaf(x[j], y[j], s);
+    }
+    s += __shfl_xor(s, 1);
+    s += __shfl_xor(s, 2);
+    s += __shfl_xor(s, 4);
+    if ((threadIdx.x & 7) == 0) {
+      const bool there = row < t.rows;
+      op.stats[w * 64 + row] = there ? lse2_of(op.lse[at * op.heads + head]) : __builtin_inff();
+      op.stats[w * 64 + 32 + row] = there ? s : 0.0f;
+      if (there) op.delta[at * op.heads + head] = s;
+    }
+  }
   if (marked) return;
   const float scale = most ? times2(op.sign, 14 - e) : 0.0f;
   const auto put = [&](char* to, const float (&x)[8]) {
@@ -505,34 +535,6 @@ __global__ __launch_bounds__(256, 2) void attention_split_rows(SplitAttnArgs a) 
       a.part_ml[slot * 2] = top;
       a.part_ml[slot * 2 + 1] = sum;
     }
-  }
-}
-
-// The statistics the backward kernels read: lse in base 2 (+inf where a row sees
-// nothing or is past its sequence) and delta = rowsum(g o), a tile of one head
-// one after another.  8 lanes a row.
-__global__ __launch_bounds__(256) void attention_split_stats(const AttnTile* tiles, int heads, int dim,
-                                                             const float* o, int64_t o_ld,
-                                                             const float* g, int64_t g_ld,
-                                                             const float* lse, float* stats) {
-  const int64_t w = blockIdx.x;
-  const int head = int(w % heads), row = threadIdx.x >> 3;
-  const AttnTile t = tiles[w / heads];
-  const int64_t at = int64_t(t.at) + min(row, t.rows - 1);
-  float s = 0;
-  for (int c = (threadIdx.x & 7) * 4; c < dim; c += 32) {
-    float x[4], y[4];
-    load_cols<4>(o + at * o_ld + int64_t(head) * dim, c, dim, x);
-    load_cols<4>(g + at * g_ld + int64_t(head) * dim, c, dim, y);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s = fmaf(x[j], y[j], s);
-  }
-  s += __shfl_xor(s, 1);
-  s += __shfl_xor(s, 2);
-  s += __shfl_xor(s, 4);
-  if ((threadIdx.x & 7) == 0) {
-    stats[w * 64 + row] = row < t.rows ? lse2_of(lse[at * heads + head]) : __builtin_inff();
-    stats[w * 64 + 32 + row] = row < t.rows ? s : 0.0f;
   }
 }
 
