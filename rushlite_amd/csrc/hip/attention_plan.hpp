@@ -72,18 +72,20 @@ inline int64_t attn_key_steps(int64_t first, int64_t lq, int64_t lk, bool causal
 }
 
 // Rows whose keys are split take parts: emit(begin, end, part) for each.  With a
-// `step`, of nearly equal length, at multiples of it; without one, of part_keys but
-// for the last, so that the parts of different rows go over the same keys together.
+// `step`, of nearly equal length, at multiples of it; without one, of part_keys, so
+// that the parts of different rows go over the same keys together, the last one half
+// shorter or longer at most.
 template <class Emit>
 inline void attn_parts(int64_t seen, int64_t part_keys, int64_t step, int64_t* next_part,
                        Emit&& emit) {
-  const int64_t parts = seen <= part_keys ? 1 : (seen + part_keys - 1) / part_keys;
-  if (parts == 1) return emit(0, seen, int64_t(-1));
+  const int64_t over = step ? part_keys - 1 : part_keys / 2;
+  const int64_t parts = seen <= part_keys ? 1 : (seen + over) / part_keys;
+  if (parts <= 1) return emit(0, seen, int64_t(-1));
   const int64_t steps = step ? (seen + step - 1) / step : 0;
   for (int64_t p = 0; p < parts; ++p) {
     const int64_t begin = step ? steps * p / parts * step : p * part_keys;
     const int64_t end = step ? steps * (p + 1) / parts * step : begin + part_keys;
-    emit(begin, std::min(seen, end), (*next_part)++);
+    emit(begin, p + 1 == parts ? seen : end, (*next_part)++);
   }
 }
 

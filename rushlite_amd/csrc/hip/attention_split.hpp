@@ -32,9 +32,9 @@
 //
 // Measured, one causal sequence of 8192, 16 heads of 128 (key heads of four
 // each): forward 0.80 ms = 343 TFLOP/s of fp32 products = 1.03 PFLOP/s of fp16, dq
-// 1.20 ms = 1.03, dk and dv 1.78 ms = 0.93, where a library's fp16 product of 8192^3 does
+// 1.18 ms = 1.05, dk and dv 1.72 ms = 0.96, where a library's fp16 product of 8192^3 does
 // 1.09 on the same card; the fp32 kernels took 22 ms for all of it.  The matrix
-// cores are busy 52, 50 and 41% of the cycles, and the clock falls by a sixth under
+// cores are busy 52, 49 and 44% of the cycles, and the clock falls by a sixth under
 // them in a loop of calls: power bounds it as much as the waits at the steps' barriers.
 #pragma once
 
