@@ -85,7 +85,10 @@ bool split_form(const AttentionPlan& plan, double scale, bool back) {
   const double q_tiles = double(plan.q_tiles.count) * double(plan.heads),
                k_tiles = double(plan.k_tiles.count) * double(plan.kv_heads);
   // Grids stay below 2^32 threads; a scale of 0 leaves no power of two to divide.
-  if (plan.dim > 128 || scale == 0 || !plan.queries || !plan.keys || 2 * (q_tiles + k_tiles) >= double(1 << 22)) return false;
+  if (plan.dim > 128 || scale == 0 || !plan.queries || !plan.keys ||
+      2 * (q_tiles + k_tiles) >= double(1 << 22) ||
+      double(plan.seqs.count) * double(plan.kv_heads) >= double(1 << 22))
+    return false;
   // In millions: the multiplications of one product in each form's steps, and the
   // bytes of a split operand's fragments.
   const double dim = double(plan.dim), f32 = plan.row_work * double(plan.kv_heads) * dim / 1e6,

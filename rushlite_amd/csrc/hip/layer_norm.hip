@@ -334,22 +334,26 @@ template <typename T>
 __global__ __launch_bounds__(1024) void norm_back_fold(const T* part, int parts, int n, T* dw,
                                                        T* db) {
   __shared__ T sums[32][33];
-  const int64_t c = int64_t(blockIdx.x) * 32 + threadIdx.x % 32, width = 2 * int64_t(n);
+  const int64_t width = 2 * int64_t(n);
   const int lane = threadIdx.x / 32;
-  T s = 0;
-  if (c < width) {
+  for (int64_t first = int64_t(blockIdx.x) * 32; first < width; first += int64_t(gridDim.x) * 32) {
+    const int64_t c = first + threadIdx.x % 32;
+    T s = 0;
+    if (c < width) {
 #pragma unroll 8
-    for (int p = lane; p < parts; p += 32) s += part[p * width + c];
-  }
-  sums[lane][threadIdx.x % 32] = s;
-  __syncthreads();
-  for (int half = 16; half >= 1; half /= 2) {
-    if (lane < half) sums[lane][threadIdx.x % 32] += sums[lane + half][threadIdx.x % 32];
+      for (int p = lane; p < parts; p += 32) s += part[p * width + c];
+    }
+    sums[lane][threadIdx.x % 32] = s;
     __syncthreads();
-  }
-  if (lane == 0 && c < width) {
-    T* out = c < n ? dw : db;
-    if (out) out[c < n ? c : c - n] = sums[0][threadIdx.x];
+    for (int half = 16; half >= 1; half /= 2) {
+      if (lane < half) sums[lane][threadIdx.x % 32] += sums[lane + half][threadIdx.x % 32];
+      __syncthreads();
+    }
+    if (lane == 0 && c < width) {
+      T* out = c < n ? dw : db;
+      if (out) out[c < n ? c : c - n] = sums[0][threadIdx.x];
+    }
+    __syncthreads();
   }
 }
 
@@ -448,7 +452,7 @@ int layer_norm_backward(Runtime* rt, NormBackArgs<T> a, T* dw, T* db) {
       }
     }
     if (a.part) {
-      norm_back_fold<T><<<dim3(uint32_t((2 * int64_t(a.n) + 31) / 32)), dim3(1024), 0,
+      norm_back_fold<T><<<dim3(uint32_t(capped((2 * int64_t(a.n) + 31) / 32, 1 << 20))), dim3(1024), 0,
                           rt->stream>>>(a.part, int(parts), a.n, dw, db);
       LMP_LAUNCH_CHECK("layer_norm_backward fold");
     }

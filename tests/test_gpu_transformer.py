@@ -133,6 +133,21 @@ def test_layer_norm_constant_and_special_rows(hip):
             assert np.array_equal(y[r], norm(hip, x[r:r + 1], None, None, 1e-5)[0][0])
 
 
+def test_layer_norm_gradients_of_a_row_of_67_million(hip):
+    """Past 2^26 columns a lane per value and partial would pass 2^32 threads a grid."""
+    n = (1 << 26) + 70
+    rng = np.random.default_rng(1)
+    x, g = rng.standard_normal((1, n), np.float32), rng.standard_normal((1, n), np.float32)
+    dx, dg, dw, db = up(hip, x), up(hip, g), hip.DeviceBuffer((n,)), hip.DeviceBuffer((n,))
+    mean, rstd = up(hip, np.array([0.25], np.float32)), up(hip, np.array([2.0], np.float32))
+    hip.check(hip.lib().lmp_k_layer_norm_backward(hip.FLOAT32, 1, n, dg.ptr, n, dx.ptr, n, None, mean.ptr, rstd.ptr, None, 0,
+                                                  dw.ptr, db.ptr))
+    assert np.array_equal(db.numpy(), g[0])
+    want = g[0].astype(np.float64) * (x[0].astype(np.float64) - 0.25) * 2
+    bound = 3 * T.U32 * np.abs(g[0]) * (np.abs(x[0]) + 0.25) * 2
+    close(dw.numpy(), want, bound)
+
+
 def test_layer_norm_backward_of_no_rows(hip):
     out = [up(hip, np.full(700, 7, np.float32)) for _ in range(2)]
     hip.check(hip.lib().lmp_k_layer_norm_backward(hip.FLOAT32, 0, 700, None, 0, None, 0, None, None, None, None, 0,
