@@ -60,7 +60,11 @@ uint32_t grid_of(int64_t work) { return uint32_t(std::clamp<int64_t>(work, 1, in
 struct Scratch {  // returned to the pool when the call ends, in stream order
   void* p = nullptr;
   ~Scratch() { if (p) scratch_free(p); }
-  bool get(size_t bytes) { return bytes == 0 || (p = scratch_alloc(bytes)) != nullptr; }
+  bool get(size_t bytes) {
+    if (p) scratch_free(p);
+    p = bytes ? scratch_alloc(bytes) : nullptr;
+    return !bytes || p;
+  }
 };
 
 AttnArgs common_args(const AttentionPlan& plan, double scale) {
@@ -262,9 +266,12 @@ int forward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale) {
     a.part = a.part_ml + slots * 2;
     return true;
   };
-  if (split_form(plan, scale, false)) {
-    if (!parts(plan.q_parts, plan.heads, kAttnSplitRows)) return LMP_ERR_OOM;
-    if (int s = split_operands(rt, plan, a, scale, false, split)) return s;
+  // Without memory for the fragments the fp32 kernels, which need none, take over.
+  int status = LMP_ERR_OOM;
+  if (split_form(plan, scale, false) && parts(plan.q_parts, plan.heads, kAttnSplitRows))
+    status = split_operands(rt, plan, a, scale, false, split);
+  if (status != LMP_ERR_OOM) {
+    if (status) return status;
     SplitAttnArgs& s = split.args;
     s.items = plan.q_blocks.at;
     s.count = plan.q_blocks.count;
@@ -273,7 +280,6 @@ int forward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale) {
     s.lse = a.lse;
     s.part = a.part;
     s.part_ml = a.part_ml;
-    int status = LMP_OK;
     with_split_dim(plan.dim, [&](auto nd) {
       status = launch_split(rt, "attention_split_rows", attention_split_rows<nd>,
                             int64_t(s.count) * plan.heads, 256,
@@ -324,16 +330,18 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
   keys.o_ld = dv_ld;
   keys.dk = dk;
   keys.dk_ld = dk_ld;
-  if (split_form(plan, scale, true)) {
-    if (int s = split_operands(rt, plan, a, scale, true, split)) return s;
+  // Rows first, then keys; each one's parts are summed before the next needs the
+  // memory.
+  const size_t slot = size_t(kAttnSplitRows) * size_t(plan.dim) * sizeof(float);
+  const size_t q_bytes = size_t(plan.q_parts) * size_t(plan.heads) * slot,
+               k_bytes = size_t(plan.k_parts) * size_t(plan.kv_heads) * slot;
+  Scratch part;
+  int status = LMP_ERR_OOM;  // as in forward()
+  if (split_form(plan, scale, true) && part.get(std::max(q_bytes, 2 * k_bytes)))
+    status = split_operands(rt, plan, a, scale, true, split);
+  if (status != LMP_ERR_OOM) {
+    if (status) return status;
     SplitAttnArgs& s = split.args;
-    // Rows first, then keys; each one's parts are summed before the next needs the
-    // memory.
-    const size_t slot = size_t(kAttnSplitRows) * size_t(plan.dim) * sizeof(float);
-    const size_t q_bytes = size_t(plan.q_parts) * size_t(plan.heads) * slot,
-                 k_bytes = size_t(plan.k_parts) * size_t(plan.kv_heads) * slot;
-    Scratch part;
-    if (!part.get(std::max(q_bytes, 2 * k_bytes))) return LMP_ERR_OOM;
     s.part = static_cast<float*>(part.p);
     s.part_dk = int64_t(k_bytes / sizeof(float));
     const auto sum = [&](const SumArgs& p, int results) -> int {
@@ -343,7 +351,6 @@ int backward(Runtime* rt, const AttentionPlan& plan, AttnArgs a, double scale, c
       LMP_LAUNCH_CHECK("attention_sum");
       return LMP_OK;
     };
-    int status = LMP_OK;
     with_split_dim(plan.dim, [&](auto nd) {
       using F = Frag<nd>;
       SplitAttnArgs r = s;
@@ -509,7 +516,7 @@ namespace {
 int check_operands(const char* name, const AttentionPlan* plan, const float* q, size_t q_ld,
                    const float* k, size_t k_ld, const float* v, size_t v_ld, double scale) {
   if (!plan) return fail(LMP_ERR_INVALID, std::string(name) + ": null plan");
-  if (!std::isfinite(scale)) return fail(LMP_ERR_INVALID, std::string(name) + ": scale is not finite");
+  if (!std::isfinite(float(scale))) return fail(LMP_ERR_INVALID, std::string(name) + ": scale is not finite");
   if ((plan->queries && !q) || (plan->keys && (!k || !v)))
     return fail(LMP_ERR_INVALID, std::string(name) + ": null buffer");
   const size_t qw = size_t(plan->heads * plan->dim), kw = size_t(plan->kv_heads * plan->dim);

@@ -141,8 +141,9 @@ def test_attention_refusals(rsl):
             rsl.attention(*args, plan)
     with pytest.raises(RuntimeError, match="3 queries and 5 keys"):
         rsl.attention_qkv(z(3, 64), plan)
-    with pytest.raises(RuntimeError, match="scale is not finite"):
-        rsl.attention(*good, plan, float("nan"))
+    for scale in (float("nan"), float("inf"), 1e300):
+        with pytest.raises(RuntimeError, match="scale is not finite"):
+            rsl.attention(*good, plan, scale)
     with pytest.raises(RuntimeError, match="multiple of kv_heads"):
         rsl.AttentionPlan([3], heads=3, kv_heads=2, head_dim=8)
     with pytest.raises(RuntimeError, match="one query length"):
