@@ -510,9 +510,20 @@ __global__ __launch_bounds__(256, 2) void attention_split_rows(SplitAttnArgs a) 
       ref = ev;
     }
     const float lift = times2(1.0f, 15 + ev - ref);
+    // `base` is a rounded product, off from the one that the fma does not round by half
+    // a unit in its last place.  Up to 2^20 that is a factor near 1 which every weight of
+    // the row has; past it the weights would leave fp16's range, so the product is
+    // rounded here too and the row's best key weighs 1.
+    if (__any(fabsf(base) > 0x1p20f)) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = s[r] * c - base;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, -base);
+    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s[r] = exp2_of(fmaf(s[r], c, -base));
+      s[r] = exp2_of(s[r]);
       sum += s[r];
       s[r] *= lift;
     }

@@ -717,3 +717,75 @@ def test_calls_repeat_bit_for_bit(hip):
         for _ in range(3):
             for a, b in zip(attend(hip, ql, kl, heads, kv, d, True, q, k, v, 0.125, g), first):
                 assert np.array_equal(a, b)
+
+
+def one_power_a_tile(a, lengths, d):
+    """Whether every tile of 32 rows of one head is one the split-fp16 kernels keep (include/lmp_hip_transformer.h)."""
+    first = 0
+    for n in lengths:
+        for at in range(first, first + n, 32):
+            rows = np.abs(a[at:min(at + 32, first + n)].reshape(-1, a.shape[1] // d, d)).max(2)
+            top = rows.max(0)
+            least = np.where(rows > 0, rows, np.inf).min(0)
+            if not ((top == 0) | ((top >= 2.0 ** -60) & (top < 2.0 ** 41) & (least * 2 ** 11 >= top))).all():
+                return False
+        first += n
+    return True
+
+
+def attend_split(hip, n, heads, kv, d, q, k, v, scale):
+    """The forward pass of one causal sequence, by the split kernels alone."""
+    assert all(one_power_a_tile(a, [n], d) for a in (q, k, v))
+    before = launches(hip)
+    got = attend(hip, [n], [n], heads, kv, d, True, q, k, v, scale)
+    assert launches(hip) - before >= 4  # the fp32 kernels launch two at most
+    return got
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", [8, 11, 15])
+def test_attention_of_long_batches_scores_past_24_bits(hip, power, sign):
+    """Scores of up to 2^25, 2^31 and 2^39, formed without an error and further apart than float32's steps at their size:
+    each row is its best key's value.
+
+    Rounding: the value's two parts hold it to 2 u, their sum rounds once, and 2^-39 of the tile's largest is lost where
+    a value is small; the weight is exactly 1.  lse: the constant log2 e, the product with it and the product with ln 2."""
+    n, heads, kv, d, scale = 1000, 16, 4, 64, 0.125
+    rng = np.random.default_rng(power)
+    q, k, v, _ = attention_inputs(rng, [n], [n], heads, kv, d)
+    q[:], k[:] = 0, 0
+    order = rng.permutation(n) - n / 2 + 0.5
+    q[:, ::d] = (sign * 2.0 ** power * (1 + np.arange(n) % 7))[:, None]
+    k[:, ::d] = (2.0 ** power * order)[:, None]
+    o, lse = attend_split(hip, n, heads, kv, d, q, k, v, scale)
+    best = np.array([(sign * order[:i + 1]).argmax() for i in range(n)])
+    want = np.repeat(v[best].reshape(n, kv, d), heads // kv, 1).reshape(n, -1).astype(np.float64)
+    close(o, want, 4 * T.U32 * np.abs(want) + 2.0 ** -39 * np.abs(v).max(), "o")
+    top = (q[:, 0].astype(np.float64) * k[best, 0] * scale)[:, None].repeat(heads, 1)
+    close(lse, top, 4 * T.U32 * np.abs(top), "lse")
+
+
+@pytest.mark.parametrize("size", [2e3, 1e4])
+def test_attention_of_long_batches_large_random_scores(hip, size):
+    """Scores of some 10^7 and 10^9: a row whose best key leads by more than the scores' rounding and 60 is that key's value,
+    every other one lies among the values that it sees."""
+    n, heads, kv, d, scale = 1000, 16, 4, 64, 0.125
+    q, k, v, _ = attention_inputs(np.random.default_rng(11), [n], [n], heads, kv, d)
+    q, k = (q * np.float32(size)), (k * np.float32(size))
+    o, lse = attend_split(hip, n, heads, kv, d, q, k, v, scale)
+    assert np.isfinite(o).all() and np.isfinite(lse).all()
+    alone = 0
+    for h in range(heads):
+        qs, ks, vs = (a.reshape(n, -1, d)[:, i].astype(np.float64) for a, i in ((q, h), (k, h // 4), (v, h // 4)))
+        s = np.where(np.tri(n, dtype=bool), qs @ ks.T * scale, -np.inf)
+        # of a score: d sums and 16 roundings as in attention_bounds, and those of its product with the constant
+        err = (d + 20) * T.U32 * scale * (np.abs(qs) @ np.abs(ks).T).max(1)
+        ranks = np.sort(s, 1)
+        lead = ranks[:, -1] - ranks[:, -2] > 2 * err + 60
+        alone += int(lead.sum())
+        got, want = o.reshape(n, heads, d)[:, h], vs[s.argmax(1)]
+        close(got[lead], want[lead], 4 * T.U32 * np.abs(want[lead]) + 2.0 ** -39 * np.abs(v).max(), "o")
+        slack = 64 * T.U32 * np.abs(v).max()
+        low, high = np.minimum.accumulate(vs, 0), np.maximum.accumulate(vs, 0)
+        assert (got >= low - slack).all() and (got <= high + slack).all()
+    assert alone > n * heads // 2
