@@ -106,8 +106,11 @@ int lmp_k_attention_plan_destroy(void* plan);
  * Short batches and single tokens run on the fp32 matrix cores.  Long ones run on
  * the fp16 matrix cores with every operand split into two fp16 parts that share a
  * power of two per 32 rows of one head: a product then errs by at most 2^-21 of
- * itself (2^-23.5 rms) and by 2^-40 of the largest one among its 32 rows; rows that
- * lie further apart than 2^12, infinities, NaN and largest values outside
+ * itself (2^-23.5 rms) and by 2^-40 of the largest one among its 32 rows.  Softmax
+ * weights, and gradients of scores, are split against the largest that their query (for
+ * dk and dv their key) has met so far, each times its tile's power of two and faded as
+ * the softmax goes on: what they multiply errs by 2^-37 of the largest such product.
+ * Rows that lie further apart than 2^12, infinities, NaN and largest values outside
  * [2^-60, 2^41) send their sequence's key head to the fp32 kernels. */
 int lmp_k_attention_f32(const void* plan, const float* q, size_t q_ld, const float* k, size_t k_ld,
                         const float* v, size_t v_ld, double scale, float* o, size_t o_ld,

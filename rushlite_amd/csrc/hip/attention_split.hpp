@@ -15,9 +15,10 @@
 // A tile with an infinity or a NaN, with a largest value outside [2^-60, 2^41) or
 // with rows more than 2^12 apart is marked, and the sequence's key head is left
 // to the fp32 kernels (attention_f32.hpp), which run over the marked ones only.
-// The forward weights are at most 1 and take a fixed power of two; P and dS of the
-// backward pass take one per query (dq) or key (dk, dv) that follows its largest
-// value so far, so that a key that few see keeps its gradient's digits.
+// Weights take a power of two per row that follows its largest so far: of P times the
+// value tile's own in the forward pass, so that a tile of large values which hardly
+// weigh leaves the others their digits; of P and dS in the backward pass, per query (dq)
+// or key (dk, dv), so that a key that few see keeps its gradient's.
 //
 // Layout.  A first kernel writes the operands as MFMA fragments: the 16 bytes of
 // each lane, a fragment's 64 lanes one after another, so that a workgroup's
@@ -56,6 +57,9 @@ typedef uint32_t w4 __attribute__((ext_vector_type(4)));
 constexpr int kIrregular = 1000;  // a marked tile's exponent
 constexpr int kZeroTile = -128;   // of a tile of zeros
 constexpr int kLeastExponent = -60, kMostExponent = 40, kRowsApart = 12;
+// Least power of two that the forward pass counts a row's weighted values in: what it
+// loses lies 2^40 below, and its factors keep above float32's smallest normal.
+constexpr int kLeastPower = -80;
 
 __device__ __forceinline__ s16 mfma_h(h8 a, h8 b, s16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -476,7 +480,8 @@ __global__ __launch_bounds__(256, 2) void attention_split_rows(SplitAttnArgs a) 
 #pragma unroll
   for (int m = 0; m < NT; ++m) acc[m] = s16(0.0f);
   float top = -__builtin_inff(), sum = 0;
-  int ref = kZeroTile;  // acc is O 2^(29 - ref)
+  float size = kLeastPower;
+  int power = kLeastPower;  // acc is O 2^(29 - power)
   for (int t = 0; t < tiles; ++t) {
     const int64_t at = int64_t(it.kt0 + tile0 + t) * a.kv_heads + kv;
     const int ek = exponent_at(a.k_exp, at), ev = exponent_at(a.v_exp, at);
@@ -498,18 +503,20 @@ __global__ __launch_bounds__(256, 2) void attention_split_rows(SplitAttnArgs a) 
     best = both_max(best);
     // Kept above zero: -inf times it stays -inf.
     const float c = fmaxf(times2(a.scale_log2e, ek + eq - 28), 1e-37f);
-    const float next = fmaxf(top, best * c), base = next > -__builtin_inff() ? next : 0.0f;
-    if (__any(next > top)) {
-      const float fade = exp2_of(top - base);
-      sum *= fade;
-      scale_acc(acc, fade);
+    const float here = best * c, next = fmaxf(top, here);
+    const float base = next > -__builtin_inff() ? next : 0.0f;
+    // The tile's weights are up to 2^(here - base), times 2^ev: 2^size follows the row's
+    // largest so far and falls with it as the weights fade; `power` lies a bit above it,
+    // so that it seldom moves.
+    if (__any(next > top || ev > power)) {
+      size = fmaxf(fmaxf(size - (next - top), float(ev) + (here - base)), float(kLeastPower));
+      const int moved = int(ceilf(size)) + 1;
+      sum *= exp2_of(top - base);
+      scale_acc(acc, exp2_of(top - base + float(power - moved)));
       top = next;
+      power = moved;
     }
-    if (ev > ref) {
-      scale_acc(acc, times2(1.0f, ref - ev));
-      ref = ev;
-    }
-    const float lift = times2(1.0f, 15 + ev - ref);
+    const float lift = times2(1.0f, 15 + ev - power);
     // `base` is a rounded product, off from the one that the fma does not round by half
     // a unit in its last place.  Up to 2^20 that is a factor near 1 which every weight of
     // the row has; past it the weights would leave fp16's range, so the product is
@@ -531,7 +538,7 @@ __global__ __launch_bounds__(256, 2) void attention_split_rows(SplitAttnArgs a) 
   }
   sum = both_sum(sum);
   if (!live) return;
-  const float back = times2(1.0f, ref - 29);
+  const float back = times2(1.0f, power - 29);
   if (it.part < 0) {
     store_lane<NT>(a.o + int64_t(it.q0 + query) * a.o_ld + int64_t(head) * a.dim, a.dim, half, acc,
                    sum > 0 ? back / sum : 0.0f);

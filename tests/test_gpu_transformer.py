@@ -789,3 +789,37 @@ def test_attention_of_long_batches_large_random_scores(hip, size):
         low, high = np.minimum.accumulate(vs, 0), np.maximum.accumulate(vs, 0)
         assert (got >= low - slack).all() and (got <= high + slack).all()
     assert alone > n * heads // 2
+
+
+@pytest.mark.parametrize("at", [0, 288])
+@pytest.mark.parametrize("weight", ["negligible", "even"])
+@pytest.mark.parametrize("power", [28, 40, 64])
+def test_attention_of_long_batches_values_of_different_sizes(hip, power, weight, at):
+    """A tile of 32 keys whose values are 2^power as large as the others', with weights that make up for it or go 2^16
+    below: the other keys' weights keep their digits."""
+    n, heads, kv, d, scale = 1000, 16, 4, 64, 0.125
+    q, k, v, g = attention_inputs(np.random.default_rng(power + at), [n], [n], heads, kv, d)
+    v *= np.float32(2.0 ** -30)
+    v[at:at + 32] *= np.float32(2.0 ** power)
+    q[:, ::d] = 8
+    k[at:at + 32, ::d] = np.float32(-np.log(2) * (power + (16 if weight == "negligible" else 0)))
+    attend_split(hip, n, heads, kv, d, q, k, v, scale)
+    check_split(hip, [n], [n], heads, kv, d, True, q, k, v, g, scale)
+
+
+def test_attention_of_long_batches_weights_that_rise_by_less_than_a_bit(hip):
+    """Every tile of keys weighs 2^0.95 as much as the one before it, and the first one's values are 2^44 as large: the power
+    of two that the weights take falls with its weight, by parts of a bit at a time.  Heads enough that no row's keys are
+    split into parts."""
+    n, heads, kv, d, scale = 1600, 64, 16, 32, 0.125
+    q, k, v, _ = attention_inputs(np.random.default_rng(5), [n], [n], heads, kv, d)
+    q, k, v = q / 32, k / 32, v / 1024
+    v[:32] *= np.float32(2.0 ** 44)
+    q[:, ::d] = 8
+    k[:, ::d] = (np.log(2) * 0.95 * (1 + np.arange(n) // 32)).astype(np.float32)[:, None]
+    o, lse = attend_split(hip, n, heads, kv, d, q, k, v, scale)
+    for h in (0, heads - 1):
+        own, keys = slice(h * d, h * d + d), slice(h // 4 * d, h // 4 * d + d)
+        one = (q[:, own], k[:, keys], v[:, keys], [n], [n], 1, 1, scale, True)
+        for a, w, b, what in zip((o[:, own], lse[:, h:h + 1]), T.attention(*one), T.attention_bounds(*one), ("o", "lse")):
+            close(a, w, b, what)
