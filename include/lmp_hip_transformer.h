@@ -65,7 +65,8 @@ typedef struct {
  * m^ = m / (1 - beta1^t) and v^ = v / (1 - beta2^t).  `step` is two int64 on the
  * device: step[0] the steps done so far (t = step[0] + 1; the call adds one),
  * step[1] the library's, 0 before the first call.  Keeping the count on the
- * device lets a recorded step be replayed.  State bits are 32 or 8.
+ * device lets a recorded step be replayed.  State bits are 32 or 8.  The buffers that
+ * a step writes (p, m, v and the scales of every tensor) do not overlap each other.
  * 8 bits: per block of values of one tensor, the largest magnitude M as a
  * float and per value a code c for sign(c) (|c| / Q)^2 M, Q = 127 for m and 255
  * for v, rounded up or down at random with the value as its expectation; a v

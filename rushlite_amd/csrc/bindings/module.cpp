@@ -509,6 +509,7 @@ PYBIND11_MODULE(_C, m) {
     }
     return shared;
   });
+  m.def("_variable_id", [](const Variable& v) { return reinterpret_cast<uintptr_t>(v.id()); });
   m.def("_storage_ptr", [](const Tensor& t) {
     return reinterpret_cast<uintptr_t>(
         lmp::tensor::detail::UnsafeTensorAccessor::getImpl(t)->raw());

@@ -349,6 +349,42 @@ __global__ __launch_bounds__(kThreads) void adamw_values(const uint8_t* codes, c
   }
 }
 
+// Two of the buffers that a step writes, if any two overlap: workgroups take them
+// without order, so an element that two entries hold would be stepped once or twice.
+struct Written {
+  uintptr_t begin, end;
+  size_t tensor;
+};
+bool find_overlap(int bits, size_t count, const lmp_adamw_tensor* tensors, Written (&pair)[2]) {
+  std::vector<Written> all;
+  all.reserve(count * (bits == 8 ? 5 : 3));
+  for (size_t i = 0; i < count; ++i) {
+    const lmp_adamw_tensor& t = tensors[i];
+    if (t.n == 0) continue;
+    const auto add = [&](const void* p, uint64_t bytes) {
+      const auto at = reinterpret_cast<uintptr_t>(p);
+      all.push_back({at, at + bytes, i});
+    };
+    const uint64_t state = t.n * (bits == 8 ? 1 : 4);
+    add(t.p, t.n * 4);
+    add(t.m, state);
+    add(t.v, state);
+    if (bits == 8) {
+      const uint64_t scales = (t.n + LMP_ADAMW_BLOCK - 1) / LMP_ADAMW_BLOCK * 4;
+      add(t.m_scale, scales);
+      add(t.v_scale, scales);
+    }
+  }
+  std::sort(all.begin(), all.end(), [](const Written& x, const Written& y) { return x.begin < y.begin; });
+  for (size_t i = 1; i < all.size(); ++i)
+    if (all[i].begin < all[i - 1].end) {
+      pair[0] = all[i - 1];
+      pair[1] = all[i];
+      return true;
+    }
+  return false;
+}
+
 }  // namespace
 }  // namespace lmp_hip
 
@@ -380,6 +416,15 @@ extern "C" int lmp_k_adamw_f32(int bits, size_t count, const lmp_adamw_tensor* t
       return fail(LMP_ERR_INVALID, which + "states of 8 bits need their scales");
     if (t.n > (uint64_t(1) << 35))
       return fail(LMP_ERR_UNSUPPORTED, which + "more than 2^35 values");
+  }
+  try {  // host memory can run out; no exception crosses the C boundary
+    Written pair[2];
+    if (find_overlap(bits, count, tensors, pair))
+      return fail(LMP_ERR_INVALID, std::string(name) + "buffers that the step writes overlap: of tensors " +
+                                       std::to_string(std::min(pair[0].tensor, pair[1].tensor)) + " and " +
+                                       std::to_string(std::max(pair[0].tensor, pair[1].tensor)));
+  } catch (const std::exception& e) {
+    return fail(LMP_ERR_OOM, std::string(name) + e.what());
   }
   LMP_RUNTIME_OR_FAIL(rt);
   AdamWArgs a{};

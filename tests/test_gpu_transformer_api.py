@@ -276,3 +276,35 @@ def test_example_trains_and_continues(rsl):
     for end, (token,) in zip((12, 17), first):
         top = np.sort(probs[end - 1])
         assert token == probs[end - 1].argmax() or top[-1] - top[-2] < 1e-4
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_takes_a_shared_parameter_once(rsl, bits):
+    """A layer that hangs in a module twice: one state and one update for each of its parameters, bit for bit those of a
+    list without repetitions."""
+    from rushlite_amd.nets import layers
+    x = np.random.default_rng(0).standard_normal((8, 300)).astype(np.float32)
+
+    class Tied(rsl.Module):
+        def __init__(self):
+            super().__init__()
+            rsl.manual_seed(3)
+            self.first = layers.Linear(300, 300)
+            self.again, self.norm, self.weights = self.first, layers.LayerNorm(300), self.first.weights
+
+        def forward(self, x):
+            return self.again(self.norm(self.first(x)))
+
+    nets = [Tied(), Tied()]
+    opts = [rsl.optim.AdamW(nets[0], lr=1e-2, bits=bits, seed=4),
+            rsl.optim.AdamW([nets[1].first.weights, nets[1].first.bias, nets[1].norm.weights, nets[1].norm.bias], lr=1e-2,
+                            bits=bits, seed=4)]
+    assert len(list(nets[0].parameters())) == 7 and len(opts[0].params) == 4
+    for _ in range(3):
+        for net, opt in zip(nets, opts):
+            opt.zero_grad()
+            (net(rsl.Variable(x)) * 0.01).sum(1).sum(0).backward()
+            opt.step()
+        for a, b in zip(*(net.parameters() for net in nets)):
+            assert np.array_equal(a.numpy(), b.numpy())

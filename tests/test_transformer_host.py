@@ -158,3 +158,50 @@ def test_plain_forms_against_differences():
                 down = fn()
                 a[i] = old
                 assert abs((up - down) / 2e-5 - grad[i]) < 1e-7
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("field,text", [
+    ("p", "tensors 0 and 1"), ("m", "tensors 0 and 1"), ("v", "tensors 0 and 1"), ("m_scale", "tensors 0 and 1"),
+    ("v_scale", "tensors 0 and 1"), ("own", "tensors 1 and 1")])
+def test_adamw_refuses_buffers_that_overlap(L, bits, field, text):
+    """One buffer in two entries, or in one entry twice, from its start or from within it; neighbours do not overlap.  600
+    values: states of 2400 or 600 bytes, three scales."""
+    from rushlite_amd import abi
+    if bits == 32 and "scale" in field:
+        pytest.skip("states of 32 bits have no scales")
+
+    def call(*tensors):
+        args = ctypes.cast((abi.AdamWTensor * len(tensors))(*tensors), ctypes.c_void_p)
+        return L.lmp_k_adamw_f32(bits, len(tensors), args, 1e-3, 0.9, 0.999, 1e-8, 1, P)
+
+    names = [n for n, _ in abi.AdamWTensor._fields_]
+    size = dict(p=2400, g=2400, m=2400 if bits == 32 else 600, v=2400 if bits == 32 else 600, m_scale=12, v_scale=12)
+    # one after another without room between them
+    at, both = 1 << 20, []
+    for _ in range(2):
+        t = {}
+        for name, n in size.items():
+            t[name] = at
+            at += n
+        both.append(t)
+    make = lambda t: abi.AdamWTensor(*[t[n] for n in names[:6]], 600, 0.0)  # noqa: E731
+    status = call(*map(make, both))
+    assert status != abi.OK and "overlap" not in L.lmp_rt_last_error().decode()  # there is no device
+    for shift in (0, size["p" if field == "own" else field] - 4):
+        bad = dict(both[1])
+        if field == "own":
+            bad["m"] = bad["p"] + shift
+        else:
+            bad[field] = both[0][field] + shift
+        refused(abi, call(make(both[0]), make(bad)), abi.ERR_INVALID, text)
+    # what has no values holds no memory
+    empty = abi.AdamWTensor(*[both[0][n] for n in names[:6]], 0, 0.0)
+    assert call(make(both[0]), empty) != abi.OK and "overlap" not in L.lmp_rt_last_error().decode()
+
+
+def test_adamw_refuses_two_variables_over_one_buffer():
+    import rushlite_amd as rsl
+    x = rsl.Variable(np.ones(3, np.float32), True, rsl.device.cpu)
+    with pytest.raises(ValueError, match="same memory"):
+        rsl.optim.AdamW([x, rsl.Variable(x.data, True)])
