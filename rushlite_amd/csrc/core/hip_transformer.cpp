@@ -64,7 +64,8 @@ void adamw_hip(int bits, const std::vector<AdamWParam>& params, const AdamWHyper
   std::vector<lmp_adamw_tensor> list;
   list.reserve(params.size());
   for (const AdamWParam& p : params) {
-    for (const Tensor* t : {&p.p, &p.m, &p.v, &p.m_scale, &p.v_scale})
+    // The gradient too: formed before the capture, nothing else may hold it at a replay.
+    for (const Tensor* t : {&p.p, &p.g, &p.m, &p.v, &p.m_scale, &p.v_scale})
       if (t->defined()) keep_for_graph(detail::UnsafeTensorAccessor::getImpl(*t));
     list.push_back({f32(p.p), f32(p.g), at(p.m), at(p.v), f32(p.m_scale), f32(p.v_scale),
                     p.p.numel(), p.decay});

@@ -308,3 +308,33 @@ def test_adamw_takes_a_shared_parameter_once(rsl, bits):
             opt.step()
         for a, b in zip(*(net.parameters() for net in nets)):
             assert np.array_equal(a.numpy(), b.numpy())
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_recorded_update_keeps_the_gradients_it_reads(rsl, bits):
+    """Only the update is recorded, after an eager backward pass; the gradients go, their memory would be another tensor's.
+    Every replay is the eager update by the same gradients."""
+    rng = np.random.default_rng(6)
+    p_np, g_np = rng.standard_normal((2, 300, 41)).astype(np.float32)
+
+    def build():
+        p = rsl.Variable(p_np, True)
+        opt = rsl.optim.AdamW([p], lr=1e-2, bits=bits, seed=3)
+        (p * rsl.Variable(g_np)).sum(1).sum(0).backward()
+        return p, opt
+
+    (eager, eager_opt), (kept, kept_opt) = build(), build()
+    graph = rsl.hip.Graph()
+    with graph.capture():
+        kept_opt.step()
+    assert kept_opt.steps == 0
+    kept_opt.zero_grad()
+    others = [rsl.Variable(np.full((300, 41), 1e6, np.float32)) for _ in range(8)]
+    for i in range(4):
+        graph.replay()
+        eager_opt.step()
+        assert np.array_equal(kept.numpy(), eager.numpy()), i
+        others.append(rsl.Variable(np.full((300, 41), -1e6, np.float32)))
+    assert kept_opt.steps == 4
+    assert all((abs(o.numpy()) == 1e6).all() for o in others)
