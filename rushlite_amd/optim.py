@@ -27,16 +27,19 @@ class AdamW:
     """p = p (1 - lr weight_decay) - lr m^ / (sqrt(v^) + eps), with m and v the running means of the gradient and its
     square and m^, v^ corrected for their start at zero.
 
-    `params`: a Module, or an iterable of Variables with requires_grad, float32 on the HIP device; a Variable that comes
-    more than once, as those of a shared layer do, is one parameter.  `weight_decay`: a number, or a function of a
-    parameter that returns one (biases and norms are often left out).  `bits`: 32 or 8.
+    `params`: a Module, whose frozen parameters (requires_grad off) are left as they are, or an iterable of Variables with
+    requires_grad; float32 on the HIP device.  A Variable that comes more than once, as those of a shared layer do, is one
+    parameter.  `weight_decay`: a number, or a function of a parameter that returns one (biases and norms are often left
+    out).  `bits`: 32 or 8.
     `seed` chooses the random bits that 8-bit states are rounded with."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, seed=0):
         if bits not in (8, 32):
             raise ValueError(f"AdamW: states have 32 or 8 bits, not {bits}")
         found, memory = {}, {}
-        for i, p in enumerate(params.parameters() if isinstance(params, Module) else params):
+        if isinstance(params, Module):
+            params = [p for p in params.parameters() if p.requires_grad]
+        for i, p in enumerate(params):
             if not isinstance(p, _C.Variable) or not p.requires_grad:
                 raise ValueError(f"AdamW: parameter {i} is not a Variable that requires a gradient")
             if _C._variable_id(p) in found:

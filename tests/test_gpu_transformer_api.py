@@ -338,3 +338,23 @@ def test_recorded_update_keeps_the_gradients_it_reads(rsl, bits):
         others.append(rsl.Variable(np.full((300, 41), -1e6, np.float32)))
     assert kept_opt.steps == 4
     assert all((abs(o.numpy()) == 1e6).all() for o in others)
+
+
+@gpu
+def test_adamw_leaves_frozen_parameters_of_a_module(rsl):
+    from rushlite_amd.nets import layers
+    rsl.manual_seed(1)
+    net = layers.SelfAttention(32, 2)
+    net.qkv.weights = rsl.Variable(net.qkv.weights.data)
+    frozen = net.qkv.weights.numpy().copy()
+    opt = rsl.optim.AdamW(net, lr=0.1)
+    assert len(opt.params) == 3 and all(p.requires_grad for p in opt.params)
+    before = [p.numpy().copy() for p in opt.params]
+    (net(rsl.Variable(np.random.default_rng(2).standard_normal((9, 32)).astype(np.float32)), net.plan([9])) * 0.1) \
+        .sum(1).sum(0).backward()
+    opt.step()
+    opt.zero_grad()
+    assert np.array_equal(net.qkv.weights.numpy(), frozen)
+    assert all((p.numpy() != b).any() for p, b in zip(opt.params, before))
+    with pytest.raises(ValueError, match="parameter 0 is not a Variable that requires a gradient"):
+        rsl.optim.AdamW(list(net.parameters()))

@@ -205,3 +205,20 @@ def test_adamw_refuses_two_variables_over_one_buffer():
     x = rsl.Variable(np.ones(3, np.float32), True, rsl.device.cpu)
     with pytest.raises(ValueError, match="same memory"):
         rsl.optim.AdamW([x, rsl.Variable(x.data, True)])
+
+
+def test_adamw_of_a_module_passes_over_frozen_parameters():
+    """What is refused here is the trained parameter's device."""
+    import rushlite_amd as rsl
+
+    class Half(rsl.Module):
+        def __init__(self):
+            super().__init__()
+            self.frozen = rsl.Variable(np.ones(3, np.float32), False, rsl.device.cpu)
+            self.trained = rsl.Variable(np.ones(3, np.float32), True, rsl.device.cpu)
+
+        def forward(self):
+            return self.frozen
+
+    with pytest.raises(ValueError, match="parameter 0 is not float32 on the HIP device"):
+        rsl.optim.AdamW(Half())
