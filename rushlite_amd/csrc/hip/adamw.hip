@@ -33,7 +33,7 @@
 namespace lmp_hip {
 namespace {
 
-constexpr int kTensors = 48;  // a launch's list: 48 x 60 bytes, inside the 4 KiB of arguments
+constexpr int kTensors = 48;  // a launch's list: 48 x 64 bytes, inside the 4 KiB of arguments
 constexpr int kThreads = 256;
 // Chunks of UNITS units of four values a lane: four units, whose loads are all on
 // their way at once, or one where four would leave compute units idle (17 thousand
@@ -70,6 +70,7 @@ struct AdamWArgs {
   int64_t* step;
   int advance;  // the last workgroup to finish advances the step
 };
+static_assert(sizeof(AdamWArgs) <= 4096);
 
 __device__ __forceinline__ double power(double base, int64_t t) {
   double r = 1;
