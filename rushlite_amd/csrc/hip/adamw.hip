@@ -144,7 +144,7 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (
     c = c * c > t ? c - 1 : c;
     c = (c + 1) * (c + 1) <= t ? c + 1 : c;
     c = float(r[j]) * (1.0f / 65536) * (2 * c + 1) < t - c * c ? c + 1 : c;
-    if (Q == 255) c = c == 0 && t > 0 ? 1.0f : c;
+    if (Q == 255) c = c == 0 && x[j] > 0 ? 1.0f : c;  // t may underflow
     c = fminf(c, float(Q));
     const int code = x[j] < 0 ? -int(c) : int(c);
     packed |= uint32_t(code & 255) << (8 * j);

@@ -823,3 +823,17 @@ def test_attention_of_long_batches_weights_that_rise_by_less_than_a_bit(hip):
         one = (q[:, own], k[:, keys], v[:, keys], [n], [n], 1, 1, scale, True)
         for a, w, b, what in zip((o[:, own], lse[:, h:h + 1]), T.attention(*one), T.attention_bounds(*one), ("o", "lse")):
             close(a, w, b, what)
+
+
+def test_adamw_8_keeps_small_second_moments_above_zero(hip):
+    """A second moment far below its block's largest is kept as the least code, also where its share of that underflows
+    float32: 2^-110 beside 2^70."""
+    n = 256
+    g = np.full(n, 2.0 ** -50, np.float32)
+    g[9], g[40:50] = 2.0 ** 40, 0
+    zero = np.zeros(1, np.float32)
+    t = [up(hip, np.zeros(n, np.float32)), up(hip, g), Bytes(hip, np.zeros(n, np.int8)), Bytes(hip, np.zeros(n, np.uint8)),
+         up(hip, zero), up(hip, zero)]
+    adamw_call(hip, 8, [(t, n)], [0.0], up(hip, np.zeros(2, np.int64)))
+    want = np.where(g == 0, 0, np.where(g > 1, 255, 1))
+    assert np.array_equal(t[3].numpy(), want)
