@@ -73,7 +73,9 @@ typedef struct {
  * above zero never becomes zero.  M below 1e-30 is stored as 0, an infinite or
  * NaN M as NaN.  The 16 random bits of each code come from MurmurHash3's 32-bit
  * finalizer over (seed, t, the tensor's place in the list, the value's place):
- * the low half for m, the high half for v.  Equal calls give equal codes. */
+ * the low half for m, the high half for v.  Equal calls give equal codes.  With states
+ * of 8 bits the parameter's root and quotient are formed to a unit in their last places
+ * (correctly rounded with states of 32, and where eps is below 2^-39 / sqrt(1 - beta2)). */
 int lmp_k_adamw_f32(int bits, size_t count, const lmp_adamw_tensor* tensors, double lr,
                     double beta1, double beta2, double eps, uint64_t seed, int64_t* step);
 

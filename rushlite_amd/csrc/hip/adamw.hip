@@ -92,7 +92,7 @@ __device__ __forceinline__ uint32_t mixed(uint32_t x) {  // MurmurHash3's 32-bit
 // One value.  Each operation on the moments rounds once (no contraction), so that a
 // state in 8 bits is a function of its inputs alone.  FAST: the parameter's root and
 // quotient to a unit in their last places, where the arithmetic is what bounds the
-// kernel.
+// kernel; they take a v below float32's smallest normal for zero (fast_enough).
 template <bool FAST>
 __device__ __forceinline__ void step_one(const AdamWArgs& a, float keep, float size, float root,
                                          float g, float& p, float& m, float& v) {
@@ -162,7 +162,7 @@ constexpr float kUnitM = float(1.0 / (127 * 127)), kUnitV = float(1.0 / (255 * 2
 
 // STREAM: accesses with the nontemporal hint (38 million parameters: 197 us without,
 // 177 with).
-template <int BITS, int kUnits, bool STREAM>
+template <int BITS, int kUnits, bool STREAM, bool FAST>
 __global__ __launch_bounds__(kThreads) void adamw_step(AdamWArgs a) {
   __shared__ float factors[2];
   const int64_t t = a.step[0] + 1;
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kThreads) void adamw_step(AdamWArgs a) {
       for (int u = 0; u < kUnits; ++u) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          step_one<false>(a, keep, size, root, gv[u][j], pv[u][j], mv[u][j], vv[u][j]);
+          step_one<FAST>(a, keep, size, root, gv[u][j], pv[u][j], mv[u][j], vv[u][j]);
         store4(p, at_of(u), pv[u]);
         store4(m, at_of(u), mv[u]);
         store4(v, at_of(u), vv[u]);
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(kThreads) void adamw_step(AdamWArgs a) {
         for (int j = 0; j < 4; ++j) {
           mv[j] = decoded<true>(mc[u], j, ms[u] * kUnitM);
           vv[j] = decoded<false>(vc[u], j, vs[u] * kUnitV);
-          step_one<true>(a, keep, size, root, gv[u][j], pv[u][j], mv[j], vv[j]);
+          step_one<FAST>(a, keep, size, root, gv[u][j], pv[u][j], mv[j], vv[j]);
           if (at + j >= n) mv[j] = vv[j] = 0.0f;
           const uint32_t r = mixed(uint32_t(at + j) ^ key_here);
           lo16[j] = r & 0xFFFF;
@@ -349,6 +349,10 @@ __global__ __launch_bounds__(kThreads) void adamw_values(const uint8_t* codes, c
     }
   }
 }
+
+// Whether eps hides what the fast root and quotient take for zero: a v below 2^-126, whose
+// corrected root is below 2^-63 / sqrt(1 - beta2), against 2^-24 of eps.
+bool fast_enough(double eps, double beta2) { return eps >= 0x1p-39 / std::sqrt(1 - beta2); }
 
 // Two of the buffers that a step writes, if any two overlap: workgroups take them
 // without order, so an element that two entries hold would be stepped once or twice.
@@ -443,6 +447,7 @@ extern "C" int lmp_k_adamw_f32(int bits, size_t count, const lmp_adamw_tensor* t
   for (size_t i = 0; i < count; ++i) values += tensors[i].n;
   // Bytes of all tensors against the memory-side cache (kStreamBytes).
   const bool stream = values * (bits == 32 ? 16 : 10) >= kStreamBytes;
+  const bool fast = fast_enough(eps, beta2);
   const bool few = values <= uint64_t(rt->cu_count) * chunk_of(4);
   const int chunk = chunk_of(few ? 1 : 4);
   uint64_t chunks = 0;
@@ -451,8 +456,14 @@ extern "C" int lmp_k_adamw_f32(int bits, size_t count, const lmp_adamw_tensor* t
     a.chunks = uint32_t(chunks);
     const dim3 grid(uint32_t(std::min<uint64_t>(chunks, uint64_t(rt->cu_count) * kGroupsPerUnit)));
     const auto run = [&](auto kernel) { kernel<<<grid, dim3(kThreads), 0, rt->stream>>>(a); };
-    if (bits == 32) run(few ? adamw_step<32, 1, false> : stream ? adamw_step<32, 4, true> : adamw_step<32, 4, false>);
-    else run(few ? adamw_step<8, 1, false> : stream ? adamw_step<8, 4, true> : adamw_step<8, 4, false>);
+    if (bits == 32)
+      run(few      ? adamw_step<32, 1, false, false>
+          : stream ? adamw_step<32, 4, true, false>
+                   : adamw_step<32, 4, false, false>);
+    else if (!fast)
+      run(few ? adamw_step<8, 1, false, false> : adamw_step<8, 4, false, false>);
+    else
+      run(few ? adamw_step<8, 1, false, true> : stream ? adamw_step<8, 4, true, true> : adamw_step<8, 4, false, true>);
     LMP_LAUNCH_CHECK("adamw_step");
     return LMP_OK;
   };

@@ -837,3 +837,23 @@ def test_adamw_8_keeps_small_second_moments_above_zero(hip):
     adamw_call(hip, 8, [(t, n)], [0.0], up(hip, np.zeros(2, np.int64)))
     want = np.where(g == 0, 0, np.where(g > 1, 255, 1))
     assert np.array_equal(t[3].numpy(), want)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-38, 1e-20])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_tiny_gradients_without_eps(hip, bits, eps):
+    """The first step is lr g / (|g| + eps) whatever g's size: second moments of 1e-39, below float32's smallest normal.
+
+    v rounds to a multiple of 2^-149, off by 7e-7 of 1e-39 at most; its root by half of that.  Ten roundings of the step
+    besides, and two of p."""
+    n, lr = 700, 0.01
+    g = (1e-18 * (1 + np.arange(n) / n) * np.where(np.arange(n) % 3, 1, -1)).astype(np.float32)
+    t = [up(hip, np.ones(n, np.float32)), up(hip, g)]
+    if bits == 32:
+        t += [up(hip, np.zeros(n, np.float32)) for _ in range(2)]
+    else:
+        t += [Bytes(hip, np.zeros(n, np.int8)), Bytes(hip, np.zeros(n, np.uint8))]
+        t += [up(hip, np.zeros(3, np.float32)) for _ in range(2)]
+    adamw_call(hip, bits, [(t, n)], [0.0], up(hip, np.zeros(2, np.int64)), hyper={**HYPER, "lr": lr, "eps": eps})
+    want = 1 - lr * g.astype(np.float64) / (np.abs(g.astype(np.float64)) + eps)
+    close(t[0].numpy(), want, lr * (3.5e-7 + 10 * T.U32) + 2 * T.U32, "p")
