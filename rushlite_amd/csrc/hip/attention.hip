@@ -78,13 +78,15 @@ AttnArgs common_args(const AttentionPlan& plan, double scale) {
 }
 
 // Whether the split-fp16 kernels run a pass: where they take less time by what
-// both forms have to do.  The rates are a fit to 155 batches on this card (1 to
-// 2048 queries, 17 to 8192 keys, 1 to 32 heads of 32, 64 and 128): the form it
-// takes is 1% slower than the faster one on average, forward, and 2% backward.
-// Some of them, fp32 | split in us: forward, one sequence of 1024, 4 heads of 128,
-// 43 | 42; 16 heads, 89 | 52; 8 queries against 8 x 8192 keys, 32 heads on 4, 147 |
-// 302; 64 queries, 896 | 404; backward, one sequence of 256, 4 heads of 64, 28 |
-// 45; of 1024, 16 heads of 64 on 4, 244 | 91.
+// both forms have to do.  The rates are a fit to batches on this card.  Over 160 (8 to
+// 2048 queries, 64 to 8192 keys, 1 to 32 heads of 32, 64 and 128) the form it takes is
+// 0.7% slower than the faster one on average, forward, and 2.6% backward; at worst 1.26
+// times as slow, forward (4 sequences of 500, 16 heads of 32: 25 | 31), and 2.3
+// times, backward (8 queries against each of 8 x 1024 keys, 8 heads of 128: 216 | 95).
+// Others, fp32 | split in us: forward, one sequence of 1024, 4 heads of 128, 42 | 38;
+// 16 heads on 4, 89 | 42; 8 queries against 8 x 8192 keys, 32 heads on 4, 149 | 304; 64
+// queries, 895 | 400; backward, one sequence of 256, 4 heads of 64, 27 | 43; of 1024, 16
+// heads of 64 on 4, 220 | 75; 8 queries against 8 x 8192 keys, 32 heads on 4, 1246 | 880.
 bool split_form(const AttentionPlan& plan, double scale, bool back) {
   const double q_tiles = double(plan.q_tiles.count) * double(plan.heads),
                k_tiles = double(plan.k_tiles.count) * double(plan.kv_heads);

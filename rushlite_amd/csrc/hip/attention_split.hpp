@@ -14,7 +14,8 @@
 // powers of two go into the factors of the scores and weights, which are exact.
 // A tile with an infinity or a NaN, with a largest value outside [2^-60, 2^41) or
 // with rows more than 2^12 apart is marked, and the sequence's key head is left
-// to the fp32 kernels (attention_f32.hpp), which run over the marked ones only.
+// to the fp32 kernels (attention_f32.hpp), which run over the marked ones only (one
+// such row of the output gradient: 8192 positions backward 20.8 ms for 3.0).
 // Weights take a power of two per row that follows its largest so far: of P times the
 // value tile's own in the forward pass, so that a tile of large values which hardly
 // weigh leaves the others their digits; of P and dS in the backward pass, per query (dq)
@@ -32,10 +33,11 @@
 //   dk, dv   S = Q K^T,   dP = dO V^T,   dV^T += dO^T P, dK^T += Q^T dS   one key
 //
 // Measured, one causal sequence of 8192, 16 heads of 128 (key heads of four
-// each): forward 0.80 ms = 343 TFLOP/s of fp32 products = 1.03 PFLOP/s of fp16, dq
+// each): forward 0.82 ms = 336 TFLOP/s of fp32 products = 1.01 PFLOP/s of fp16 (0.80 ms
+// without the two comparisons a step that keep large scores and large values sound), dq
 // 1.18 ms = 1.05, dk and dv 1.72 ms = 0.96, where a library's fp16 product of 8192^3 does
 // 1.09 on the same card; the fp32 kernels took 22 ms for all of it.  The matrix
-// cores are busy 52, 49 and 44% of the cycles, and the clock falls by a sixth under
+// cores are busy 51, 49 and 44% of the cycles, and the clock falls by a sixth under
 // them in a loop of calls: power bounds it as much as the waits at the steps' barriers.
 #pragma once
 
