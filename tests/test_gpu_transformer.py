@@ -857,3 +857,14 @@ def test_adamw_of_tiny_gradients_without_eps(hip, bits, eps):
     adamw_call(hip, bits, [(t, n)], [0.0], up(hip, np.zeros(2, np.int64)), hyper={**HYPER, "lr": lr, "eps": eps})
     want = 1 - lr * g.astype(np.float64) / (np.abs(g.astype(np.float64)) + eps)
     close(t[0].numpy(), want, lr * (3.5e-7 + 10 * T.U32) + 2 * T.U32, "p")
+
+
+@pytest.mark.parametrize("n", [(1 << 21) + 5, (1 << 25) + 300])
+def test_adamw_8_of_tiny_gradients_in_long_tensors(hip, n):
+    """As above, with states of 8 bits and eps 0, past the sizes at which a lane takes four units and accesses stream."""
+    lr = 0.01
+    g = np.resize((1e-18 * np.where(np.arange(256) % 3, 1, -1)).astype(np.float32), n)
+    t = [up(hip, np.ones(n, np.float32)), up(hip, g), Bytes(hip, np.zeros(n, np.int8)), Bytes(hip, np.zeros(n, np.uint8))]
+    t += [up(hip, np.zeros(-(-n // 256), np.float32)) for _ in range(2)]
+    adamw_call(hip, 8, [(t, n)], [0.0], up(hip, np.zeros(2, np.int64)), hyper={**HYPER, "lr": lr, "eps": 0.0})
+    close(t[0].numpy(), 1 - lr * np.sign(g.astype(np.float64)), lr * (7e-7 + 10 * T.U32) + 2 * T.U32, "p")
