@@ -1,6 +1,7 @@
 /*
  * lmp_hip_transformer.h -- C ABI of the transformer-training operators of
- * liblmp_hip.so: layer normalisation, the AdamW step and packed attention.
+ * liblmp_hip.so: layer normalisation, the AdamW step, packed attention, rotary
+ * positions, dropout, gated linear layers and cross entropy over a vocabulary.
  *
  * The reference has none of these; they follow the conventions of lmp_hip.h:
  * every entry point returns an lmp_status and leaves its message in
@@ -130,6 +131,94 @@ int lmp_k_attention_backward_f32(const void* plan, const float* q, size_t q_ld, 
                                  const float* o, size_t o_ld, const float* lse, const float* g,
                                  size_t g_ld, float* dq, size_t dq_ld, float* dk, size_t dk_ld,
                                  float* dv, size_t dv_ld);
+
+/* ------------------------------------------------------- rotary positions */
+
+/* y = x with the pairs of its first `heads` vectors of each row turned by the row's
+ * position.  A row has `cols` values: the vectors of head_dim values one after another,
+ * then what is copied as it is (the values of a projection to queries, keys and values).
+ * Of each vector the first rotary_dim values (even, head_dim at most) turn and the others
+ * are copied: pair j, at values (j, j + rotary_dim / 2) or with interleaved != 0 at
+ * (2 j, 2 j + 1), becomes
+ *   scale (u cos a - v sin a, v cos a + u sin a),  a = positions[row] * frequencies[j],
+ * with inverse != 0 by -a: the gradient of the same call.  dtype is LMP_FLOAT32 or
+ * LMP_FLOAT64 for x and y; positions (int64) and frequencies (float64, rotary_dim / 2
+ * radians per position) are on the device.  Angles are formed in 64 bits: for float32 a
+ * turned value errs by 2^-20 of its pair's larger one, and besides by |a| 2^-51 of both.
+ * y may be x with the same leading dimension, or rows beside x's; another overlap is
+ * refused. */
+int lmp_k_rotary(int dtype, size_t rows, size_t cols, size_t heads, size_t head_dim,
+                 size_t rotary_dim, int interleaved, const void* x, size_t ldx,
+                 const int64_t* positions, const double* frequencies, double scale, int inverse,
+                 void* y, size_t ldy);
+
+/* ---------------------------------------------------------------- dropout */
+
+/* y = residual + (kept ? x / (1 - rate) : 0) over n contiguous values (residual null: 0),
+ * rate in [0, 1].  What is kept comes from Philox4x32-10 with the seed's halves as its key
+ * and (place / 4, number of the call), low halves first, as its counter: value i takes word
+ * i % 4 and is kept if that is at least rate * 2^32 (rounded).  `state` is two int64 on the
+ * device: state[0] the number of this call, which the call advances by one, state[1] the
+ * library's, 0 before the first call.  Keeping it on the device lets a recorded call draw
+ * afresh at every replay.  `used` (one int64 on the device, or null where no backward pass
+ * follows) takes the number of this call.  What is dropped, infinities and NaN too, leaves
+ * no trace.  y may be x or residual. */
+int lmp_k_dropout(int dtype, size_t n, const void* x, const void* residual, double rate,
+                  uint64_t seed, int64_t* state, int64_t* used, void* y);
+
+/* dx = kept ? g / (1 - rate) : 0 by what the call numbered *used kept (the residual's
+ * gradient is g).  dx may be g. */
+int lmp_k_dropout_backward(int dtype, size_t n, const void* g, double rate, uint64_t seed,
+                           const int64_t* used, void* dx);
+
+/* ----------------------------------------------------------- gated linear */
+
+typedef enum {
+  LMP_GATE_SILU = 0,      /* a / (1 + e^-a) */
+  LMP_GATE_GELU = 1,      /* a Phi(a), Phi the normal distribution's */
+  LMP_GATE_GELU_TANH = 2, /* a / 2 (1 + tanh(sqrt(2 / pi) (a + 0.044715 a^3))) */
+  LMP_GATE_RELU = 3,      /* max(a, 0); its slope at 0 is 0 */
+  LMP_GATE_SIGMOID = 4,   /* 1 / (1 + e^-a) */
+  LMP_GATE_COUNT = 5
+} lmp_gate;
+
+/* h = act(a) u for [a | u] = x w + bias: x [rows, in], w [in, 2 hidden] whose first
+ * `hidden` columns are the gate's, bias 2 hidden values or null (0), h [rows, hidden].
+ * pre [rows, 2 hidden] takes [a | u] for the backward pass (null where none follows).
+ * in and hidden are positive.  Outputs do not overlap operands, here and below. */
+int lmp_k_gated_linear_f32(int gate, size_t rows, size_t in, size_t hidden, const float* x,
+                           size_t ldx, const float* w, size_t ldw, const float* bias, float* h,
+                           size_t ldh, float* pre, size_t ldpre);
+
+/* The gradients from the output gradient g [rows, hidden] and the pre that the forward call
+ * wrote: with d = [g u act'(a) | g act(a)], dx = d w^T, dw = x^T d and db the column sums
+ * of d.  Each of dx, dw and db may be null where it is not wanted (x is read for dw, w for
+ * dx). */
+int lmp_k_gated_linear_backward_f32(int gate, size_t rows, size_t in, size_t hidden,
+                                    const float* g, size_t ldg, const float* x, size_t ldx,
+                                    const float* w, size_t ldw, const float* pre, size_t ldpre,
+                                    float* dx, size_t lddx, float* dw, size_t lddw, float* db);
+
+/* -------------------------------------- cross entropy over a vocabulary */
+
+/* loss[i] = log sum_v exp(z_iv) - z_i,t of z = x w + bias: x [rows, in], w [in, vocab],
+ * bias vocab values or null (0), t = targets[i] (int64, on the device).  A row whose target
+ * is negative is not counted: its loss is 0, whatever it holds.  A target of vocab or more
+ * makes its row's loss NaN.  A logit of -inf has no share; a row of nothing else has the loss
+ * NaN.  The logits are formed in pieces and never held whole.  in and vocab are positive. */
+int lmp_k_linear_cross_entropy_f32(size_t rows, size_t in, size_t vocab, const float* x,
+                                   size_t ldx, const float* w, size_t ldw, const float* bias,
+                                   const int64_t* targets, float* loss);
+
+/* The losses and, of sum_i weights[i] loss[i] (weights null: 1 each), the gradients dx
+ * [rows, in], dw [in, vocab] and db (vocab values), each null where it is not wanted (db
+ * only with dw).  A row that is not counted has no part in them, whatever it and its weight
+ * hold. */
+int lmp_k_linear_cross_entropy_grad_f32(size_t rows, size_t in, size_t vocab, const float* x,
+                                        size_t ldx, const float* w, size_t ldw,
+                                        const float* bias, const int64_t* targets,
+                                        const float* weights, float* loss, float* dx,
+                                        size_t lddx, float* dw, size_t lddw, float* db);
 
 #ifdef __cplusplus
 }

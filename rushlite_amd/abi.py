@@ -61,6 +61,7 @@ class PoolStats(C.Structure):
 
 ADAMW_BLOCK = 256  # values that share one scale of an 8-bit state
 ATTENTION_MAX_DIM = 256
+GATE = dict(silu=0, gelu=1, gelu_tanh=2, relu=3, sigmoid=4)
 
 
 class AdamWTensor(C.Structure):
@@ -137,6 +138,15 @@ TRANSFORMER_SIGNATURES = {
     "lmp_k_attention_f32": (_i, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _d, _vp, _sz, _vp]),
     "lmp_k_attention_backward_f32": (_i, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _d, _vp, _sz, _vp,
                                           _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz]),
+    "lmp_k_rotary": (_i, [_i, _sz, _sz, _sz, _sz, _sz, _i, _vp, _sz, _vp, _vp, _d, _i, _vp, _sz]),
+    "lmp_k_dropout": (_i, [_i, _sz, _vp, _vp, _d, C.c_uint64, _vp, _vp, _vp]),
+    "lmp_k_dropout_backward": (_i, [_i, _sz, _vp, _d, C.c_uint64, _vp, _vp]),
+    "lmp_k_gated_linear_f32": (_i, [_i, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _sz]),
+    "lmp_k_gated_linear_backward_f32": (_i, [_i, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp,
+                                             _sz, _vp, _sz, _vp, _sz, _vp]),
+    "lmp_k_linear_cross_entropy_f32": (_i, [_sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp]),
+    "lmp_k_linear_cross_entropy_grad_f32": (_i, [_sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp,
+                                                 _vp, _vp, _sz, _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,59 @@
+// The gates of a gated linear layer: act(a) and act'(a) in float32.
+//
+//   silu       a s(a)                        s the logistic function
+//   gelu       a Phi(a)                      Phi the normal distribution's
+//   gelu_tanh  a s(2 c (a + k a^3))          c = sqrt(2 / pi), k = 0.044715: a / 2 (1 + tanh(c (a + k a^3)))
+//   relu       max(a, 0)
+//   sigmoid    s(a)
+//
+// s(v) = 1 / (1 + e^-v) and 1 - s(v) = 1 / (1 + e^v) are formed each by itself, and Phi from
+// the complementary error function, so that small values keep their digits.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "lmp_hip_transformer.h"
+
+namespace lmp_hip {
+namespace {
+
+// The larger of s(v) and s(-v) is 1 / (1 + e^-|v|), the smaller e^-|v| times that.
+__device__ __forceinline__ void logistic(float v, float& s, float& rest) {
+  const float e = expf(-fabsf(v)), big = 1.0f / (1.0f + e), small = e * big;
+  s = v < 0 ? small : big;
+  rest = v < 0 ? big : small;
+}
+
+__device__ __forceinline__ void gate_of(int gate, float a, float& act, float& slope) {
+  constexpr float kTwoC = 1.5957691216057308f, kCube = 0.044715f;
+  float s, rest;
+  switch (gate) {
+    case LMP_GATE_SILU:
+      logistic(a, s, rest);
+      act = a * s;
+      slope = s + act * rest;
+      return;
+    case LMP_GATE_GELU:
+      s = 0.5f * erfcf(a * -0.70710678118654752f);
+      act = a * s;
+      slope = s + a * expf(a * a * -0.5f) * 0.39894228040143268f;
+      return;
+    case LMP_GATE_GELU_TANH:
+      logistic(a * kTwoC * (1.0f + kCube * a * a), s, rest);
+      act = a * s;
+      slope = s + act * rest * (kTwoC * (1.0f + 3.0f * kCube * a * a));
+      return;
+    case LMP_GATE_RELU:
+      act = a < 0.0f ? 0.0f : a;
+      slope = a > 0.0f ? 1.0f : 0.0f;
+      return;
+    default:
+      logistic(a, s, rest);
+      act = s;
+      slope = s * rest;
+      return;
+  }
+}
+
+}  // namespace
+}  // namespace lmp_hip
