@@ -25,9 +25,11 @@ from .grad_mode import no_grad
 from .graphs import Graph as _Graph
 from . import optim
 from .nets.Module import Module
+from .random import Generator, dropout
 
 # rsl.hip.Graph (and its rsl.cuda alias): whole-step HIP graphs.
 hip.Graph = _Graph  # noqa: F405
 cuda.Graph = _Graph  # noqa: F405
 
-__all__ = ["Variable", "Module", "capture_on", "capture", "no_grad", "optim"]
+__all__ = ["Variable", "Module", "capture_on", "capture", "no_grad", "optim", "Generator",
+           "dropout"]

@@ -4,6 +4,7 @@
 
 #include <cmath>
 #include <optional>
+#include <string>
 
 #include "transformer.hpp"
 
@@ -69,6 +70,56 @@ void bind_transformer(py::module_& m) {
       py::arg("rows"), py::arg("plan"), py::arg("scale") = py::none(),
       "attention() with q, k and v side by side in the rows of one projection: "
       "[queries, (heads + 2 kv_heads) * head_dim].");
+
+  m.def(
+      "rotary",
+      [](const Variable& x, const Variable& positions, const Tensor& frequencies, int64_t heads,
+         int64_t head_dim, bool interleaved, Scalar scale) {
+        if (heads < 0 || head_dim < 0) throw py::value_error("rotary: negative heads or head_dim");
+        return ag::ops::rotary(x, positions.data(), frequencies,
+                               {size_t(heads), size_t(head_dim), interleaved, scale});
+      },
+      py::arg("x"), py::arg("positions"), py::arg("frequencies"), py::kw_only(), py::arg("heads"),
+      py::arg("head_dim"), py::arg("interleaved") = false, py::arg("scale") = 1.0,
+      "x [rows, columns] with the pairs of its first heads * head_dim columns turned by "
+      "positions[row] * frequencies[pair]; layers.Rotary holds the frequencies.");
+  m.def(
+      "_dropout",
+      [](const Variable& x, const Variable* residual, Scalar rate, uint64_t seed, Tensor state) {
+        return ag::ops::dropout(x, residual, rate, seed, state);
+      },
+      py::arg("x"), py::arg("residual").none(true), py::arg("rate"), py::arg("seed"),
+      py::arg("state"));
+  m.def(
+      "gated_linear",
+      [](const Variable& x, const Variable& w, const Variable* b, const std::string& gate) {
+        static const char* const names[] = {"silu", "gelu", "gelu_tanh", "relu", "sigmoid"};
+        for (int i = 0; i < 5; ++i)
+          if (gate == names[i]) return ag::ops::gated_linear(x, w, b, i);
+        throw py::value_error("gated_linear: unknown gate '" + gate +
+                              "' (silu, gelu, gelu_tanh, relu or sigmoid)");
+      },
+      py::arg("x"), py::arg("w"), py::arg("b").none(true) = py::none(), py::arg("gate") = "silu",
+      "act(a) * u for [a | u] = x @ w + b: the gate's columns of w first, then as many more.");
+  m.def(
+      "linear_cross_entropy",
+      [](const Variable& x, const Variable& w, const Variable* b, const Variable& targets,
+         const Variable* weights) {
+        return ag::ops::linear_cross_entropy(x, w, b, targets.data(),
+                                             weights ? weights->data() : Tensor());
+      },
+      py::arg("x"), py::arg("w"), py::arg("b").none(true), py::arg("targets"),
+      py::arg("weights").none(true) = py::none(),
+      "The softmax cross entropies of the rows of x @ w + b against targets (int64; a negative one "
+      "is not counted), summed with weights (finite) or averaged over what counts, of shape [1].  "
+      "The logits are never held whole, and the gradients are formed with the losses.");
+  m.def(
+      "linear_cross_entropy_rows",
+      [](const Variable& x, const Variable& w, const Variable* b, const Variable& targets) {
+        return Variable(ag::ops::linear_cross_entropy_rows(x, w, b, targets.data()), false);
+      },
+      py::arg("x"), py::arg("w"), py::arg("b").none(true), py::arg("targets"),
+      "The cross entropy of each row, without a gradient (scoring).");
 
   // One AdamW step over lists of tensors (optim.AdamW): per parameter (p, g, m,
   // v, m_scale, v_scale, decay), the scales None for states of 32 bits.

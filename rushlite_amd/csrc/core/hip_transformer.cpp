@@ -85,6 +85,79 @@ Tensor adamw_decode_hip(bool signed_codes, const Tensor& codes, const Tensor& sc
   return out;
 }
 
+Tensor rotary_hip(const Tensor& x, const Tensor& positions, const Tensor& frequencies,
+                  const RotaryShape& r, bool inverse) {
+  Tensor y = empty(x.shape(), x.device(), x.type());
+  const size_t rows = x.shape()[0], cols = x.shape()[1];
+  if (x.numel()) count_launch();
+  hip_ok(lmp_k_rotary(int(x.type()), rows, cols, r.heads, r.head_dim, 2 * frequencies.numel(),
+                      r.interleaved ? 1 : 0, at(x), cols, static_cast<const int64_t*>(at(positions)),
+                      static_cast<const double*>(at(frequencies)), r.scale, inverse ? 1 : 0, at(y),
+                      cols),
+         "lmp_k_rotary");
+  return y;
+}
+
+Tensor dropout_hip(const Tensor& x, const Tensor& residual, Scalar rate, uint64_t seed,
+                   Tensor& state, Tensor* used) {
+  Tensor y = empty(x.shape(), x.device(), x.type());
+  count_launch();
+  hip_ok(lmp_k_dropout(int(x.type()), x.numel(), at(x), at(residual), rate, seed,
+                       static_cast<int64_t*>(at(state)), static_cast<int64_t*>(at(*used)), at(y)),
+         "lmp_k_dropout");
+  return y;
+}
+
+Tensor dropout_backward_hip(const Tensor& g, Scalar rate, uint64_t seed, const Tensor& used) {
+  Tensor dx = empty(g.shape(), g.device(), g.type());
+  if (g.numel()) count_launch();
+  hip_ok(lmp_k_dropout_backward(int(g.type()), g.numel(), at(g), rate, seed,
+                                static_cast<const int64_t*>(at(used)), at(dx)),
+         "lmp_k_dropout_backward");
+  return dx;
+}
+
+GatedOut gated_linear_hip(int gate, const Tensor& x, const Tensor& w, const Tensor& bias,
+                          bool keep) {
+  const size_t rows = x.shape()[0], in = x.shape()[1], width = w.shape()[1];
+  GatedOut out{empty({rows, width / 2}, x.device(), x.type()), {}};
+  if (keep) out.pre = empty({rows, width}, x.device(), x.type());
+  if (rows) count_launch();
+  hip_ok(lmp_k_gated_linear_f32(gate, rows, in, width / 2, f32(x), in, f32(w), width, f32(bias),
+                                f32(out.h), width / 2, f32(out.pre), width),
+         "lmp_k_gated_linear_f32");
+  return out;
+}
+
+void gated_linear_backward_hip(int gate, const Tensor& g, const Tensor& x, const Tensor& w,
+                               const Tensor& pre, Tensor* dx, Tensor* dw, Tensor* db) {
+  const size_t rows = x.shape()[0], in = x.shape()[1], width = w.shape()[1];
+  count_launch();
+  hip_ok(lmp_k_gated_linear_backward_f32(gate, rows, in, width / 2, f32(g), width / 2, f32(x), in,
+                                         f32(w), width, f32(pre), width, f32(*dx), in, f32(*dw),
+                                         width, f32(*db)),
+         "lmp_k_gated_linear_backward_f32");
+}
+
+Tensor linear_cross_entropy_hip(const Tensor& x, const Tensor& w, const Tensor& bias,
+                                const Tensor& targets, const Tensor& weights, Tensor* dx,
+                                Tensor* dw, Tensor* db) {
+  const size_t rows = x.shape()[0], in = x.shape()[1], vocab = w.shape()[1];
+  Tensor loss = empty({rows}, x.device(), x.type());
+  const auto* t = static_cast<const int64_t*>(at(targets));
+  if (rows) count_launch();
+  if (weights.defined())
+    hip_ok(lmp_k_linear_cross_entropy_grad_f32(rows, in, vocab, f32(x), in, f32(w), vocab, f32(bias),
+                                               t, f32(weights), f32(loss), f32(*dx), in, f32(*dw),
+                                               vocab, f32(*db)),
+           "lmp_k_linear_cross_entropy_grad_f32");
+  else
+    hip_ok(lmp_k_linear_cross_entropy_f32(rows, in, vocab, f32(x), in, f32(w), vocab, f32(bias), t,
+                                          f32(loss)),
+           "lmp_k_linear_cross_entropy_f32");
+  return loss;
+}
+
 }  // namespace
 
 constexpr DeviceType kHip = DeviceType::HIP;
@@ -92,6 +165,12 @@ LMP_REGISTER_DISPATCH(layer_norm_stub, kHip, layer_norm_hip)
 LMP_REGISTER_DISPATCH(layer_norm_backward_stub, kHip, layer_norm_backward_hip)
 LMP_REGISTER_DISPATCH(attention_stub, kHip, attention_hip)
 LMP_REGISTER_DISPATCH(attention_backward_stub, kHip, attention_backward_hip)
+LMP_REGISTER_DISPATCH(rotary_stub, kHip, rotary_hip)
+LMP_REGISTER_DISPATCH(dropout_stub, kHip, dropout_hip)
+LMP_REGISTER_DISPATCH(dropout_backward_stub, kHip, dropout_backward_hip)
+LMP_REGISTER_DISPATCH(gated_linear_stub, kHip, gated_linear_hip)
+LMP_REGISTER_DISPATCH(gated_linear_backward_stub, kHip, gated_linear_backward_hip)
+LMP_REGISTER_DISPATCH(linear_cross_entropy_stub, kHip, linear_cross_entropy_hip)
 LMP_REGISTER_DISPATCH(adamw_stub, kHip, adamw_hip)
 LMP_REGISTER_DISPATCH(adamw_decode_stub, kHip, adamw_decode_hip)
 

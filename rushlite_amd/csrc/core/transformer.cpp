@@ -8,6 +8,12 @@ LMP_DEFINE_DISPATCH(layer_norm_fn, layer_norm_stub)
 LMP_DEFINE_DISPATCH(layer_norm_backward_fn, layer_norm_backward_stub)
 LMP_DEFINE_DISPATCH(attention_fn, attention_stub)
 LMP_DEFINE_DISPATCH(attention_backward_fn, attention_backward_stub)
+LMP_DEFINE_DISPATCH(rotary_fn, rotary_stub)
+LMP_DEFINE_DISPATCH(dropout_fn, dropout_stub)
+LMP_DEFINE_DISPATCH(dropout_backward_fn, dropout_backward_stub)
+LMP_DEFINE_DISPATCH(gated_linear_fn, gated_linear_stub)
+LMP_DEFINE_DISPATCH(gated_linear_backward_fn, gated_linear_backward_stub)
+LMP_DEFINE_DISPATCH(linear_cross_entropy_fn, linear_cross_entropy_stub)
 LMP_DEFINE_DISPATCH(adamw_fn, adamw_stub)
 LMP_DEFINE_DISPATCH(adamw_decode_fn, adamw_decode_stub)
 
@@ -207,6 +213,165 @@ Variable attention_qkv(const Variable& rows, const AttentionPlan& plan, Scalar s
                                                   out.grad(), slice(d, 0), slice(d, 1),
                                                   slice(d, 2));
                   in[0].incr_grad_owned(d);
+                });
+}
+
+Variable rotary(const Variable& x, const Tensor& positions, const Tensor& frequencies,
+                const tops::RotaryShape& shape) {
+  const Tensor& xt = x.data();
+  LMP_CHECK(xt.type() == DataType::Float32 || xt.type() == DataType::Float64)
+      << "rotary: x must be float32 or float64";
+  LMP_CHECK(xt.shape().size() == 2) << "rotary: x must have two axes, not " << xt.shape();
+  LMP_CHECK(positions.type() == DataType::Int64 && positions.numel() == xt.shape()[0] &&
+            positions.device() == xt.device())
+      << "rotary: positions must be int64 on x's device, one for each of its "
+      << xt.shape()[0] << " rows";
+  LMP_CHECK(frequencies.type() == DataType::Float64 && frequencies.device() == xt.device())
+      << "rotary: frequencies must be float64 on x's device";
+  LMP_CHECK(2 * frequencies.numel() <= shape.head_dim)
+      << "rotary: " << frequencies.numel() << " pairs do not fit heads of " << shape.head_dim;
+  // Inputs made before a capture are read at every replay.
+  for (const Tensor* t : {&positions, &frequencies})
+    tensor::keep_for_graph(tensor::detail::UnsafeTensorAccessor::getImpl(*t));
+  const Tensor y = tops::rotary_stub()(xt.device(), xt, positions, frequencies, shape, false);
+  return result(y, {x}, "RotaryBackward",
+                [positions, frequencies, shape](const Variable& out, variable_list& in) {
+                  in[0].incr_grad_owned(tops::rotary_stub()(out.data().device(), out.grad(),
+                                                            positions, frequencies, shape, true));
+                });
+}
+
+Variable dropout(const Variable& x, const Variable* residual, Scalar rate, uint64_t seed,
+                 Tensor state) {
+  const Tensor& xt = x.data();
+  LMP_CHECK(xt.type() == DataType::Float32 || xt.type() == DataType::Float64)
+      << "dropout: x must be float32 or float64";
+  LMP_CHECK(!residual || (residual->data().type() == xt.type() &&
+                          residual->data().device() == xt.device() &&
+                          residual->data().shape() == xt.shape()))
+      << "dropout: the residual must be of x's type, device and shape";
+  LMP_CHECK(state.type() == DataType::Int64 && state.numel() == 2 && state.device() == xt.device())
+      << "dropout: the generator is not on x's device";
+  variable_list ins{x};
+  if (residual) ins.push_back(*residual);
+  Tensor used;
+  if (x.requires_grad() && wants_grad(ins)) used = empty({1}, xt.device(), DataType::Int64);
+  tensor::keep_for_graph(tensor::detail::UnsafeTensorAccessor::getImpl(state));
+  const Tensor y = tops::dropout_stub()(xt.device(), xt, residual ? residual->data() : Tensor(),
+                                        rate, seed, state, &used);
+  return result(y, std::move(ins), "DropoutBackward",
+                [rate, seed, used](const Variable& out, variable_list& in) {
+                  if (in[0].requires_grad())
+                    in[0].incr_grad_owned(tops::dropout_backward_stub()(
+                        out.data().device(), out.grad(), rate, seed, used));
+                  if (in.size() > 1 && in[1].requires_grad()) in[1].incr_grad(out.grad());
+                });
+}
+
+namespace {
+
+// x [rows, in], w [in, width], b [width], all float32 on one device.
+void check_linear(const char* name, const Variable& x, const Variable& w, const Variable* b) {
+  const Tensor &xt = x.data(), &wt = w.data();
+  const auto fits = [&](const Tensor& t) {
+    return t.type() == DataType::Float32 && t.device() == xt.device();
+  };
+  LMP_CHECK(fits(xt) && fits(wt) && (!b || fits(b->data())))
+      << name << ": x, the weights and the bias must be float32 on one device";
+  LMP_CHECK(xt.shape().size() == 2 && wt.shape().size() == 2 && xt.shape()[1] == wt.shape()[0])
+      << name << ": x " << xt.shape() << " and weights " << wt.shape() << " do not multiply";
+  LMP_CHECK(!b || b->data().shape() == std::vector<size_t>{wt.shape()[1]})
+      << name << ": the bias must have " << wt.shape()[1] << " values";
+}
+
+}  // namespace
+
+Variable gated_linear(const Variable& x, const Variable& w, const Variable* b, int gate) {
+  check_linear("gated_linear", x, w, b);
+  LMP_CHECK(w.data().shape()[1] % 2 == 0)
+      << "gated_linear: the weights' columns are the gate's and as many more, not "
+      << w.data().shape()[1];
+  variable_list ins{x, w};
+  if (b) ins.push_back(*b);
+  const tops::GatedOut out = tops::gated_linear_stub()(
+      x.data().device(), gate, x.data(), w.data(), b ? b->data() : Tensor(), wants_grad(ins));
+  return result(out.h, std::move(ins), "GatedLinearBackward",
+                [gate, pre = out.pre](const Variable& h, variable_list& in) {
+                  Tensor d[3];
+                  for (size_t i = 0; i < in.size(); ++i)
+                    if (in[i].requires_grad()) d[i] = empty_like(in[i].data());
+                  tops::gated_linear_backward_stub()(h.data().device(), gate, h.grad(),
+                                                     in[0].data(), in[1].data(), pre, &d[0], &d[1],
+                                                     &d[2]);
+                  for (size_t i = 0; i < in.size(); ++i)
+                    if (d[i].defined()) in[i].incr_grad_owned(d[i]);
+                });
+}
+
+namespace {
+
+void check_targets(const Variable& x, const Tensor& targets, const Tensor& weights) {
+  const size_t rows = x.data().shape()[0];
+  LMP_CHECK(targets.type() == DataType::Int64 && targets.numel() == rows &&
+            targets.device() == x.data().device())
+      << "linear_cross_entropy: targets must be int64 on x's device, one for each of its " << rows
+      << " rows";
+  LMP_CHECK(!weights.defined() ||
+            (weights.type() == DataType::Float32 && weights.numel() == rows &&
+             weights.device() == x.data().device()))
+      << "linear_cross_entropy: weights must be float32 on x's device, one for each of its " << rows
+      << " rows";
+  LMP_CHECK(rows > 0) << "linear_cross_entropy: no rows";
+}
+
+}  // namespace
+
+Tensor linear_cross_entropy_rows(const Variable& x, const Variable& w, const Variable* b,
+                                 const Tensor& targets) {
+  check_linear("linear_cross_entropy", x, w, b);
+  check_targets(x, targets, Tensor());
+  tensor::keep_for_graph(tensor::detail::UnsafeTensorAccessor::getImpl(targets));
+  Tensor none;
+  return tops::linear_cross_entropy_stub()(x.data().device(), x.data(), w.data(),
+                                           b ? b->data() : Tensor(), targets, Tensor(), &none,
+                                           &none, &none);
+}
+
+Variable linear_cross_entropy(const Variable& x, const Variable& w, const Variable* b,
+                              const Tensor& targets, const Tensor& weights) {
+  check_linear("linear_cross_entropy", x, w, b);
+  check_targets(x, targets, weights);
+  const size_t rows = x.data().shape()[0];
+  for (const Tensor* t : {&targets, &weights})
+    if (t->defined())
+      tensor::keep_for_graph(tensor::detail::UnsafeTensorAccessor::getImpl(*t));
+  Tensor share;
+  if (weights.defined()) {
+    share = weights.reshape({rows});
+  } else {
+    const Tensor t = targets.reshape({rows});
+    const Tensor counted =
+        tops::ge(t, tensor::scalar_like(t, 0)) * tensor::scalar_like(x.data(), 1);
+    share = counted / tops::clamp(tops::sum(counted, 0), 1, double(rows));
+  }
+  variable_list ins{x, w};
+  if (b) ins.push_back(*b);
+  Tensor d[3];
+  const bool rg = wants_grad(ins);
+  if (rg) {
+    for (size_t i = 0; i < ins.size(); ++i)
+      if (ins[i].requires_grad()) d[i] = empty_like(ins[i].data());
+    // The bias' gradient rides with the weights'.
+    if (d[2].defined() && !d[1].defined()) d[1] = empty_like(w.data());
+  }
+  const Tensor loss = tops::linear_cross_entropy_stub()(
+      x.data().device(), x.data(), w.data(), b ? b->data() : Tensor(), targets,
+      rg ? share : Tensor(), &d[0], &d[1], &d[2]);
+  return result(tops::sum(tops::mul(loss, share), 0), std::move(ins), "LinearCrossEntropyBackward",
+                [d0 = d[0], d1 = d[1], d2 = d[2]](const Variable& out, variable_list& in) {
+                  const Tensor* d[3] = {&d0, &d1, &d2};
+                  for (size_t i = 0; i < in.size(); ++i)
+                    if (in[i].requires_grad()) in[i].incr_grad(tops::mul(*d[i], out.grad()));
                 });
 }
 

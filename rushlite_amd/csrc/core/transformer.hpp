@@ -1,6 +1,8 @@
 // Transformer-training operators over tensors and variables: layer norm, packed
-// attention and the AdamW step (include/lmp_hip_transformer.h).  The reference
-// has none of them; they run on the HIP device only, as every op here does.
+// attention, the AdamW step, rotary positions, dropout, gated linear layers and
+// the cross entropy over a vocabulary (include/lmp_hip_transformer.h).  The
+// reference has none of them; they run on the HIP device only, as every op here
+// does.
 #pragma once
 
 #include <memory>
@@ -47,7 +49,45 @@ using adamw_fn = void (*)(int bits, const std::vector<AdamWParam>& params, const
 using adamw_decode_fn = Tensor (*)(bool signed_codes, const Tensor& codes, const Tensor& scales,
                                    size_t n);
 
+// Pairs of the first heads * head_dim columns turned by position x frequency.
+struct RotaryShape {
+  size_t heads, head_dim;
+  bool interleaved;
+  Scalar scale;
+};
+using rotary_fn = Tensor (*)(const Tensor& x, const Tensor& positions, const Tensor& frequencies,
+                             const RotaryShape& shape, bool inverse);
+
+// The call's number goes to *used where `used` is defined.
+using dropout_fn = Tensor (*)(const Tensor& x, const Tensor& residual, Scalar rate, uint64_t seed,
+                              Tensor& state, Tensor* used);
+using dropout_backward_fn = Tensor (*)(const Tensor& g, Scalar rate, uint64_t seed,
+                                       const Tensor& used);
+
+// h, and [a | u] where `keep` (else left undefined); bias may be undefined.
+struct GatedOut {
+  Tensor h, pre;
+};
+using gated_linear_fn = GatedOut (*)(int gate, const Tensor& x, const Tensor& w, const Tensor& bias,
+                                     bool keep);
+// Writes those of dx, dw and db that are defined.
+using gated_linear_backward_fn = void (*)(int gate, const Tensor& g, const Tensor& x,
+                                          const Tensor& w, const Tensor& pre, Tensor* dx,
+                                          Tensor* dw, Tensor* db);
+
+// The losses of the rows; with `weights` defined also those of dx, dw and db that
+// are defined, of the weighted sum.
+using linear_cross_entropy_fn = Tensor (*)(const Tensor& x, const Tensor& w, const Tensor& bias,
+                                           const Tensor& targets, const Tensor& weights, Tensor* dx,
+                                           Tensor* dw, Tensor* db);
+
 LMP_DECLARE_DISPATCH(layer_norm_fn, layer_norm_stub)
+LMP_DECLARE_DISPATCH(rotary_fn, rotary_stub)
+LMP_DECLARE_DISPATCH(dropout_fn, dropout_stub)
+LMP_DECLARE_DISPATCH(dropout_backward_fn, dropout_backward_stub)
+LMP_DECLARE_DISPATCH(gated_linear_fn, gated_linear_stub)
+LMP_DECLARE_DISPATCH(gated_linear_backward_fn, gated_linear_backward_stub)
+LMP_DECLARE_DISPATCH(linear_cross_entropy_fn, linear_cross_entropy_stub)
 LMP_DECLARE_DISPATCH(layer_norm_backward_fn, layer_norm_backward_stub)
 LMP_DECLARE_DISPATCH(attention_fn, attention_stub)
 LMP_DECLARE_DISPATCH(attention_backward_fn, attention_backward_stub)
@@ -88,6 +128,23 @@ Variable layer_norm(const Variable& x, const Variable* w, const Variable* b, Sca
 // and v [keys, kv_heads * dim].
 Variable attention(const Variable& q, const Variable& k, const Variable& v,
                    const AttentionPlan& plan, Scalar scale);
+// x [rows, columns] with the pairs of its first heads * head_dim columns turned by
+// positions[row] * frequencies[pair] (int64 and float64 tensors); a head's first
+// 2 * frequencies values turn.
+Variable rotary(const Variable& x, const Tensor& positions, const Tensor& frequencies,
+                const tensor::ops::RotaryShape& shape);
+// residual + (kept ? x / (1 - rate) : 0); `state` (two int64) counts the calls.
+Variable dropout(const Variable& x, const Variable* residual, Scalar rate, uint64_t seed,
+                 Tensor state);
+// act(a) u for [a | u] = x w + b.
+Variable gated_linear(const Variable& x, const Variable& w, const Variable* b, int gate);
+// The cross entropies of the rows of x w + b against targets (int64), without a gradient.
+Tensor linear_cross_entropy_rows(const Variable& x, const Variable& w, const Variable* b,
+                                 const Tensor& targets);
+// Their sum weighted by `weights` ([rows] float32; undefined: the mean over the rows whose
+// targets are not negative), of shape [1].  The gradients are formed with the losses.
+Variable linear_cross_entropy(const Variable& x, const Variable& w, const Variable* b,
+                              const Tensor& targets, const Tensor& weights);
 // The same with q, k and v side by side in the rows of one projection:
 // [queries, (heads + 2 kv_heads) * dim].
 Variable attention_qkv(const Variable& rows, const AttentionPlan& plan, Scalar scale);
