@@ -11,12 +11,12 @@
 #include <string>
 
 #include "common.hpp"
+#include "gemm_half.hpp"
+#include "half_products.hpp"
 #include "lmp_hip_transformer.h"
+#include "strips.hpp"
 
 namespace lmp_hip {
-
-int clear_f32(Runtime* rt, float* p, size_t rows, size_t cols, size_t ld);
-
 namespace {
 
 // Bytes of one piece's logits: well inside the 256 MB memory-side cache, so that what
@@ -101,6 +101,160 @@ __global__ __launch_bounds__(1024) void loss_rows(LossArgs a) {
   }
 }
 
+// ------------------------------------------------------- on the fp16 matrix cores
+
+// The largest logit and the sum of exponents below it of a row's 64 columns, for each wave
+// column of the tiles.
+struct HalfLogits {
+  const float* bias;
+  float* z;      // [rows, vocab], or null
+  Softmax* part;  // [rows, parts]
+  int parts;
+  const int64_t* targets;
+  float* hit;  // [rows]: the target's logit
+};
+
+// e^x for x <= 0: 2^(x log2 e) with what rounding the product leaves out put back, so that
+// it errs by two units, not by |x| of them.
+__device__ __forceinline__ float exp_below(float x) {
+  constexpr float kHi = 1.44269504088896341f, kLo = 1.925963033500e-8f, kLn2 = 0.69314718055994531f;
+  const float t = x * kHi, e = __builtin_amdgcn_exp2f(t);
+  const float rest = __builtin_fmaf(x, kHi, -t) + x * kLo;
+  return t < -160.0f ? 0.0f : __builtin_fmaf(e, rest * kLn2, e);
+}
+
+__device__ __forceinline__ float over_eight(float x, bool most) {
+#define LMP_STEP(ctrl)                                                                                          \
+  {                                                                                                             \
+    const float y = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, 0xF, 0xF, false)); \
+    x = most ? fmaxf(x, y) : x + y;                                                                             \
+  }
+  LMP_STEP(0xB1);
+  LMP_STEP(0x4E);
+  LMP_STEP(0x141);
+#undef LMP_STEP
+  return x;
+}
+
+template <int NT, int MINB, class C>
+__global__ __launch_bounds__(NT, MINB) void half_logits(HalfArgs g, HalfLogits o) {
+  static_assert(NT == C::THREADS, "one lane per thread of the configuration");
+  __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
+  hv16 acc[C::TM][C::TN];
+  const HalfItem at = half_item(g, int(blockIdx.x));
+  const int n0 = at.tile_n * C::BN;
+  const bool scaled = half_tile<C, false, false>(g, at, n0, [&](int c) { return min(c, g.n - 1 - n0); }, smem, acc);
+  const int wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % C::WN, col0 = n0 + wn * 64;
+  const uint32_t* const tops[2] = {g.b_top + col0, g.b_top + col0 + 32};
+  half_epilogue<C>(g, at, scaled, smem, tops, acc, [&](int row, int c4, hv4 (&v)[2]) {
+    const float low = -__builtin_huge_valf();
+    const int64_t target = row < g.m ? o.targets[row] : -1;
+    float top = low;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int col = col0 + 32 * j + c4;
+      if (o.bias) v[j] = v[j] + load_four(o.bias, col, g.n);
+      if (o.z && row < g.m) store_four(o.z + int64_t(row) * g.n, col, g.n, v[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (target == col + e && col + e < g.n) o.hit[row] = v[j][e];
+        if (col + e >= g.n) v[j][e] = low;
+        top = fmaxf(top, v[j][e]);  // of NaN the other one
+      }
+    }
+    top = over_eight(top, true);
+    const float from = top > low ? top : 0.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += exp_below(v[j][e] - from);
+    sum = over_eight(sum, false);
+    if (c4 == 0 && row < g.m) o.part[int64_t(row) * o.parts + at.tile_n * C::WN + wn] = {top, sum};
+  });
+}
+
+// What the gradient of a row's logits needs: dz = e^(z - top) factor - [v = target] weight.
+struct LossRow {
+  float top, factor, weight;
+  int target;  // -1: not counted, or past the vocabulary (whose factor is NaN)
+};
+
+// The rows' losses from their parts, a wave a row; with `info` what the gradient needs, and
+// |weight|, which no |dz| passes, as the row's largest magnitude.
+struct HalfRows {
+  int64_t rows;
+  int parts, vocab;
+  const Softmax* part;
+  const float* hit;
+  const int64_t* targets;
+  const float* weights;
+  float* loss;
+  LossRow* info;
+  uint32_t* row_top;
+};
+__global__ __launch_bounds__(256) void half_loss_rows(HalfRows a) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); row < a.rows; row += int64_t(gridDim.x) * 4) {
+    const int64_t t = a.targets[row];
+    const Softmax* p = a.part + row * a.parts;
+    Softmax s{-__builtin_huge_valf(), 0.0f};
+    for (int i = lane; i < a.parts; i += 64) s = joined(s, p[i]);
+    for (int off = 1; off < 64; off *= 2) s = joined(s, {__shfl_xor(s.top, off), __shfl_xor(s.sum, off)});
+    if (lane) continue;
+    const bool counted = t >= 0, known = t < a.vocab;
+    const float nan = __builtin_nanf("");
+    a.loss[row] = !counted ? 0.0f : known ? logf(s.sum) - (a.hit[row] - s.top) : nan;
+    if (a.info) {
+      const float w = !counted ? 0.0f : !known ? nan : a.weights ? a.weights[row] : 1.0f;
+      a.info[row] = {s.top, w / s.sum, w, counted && known ? int(t) : counted ? -2 : -1};
+      a.row_top[row] = magnitude(w);
+    }
+  }
+}
+
+// dz over z, with its columns' largest magnitudes and (SUMS) their sums over each strip.
+struct HalfGrad {
+  StripShape s;
+  float* z;
+  const LossRow* info;
+  uint32_t* col_top;
+  float* sums;  // [strips, vocab]
+};
+template <bool SUMS>
+__global__ __launch_bounds__(kStripThreads) void half_loss_grad(HalfGrad o) {
+  const int col = strip_col(), n = o.s.cols;
+  uint32_t top[4] = {0, 0, 0, 0};
+  hv4 sum = hv4(0.0f);
+  const int64_t end = strip_end(o.s);
+#pragma unroll 4
+  for (int64_t row = strip_begin(o.s); row < end; ++row) {
+    const LossRow r = o.info[row];
+    float* z = o.z + row * n;
+    hv4 v = load_four(z, col, n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p = exp_below(v[e] - r.top) * r.factor;
+      v[e] = r.target == -1 ? 0.0f : col + e == r.target ? p - r.weight : p;
+      top[e] = max(top[e], magnitude(v[e]));
+    }
+    store_four(z, col, n, v);
+    if constexpr (SUMS) sum = sum + v;
+  }
+  raise_cols(o.col_top, col, n, top);
+  if constexpr (SUMS) store_four(o.sums + int64_t(blockIdx.y) * n, col, n, sum);
+}
+
+// The rows of x, zeros in place of those that are not counted: 0 x infinity would be NaN.
+__global__ __launch_bounds__(256) void counted_rows(const float* x, int64_t ldx, int64_t rows, int in,
+                                                    const int64_t* targets, float* out) {
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const bool counted = targets[row] >= 0;
+    for (int i = threadIdx.x * 4; i < in; i += 1024)
+      store_four(out + row * in, i, in, counted ? load_four(x + row * ldx, i, in) : hv4(0.0f));
+  }
+}
+
 struct LossCall {
   size_t rows, in, vocab;
   const float* x;
@@ -129,11 +283,111 @@ int check_loss(const std::string& name, const LossCall& c) {
   return LMP_OK;
 }
 
+// From this many multiply-adds a product on, the fp16 matrix cores make up for the passes
+// that find the largest magnitudes.
+constexpr uint64_t kHalfWork = uint64_t(1) << 28;
+
+int run_loss_half(Runtime* rt, const LossCall& c) {
+  const bool grad = c.dx || c.dw;
+  // Pieces of whole tiles of rows.
+  const size_t fit = std::max<size_t>(256, kPieceBytes / (c.vocab * sizeof(float)) / 256 * 256);
+  const size_t pieces = grad ? (c.rows + fit - 1) / fit : 1;
+  size_t each = (c.rows + pieces - 1) / pieces;
+  if (pieces > 1) each = (each + 255) / 256 * 256;
+  // A product's K takes 32 rows: fewer at the end join the last piece.
+  const size_t most = std::min(c.rows, each + 31);
+  const HalfPlan plan = half_plan(rt->cu_count, 0, int64_t(most), int64_t(c.vocab), int64_t(c.in), false);
+  if (plan.cfg < 0) return fail(LMP_ERR_UNSUPPORTED, "linear_cross_entropy: more tiles than a grid holds");
+  const int bn = kHalfTiles[plan.cfg].bn, parts = int((c.vocab + bn - 1) / bn) * (bn / 64);
+  const StripShape strips = strips_of(rt, most, c.vocab);
+  // The workspace, each part a multiple of 256 bytes.
+  size_t total = 0;
+  const auto room = [&](size_t words) {
+    const size_t at = total;
+    total += (words + 63) / 64 * 64;
+    return at;
+  };
+  const size_t at_z = room(grad ? most * c.vocab : 0), at_x = room(c.dw ? c.rows * c.in : 0);
+  const size_t at_part = room(most * size_t(parts) * 2), at_hit = room(most), at_info = room(grad ? most * 4 : 0);
+  const size_t at_sums = room(c.db ? size_t(strips.strips) * c.vocab : 0), at_db = room(c.db ? c.vocab : 0);
+  const size_t at_tops = total;
+  const size_t at_xr = room(half_tops_room(c.rows)), at_wc = room(half_tops_room(c.vocab));
+  const size_t at_xc = room(c.dw ? half_tops_room(c.in) : 0), at_wr = room(c.dx ? half_tops_room(c.in) : 0);
+  const size_t at_dr = room(grad ? half_tops_room(most) : 0), at_dc = room(grad ? half_tops_room(c.vocab) : 0);
+  float* base = static_cast<float*>(scratch_alloc(total * sizeof(float)));
+  if (!base) return LMP_ERR_OOM;
+  uint32_t* words = reinterpret_cast<uint32_t*>(base);
+  uint32_t *x_row = words + at_xr, *w_col = words + at_wc, *x_col = words + at_xc, *w_row = words + at_wr;
+  uint32_t *d_row = words + at_dr, *d_col = words + at_dc;
+  const float* x = c.x;
+  size_t ldx = c.ldx;
+  const auto piece = [&](size_t at, size_t n) -> int {
+    const float* xp = x + at * ldx;
+    const HalfArgs g = half_args(xp, int(ldx), c.w, int(c.ldw), int(n), int(c.vocab), int(c.in), x_row + at, w_col, plan);
+    float* z = grad ? base + at_z : nullptr;
+    Softmax* part = reinterpret_cast<Softmax*>(base + at_part);
+    LossRow* info = grad ? reinterpret_cast<LossRow*>(base + at_info) : nullptr;
+    const HalfLogits o{c.bias, z, part, parts, c.targets + at, base + at_hit};
+    if (int s = with_half_cfg(plan.cfg, [&](auto cfg) -> int {
+          using C = decltype(cfg);
+          half_logits<C::THREADS, C::MINB, C><<<dim3(half_items(g)), dim3(C::THREADS), 0, rt->stream>>>(g, o);
+          LMP_LAUNCH_CHECK("half_logits");
+          return LMP_OK;
+        }))
+      return s;
+    const HalfRows r{int64_t(n), parts, int(c.vocab), part, base + at_hit, c.targets + at,
+                     c.weights ? c.weights + at : nullptr, c.loss + at, info, d_row};
+    half_loss_rows<<<dim3(uint32_t(std::min<size_t>((n + 3) / 4, 65536))), dim3(256), 0, rt->stream>>>(r);
+    LMP_LAUNCH_CHECK("half_loss_rows");
+    if (!grad) return LMP_OK;
+    if (at)
+      if (int s = clear_words(rt, d_col, half_tops_room(c.vocab))) return s;
+    StripShape mine = strips;
+    mine.rows = int64_t(n);
+    mine.strips = int((int64_t(n) + mine.each - 1) / mine.each);
+    const HalfGrad d{mine, z, info, d_col, base + at_sums};
+    if (c.db) half_loss_grad<true><<<strip_grid(mine), dim3(kStripThreads), 0, rt->stream>>>(d);
+    else half_loss_grad<false><<<strip_grid(mine), dim3(kStripThreads), 0, rt->stream>>>(d);
+    LMP_LAUNCH_CHECK("half_loss_grad");
+    if (c.db) {
+      float* to = at ? base + at_db : c.db;
+      if (int s = lmp_k_reduce(LMP_RED_SUM, LMP_FLOAT32, to, base + at_sums, 1, size_t(mine.strips), c.vocab)) return s;
+      if (at)
+        if (int s = lmp_k_add_inplace(LMP_FLOAT32, c.db, to, c.vocab)) return s;
+    }
+    return half_backward(rt, {n, c.in, c.vocab, z, c.vocab, d_row, d_col, xp, ldx, x_col, c.w, c.ldw, w_row,
+                              c.dx ? c.dx + at * c.lddx : nullptr, c.lddx, c.dw, c.lddw, at > 0});
+  };
+  const auto run = [&]() -> int {
+    if (int s = clear_words(rt, words + at_tops, total - at_tops)) return s;
+    if (c.dw) {
+      counted_rows<<<dim3(uint32_t(std::min<size_t>(c.rows, 65536))), dim3(256), 0, rt->stream>>>(
+          c.x, int64_t(c.ldx), int64_t(c.rows), int(c.in), c.targets, base + at_x);
+      LMP_LAUNCH_CHECK("counted_rows");
+      x = base + at_x;
+      ldx = c.in;
+    }
+    if (int s = half_tops(rt, x, c.rows, c.in, ldx, x_row, c.dw ? x_col : nullptr)) return s;
+    if (int s = half_tops(rt, c.w, c.in, c.vocab, c.ldw, c.dx ? w_row : nullptr, w_col)) return s;
+    for (size_t at = 0, n; at < c.rows; at += n) {
+      n = c.rows - at <= most ? c.rows - at : each;
+      if (int s = piece(at, n)) return s;
+    }
+    return LMP_OK;
+  };
+  const int rc = run();
+  scratch_free(base);
+  return rc;
+}
+
 int run_loss(Runtime* rt, const LossCall& c) {
   if (c.rows == 0) {
     if (int s = clear_f32(rt, c.dw, c.in, c.vocab, c.lddw)) return s;
     return clear_f32(rt, c.db, 1, c.vocab, c.vocab);
   }
+  if (half_fits(c.rows, c.in, c.vocab, std::max({c.ldx, c.ldw, c.vocab})) &&
+      uint64_t(c.rows) * c.in * c.vocab >= kHalfWork)
+    return run_loss_half(rt, c);
   const size_t fit = std::max<size_t>(256, kPieceBytes / (c.vocab * sizeof(float)));
   const size_t pieces = (c.rows + fit - 1) / fit, each = (c.rows + pieces - 1) / pieces;
   const size_t logits = (each * c.vocab + 3) / 4 * 4;

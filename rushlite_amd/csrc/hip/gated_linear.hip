@@ -3,6 +3,10 @@
 //
 //   pre = x W + b = [a | u],  h = act(a) u
 //   d = [g u act'(a) | g act(a)],  dx = d W^T,  dW = x^T d,  db = the column sums of d
+//
+// Large layers run on the fp16 matrix cores (gemm_half.hpp): forward as one kernel, whose
+// epilogue forms h; backward d in one pass, with the largest magnitudes and the column sums,
+// then both products in one launch.  Smaller ones take the framework's fp32 products.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -11,7 +15,10 @@
 
 #include "common.hpp"
 #include "gate.hpp"
+#include "gemm_half.hpp"
+#include "half_products.hpp"
 #include "lmp_hip_transformer.h"
+#include "strips.hpp"
 
 namespace lmp_hip {
 namespace {
@@ -59,24 +66,117 @@ int launch_gate(Runtime* rt, const GateArgs& a) {
   return LMP_OK;
 }
 
-__global__ __launch_bounds__(kThreads) void clear_rows(float* p, int64_t rows, int cols, int64_t ld) {
-  const int64_t total = rows * cols;
-  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < total; i += int64_t(gridDim.x) * kThreads)
-    p[i / cols * ld + i % cols] = 0.0f;
+// ------------------------------------------------------- on the fp16 matrix cores
+
+struct HalfGated {
+  int gate, hidden;
+  const float* bias;
+  float* h;
+  int64_t ldh;
+  float* pre;
+  int64_t ldpre;
+};
+
+// h (and pre) of a tile: its block columns are the gate's and the other half's by turns, so
+// that a lane ends with both of a hidden value.
+template <int NT, int MINB, class C>
+__global__ __launch_bounds__(NT, MINB) void half_gated(HalfArgs g, HalfGated o) {
+  static_assert(NT == C::THREADS, "one lane per thread of the configuration");
+  __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
+  hv16 acc[C::TM][C::TN];
+  const HalfItem at = half_item(g, int(blockIdx.x));
+  const int h0 = at.tile_n * (C::BN / 2);
+  const int left = o.hidden - 1 - h0;
+  const auto local = [&](int c) {
+    const int block = c / 32;
+    return min(block / 2 * 32 + c % 32, left) + (block & 1) * o.hidden;
+  };
+  const bool scaled = half_tile<C, false, false>(g, at, h0, local, smem, acc);
+  const int wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % C::WN;
+  const int col0 = h0 + wn * 32;
+  const uint32_t* const tops[2] = {g.b_top + col0, g.b_top + o.hidden + col0};
+  half_epilogue<C>(g, at, scaled, smem, tops, acc, [&](int row, int c4, hv4 (&v)[2]) {
+    const int col = col0 + c4;
+    if (row >= g.m || col >= o.hidden) return;
+    if (o.bias) {
+      v[0] = v[0] + load_four(o.bias, col, o.hidden);
+      v[1] = v[1] + load_four(o.bias + o.hidden, col, o.hidden);
+    }
+    hv4 h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float act, slope;
+      gate_of(o.gate, v[0][e], act, slope);
+      h[e] = act * v[1][e];
+    }
+    store_four(o.h + row * o.ldh, col, o.hidden, h);
+    if (o.pre) {
+      float* p = o.pre + row * o.ldpre;
+      store_four(p, col, o.hidden, v[0]);
+      store_four(p + o.hidden, col, o.hidden, v[1]);
+    }
+  });
+}
+
+// d with its largest magnitudes, and (SUMS) the columns' sums of each strip of rows.
+struct HalfGate {
+  GateArgs a;
+  StripShape s;
+  uint32_t *row_top, *col_top;
+  float* sums;  // [strips, 2 hidden]
+};
+template <bool SUMS>
+__global__ __launch_bounds__(kStripThreads) void half_gate(HalfGate o) {
+  const GateArgs& a = o.a;
+  const int col = strip_col(), n = a.hidden;
+  uint32_t top0[4] = {0, 0, 0, 0}, top1[4] = {0, 0, 0, 0};
+  hv4 sum0 = hv4(0.0f), sum1 = hv4(0.0f);
+  const int64_t end = strip_end(o.s);
+#pragma unroll 2
+  for (int64_t row = strip_begin(o.s); row < end; ++row) {
+    const float* p = a.pre + row * a.ldpre;
+    const hv4 x = load_four(p, col, n), u = load_four(p + n, col, n), g = load_four(a.g + row * a.ldg, col, n);
+    hv4 d0, d1;
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float act, slope;
+      gate_of(a.gate, x[e], act, slope);
+      d0[e] = g[e] * u[e] * slope;
+      d1[e] = g[e] * act;
+      const uint32_t m0 = col + e < n ? magnitude(d0[e]) : 0, m1 = col + e < n ? magnitude(d1[e]) : 0;
+      top0[e] = max(top0[e], m0);
+      top1[e] = max(top1[e], m1);
+      most = max(most, max(m0, m1));
+    }
+    float* out = a.out + row * a.ldo;
+    store_four(out, col, n, d0);
+    store_four(out + n, col, n, d1);
+    if constexpr (SUMS) {
+      sum0 = sum0 + d0;
+      sum1 = sum1 + d1;
+    }
+    raise_row(o.row_top + row, most);
+  }
+  raise_cols(o.col_top, col, n, top0);
+  raise_cols(o.col_top + n, col, n, top1);
+  if constexpr (SUMS) {
+    float* sums = o.sums + int64_t(blockIdx.y) * 2 * n;
+    store_four(sums, col, n, sum0);
+    store_four(sums + n, col, n, sum1);
+  }
+}
+
+// From this many multiply-adds a product on, the fp16 matrix cores make up for the passes
+// that find the largest magnitudes.
+constexpr uint64_t kHalfWork = uint64_t(1) << 28;
+
+bool use_half(size_t rows, size_t in, size_t hidden, size_t most_ld) {
+  return half_fits(rows, in, 2 * hidden, std::max(most_ld, 2 * hidden)) && hidden >= 32 &&
+         uint64_t(rows) * in * 2 * hidden >= kHalfWork;
 }
 
 }  // namespace
-
-// Zeros in `cols` columns of `rows` rows (the gradients of no rows).
-int clear_f32(Runtime* rt, float* p, size_t rows, size_t cols, size_t ld) {
-  if (!p || rows == 0 || cols == 0) return LMP_OK;
-  const size_t groups = (rows * cols + kThreads - 1) / kThreads;
-  clear_rows<<<dim3(uint32_t(std::min<size_t>(groups, 65536))), dim3(kThreads), 0, rt->stream>>>(
-      p, int64_t(rows), int(cols), int64_t(ld));
-  LMP_LAUNCH_CHECK("clear");
-  return LMP_OK;
-}
-
 namespace {
 
 int check_gated(const std::string& name, int gate, size_t rows, size_t in, size_t hidden) {
@@ -105,6 +205,30 @@ extern "C" int lmp_k_gated_linear_f32(int gate, size_t rows, size_t in, size_t h
   if (std::max({ldx, ldw, ldh, pre ? ldpre : 0}) >= kGemmMaxExtent)
     return fail(LMP_ERR_UNSUPPORTED, name + "dimension of 2^31 - 4096 or more");
   LMP_RUNTIME_OR_FAIL(rt);
+  if (use_half(rows, in, hidden, std::max(ldx, ldw))) {
+    const size_t of_x = half_tops_room(rows), of_w = half_tops_room(2 * hidden);
+    uint32_t* tops = static_cast<uint32_t*>(scratch_alloc((of_x + of_w) * sizeof(uint32_t)));
+    if (!tops) return LMP_ERR_OOM;
+    const auto run = [&]() -> int {
+      if (int s = clear_words(rt, tops, of_x + of_w)) return s;
+      if (int s = half_tops(rt, x, rows, in, ldx, tops, nullptr)) return s;
+      if (int s = half_tops(rt, w, in, 2 * hidden, ldw, nullptr, tops + of_x)) return s;
+      // A tile of BN columns holds BN / 2 hidden values: the plan's columns are twice as many.
+      const HalfPlan plan = half_plan(rt->cu_count, 0, int64_t(rows), 2 * int64_t(hidden), int64_t(in), false);
+      if (plan.cfg < 0) return fail(LMP_ERR_UNSUPPORTED, name + "more tiles than a grid holds");
+      const HalfArgs g = half_args(x, int(ldx), w, int(ldw), int(rows), int(2 * hidden), int(in), tops, tops + of_x, plan);
+      const HalfGated o{gate, int(hidden), bias, h, int64_t(ldh), pre, int64_t(ldpre)};
+      return with_half_cfg(plan.cfg, [&](auto cfg) -> int {
+        using C = decltype(cfg);
+        half_gated<C::THREADS, C::MINB, C><<<dim3(half_items(g)), dim3(C::THREADS), 0, rt->stream>>>(g, o);
+        LMP_LAUNCH_CHECK("half_gated");
+        return LMP_OK;
+      });
+    };
+    const int rc = run();
+    scratch_free(tops);
+    return rc;
+  }
   float* z = pre;
   if (!z) {
     z = static_cast<float*>(scratch_alloc(rows * 2 * hidden * sizeof(float)));
@@ -139,6 +263,36 @@ extern "C" int lmp_k_gated_linear_backward_f32(int gate, size_t rows, size_t in,
   if (rows == 0) {
     if (int s = clear_f32(rt, dw, in, width, lddw)) return s;
     return clear_f32(rt, db, 1, width, width);
+  }
+  if (use_half(rows, in, hidden, std::max(dw ? ldx : 0, dx ? ldw : 0))) {
+    const StripShape strips = strips_of(rt, rows, hidden);
+    const size_t of_d = (rows * width + 63) / 64 * 64, of_sums = db ? (size_t(strips.strips) * width + 63) / 64 * 64 : 0;
+    const size_t of_x = half_tops_room(in), of_row = half_tops_room(rows), of_col = half_tops_room(width);
+    const size_t of_tops = 2 * of_x + of_row + of_col;
+    float* d = static_cast<float*>(scratch_alloc((of_d + of_sums + of_tops) * sizeof(float)));
+    if (!d) return LMP_ERR_OOM;
+    float* sums = d + of_d;
+    uint32_t* x_col = reinterpret_cast<uint32_t*>(sums + of_sums);
+    uint32_t *w_row = x_col + of_x, *d_row = w_row + of_x, *d_col = d_row + of_row;
+    const auto run = [&]() -> int {
+      if (int s = clear_words(rt, x_col, of_tops)) return s;
+      if (dw)
+        if (int s = half_tops(rt, x, rows, in, ldx, nullptr, x_col)) return s;
+      if (dx)
+        if (int s = half_tops(rt, w, in, width, ldw, w_row, nullptr)) return s;
+      const HalfGate o{{gate, int64_t(rows), int(hidden), pre, int64_t(ldpre), g, int64_t(ldg), d, int64_t(width)},
+                       strips, d_row, d_col, sums};
+      if (db) half_gate<true><<<strip_grid(strips), dim3(kStripThreads), 0, rt->stream>>>(o);
+      else half_gate<false><<<strip_grid(strips), dim3(kStripThreads), 0, rt->stream>>>(o);
+      LMP_LAUNCH_CHECK("half_gate");
+      if (db)
+        if (int s = lmp_k_reduce(LMP_RED_SUM, LMP_FLOAT32, db, sums, 1, size_t(strips.strips), width)) return s;
+      return half_backward(rt, {rows, in, width, d, width, d_row, d_col, x, ldx, x_col, w, ldw, w_row, dx, lddx, dw,
+                                lddw, false});
+    };
+    const int rc = run();
+    scratch_free(d);
+    return rc;
   }
   float* d = static_cast<float*>(scratch_alloc(rows * width * sizeof(float)));
   if (!d) return LMP_ERR_OOM;

@@ -161,4 +161,55 @@ inline bool bf3_pair_fits(uint64_t a, uint64_t b, int threads) {
   return a + b <= kMaxGridThreads / uint64_t(threads);
 }
 
+// ---------------------------------------------- products on the fp16 matrix cores
+
+constexpr int kHalfK = 32;  // k values per step
+
+struct HalfPlan {
+  int cfg = -1;  // index into kHalfTiles; -1: no launch fits a grid
+  int splits = 1;
+};
+
+// Time of one 32-wide k step of a workgroup, in us: `alone` on its CU, and `shared` per
+// workgroup where several take turns; `ends`: its first loads and its tile's way out.
+struct HalfTile {
+  int bm, bn, threads;
+  float alone, shared, ends;
+};
+constexpr HalfTile kHalfTiles[] = {{256, 256, 512, 2.9f, 2.9f, 11.0f},
+                                   {256, 128, 512, 1.6f, 1.65f, 7.0f},
+                                   {128, 128, 512, 1.0f, 0.92f, 5.0f},
+                                   {64, 128, 256, 0.75f, 0.56f, 4.0f}};
+
+// Modelled time of tiles of one configuration in `splits` parts of K.
+inline float half_time(const HalfTile& t, int64_t cus, int64_t items, int64_t steps) {
+  const float load = float((items + cus - 1) / cus);
+  return load * t.ends + float(steps) * std::max(t.alone, load * t.shared);
+}
+
+// Tiles (and, with `splits`, the split of K) with the least modelled time; partials stay
+// within `scratch` bytes and a split keeps at least 128 k.
+inline HalfPlan half_plan(int64_t cus, int64_t scratch, int64_t m, int64_t n, int64_t k, bool split) {
+  const int64_t steps = (k + kHalfK - 1) / kHalfK;
+  HalfPlan plan;
+  float best = 0.0f;
+  for (int c = 0; c < int(std::size(kHalfTiles)); ++c) {
+    const HalfTile& t = kHalfTiles[c];
+    const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
+    for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
+      if (s > 1 && (!split || steps / s < 4 || int64_t(s) * m * n > scratch / int64_t(sizeof(float)))) break;
+      if (uint64_t(tiles) * uint64_t(s) > kMaxGridThreads / uint64_t(t.threads)) break;
+      float us = half_time(t, cus, tiles * s, (steps + s - 1) / s);
+      if (s > 1) us += 3.0f + float(s + 1) * float(m) * float(n) * (4.0f / 5e6f);
+      if (plan.cfg < 0 || us < best) {
+        best = us;
+        plan.cfg = c;
+        plan.splits = s;
+      }
+      if (tiles * s > 8 * cus) break;
+    }
+  }
+  return plan;
+}
+
 }  // namespace lmp_hip

@@ -154,7 +154,9 @@ def test_dropout_rates_and_what_is_dropped(hip):
 # ------------------------------------------------------------ gated linear
 
 GATED = [(1, 1, 1), (1, 7, 3), (3, 5, 4), (2, 64, 33), (32, 64, 64), (5, 300, 70), (33, 40, 129), (31, 1000, 96), (32, 1024, 515),
-         (64, 32, 200), (70, 129, 65), (129, 128, 128), (300, 77, 260), (200, 512, 300), (1000, 64, 31), (513, 256, 640)]
+         (64, 32, 200), (70, 129, 65), (129, 128, 128), (300, 77, 260), (200, 512, 300), (1000, 64, 31), (513, 256, 640),
+         # on the fp16 matrix cores
+         (700, 400, 600), (1031, 257, 521), (32, 2048, 2100), (4000, 33, 1037), (6007, 300, 97), (130, 4097, 300)]
 
 
 def gated(hip, gate, x, w, b, g, pads=(0, 0, 0, 0), want=(True, True, True), keep=True):
@@ -203,7 +205,7 @@ def test_gated_linear(hip, gate, rows, k, n):
 def test_gated_linear_relu_is_exact_on_integers(hip):
     """Small whole numbers: every product and sum is exact, so ReLU's two sides are too, at 0 as well."""
     rng = np.random.default_rng(4)
-    for rows, k, n in ((3, 5, 4), (40, 33, 70), (300, 64, 129)):
+    for rows, k, n in ((3, 5, 4), (40, 33, 70), (300, 64, 129), (301, 700, 701)):
         x, w, g = (rng.integers(-3, 4, s).astype(np.float32) for s in ((rows, k), (k, 2 * n), (rows, n)))
         for got, want in zip(gated(hip, "relu", x, w, None, g), D.gated("relu", x, w, None, g)):
             assert np.array_equal(got, want)
@@ -211,7 +213,7 @@ def test_gated_linear_relu_is_exact_on_integers(hip):
 
 def test_gated_linear_parts_of_the_backward(hip):
     rng = np.random.default_rng(6)
-    for rows, k, n in ((5, 9, 6), (200, 70, 140)):
+    for rows, k, n in ((5, 9, 6), (200, 70, 140), (300, 700, 701)):
         x, w, g = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (k, 2 * n), (rows, n)))
         want, bound = D.gated("silu", x, w, None, g), D.gated_bounds("silu", x, w, None, g)
         for parts in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (1, 0, 1), (0, 1, 1)):
@@ -233,7 +235,7 @@ def test_gated_linear_special_values(hip):
     """Infinities and NaN in one row touch no other; gates far out are 0, a or 1; operands far apart and past the split's
     range come out as float32's products give them."""
     rng = np.random.default_rng(8)
-    for rows, k, n in ((6, 40, 30), (150, 64, 130)):
+    for rows, k, n in ((6, 40, 30), (150, 64, 130), (300, 700, 701)):
         x, w, g = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (k, 2 * n), (rows, n)))
         clean = gated(hip, "silu", x, w, None, g)
         x[2, 3], x[4, 0] = np.nan, np.inf
@@ -252,9 +254,10 @@ def test_gated_linear_special_values(hip):
         act = np.array([0, 1, 0, 1, 0.5]) if gate == "sigmoid" else np.maximum(x[:, 0].astype(np.float64), 0)
         close(h, act * u, 1e-5 * np.abs(act * u) + 1e-38, gate)
     # one row and one column far larger than the others, and far smaller
-    x, w = rng.standard_normal((70, 96)).astype(np.float32), rng.standard_normal((96, 140)).astype(np.float32)
-    g = rng.standard_normal((70, 70)).astype(np.float32)
-    for scale in (1e-20, 1e-12, 1e12):
+    for rows, k, n, scale in [(*size, scale) for size in ((70, 96, 70), (400, 600, 700)) for scale in (1e-20, 1e-12, 1e12)]:
+        x, w, g = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (k, 2 * n), (rows, n)))
+        if k > 96:
+            w *= np.float32(k ** -0.5)
         xs, gs = x.copy(), g.copy()
         xs[5] *= np.float32(scale)
         gs[9] *= np.float32(scale)
@@ -266,7 +269,9 @@ def test_gated_linear_special_values(hip):
 # ----------------------------------------------------------- cross entropy
 
 LOSS = [(1, 1, 1), (1, 3, 2), (3, 5, 7), (32, 64, 10), (7, 33, 1000), (64, 16, 129), (40, 130, 515), (130, 64, 1024),
-        (33, 100, 4099), (300, 40, 333), (65, 7, 20001), (129, 256, 640)]
+        (33, 100, 4099), (300, 40, 333), (65, 7, 20001), (129, 256, 640),
+        # on the fp16 matrix cores
+        (1031, 257, 1021), (40, 1000, 7001), (3000, 33, 2801), (32, 600, 14100), (9000, 520, 64), (777, 1111, 513)]
 
 
 def loss(hip, x, w, b, targets, weights=None, pads=(0, 0), grads=True, want=(True, True, True)):
@@ -315,7 +320,11 @@ def test_cross_entropy(hip, rows, k, vocab):
 def test_cross_entropy_in_several_pieces(hip):
     """More logits than one piece of the workspace holds."""
     rng = np.random.default_rng(1)
-    rows, k, vocab = 2300, 12, 30011
+    for rows, k, vocab in ((2300, 12, 30011), (2300, 40, 30011), (1050, 64, 33000)):
+        several_pieces(hip, rng, rows, k, vocab)
+
+
+def several_pieces(hip, rng, rows, k, vocab):
     x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
     targets = rng.integers(-vocab // 4, vocab, rows)
     check_loss(hip, x, w, rng.standard_normal(vocab).astype(np.float32), targets, rng.random(rows).astype(np.float32))
@@ -323,7 +332,7 @@ def test_cross_entropy_in_several_pieces(hip):
 
 def test_cross_entropy_rows_that_do_not_count_leave_no_trace(hip):
     rng = np.random.default_rng(2)
-    for rows, k, vocab in ((9, 20, 50), (140, 64, 700)):
+    for rows, k, vocab in ((9, 20, 50), (140, 64, 700), (700, 500, 1009)):
         x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
         targets, weights = rng.integers(0, vocab, rows), rng.random(rows).astype(np.float32)
         targets[[1, 4]] = -1, -(1 << 40)
@@ -338,26 +347,41 @@ def test_cross_entropy_rows_that_do_not_count_leave_no_trace(hip):
 
 def test_cross_entropy_targets_past_the_vocabulary(hip):
     rng = np.random.default_rng(3)
-    x, w = rng.standard_normal((6, 8)).astype(np.float32), rng.standard_normal((8, 33)).astype(np.float32)
-    targets = np.array([0, 33, 5, 1 << 40, 32, 2])
-    value, dx, dw, _ = loss(hip, x, w, None, targets)
-    assert np.isnan(value[[1, 3]]).all() and np.isnan(dx[[1, 3]]).all() and np.isnan(dw).all()
-    good = [0, 2, 4, 5]
-    want, bound = D.cross_entropy(x[good], w, None, targets[good]), D.cross_entropy_bounds(x[good], w, None, targets[good])
-    close(value[good], want[0], bound[0])
-    close(dx[good], want[1], bound[1])
-    assert np.array_equal(np.isnan(loss(hip, x, w, None, targets, grads=False)), np.isnan(value))
+    for rows, k, vocab in ((6, 8, 33), (700, 500, 1009)):
+        x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
+        targets = rng.integers(0, vocab, rows)
+        targets[[1, 3, 4]] = vocab, 1 << 40, vocab - 1
+        value, dx, dw, _ = loss(hip, x, w, None, targets)
+        assert np.isnan(value[[1, 3]]).all() and np.isnan(dx[[1, 3]]).all() and np.isnan(dw).all()
+        good = [r for r in range(rows) if r not in (1, 3)]
+        want, bound = D.cross_entropy(x[good], w, None, targets[good]), D.cross_entropy_bounds(x[good], w, None, targets[good])
+        close(value[good], want[0], bound[0])
+        close(dx[good], want[1], bound[1])
+        assert np.array_equal(np.isnan(loss(hip, x, w, None, targets, grads=False)), np.isnan(value))
 
 
 def test_cross_entropy_of_barred_and_extreme_logits(hip):
     """A bias of -inf, or of the lowest float, bars a word; a target so barred has an infinite loss; logits of 1e30 give
     weights of 0 and 1; one NaN logit makes its row NaN."""
     rng = np.random.default_rng(4)
-    x, w = rng.standard_normal((5, 16)).astype(np.float32), rng.standard_normal((16, 300)).astype(np.float32)
-    targets = np.array([0, 7, 299, 100, 5])
+    for rows, k, vocab in ((5, 16, 300), (500, 600, 1001)):
+        barred(hip, rng, rows, k, vocab)
+    big = np.zeros((2, 1), np.float32) + 1e15
+    wide = np.array([[1e15, -1e15, 0]], np.float32)
+    value, dx, dw, _ = loss(hip, big, wide, None, np.array([0, 2]))
+    assert value[0] == 0 and abs(value[1] / 1e30 - 1) < 1e-6
+    assert np.array_equal(dw, [[1e15 * np.float32(1), 0, -1e15 * np.float32(1)]])
+
+
+def barred(hip, rng, rows, k, vocab):
+    x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
+    if k > 16:
+        w *= np.float32(k ** -0.5)
+    targets = rng.integers(0, vocab, rows)
+    targets[[1, 2]] = 7, vocab - 1
     for low in (-np.inf, np.finfo(np.float32).min):
-        b = np.where(np.arange(300) % 2 == 0, 0, low).astype(np.float32)
-        b[[7, 299, 5]] = 0
+        b = np.where(np.arange(vocab) % 2 == 0, 0, low).astype(np.float32)
+        b[targets] = 0
         open_ = b == 0
         want = D.cross_entropy(x, w[:, open_], None, np.cumsum(open_)[targets] - 1)
         bound = D.cross_entropy_bounds(x, w[:, open_], None, np.cumsum(open_)[targets] - 1)
@@ -366,31 +390,29 @@ def test_cross_entropy_of_barred_and_extreme_logits(hip):
         close(got[1], want[1], bound[1])
         close(got[2][:, open_], want[2], bound[2])
         assert (got[2][:, ~open_] == 0).all() and (got[3][~open_] == 0).all()
+    targets[targets == 1] = 2
     targets[1] = 1
-    value = loss(hip, x, w, b := np.where(np.arange(300) == 1, -np.inf, 0).astype(np.float32), targets, grads=False)
+    b = np.where(np.arange(vocab) == 1, -np.inf, 0).astype(np.float32)
+    value = loss(hip, x, w, b, targets, grads=False)
     assert value[1] == np.inf and np.isfinite(np.delete(value, 1)).all()
-    assert np.isnan(loss(hip, x, w, np.full(300, -np.inf, np.float32), targets, grads=False)).all()
+    assert np.isnan(loss(hip, x, w, np.full(vocab, -np.inf, np.float32), targets, grads=False)).all()
     b[:] = 0
     b[9] = np.nan
     assert np.isnan(loss(hip, x, w, b, targets, grads=False)).all()
-    big = np.zeros((2, 1), np.float32) + 1e15
-    wide = np.array([[1e15, -1e15, 0]], np.float32)
-    value, dx, dw, _ = loss(hip, big, wide, None, np.array([0, 2]))
-    assert value[0] == 0 and abs(value[1] / 1e30 - 1) < 1e-6
-    assert np.array_equal(dw, [[1e15 * np.float32(1), 0, -1e15 * np.float32(1)]])
 
 
 def test_cross_entropy_without_parts(hip):
     rng = np.random.default_rng(5)
-    x, w = rng.standard_normal((70, 40)).astype(np.float32), rng.standard_normal((40, 90)).astype(np.float32)
-    targets = rng.integers(0, 90, 70)
-    full = loss(hip, x, w, None, targets)
-    bound = D.cross_entropy_bounds(x, w, None, targets)
-    for want in ((True, False, False), (False, True, False), (False, True, True), (False, False, False)):
-        got = loss(hip, x, w, None, targets, want=want)
-        for a, f, e, t in zip(got, full, bound, (True, *want)):
-            if t:
-                close(a, f.astype(np.float64), 2 * e)
+    for rows, k, vocab in ((70, 40, 90), (600, 500, 1003)):
+        x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
+        targets = rng.integers(0, vocab, rows)
+        full = loss(hip, x, w, None, targets)
+        bound = D.cross_entropy_bounds(x, w, None, targets)
+        for want in ((True, False, False), (False, True, False), (False, True, True), (False, False, False)):
+            got = loss(hip, x, w, None, targets, want=want)
+            for a, f, e, t in zip(got, full, bound, (True, *want)):
+                if t:
+                    close(a, f.astype(np.float64), 2 * e)
     dw, db, spare = (up(hip, np.full(s, 7, np.float32)) for s in ((4, 9), (8,), (3, 4)))
     hip.check(hip.lib().lmp_k_linear_cross_entropy_grad_f32(0, 4, 8, None, 4, None, 8, None, None, None, None, spare.ptr, 4, dw.ptr,
                                                             9, db.ptr))
