@@ -12,9 +12,9 @@
 
 #include "common.hpp"
 #include "gemm_half.hpp"
+#include "half_panels.hpp"
 #include "half_products.hpp"
 #include "lmp_hip_transformer.h"
-#include "strips.hpp"
 
 namespace lmp_hip {
 namespace {
@@ -138,15 +138,13 @@ __device__ __forceinline__ float over_eight(float x, bool most) {
 
 template <int NT, int MINB, class C>
 __global__ __launch_bounds__(NT, MINB) void half_logits(HalfArgs g, HalfLogits o) {
-  static_assert(NT == C::THREADS, "one lane per thread of the configuration");
+  static_assert(NT == C::THREADS && C::TN == 2, "a wave has 64 columns");
   __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
   hv16 acc[C::TM][C::TN];
   const HalfItem at = half_item(g, int(blockIdx.x));
-  const int n0 = at.tile_n * C::BN;
-  const bool scaled = half_tile<C, false, false>(g, at, n0, [&](int c) { return min(c, g.n - 1 - n0); }, smem, acc);
-  const int wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % C::WN, col0 = n0 + wn * 64;
-  const uint32_t* const tops[2] = {g.b_top + col0, g.b_top + col0 + 32};
-  half_epilogue<C>(g, at, scaled, smem, tops, acc, [&](int row, int c4, hv4 (&v)[2]) {
+  half_tile<C>(g, at, smem, acc);
+  const int wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % C::WN, col0 = at.tile_n * C::BN + wn * 64;
+  half_epilogue<C>(g, at, smem, acc, [&](int row, int c4, hv4 (&v)[2]) {
     const float low = -__builtin_huge_valf();
     const int64_t target = row < g.m ? o.targets[row] : -1;
     float top = low;
@@ -208,52 +206,29 @@ __global__ __launch_bounds__(256) void half_loss_rows(HalfRows a) {
     if (a.info) {
       const float w = !counted ? 0.0f : !known ? nan : a.weights ? a.weights[row] : 1.0f;
       a.info[row] = {s.top, w / s.sum, w, counted && known ? int(t) : counted ? -2 : -1};
-      a.row_top[row] = magnitude(w);
+      a.row_top[row] = finite_magnitude(w);
     }
   }
 }
 
-// dz over z, with its columns' largest magnitudes and (SUMS) their sums over each strip.
-struct HalfGrad {
-  StripShape s;
-  float* z;
+// dz, formed from the logits.
+struct LossGradient {
+  int64_t rows;
+  int cols;
+  const float* z;  // [rows, cols]
   const LossRow* info;
-  uint32_t* col_top;
-  float* sums;  // [strips, vocab]
-};
-template <bool SUMS>
-__global__ __launch_bounds__(kStripThreads) void half_loss_grad(HalfGrad o) {
-  const int col = strip_col(), n = o.s.cols;
-  uint32_t top[4] = {0, 0, 0, 0};
-  hv4 sum = hv4(0.0f);
-  const int64_t end = strip_end(o.s);
-#pragma unroll 4
-  for (int64_t row = strip_begin(o.s); row < end; ++row) {
-    const LossRow r = o.info[row];
-    float* z = o.z + row * n;
-    hv4 v = load_four(z, col, n);
+  __device__ __forceinline__ hv4 load(int64_t row, int col) const {
+    const LossRow r = info[row];
+    hv4 v = load_four(z + row * cols, col, cols);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float p = exp_below(v[e] - r.top) * r.factor;
-      v[e] = r.target == -1 ? 0.0f : col + e == r.target ? p - r.weight : p;
-      top[e] = max(top[e], magnitude(v[e]));
+      v[e] = r.target == -1 || col + e >= cols ? 0.0f : col + e == r.target ? p - r.weight : p;
     }
-    store_four(z, col, n, v);
-    if constexpr (SUMS) sum = sum + v;
+    return v;
   }
-  raise_cols(o.col_top, col, n, top);
-  if constexpr (SUMS) store_four(o.sums + int64_t(blockIdx.y) * n, col, n, sum);
-}
-
-// The rows of x, zeros in place of those that are not counted: 0 x infinity would be NaN.
-__global__ __launch_bounds__(256) void counted_rows(const float* x, int64_t ldx, int64_t rows, int in,
-                                                    const int64_t* targets, float* out) {
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const bool counted = targets[row] >= 0;
-    for (int i = threadIdx.x * 4; i < in; i += 1024)
-      store_four(out + row * in, i, in, counted ? load_four(x + row * ldx, i, in) : hv4(0.0f));
-  }
-}
+  __device__ __forceinline__ int place(int col) const { return col; }
+};
 
 struct LossCall {
   size_t rows, in, vocab;
@@ -289,41 +264,38 @@ constexpr uint64_t kHalfWork = uint64_t(1) << 28;
 
 int run_loss_half(Runtime* rt, const LossCall& c) {
   const bool grad = c.dx || c.dw;
-  // Pieces of whole tiles of rows.
+  // Pieces of whole groups of panels.
   const size_t fit = std::max<size_t>(256, kPieceBytes / (c.vocab * sizeof(float)) / 256 * 256);
   const size_t pieces = grad ? (c.rows + fit - 1) / fit : 1;
-  size_t each = (c.rows + pieces - 1) / pieces;
-  if (pieces > 1) each = (each + 255) / 256 * 256;
-  // A product's K takes 32 rows: fewer at the end join the last piece.
-  const size_t most = std::min(c.rows, each + 31);
-  const HalfPlan plan = half_plan(rt->cu_count, 0, int64_t(most), int64_t(c.vocab), int64_t(c.in), false);
+  const size_t each = pieces > 1 ? ((c.rows + pieces - 1) / pieces + 255) / 256 * 256 : c.rows;
+  const HalfPlan plan = half_plan(rt->cu_count, 0, int64_t(each), int64_t(c.vocab), int64_t(c.in), false);
   if (plan.cfg < 0) return fail(LMP_ERR_UNSUPPORTED, "linear_cross_entropy: more tiles than a grid holds");
   const int bn = kHalfTiles[plan.cfg].bn, parts = int((c.vocab + bn - 1) / bn) * (bn / 64);
-  const StripShape strips = strips_of(rt, most, c.vocab);
-  // The workspace, each part a multiple of 256 bytes.
-  size_t total = 0;
-  const auto room = [&](size_t words) {
-    const size_t at = total;
-    total += (words + 63) / 64 * 64;
-    return at;
-  };
-  const size_t at_z = room(grad ? most * c.vocab : 0), at_x = room(c.dw ? c.rows * c.in : 0);
-  const size_t at_part = room(most * size_t(parts) * 2), at_hit = room(most), at_info = room(grad ? most * 4 : 0);
-  const size_t at_sums = room(c.db ? size_t(strips.strips) * c.vocab : 0), at_db = room(c.db ? c.vocab : 0);
-  const size_t at_tops = total;
-  const size_t at_xr = room(half_tops_room(c.rows)), at_wc = room(half_tops_room(c.vocab));
-  const size_t at_xc = room(c.dw ? half_tops_room(c.in) : 0), at_wr = room(c.dx ? half_tops_room(c.in) : 0);
-  const size_t at_dr = room(grad ? half_tops_room(most) : 0), at_dc = room(grad ? half_tops_room(c.vocab) : 0);
-  float* base = static_cast<float*>(scratch_alloc(total * sizeof(float)));
+  const size_t strips = c.db ? size_t(most_strips(rt, int64_t(each), int64_t(c.vocab))) : 0;
+  HalfRoom room;
+  const size_t of_xr = room.take(half_tops_words(c.rows)), of_wc = room.take(half_tops_words(c.vocab));
+  const size_t of_xc = room.take(c.dw ? half_tops_words(c.in) : 0), of_wr = room.take(c.dx ? half_tops_words(c.in) : 0);
+  const size_t of_dr = room.take(grad ? half_tops_words(each) : 0), of_dc = room.take(grad ? half_tops_words(c.vocab) : 0);
+  const size_t tops = room.words;
+  const size_t at_part = room.take(each * size_t(parts) * 2), at_hit = room.take(each), at_info = room.take(grad ? each * 4 : 0);
+  const size_t at_sums = room.take(strips * c.vocab), at_db = room.take(c.db ? c.vocab : 0);
+  const size_t at_z = room.take(grad ? each * c.vocab : 0);
+  const size_t at_xr = room.take(half_panel_words(c.rows, c.in)), at_wc = room.take(half_panel_words(c.vocab, c.in));
+  const size_t at_xc = room.take(c.dw ? half_panel_words(c.in, c.rows) : 0);
+  const size_t at_wr = room.take(c.dx ? half_panel_words(c.in, c.vocab) : 0);
+  const size_t at_dr = room.take(c.dx ? half_panel_words(each, c.vocab) : 0);
+  const size_t at_dc = room.take(c.dw ? half_panel_words(c.vocab, each) : 0);
+  float* base = static_cast<float*>(scratch_alloc(room.words * sizeof(float)));
   if (!base) return LMP_ERR_OOM;
   uint32_t* words = reinterpret_cast<uint32_t*>(base);
-  uint32_t *x_row = words + at_xr, *w_col = words + at_wc, *x_col = words + at_xc, *w_row = words + at_wr;
-  uint32_t *d_row = words + at_dr, *d_col = words + at_dc;
-  const float* x = c.x;
-  size_t ldx = c.ldx;
+  const auto panels = [&](size_t at, size_t k, size_t of) {
+    return HalfPanels{reinterpret_cast<char*>(words + at), int64_t(half_stride(k)), words + of};
+  };
+  const HalfPanels none{}, xr = panels(at_xr, c.in, of_xr), wc = panels(at_wc, c.in, of_wc);
+  const HalfPanels xc = c.dw ? panels(at_xc, c.rows, of_xc) : none, wr = c.dx ? panels(at_wr, c.vocab, of_wr) : none;
   const auto piece = [&](size_t at, size_t n) -> int {
-    const float* xp = x + at * ldx;
-    const HalfArgs g = half_args(xp, int(ldx), c.w, int(c.ldw), int(n), int(c.vocab), int(c.in), x_row + at, w_col, plan);
+    const HalfPanels mine{xr.panels + int64_t(at / 64) * xr.stride, xr.stride, xr.tops + at};
+    const HalfArgs g = half_args(mine, wc, int(n), int(c.vocab), int(c.in), plan);
     float* z = grad ? base + at_z : nullptr;
     Softmax* part = reinterpret_cast<Softmax*>(base + at_part);
     LossRow* info = grad ? reinterpret_cast<LossRow*>(base + at_info) : nullptr;
@@ -336,43 +308,39 @@ int run_loss_half(Runtime* rt, const LossCall& c) {
         }))
       return s;
     const HalfRows r{int64_t(n), parts, int(c.vocab), part, base + at_hit, c.targets + at,
-                     c.weights ? c.weights + at : nullptr, c.loss + at, info, d_row};
+                     c.weights ? c.weights + at : nullptr, c.loss + at, info, words + of_dr};
     half_loss_rows<<<dim3(uint32_t(std::min<size_t>((n + 3) / 4, 65536))), dim3(256), 0, rt->stream>>>(r);
     LMP_LAUNCH_CHECK("half_loss_rows");
     if (!grad) return LMP_OK;
     if (at)
-      if (int s = clear_words(rt, d_col, half_tops_room(c.vocab))) return s;
-    StripShape mine = strips;
-    mine.rows = int64_t(n);
-    mine.strips = int((int64_t(n) + mine.each - 1) / mine.each);
-    const HalfGrad d{mine, z, info, d_col, base + at_sums};
-    if (c.db) half_loss_grad<true><<<strip_grid(mine), dim3(kStripThreads), 0, rt->stream>>>(d);
-    else half_loss_grad<false><<<strip_grid(mine), dim3(kStripThreads), 0, rt->stream>>>(d);
-    LMP_LAUNCH_CHECK("half_loss_grad");
-    if (c.db) {
-      float* to = at ? base + at_db : c.db;
-      if (int s = lmp_k_reduce(LMP_RED_SUM, LMP_FLOAT32, to, base + at_sums, 1, size_t(mine.strips), c.vocab)) return s;
-      if (at)
-        if (int s = lmp_k_add_inplace(LMP_FLOAT32, c.db, to, c.vocab)) return s;
+      if (int s = clear_words(rt, words + of_dc, half_tops_words(c.vocab))) return s;
+    const HalfPanels dr = c.dx ? panels(at_dr, c.vocab, of_dr) : none, dc = c.dw ? panels(at_dc, n, of_dc) : none;
+    const LossGradient of_d{int64_t(n), int(c.vocab), z, info};
+    if (c.dw) {
+      const auto job = tops_job(rt, of_d, nullptr, dc.tops, c.db ? base + at_sums : nullptr);
+      if (int s = run_panel_jobs(rt, job, NoJob{})) return s;
+      if (c.db) {
+        float* to = at ? base + at_db : c.db;
+        const size_t mine_strips = size_t(job.blocks / job.col_blocks);
+        if (int s = lmp_k_reduce(LMP_RED_SUM, LMP_FLOAT32, to, base + at_sums, 1, mine_strips, c.vocab)) return s;
+        if (at)
+          if (int s = lmp_k_add_inplace(LMP_FLOAT32, c.db, to, c.vocab)) return s;
+      }
     }
-    return half_backward(rt, {n, c.in, c.vocab, z, c.vocab, d_row, d_col, xp, ldx, x_col, c.w, c.ldw, w_row,
-                              c.dx ? c.dx + at * c.lddx : nullptr, c.lddx, c.dw, c.lddw, at > 0});
+    if (int s = run_panel_jobs(rt, pack_job(of_d, dr, dc), NoJob{})) return s;
+    HalfPanels xp = xc;  // K of dw from this piece's first row on
+    if (c.dw) xp.panels += int64_t(at / kHalfK) * kHalfStep;
+    return half_backward(rt, {n, c.in, c.vocab, dr, dc, xp, wr, c.dx ? c.dx + at * c.lddx : nullptr, c.lddx, c.dw, c.lddw,
+                              at > 0, 0});
   };
   const auto run = [&]() -> int {
-    if (int s = clear_words(rt, words + at_tops, total - at_tops)) return s;
-    if (c.dw) {
-      counted_rows<<<dim3(uint32_t(std::min<size_t>(c.rows, 65536))), dim3(256), 0, rt->stream>>>(
-          c.x, int64_t(c.ldx), int64_t(c.rows), int(c.in), c.targets, base + at_x);
-      LMP_LAUNCH_CHECK("counted_rows");
-      x = base + at_x;
-      ldx = c.in;
-    }
-    if (int s = half_tops(rt, x, c.rows, c.in, ldx, x_row, c.dw ? x_col : nullptr)) return s;
-    if (int s = half_tops(rt, c.w, c.in, c.vocab, c.ldw, c.dx ? w_row : nullptr, w_col)) return s;
-    for (size_t at = 0, n; at < c.rows; at += n) {
-      n = c.rows - at <= most ? c.rows - at : each;
-      if (int s = piece(at, n)) return s;
-    }
+    if (int s = clear_words(rt, words, tops)) return s;
+    const MatrixSource of_x{int64_t(c.rows), int(c.in), c.x, int64_t(c.ldx), c.targets};
+    const MatrixSource of_w{int64_t(c.in), int(c.vocab), c.w, int64_t(c.ldw), nullptr};
+    if (int s = run_panel_jobs(rt, tops_job(rt, of_w, wr.tops, wc.tops), tops_job(rt, of_x, xr.tops, xc.tops))) return s;
+    if (int s = run_panel_jobs(rt, pack_job(of_w, wr, wc), pack_job(of_x, xr, xc))) return s;
+    for (size_t at = 0; at < c.rows; at += each)
+      if (int s = piece(at, std::min(each, c.rows - at))) return s;
     return LMP_OK;
   };
   const int rc = run();
@@ -385,7 +353,7 @@ int run_loss(Runtime* rt, const LossCall& c) {
     if (int s = clear_f32(rt, c.dw, c.in, c.vocab, c.lddw)) return s;
     return clear_f32(rt, c.db, 1, c.vocab, c.vocab);
   }
-  if (half_fits(c.rows, c.in, c.vocab, std::max({c.ldx, c.ldw, c.vocab})) &&
+  if (half_fits(c.rows, c.in, c.vocab) &&
       uint64_t(c.rows) * c.in * c.vocab >= kHalfWork)
     return run_loss_half(rt, c);
   const size_t fit = std::max<size_t>(256, kPieceBytes / (c.vocab * sizeof(float)));

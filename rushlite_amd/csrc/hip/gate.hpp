@@ -12,6 +12,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "lmp_hip_transformer.h"
 
 namespace lmp_hip {
@@ -24,34 +26,41 @@ __device__ __forceinline__ void logistic(float v, float& s, float& rest) {
   rest = v < 0 ? big : small;
 }
 
-__device__ __forceinline__ void gate_of(int gate, float a, float& act, float& slope) {
+template <int GATE>
+__device__ __forceinline__ void gate_at(float a, float& act, float& slope) {
   constexpr float kTwoC = 1.5957691216057308f, kCube = 0.044715f;
   float s, rest;
+  if constexpr (GATE == LMP_GATE_SILU) {
+    logistic(a, s, rest);
+    act = a * s;
+    slope = s + act * rest;
+  } else if constexpr (GATE == LMP_GATE_GELU) {
+    s = 0.5f * erfcf(a * -0.70710678118654752f);
+    act = a * s;
+    slope = s + a * expf(a * a * -0.5f) * 0.39894228040143268f;
+  } else if constexpr (GATE == LMP_GATE_GELU_TANH) {
+    logistic(a * kTwoC * (1.0f + kCube * a * a), s, rest);
+    act = a * s;
+    slope = s + act * rest * (kTwoC * (1.0f + 3.0f * kCube * a * a));
+  } else if constexpr (GATE == LMP_GATE_RELU) {
+    act = a < 0.0f ? 0.0f : a;
+    slope = a > 0.0f ? 1.0f : 0.0f;
+  } else {
+    logistic(a, s, rest);
+    act = s;
+    slope = s * rest;
+  }
+}
+
+// Calls f with the gate as a constant.
+template <class F>
+__host__ __device__ __forceinline__ auto with_gate(int gate, F&& f) {
   switch (gate) {
-    case LMP_GATE_SILU:
-      logistic(a, s, rest);
-      act = a * s;
-      slope = s + act * rest;
-      return;
-    case LMP_GATE_GELU:
-      s = 0.5f * erfcf(a * -0.70710678118654752f);
-      act = a * s;
-      slope = s + a * expf(a * a * -0.5f) * 0.39894228040143268f;
-      return;
-    case LMP_GATE_GELU_TANH:
-      logistic(a * kTwoC * (1.0f + kCube * a * a), s, rest);
-      act = a * s;
-      slope = s + act * rest * (kTwoC * (1.0f + 3.0f * kCube * a * a));
-      return;
-    case LMP_GATE_RELU:
-      act = a < 0.0f ? 0.0f : a;
-      slope = a > 0.0f ? 1.0f : 0.0f;
-      return;
-    default:
-      logistic(a, s, rest);
-      act = s;
-      slope = s * rest;
-      return;
+    case LMP_GATE_SILU: return f(std::integral_constant<int, LMP_GATE_SILU>{});
+    case LMP_GATE_GELU: return f(std::integral_constant<int, LMP_GATE_GELU>{});
+    case LMP_GATE_GELU_TANH: return f(std::integral_constant<int, LMP_GATE_GELU_TANH>{});
+    case LMP_GATE_RELU: return f(std::integral_constant<int, LMP_GATE_RELU>{});
+    default: return f(std::integral_constant<int, LMP_GATE_SIGMOID>{});
   }
 }
 

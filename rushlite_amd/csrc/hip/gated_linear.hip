@@ -4,9 +4,10 @@
 //   pre = x W + b = [a | u],  h = act(a) u
 //   d = [g u act'(a) | g act(a)],  dx = d W^T,  dW = x^T d,  db = the column sums of d
 //
-// Large layers run on the fp16 matrix cores (gemm_half.hpp): forward as one kernel, whose
-// epilogue forms h; backward d in one pass, with the largest magnitudes and the column sums,
-// then both products in one launch.  Smaller ones take the framework's fp32 products.
+// Large layers run on the fp16 matrix cores (gemm_half.hpp), their columns 32 of the one half
+// and 32 of the other by turns: forward the product's epilogue forms h; backward d is
+// formed where it is split, and never held whole.  Smaller ones take the framework's fp32
+// products.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -16,9 +17,9 @@
 #include "common.hpp"
 #include "gate.hpp"
 #include "gemm_half.hpp"
+#include "half_panels.hpp"
 #include "half_products.hpp"
 #include "lmp_hip_transformer.h"
-#include "strips.hpp"
 
 namespace lmp_hip {
 namespace {
@@ -46,7 +47,7 @@ __global__ __launch_bounds__(kThreads) void gate_rows(GateArgs a) {
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const float p = a.pre[row * a.ldpre + col], u = a.pre[row * a.ldpre + a.hidden + col];
     float act, slope;
-    gate_of(a.gate, p, act, slope);
+    with_gate(a.gate, [&](auto gate) { gate_at<decltype(gate)::value>(p, act, slope); });
     if constexpr (BACK) {
       const float g = a.g[row * a.ldg + col];
       a.out[row * a.ldo + col] = g * u * slope;
@@ -68,6 +69,55 @@ int launch_gate(Runtime* rt, const GateArgs& a) {
 
 // ------------------------------------------------------- on the fp16 matrix cores
 
+// Columns by turns: how many there are, and what half and column of it column `col` is.
+inline size_t turned_cols(size_t hidden) { return (hidden + 31) / 32 * 64; }
+__device__ __forceinline__ int second_half(int col) { return col / 32 & 1; }
+__device__ __forceinline__ int half_col(int col) { return col / 64 * 32 + col % 32; }
+
+struct GatedWeights {
+  int64_t rows;
+  int cols;
+  const float* w;
+  int64_t ld;
+  int hidden;
+  __device__ __forceinline__ hv4 load(int64_t row, int col) const {
+    return load_four(w + row * ld + second_half(col) * hidden, half_col(col), hidden);
+  }
+  __device__ __forceinline__ int place(int) const { return -1; }
+};
+
+// d, formed from pre and g.
+template <int GATE>
+struct GatedGradient {
+  int64_t rows;
+  int cols, hidden;
+  const float* pre;
+  int64_t ldpre;
+  const float* g;
+  int64_t ldg;
+  __device__ __forceinline__ hv4 load(int64_t row, int col) const {
+    const int c = half_col(col);
+    const bool second = second_half(col);
+    const float* p = pre + row * ldpre;
+    const hv4 a = load_four(p, c, hidden), gr = load_four(g + row * ldg, c, hidden);
+    hv4 u = hv4(0.0f);
+    if (!second) u = load_four(p + hidden, c, hidden);
+    hv4 d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float act, slope;
+      gate_at<GATE>(a[e], act, slope);
+      d[e] = second ? gr[e] * act : gr[e] * u[e] * slope;
+    }
+    return d;
+  }
+  // Where d's column is in db, or -1.
+  __device__ __forceinline__ int place(int col) const {
+    const int c = half_col(col);
+    return c < hidden ? c + second_half(col) * hidden : -1;
+  }
+};
+
 struct HalfGated {
   int gate, hidden;
   const float* bias;
@@ -77,25 +127,17 @@ struct HalfGated {
   int64_t ldpre;
 };
 
-// h (and pre) of a tile: its block columns are the gate's and the other half's by turns, so
-// that a lane ends with both of a hidden value.
+// h (and pre) of a tile: a lane ends with both halves of a hidden value.
 template <int NT, int MINB, class C>
 __global__ __launch_bounds__(NT, MINB) void half_gated(HalfArgs g, HalfGated o) {
-  static_assert(NT == C::THREADS, "one lane per thread of the configuration");
+  static_assert(NT == C::THREADS && C::TN == 2, "a wave has 32 columns of each half");
   __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
   hv16 acc[C::TM][C::TN];
   const HalfItem at = half_item(g, int(blockIdx.x));
-  const int h0 = at.tile_n * (C::BN / 2);
-  const int left = o.hidden - 1 - h0;
-  const auto local = [&](int c) {
-    const int block = c / 32;
-    return min(block / 2 * 32 + c % 32, left) + (block & 1) * o.hidden;
-  };
-  const bool scaled = half_tile<C, false, false>(g, at, h0, local, smem, acc);
+  half_tile<C>(g, at, smem, acc);
   const int wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % C::WN;
-  const int col0 = h0 + wn * 32;
-  const uint32_t* const tops[2] = {g.b_top + col0, g.b_top + o.hidden + col0};
-  half_epilogue<C>(g, at, scaled, smem, tops, acc, [&](int row, int c4, hv4 (&v)[2]) {
+  const int col0 = at.tile_n * (C::BN / 2) + wn * 32;
+  half_epilogue<C>(g, at, smem, acc, [&](int row, int c4, hv4 (&v)[2]) {
     const int col = col0 + c4;
     if (row >= g.m || col >= o.hidden) return;
     if (o.bias) {
@@ -103,12 +145,14 @@ __global__ __launch_bounds__(NT, MINB) void half_gated(HalfArgs g, HalfGated o) 
       v[1] = v[1] + load_four(o.bias + o.hidden, col, o.hidden);
     }
     hv4 h;
+    with_gate(o.gate, [&](auto gate) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float act, slope;
-      gate_of(o.gate, v[0][e], act, slope);
-      h[e] = act * v[1][e];
-    }
+      for (int e = 0; e < 4; ++e) {
+        float act, slope;
+        gate_at<decltype(gate)::value>(v[0][e], act, slope);
+        h[e] = act * v[1][e];
+      }
+    });
     store_four(o.h + row * o.ldh, col, o.hidden, h);
     if (o.pre) {
       float* p = o.pre + row * o.ldpre;
@@ -118,62 +162,92 @@ __global__ __launch_bounds__(NT, MINB) void half_gated(HalfArgs g, HalfGated o) 
   });
 }
 
-// d with its largest magnitudes, and (SUMS) the columns' sums of each strip of rows.
-struct HalfGate {
-  GateArgs a;
-  StripShape s;
-  uint32_t *row_top, *col_top;
-  float* sums;  // [strips, 2 hidden]
-};
-template <bool SUMS>
-__global__ __launch_bounds__(kStripThreads) void half_gate(HalfGate o) {
-  const GateArgs& a = o.a;
-  const int col = strip_col(), n = a.hidden;
-  uint32_t top0[4] = {0, 0, 0, 0}, top1[4] = {0, 0, 0, 0};
-  hv4 sum0 = hv4(0.0f), sum1 = hv4(0.0f);
-  const int64_t end = strip_end(o.s);
-#pragma unroll 2
-  for (int64_t row = strip_begin(o.s); row < end; ++row) {
-    const float* p = a.pre + row * a.ldpre;
-    const hv4 x = load_four(p, col, n), u = load_four(p + n, col, n), g = load_four(a.g + row * a.ldg, col, n);
-    hv4 d0, d1;
-    uint32_t most = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float act, slope;
-      gate_of(a.gate, x[e], act, slope);
-      d0[e] = g[e] * u[e] * slope;
-      d1[e] = g[e] * act;
-      const uint32_t m0 = col + e < n ? magnitude(d0[e]) : 0, m1 = col + e < n ? magnitude(d1[e]) : 0;
-      top0[e] = max(top0[e], m0);
-      top1[e] = max(top1[e], m1);
-      most = max(most, max(m0, m1));
-    }
-    float* out = a.out + row * a.ldo;
-    store_four(out, col, n, d0);
-    store_four(out + n, col, n, d1);
-    if constexpr (SUMS) {
-      sum0 = sum0 + d0;
-      sum1 = sum1 + d1;
-    }
-    raise_row(o.row_top + row, most);
-  }
-  raise_cols(o.col_top, col, n, top0);
-  raise_cols(o.col_top + n, col, n, top1);
-  if constexpr (SUMS) {
-    float* sums = o.sums + int64_t(blockIdx.y) * 2 * n;
-    store_four(sums, col, n, sum0);
-    store_four(sums + n, col, n, sum1);
-  }
-}
-
 // From this many multiply-adds a product on, the fp16 matrix cores make up for the passes
 // that find the largest magnitudes.
 constexpr uint64_t kHalfWork = uint64_t(1) << 28;
 
-bool use_half(size_t rows, size_t in, size_t hidden, size_t most_ld) {
-  return half_fits(rows, in, 2 * hidden, std::max(most_ld, 2 * hidden)) && hidden >= 32 &&
-         uint64_t(rows) * in * 2 * hidden >= kHalfWork;
+bool use_half(size_t rows, size_t in, size_t hidden) {
+  return half_fits(rows, in, 2 * hidden) && hidden >= 32 && uint64_t(rows) * in * 2 * hidden >= kHalfWork;
+}
+
+// The workspace as panels and their rows' magnitudes.
+HalfPanels panels_at(uint32_t* base, size_t panels, size_t k, size_t tops) {
+  return {reinterpret_cast<char*>(base + panels), int64_t(half_stride(k)), base + tops};
+}
+
+int gated_half(Runtime* rt, int gate, size_t rows, size_t in, size_t hidden, const float* x, size_t ldx,
+               const float* w, size_t ldw, const float* bias, float* h, size_t ldh, float* pre, size_t ldpre) {
+  const size_t cols = turned_cols(hidden);
+  const HalfPlan plan = half_plan(rt->cu_count, 0, int64_t(rows), int64_t(cols), int64_t(in), false);
+  if (plan.cfg < 0) return fail(LMP_ERR_UNSUPPORTED, "gated_linear: more tiles than a grid holds");
+  HalfRoom room;
+  const size_t at_x = room.take(half_tops_words(rows)), at_w = room.take(half_tops_words(cols)), tops = room.words;
+  const size_t x_panels = room.take(half_panel_words(rows, in)), w_panels = room.take(half_panel_words(cols, in));
+  uint32_t* base = static_cast<uint32_t*>(scratch_alloc(room.words * sizeof(uint32_t)));
+  if (!base) return LMP_ERR_OOM;
+  const HalfPanels xr = panels_at(base, x_panels, in, at_x), wc = panels_at(base, w_panels, in, at_w), none{};
+  const MatrixSource of_x{int64_t(rows), int(in), x, int64_t(ldx), nullptr};
+  const GatedWeights of_w{int64_t(in), int(cols), w, int64_t(ldw), int(hidden)};
+  const auto run = [&]() -> int {
+    if (int s = clear_words(rt, base, tops)) return s;
+    if (int s = run_panel_jobs(rt, tops_job(rt, of_w, nullptr, wc.tops), tops_job(rt, of_x, xr.tops, nullptr))) return s;
+    if (int s = run_panel_jobs(rt, pack_job(of_w, none, wc), pack_job(of_x, xr, none))) return s;
+    const HalfArgs g = half_args(xr, wc, int(rows), int(cols), int(in), plan);
+    const HalfGated o{gate, int(hidden), bias, h, int64_t(ldh), pre, int64_t(ldpre)};
+    return with_half_cfg(plan.cfg, [&](auto cfg) -> int {
+      using C = decltype(cfg);
+      half_gated<C::THREADS, C::MINB, C><<<dim3(half_items(g)), dim3(C::THREADS), 0, rt->stream>>>(g, o);
+      LMP_LAUNCH_CHECK("half_gated");
+      return LMP_OK;
+    });
+  };
+  const int rc = run();
+  scratch_free(base);
+  return rc;
+}
+
+int gated_half_backward(Runtime* rt, int gate, size_t rows, size_t in, size_t hidden, const float* g, size_t ldg,
+                        const float* x, size_t ldx, const float* w, size_t ldw, const float* pre, size_t ldpre,
+                        float* dx, size_t lddx, float* dw, size_t lddw, float* db) {
+  const size_t cols = turned_cols(hidden), width = 2 * hidden;
+  const size_t most = size_t(most_strips(rt, int64_t(rows), int64_t(cols)));
+  HalfRoom room;
+  const size_t at_dr = room.take(half_tops_words(rows)), at_dc = room.take(half_tops_words(cols));
+  const size_t at_x = room.take(half_tops_words(in)), at_w = room.take(half_tops_words(in)), tops = room.words;
+  const size_t d_rows = room.take(dx ? half_panel_words(rows, cols) : 0);
+  const size_t d_cols = room.take(dw ? half_panel_words(cols, rows) : 0);
+  const size_t x_panels = room.take(dw ? half_panel_words(in, rows) : 0);
+  const size_t w_panels = room.take(dx ? half_panel_words(in, cols) : 0);
+  const size_t at_sums = room.take(db ? most * width : 0);
+  uint32_t* base = static_cast<uint32_t*>(scratch_alloc(room.words * sizeof(uint32_t)));
+  if (!base) return LMP_ERR_OOM;
+  HalfPanels none{}, dr = none, dc = none, xc = none, wr = none;
+  if (dx) dr = panels_at(base, d_rows, cols, at_dr), wr = panels_at(base, w_panels, cols, at_w);
+  if (dw) dc = panels_at(base, d_cols, rows, at_dc), xc = panels_at(base, x_panels, rows, at_x);
+  float* sums = db ? reinterpret_cast<float*>(base + at_sums) : nullptr;
+  const MatrixSource of_x{dw ? int64_t(rows) : 0, int(in), x, int64_t(ldx), nullptr};
+  const GatedWeights of_w{dx ? int64_t(in) : 0, int(cols), w, int64_t(ldw), int(hidden)};
+  size_t strips = 0;
+  const auto run = [&]() -> int {
+    if (int s = clear_words(rt, base, tops)) return s;
+    if (int s = run_panel_jobs(rt, tops_job(rt, of_w, wr.tops, nullptr), tops_job(rt, of_x, nullptr, xc.tops))) return s;
+    if (int s = run_panel_jobs(rt, pack_job(of_w, wr, none), pack_job(of_x, none, xc))) return s;
+    if (int s = with_gate(gate, [&](auto gt) -> int {
+          const GatedGradient<decltype(gt)::value> of_d{int64_t(rows), int(cols), int(hidden), pre, int64_t(ldpre), g, int64_t(ldg)};
+          auto job = tops_job(rt, of_d, dr.tops, dc.tops, sums);
+          job.sums_ld = int64_t(width);
+          strips = size_t(job.blocks / job.col_blocks);
+          if (int e = run_panel_jobs(rt, job, NoJob{})) return e;
+          return dx || dw ? run_panel_jobs(rt, pack_job(of_d, dr, dc), NoJob{}) : LMP_OK;
+        }))
+      return s;
+    if (db)
+      if (int s = lmp_k_reduce(LMP_RED_SUM, LMP_FLOAT32, db, sums, 1, strips, width)) return s;
+    return half_backward(rt, {rows, in, cols, dr, dc, xc, wr, dx, lddx, dw, lddw, false, hidden});
+  };
+  const int rc = run();
+  scratch_free(base);
+  return rc;
 }
 
 }  // namespace
@@ -205,30 +279,8 @@ extern "C" int lmp_k_gated_linear_f32(int gate, size_t rows, size_t in, size_t h
   if (std::max({ldx, ldw, ldh, pre ? ldpre : 0}) >= kGemmMaxExtent)
     return fail(LMP_ERR_UNSUPPORTED, name + "dimension of 2^31 - 4096 or more");
   LMP_RUNTIME_OR_FAIL(rt);
-  if (use_half(rows, in, hidden, std::max(ldx, ldw))) {
-    const size_t of_x = half_tops_room(rows), of_w = half_tops_room(2 * hidden);
-    uint32_t* tops = static_cast<uint32_t*>(scratch_alloc((of_x + of_w) * sizeof(uint32_t)));
-    if (!tops) return LMP_ERR_OOM;
-    const auto run = [&]() -> int {
-      if (int s = clear_words(rt, tops, of_x + of_w)) return s;
-      if (int s = half_tops(rt, x, rows, in, ldx, tops, nullptr)) return s;
-      if (int s = half_tops(rt, w, in, 2 * hidden, ldw, nullptr, tops + of_x)) return s;
-      // A tile of BN columns holds BN / 2 hidden values: the plan's columns are twice as many.
-      const HalfPlan plan = half_plan(rt->cu_count, 0, int64_t(rows), 2 * int64_t(hidden), int64_t(in), false);
-      if (plan.cfg < 0) return fail(LMP_ERR_UNSUPPORTED, name + "more tiles than a grid holds");
-      const HalfArgs g = half_args(x, int(ldx), w, int(ldw), int(rows), int(2 * hidden), int(in), tops, tops + of_x, plan);
-      const HalfGated o{gate, int(hidden), bias, h, int64_t(ldh), pre, int64_t(ldpre)};
-      return with_half_cfg(plan.cfg, [&](auto cfg) -> int {
-        using C = decltype(cfg);
-        half_gated<C::THREADS, C::MINB, C><<<dim3(half_items(g)), dim3(C::THREADS), 0, rt->stream>>>(g, o);
-        LMP_LAUNCH_CHECK("half_gated");
-        return LMP_OK;
-      });
-    };
-    const int rc = run();
-    scratch_free(tops);
-    return rc;
-  }
+  if (use_half(rows, in, hidden))
+    return gated_half(rt, gate, rows, in, hidden, x, ldx, w, ldw, bias, h, ldh, pre, ldpre);
   float* z = pre;
   if (!z) {
     z = static_cast<float*>(scratch_alloc(rows * 2 * hidden * sizeof(float)));
@@ -264,36 +316,8 @@ extern "C" int lmp_k_gated_linear_backward_f32(int gate, size_t rows, size_t in,
     if (int s = clear_f32(rt, dw, in, width, lddw)) return s;
     return clear_f32(rt, db, 1, width, width);
   }
-  if (use_half(rows, in, hidden, std::max(dw ? ldx : 0, dx ? ldw : 0))) {
-    const StripShape strips = strips_of(rt, rows, hidden);
-    const size_t of_d = (rows * width + 63) / 64 * 64, of_sums = db ? (size_t(strips.strips) * width + 63) / 64 * 64 : 0;
-    const size_t of_x = half_tops_room(in), of_row = half_tops_room(rows), of_col = half_tops_room(width);
-    const size_t of_tops = 2 * of_x + of_row + of_col;
-    float* d = static_cast<float*>(scratch_alloc((of_d + of_sums + of_tops) * sizeof(float)));
-    if (!d) return LMP_ERR_OOM;
-    float* sums = d + of_d;
-    uint32_t* x_col = reinterpret_cast<uint32_t*>(sums + of_sums);
-    uint32_t *w_row = x_col + of_x, *d_row = w_row + of_x, *d_col = d_row + of_row;
-    const auto run = [&]() -> int {
-      if (int s = clear_words(rt, x_col, of_tops)) return s;
-      if (dw)
-        if (int s = half_tops(rt, x, rows, in, ldx, nullptr, x_col)) return s;
-      if (dx)
-        if (int s = half_tops(rt, w, in, width, ldw, w_row, nullptr)) return s;
-      const HalfGate o{{gate, int64_t(rows), int(hidden), pre, int64_t(ldpre), g, int64_t(ldg), d, int64_t(width)},
-                       strips, d_row, d_col, sums};
-      if (db) half_gate<true><<<strip_grid(strips), dim3(kStripThreads), 0, rt->stream>>>(o);
-      else half_gate<false><<<strip_grid(strips), dim3(kStripThreads), 0, rt->stream>>>(o);
-      LMP_LAUNCH_CHECK("half_gate");
-      if (db)
-        if (int s = lmp_k_reduce(LMP_RED_SUM, LMP_FLOAT32, db, sums, 1, size_t(strips.strips), width)) return s;
-      return half_backward(rt, {rows, in, width, d, width, d_row, d_col, x, ldx, x_col, w, ldw, w_row, dx, lddx, dw,
-                                lddw, false});
-    };
-    const int rc = run();
-    scratch_free(d);
-    return rc;
-  }
+  if (use_half(rows, in, hidden))
+    return gated_half_backward(rt, gate, rows, in, hidden, g, ldg, x, ldx, w, ldw, pre, ldpre, dx, lddx, dw, lddw, db);
   float* d = static_cast<float*>(scratch_alloc(rows * width * sizeof(float)));
   if (!d) return LMP_ERR_OOM;
   const auto run = [&]() -> int {

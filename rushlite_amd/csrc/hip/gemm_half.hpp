@@ -7,18 +7,25 @@
 // (gemm_bf3.hpp), with a product's error near that of rounding its operands: a sum's
 // error is its own roundings'.
 //
-// Range.  Each row of A and each column of B has a power of two that takes its
-// largest magnitude to [2^14, 2^15), found in a pass of its own (or by the kernel that
-// makes the operand): values down to 2^-17 of the largest keep both parts whole,
-// smaller ones lose at most 2^-40 of it.  The two powers leave the sum at the end, exactly.
-// An infinity or a NaN leaves a sum that is not finite; a workgroup that finds one
-// forms its tile again with fp32 MFMAs on the operands as they are.
+// Range.  Each row of A and each column of B has a power of two that takes its largest
+// finite magnitude to [2^14, 2^15): values down to 2^-17 of the largest keep both parts
+// whole, smaller ones lose at most 2^-40 of it.  The two powers leave the sum at the end,
+// exactly.  An infinity keeps its sign in h and has m = 0; it leaves a sum that is not
+// finite, and a workgroup that finds one forms its tile again with the parts h that are not
+// finite left out of the two small products, where 0 x infinity would be NaN.
 //
-// Structure.  A workgroup owns a BM x BN tile, its waves TM x TN blocks of 32 x 32; K
-// advances 32 at a time through two LDS stages with one barrier a step.  Loads go
-// through registers, one step ahead, are split there (five VALU operations a pair)
-// and stored as two planes of 16-byte octets, [plane][k / 8][row], in which a fragment of
-// one MFMA is one conflict-free 128-bit read a lane.
+// Operands are split once, by kernels of their own (half_products.hip), into panels of 64
+// rows of A, or columns of B:
+//   [row / 64][k / 8][part][row % 64][k % 8], K filled up with zeros to a multiple of 32, rows to 256,
+// so that 64 rows of one octet are a kilobyte in a row, which one wave's load takes to LDS
+// as it is, and in which a fragment of an MFMA is one conflict-free 128-bit read a lane.
+//
+// Structure.  A workgroup owns a BM x BN tile, its waves TM x TN blocks of 32 x 32.  K
+// advances 32 at a time through two LDS stages, each half's fragments read while the products
+// of the half before run.  One barrier a step, in its middle: the stage has been read by
+// then, the next one has arrived, and the loads of the one after it start, a whole step
+// ahead of their use.  Bound by the matrix cores: of a 256 x 256 step's 3072 cycles of MFMA
+// the LDS takes 2048.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -27,6 +34,7 @@
 #include <type_traits>
 
 #include "gemm_plan.hpp"
+#include "half_products.hpp"
 
 namespace lmp_hip {
 namespace {
@@ -39,28 +47,26 @@ typedef float hv4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef float hv16 __attribute__((ext_vector_type(16)));
 typedef uint32_t hu4 __attribute__((ext_vector_type(4)));
 typedef int hi4 __attribute__((ext_vector_type(4)));
+typedef uint16_t hw8 __attribute__((ext_vector_type(8)));
 
 // Kept out of the templates: a target builtin inside a kernel template keeps the host
 // pass from emitting the kernel's launch stub.
 __device__ __forceinline__ hv16 mfma_f16(hf8 a, hf8 b, hv16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ hv16 mfma_full(float a, float b, hv16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+// 16 bytes a lane from memory to LDS: lane l's to lds + 16 l.
+__device__ __forceinline__ void panel_load(const char* src, char* lds) {
+  __builtin_amdgcn_global_load_lds(reinterpret_cast<const float*>(src), reinterpret_cast<float*>(lds), 16, 0, 0);
 }
-// Two values times s into the two parts, packed.
-__device__ __forceinline__ void half_pair(float x, float y, float s, uint32_t& h, uint32_t& m) {
-  const hf2 a = __builtin_convertvector(hv2{x * s, y * s}, hf2);
-  hf2 b;
-  b.x = _Float16(__builtin_fmaf(x, s, -float(a.x)));
-  b.y = _Float16(__builtin_fmaf(y, s, -float(a.y)));
-  h = __builtin_bit_cast(uint32_t, a);
-  m = __builtin_bit_cast(uint32_t, b);
+// This wave's loads and LDS accesses are done, and then the workgroup's.
+__device__ __forceinline__ void panels_settled() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(7 << 4);
+  asm volatile("s_barrier" ::: "memory");
 }
 
-// The exponent of a row's power of two from the bits of its largest magnitude: [2^14,
-// 2^15) where that is at least 2^-112 and finite.  Subnormal rows and rows of zeros take
-// 2^126; infinities and NaN leave their mark whatever they are multiplied by.
+// The exponent of a row's power of two from the bits of its largest finite magnitude: [2^14,
+// 2^15) where that is at least 2^-112.  Smaller rows and rows of zeros take 2^126.
 __device__ __forceinline__ int half_exponent(uint32_t top) { return min(141 - int(top >> 23), 126); }
 __device__ __forceinline__ float power_of(int e) {
   return __builtin_bit_cast(float, uint32_t(e + 127) << 23);
@@ -71,115 +77,25 @@ struct HalfCfg {
   static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, MINB = MINB_;
   static constexpr int NW = WM * WN, THREADS = 64 * NW;
   static constexpr int BM = WM * TM * 32, BN = WN * TN * 32;
-  static constexpr int A_OCT = BM * 16 + 64, B_OCT = BN * 16 + 64;  // bytes
-  static constexpr int A_PLANE = 4 * A_OCT, B_PLANE = 4 * B_OCT;
-  static constexpr int STAGE = 2 * (A_PLANE + B_PLANE);
-  static constexpr int SMEM = 2 * STAGE + 16;  // the stages and the fallback's flag
-  static_assert(2 * STAGE >= NW * 32 * 36 * 4, "the epilogue's wave tiles fit");
-  static_assert(2 * STAGE >= kHalfK * (BM + BN + 8) * 4, "the fallback's panels fit");
+  static constexpr int A_PANELS = BM / 64, PANELS = (BM + BN) / 64;
+  static constexpr int STAGE = PANELS * kHalfStep;
+  static constexpr int LOADS = PANELS * 8 / NW;  // of a wave, a step
+  static constexpr int SMEM = 2 * STAGE + 16;    // the stages and the flag of sums that are not finite
+  static_assert((TM == 1 || TM % 2 == 0) && TN % 2 == 0, "a wave's blocks are whole panels, or half of one");
+  static_assert(2 * STAGE >= NW * 16 * (32 * TN + 4) * 4, "the epilogue's wave tiles fit");
+  static_assert(BM % 64 == 0 && BN % 64 == 0 && LOADS * NW == PANELS * 8, "whole panels, split evenly");
 };
 
-// One operand's panel of R rows (of m or n) x 32 k on its way from memory to LDS.  A
-// thread holds ITEMS items of eight consecutive k of one row.  KMAJOR: k is contiguous.
-template <int R, int THREADS, bool KMAJOR>
-struct HalfPanel {
-  static constexpr int ITEMS = R * 4 / THREADS;
-  static constexpr int PAIRS = ITEMS * 4;
-  static_assert(ITEMS * THREADS == R * 4, "items split evenly over the threads");
-  // A load's address is a uniform base and the lane's own 32-bit offset, constant over K.
-  const char* base;
-  int ld, k[ITEMS], off[ITEMS];
-  uint32_t at[ITEMS];
-  float s[ITEMS];  // the row's power of two
-  float v[ITEMS][8];
-
-  static __device__ __forceinline__ int row_of(int i) {
-    const int q = int(threadIdx.x) + i * THREADS;
-    return KMAJOR ? q / 4 : q % R;
-  }
-  // `origin`: the value at k = 0 of the tile's first row; `local(r)`: how many rows after it
-  // the tile's r-th is; `k0` the first k that load() reads; `tops`: the bits of the largest
-  // magnitudes, from the tile's first row on.
-  template <class Local>
-  __device__ __forceinline__ void init(const float* origin, int ld_, Local&& local, int k0,
-                                       int oct_bytes, const uint32_t* tops) {
-    ld = ld_;
-    base = reinterpret_cast<const char*>(origin + (KMAJOR ? int64_t(k0) : int64_t(k0) * ld));
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int q = int(threadIdx.x) + i * THREADS;
-      const int row = row_of(i), oct = KMAJOR ? q % 4 : q / R;
-      k[i] = 8 * oct;
-      const int r = local(row);
-      at[i] = 4u * (KMAJOR ? uint32_t(r) * uint32_t(ld) + uint32_t(k[i]) : uint32_t(k[i]) * uint32_t(ld) + uint32_t(r));
-      off[i] = oct * oct_bytes + row * 16;
-      s[i] = power_of(half_exponent(tops[r]));
-    }
-  }
-  __device__ __forceinline__ const float* place(int64_t bytes, int i) const {
-    return reinterpret_cast<const float*>(base + bytes + at[i]);
-  }
-  __device__ __forceinline__ void load(int i) {
-    if constexpr (KMAJOR) {
-#pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        const hv4_any x = *reinterpret_cast<const hv4_any*>(place(4 * j, i));
-        v[i][j] = x.x; v[i][j + 1] = x.y; v[i][j + 2] = x.z; v[i][j + 3] = x.w;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = *place(int64_t(j) * ld * 4, i);
-    }
-  }
-  __device__ __forceinline__ void move(int advance) { base += int64_t(advance) * (KMAJOR ? 4 : 4 * int64_t(ld)); }
-  __device__ __forceinline__ void load_all(int advance) {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) load(i);
-    move(advance);
-  }
-  // A step of `left` values of k that starts `after` k past the base, zeros after them.
-  __device__ __forceinline__ void load_tail(int after, int left) {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[i][j] = 0.0f;
-        if (k[i] + j < left) v[i][j] = *place(int64_t(after + j) * (KMAJOR ? 4 : 4 * int64_t(ld)), i);
-      }
-  }
-  __device__ __forceinline__ void put(int i, char* lds, int plane, const uint32_t (&h)[4],
-                                      const uint32_t (&m)[4]) const {
-    *reinterpret_cast<hu4*>(lds + off[i]) = hu4{h[0], h[1], h[2], h[3]};
-    *reinterpret_cast<hu4*>(lds + off[i] + plane) = hu4{m[0], m[1], m[2], m[3]};
-  }
-  __device__ __forceinline__ void store_all(char* lds, int plane) const {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      uint32_t h[4], m[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) half_pair(v[i][2 * j], v[i][2 * j + 1], s[i], h[j], m[j]);
-      put(i, lds, plane, h, m);
-    }
-  }
-  // The values themselves, [k][row] with R + 4 values per k (the fallback).
-  __device__ __forceinline__ void store_values(float* lds) const {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int row = row_of(i);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) lds[(k[i] + j) * (R + 4) + row] = v[i][j];
-    }
-  }
-};
-
-// A product op(A) [m, k] op(B) [k, n].  `a_top` and `b_top`: the bits of the largest
-// magnitude of each row of op(A) and column of op(B), rounded up to 256 of them.
+// A product op(A) [m, k] op(B) [k, n] of panels.  `a_top` and `b_top`: the bits of the
+// largest finite magnitude of each row of op(A) and column of op(B), rounded up to 256 of them.
 struct HalfArgs {
-  const float *a, *b;
-  int m, n, k, lda, ldb;  // lda, ldb below 2^22: a panel's offsets fit 32 bits
+  const char *a, *b;
+  int64_t a_stride, b_stride;  // bytes from panel to panel
+  int m, n;
+  int steps;  // 32-wide k steps
   const uint32_t *a_top, *b_top;
   int tiles_m, tiles_n;
-  int splits, steps_per_split;  // K splits, and 32-wide k steps in each
+  int splits, steps_per_split;
 };
 
 // Where a work item lies: its tile's origin in tiles, and its split of K.
@@ -203,19 +119,23 @@ __device__ __forceinline__ HalfItem half_item(const HalfArgs& g, int id) {
   return {group * kGroup + in_group % gsize, in_group / gsize, split};
 }
 
+// The parts that are finite, zeros in place of the others.
+__device__ __forceinline__ hf8 finite_parts(hf8 x) {
+  const hw8 b = __builtin_bit_cast(hw8, x);
+  hw8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (b[i] & 0x7c00) == 0x7c00 ? uint16_t(0) : b[i];
+  return __builtin_bit_cast(hf8, r);
+}
+
 // The tile's sums, scaled by the powers of two of rows and columns, into acc: block (i, j)
 // of the wave, register r: row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32.
-// The tile's first column of op(B) is b0, its c-th lies b_local(c) after it; rows and
-// columns past the matrix repeat one of it.  Returns false where the sums come from the
-// fallback: unscaled.
-template <class C, bool TA, bool TB, class Local>
-__device__ __forceinline__ bool half_tile(const HalfArgs& g, const HalfItem& at, int b0, Local&& b_local,
-                                          char* smem, hv16 (&acc)[C::TM][C::TN]) {
-  constexpr int TM = C::TM, TN = C::TN, MM = TM * TN;
-  const int m0 = at.tile_m * C::BM;
-  const int k_begin = at.split * g.steps_per_split * kHalfK;
-  const int k_len = min(g.k - k_begin, g.steps_per_split * kHalfK);
-  const int full = k_len / kHalfK, left = k_len % kHalfK, steps = full + (left ? 1 : 0);
+template <class C>
+__device__ __forceinline__ void half_tile(const HalfArgs& g, const HalfItem& at, char* smem,
+                                          hv16 (&acc)[C::TM][C::TN]) {
+  constexpr int TM = C::TM, TN = C::TN;
+  const int first = at.split * g.steps_per_split;
+  const int steps = min(g.steps - first, g.steps_per_split);
   int* flag = reinterpret_cast<int*>(smem + 2 * C::STAGE);
   if (threadIdx.x == 0) *flag = 0;  // set after the K loop's barriers
 
@@ -224,37 +144,40 @@ __device__ __forceinline__ bool half_tile(const HalfArgs& g, const HalfItem& at,
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int li = lane & 31, lh = lane >> 5;
 
-  const auto a_local = [&](int r) { return min(r, g.m - 1 - m0); };
-  const float* a_origin = g.a + (TA ? int64_t(m0) : int64_t(m0) * g.lda);
-  const float* b_origin = g.b + (TB ? int64_t(b0) * g.ldb : int64_t(b0));
-  using PA = HalfPanel<C::BM, C::THREADS, !TA>;
-  using PB = HalfPanel<C::BN, C::THREADS, TB>;
-  PA pa;
-  PB pb;
-  // Loads past the last whole step repeat it (and are not used); a split without a whole
-  // step reads the 32 k before the end of K for them (K >= 32).
-  const int k_load = min(k_begin, g.k - kHalfK);
-  pa.init(a_origin, g.lda, a_local, k_load, C::A_OCT, g.a_top + m0);
-  pb.init(b_origin, g.ldb, b_local, k_load, C::B_OCT, g.b_top + b0);
+  // A wave's loads of a step: `unit` kilobytes from its own first one on.
+  const char* src[C::LOADS];
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+  for (int i = 0; i < C::LOADS; ++i) {
+    const int unit = wave * C::LOADS + i, panel = unit / 8;
+    src[i] = (panel < C::A_PANELS ? g.a + (int64_t(at.tile_m) * C::A_PANELS + panel) * g.a_stride
+                                  : g.b + (int64_t(at.tile_n) * (C::BN / 64) + panel - C::A_PANELS) * g.b_stride) +
+             int64_t(first) * kHalfStep + unit % 8 * 1024;
+  }
+  char* const to = smem + wave * (C::LOADS * 1024);
+  uint32_t ahead = lane * 16;  // of the next step to load
+  const auto issue = [&](int stage) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = hv16(0.0f);
-
-  const int a_at = lh * C::A_OCT + (wm * TM * 32 + li) * 16;
-  const int b_at = 2 * C::A_PLANE + lh * C::B_OCT + (wn * TN * 32 + li) * 16;
-  // Fragments of 16 k: the leading parts of B in two sets, so that the next ones are read
-  // while the leading product runs.
-  hf8 ah[TM], am[TM], bh[2][TN], bm[TN];
-  const auto read_a = [&](hf8 (&f)[TM], const char* s, int plane, int kh) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-      f[i] = *reinterpret_cast<const hf8*>(s + plane * C::A_PLANE + kh * 2 * C::A_OCT + a_at + i * 512);
+    for (int i = 0; i < C::LOADS; ++i) panel_load(src[i] + ahead, to + stage * C::STAGE + i * 1024);
+    ahead += kHalfStep;
   };
-  const auto read_b = [&](hf8 (&f)[TN], const char* s, int plane, int kh) {
+
+  // Fragments of 16 k: A's blocks lie in panels of two, a part a kilobyte on, an octet two.
+  const int a_at = lh * 2048 + wm * TM * 32 / 64 * kHalfStep + wm * TM * 32 % 64 * 16 + li * 16;
+  const int b_at = C::A_PANELS * kHalfStep + lh * 2048 + wn * TN * 32 / 64 * kHalfStep + wn * TN * 32 % 64 * 16 + li * 16;
+  struct Fragments {
+    hf8 ah[TM], am[TM], bh[TN], bm[TN];
+  };
+  const auto read = [&](Fragments& f, const char* stage, int half) {
+    const char* a = stage + half * 4096 + a_at;
+    const char* b = stage + half * 4096 + b_at;
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-      f[j] = *reinterpret_cast<const hf8*>(s + plane * C::B_PLANE + kh * 2 * C::B_OCT + b_at + j * 512);
+    for (int i = 0; i < TM; ++i) f.ah[i] = *reinterpret_cast<const hf8*>(a + i / 2 * kHalfStep + i % 2 * 512);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) f.bm[j] = *reinterpret_cast<const hf8*>(b + 1024 + j / 2 * kHalfStep + j % 2 * 512);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) f.bh[j] = *reinterpret_cast<const hf8*>(b + j / 2 * kHalfStep + j % 2 * 512);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) f.am[i] = *reinterpret_cast<const hf8*>(a + 1024 + i / 2 * kHalfStep + i % 2 * 512);
   };
   const auto product = [&](const hf8 (&x)[TM], const hf8 (&y)[TN]) {
 #pragma unroll
@@ -262,99 +185,49 @@ __device__ __forceinline__ bool half_tile(const HalfArgs& g, const HalfItem& at,
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = mfma_f16(x[i], y[j], acc[i][j]);
   };
+  const auto products = [&](const Fragments& f) {
+    product(f.ah, f.bm);
+    product(f.am, f.bh);
+    product(f.ah, f.bh);
+  };
+  // A half's products with the next half's reads among them: 0x8 MFMA, 0x100 LDS read.
+  const auto order = [&]() {
+    constexpr int READS = 2 * (TM + TN), MFMAS = 3 * TM * TN, EACH = MFMAS * 2 / 3 / READS > 0 ? MFMAS * 2 / 3 / READS : 1;
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, MFMAS - READS * EACH > 0 ? MFMAS - READS * EACH : 1, 0);
+  };
 
-  // The step with the end of K first (when 32 does not divide it), then the whole ones:
-  // stage t % 2 holds step t, the registers the one after it.
-  int ahead = full;  // whole steps not loaded yet
-  const auto advance = [&]() { return ahead > 1 ? kHalfK : 0; };
-  if (left) {
-    pa.load_tail(k_begin - k_load + full * kHalfK, left);
-    pb.load_tail(k_begin - k_load + full * kHalfK, left);
-  } else {
-    pa.load_all(advance());
-    pb.load_all(advance());
-    --ahead;
-  }
-  pa.store_all(smem, C::A_PLANE);
-  pb.store_all(smem + 2 * C::A_PLANE, C::B_PLANE);
-  {
-    const int adv = advance();
-    pa.load_all(adv);
-    pb.load_all(adv);
-    --ahead;
-  }
-  // The leading product of a step's second half is held past the barrier; zeros at first.
 #pragma unroll
-  for (int i = 0; i < TM; ++i) ah[i] = hf8(0);
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
-  for (int j = 0; j < TN; ++j) bh[1][j] = hf8(0);
-  constexpr int PAIRS = PA::PAIRS + PB::PAIRS;
-  const auto step = [&](auto stage_c) {
+    for (int j = 0; j < TN; ++j) acc[i][j] = hv16(0.0f);
+  issue(0);
+  if (steps > 1) issue(1);
+  panels_settled();
+  Fragments f0, f1;
+  read(f0, smem, 0);
+  const auto step = [&](auto stage_c, int t) {
     constexpr int stage = decltype(stage_c)::value;
     const char* s = smem + stage * C::STAGE;
-    char* d = smem + (stage ^ 1) * C::STAGE;
-    __syncthreads();
-    const int adv = advance();
-    --ahead;
-    read_a(am, s, 1, 0);
-    read_b(bh[0], s, 0, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    product(ah, bh[1]);
-    __builtin_amdgcn_sched_barrier(0);
-    read_a(ah, s, 0, 0);
-    read_b(bm, s, 1, 0);
-    uint32_t h[4], m[4];
-#pragma unroll
-    for (int c = 0; c < PAIRS; ++c) {
-      // The five products of the step in order, spread over the pairs; each one's fragments
-      // are read when their registers fall free, a product ahead of it.
-      const int q0 = c * 5 * MM / PAIRS, q1 = (c + 1) * 5 * MM / PAIRS;
-      const bool of_a = c < PA::PAIRS;
-      const int ca = of_a ? c : c - PA::PAIRS;
-      const int it = ca / 4, pr = ca % 4;
-      if (of_a) half_pair(pa.v[it][2 * pr], pa.v[it][2 * pr + 1], pa.s[it], h[pr], m[pr]);
-      else half_pair(pb.v[it][2 * pr], pb.v[it][2 * pr + 1], pb.s[it], h[pr], m[pr]);
-#pragma unroll
-      for (int q = q0; q < q1; ++q) {
-        if (q == MM) read_a(am, s, 1, 1);
-        if (q == 2 * MM) read_b(bh[1], s, 0, 1);
-        if (q == 2 * MM) read_b(bm, s, 1, 1);
-        if (q == 3 * MM) read_a(ah, s, 0, 1);
-        const int pp = q / MM, i = (q % MM) / TN, j = q % TN;
-        const hf8 x = pp == 0 || pp == 3 ? am[i] : ah[i];
-        const hf8 y = pp == 0 || pp == 2 ? bh[0][j] : pp == 3 ? bh[1][j] : bm[j];
-        acc[i][j] = mfma_f16(x, y, acc[i][j]);
-      }
-      if (of_a && pr == 3) {
-        pa.put(it, d, C::A_PLANE, h, m);
-        pa.load(it);
-      }
-      if (!of_a && pr == 3) {
-        pb.put(it, d + 2 * C::A_PLANE, C::B_PLANE, h, m);
-        pb.load(it);
-      }
-      // Masks: 0x8 MFMA, 0x100 LDS read, 0x2 VALU.
-#pragma unroll
-      for (int q = q0; q < q1; ++q) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-      }
-      if (c < PAIRS - 1) __builtin_amdgcn_sched_barrier(0);
-    }
-    pa.move(adv);
-    pb.move(adv);
+    read(f1, s, 1);
+    products(f0);
+    order();
+    panels_settled();
+    if (t + 2 < steps) issue(stage);
+    read(f0, smem + (stage ^ 1) * C::STAGE, 0);  // after the last step: of no use
+    products(f1);
+    order();
   };
   int t = 0;
   while (t + 1 < steps) {
-    step(std::integral_constant<int, 0>{});
-    ++t;
-    step(std::integral_constant<int, 1>{});
-    ++t;
+    step(std::integral_constant<int, 0>{}, t++);
+    step(std::integral_constant<int, 1>{}, t++);
   }
-  if (t < steps) step(std::integral_constant<int, 0>{});
-  product(ah, bh[1]);
-  __syncthreads();
+  if (t < steps) step(std::integral_constant<int, 0>{}, t);
 
   uint32_t top = 0;
 #pragma unroll
@@ -366,47 +239,30 @@ __device__ __forceinline__ bool half_tile(const HalfArgs& g, const HalfItem& at,
         top = max(top, __builtin_bit_cast(uint32_t, float(acc[i][j][r])) & 0x7fffffffu);
   if (top >= 0x7f800000u) *flag = 1;
   __syncthreads();
-  if (!*flag) return true;
+  if (!*flag) return;
 
-  // fp32 MFMAs on the values as they are.
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = hv16(0.0f);
-  pa.init(a_origin, g.lda, a_local, k_load, C::A_OCT, g.a_top + m0);
-  pb.init(b_origin, g.ldb, b_local, k_load, C::B_OCT, g.b_top + b0);
-  constexpr int PITCH_A = C::BM + 4, PITCH_B = C::BN + 4;
-  float* sa = reinterpret_cast<float*>(smem);
-  float* sb = sa + kHalfK * PITCH_A;
+  ahead = lane * 16;
 #pragma unroll 1
   for (int u = 0; u < steps; ++u) {
-    if (u == 0 && left) {
-      pa.load_tail(k_begin - k_load + full * kHalfK, left);
-      pb.load_tail(k_begin - k_load + full * kHalfK, left);
-    } else {
-      const int adv = u + 1 < steps ? kHalfK : 0;
-      pa.load_all(adv);
-      pb.load_all(adv);
+    issue(0);
+    panels_settled();
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      read(f0, smem, half);
+      product(f0.ah, f0.bh);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) f0.ah[i] = finite_parts(f0.ah[i]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) f0.bh[j] = finite_parts(f0.bh[j]);
+      product(f0.ah, f0.bm);
+      product(f0.am, f0.bh);
     }
-    __syncthreads();  // the step before is read
-    pa.store_values(sa);
-    pb.store_values(sb);
-    __syncthreads();
-#pragma unroll 4
-    for (int k = 0; k < kHalfK; k += 2) {
-      float xa[TM], xb[TN];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) xa[i] = sa[(k + lh) * PITCH_A + (wm * TM + i) * 32 + li];
-#pragma unroll
-      for (int j = 0; j < TN; ++j) xb[j] = sb[(k + lh) * PITCH_B + (wn * TN + j) * 32 + li];
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mfma_full(xa[i], xb[j], acc[i][j]);
-    }
+    panels_settled();
   }
-  __syncthreads();  // the epilogue writes over the panels
-  return false;
 }
 
 // Calls f(row, column, values) for every four consecutive columns of the wave's rows: values
@@ -414,9 +270,7 @@ __device__ __forceinline__ bool half_tile(const HalfArgs& g, const HalfItem& at,
 // of every block), unscaled.  Through a wave-private LDS tile of 16 rows (LDS requests
 // of one wave complete in order).
 template <class C, class F>
-__device__ __forceinline__ void half_epilogue(const HalfArgs& g, const HalfItem& at, bool scaled,
-                                              char* smem, const uint32_t* const (&b_tops)[C::TN],
-                                              hv16 (&acc)[C::TM][C::TN], F&& f) {
+__device__ __forceinline__ void half_epilogue(const HalfArgs& g, const HalfItem& at, char* smem, hv16 (&acc)[C::TM][C::TN], F&& f) {
   constexpr int TM = C::TM, TN = C::TN, PITCH = 32 * TN + 4;
   static_assert(2 * C::STAGE >= C::NW * 16 * PITCH * 4, "the wave tiles fit");
   const int lane = threadIdx.x & 63;
@@ -429,7 +283,7 @@ __device__ __forceinline__ void half_epilogue(const HalfArgs& g, const HalfItem&
 #pragma unroll
   for (int j = 0; j < TN; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) eb[j][e] = scaled ? half_exponent(b_tops[j][c4 + e]) : 0;
+    for (int e = 0; e < 4; ++e) eb[j][e] = half_exponent(g.b_top[at.tile_n * C::BN + wn * TN * 32 + j * 32 + c4 + e]);
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -444,7 +298,7 @@ __device__ __forceinline__ void half_epilogue(const HalfArgs& g, const HalfItem&
       for (int q = 0; q < 2; ++q) {
         const int rr = q * 8 + (lane >> 3);
         const int row = at.tile_m * C::BM + (wm * TM + i) * 32 + half * 16 + rr;
-        const int ea = scaled ? half_exponent(g.a_top[row]) : 0;
+        const int ea = half_exponent(g.a_top[row]);
         hv4 v[TN];
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
@@ -469,9 +323,9 @@ __device__ __forceinline__ void store_four(float* row, int col, int n, hv4 v) {
   }
 }
 
-using HalfBig = HalfCfg<2, 4, 4, 2, 1>;   // 256 x 256, 8 waves of 128 x 64
+using HalfBig = HalfCfg<2, 4, 4, 2, 2>;    // 256 x 256, 8 waves of 128 x 64
 using HalfWide = HalfCfg<4, 2, 2, 2, 2>;  // 256 x 128, 8 waves of 64 x 64
-using HalfMid = HalfCfg<4, 2, 1, 2, 4>;   // 128 x 128, 8 waves of 32 x 64, two a CU
+using HalfMid = HalfCfg<2, 2, 2, 2, 2>;   // 128 x 128, 4 waves of 64 x 64, two a CU
 using HalfFlat = HalfCfg<2, 2, 1, 2, 2>;  // 64 x 128, 4 waves of 32 x 64, three a CU
 
 // kHalfTiles is what these types are.
@@ -494,12 +348,11 @@ int with_half_cfg(int cfg, F&& f) {
 }
 
 // The launch arguments of a product under `plan`.
-inline HalfArgs half_args(const float* a, int lda, const float* b, int ldb, int m, int n, int k,
-                          const uint32_t* a_top, const uint32_t* b_top, const HalfPlan& plan) {
+inline HalfArgs half_args(const HalfPanels& a, const HalfPanels& b, int m, int n, int k, const HalfPlan& plan) {
   const HalfTile& t = kHalfTiles[plan.cfg];
   const int steps = (k + kHalfK - 1) / kHalfK, each = (steps + plan.splits - 1) / plan.splits;
-  return {a, b, m, n, k, lda, ldb, a_top, b_top, (m + t.bm - 1) / t.bm, (n + t.bn - 1) / t.bn,
-          (steps + each - 1) / each, each};
+  return {a.panels, b.panels, a.stride, b.stride, m, n, steps, a.tops, b.tops, (m + t.bm - 1) / t.bm,
+          (n + t.bn - 1) / t.bn, (steps + each - 1) / each, each};
 }
 inline uint32_t half_items(const HalfArgs& g) { return uint32_t(int64_t(g.tiles_m) * g.tiles_n * g.splits); }
 

@@ -163,7 +163,8 @@ inline bool bf3_pair_fits(uint64_t a, uint64_t b, int threads) {
 
 // ---------------------------------------------- products on the fp16 matrix cores
 
-constexpr int kHalfK = 32;  // k values per step
+constexpr int kHalfK = 32;         // k values per step
+constexpr int kHalfStep = 8192;    // bytes of a panel's step: 64 rows, both parts
 
 struct HalfPlan {
   int cfg = -1;  // index into kHalfTiles; -1: no launch fits a grid
@@ -178,7 +179,7 @@ struct HalfTile {
 };
 constexpr HalfTile kHalfTiles[] = {{256, 256, 512, 2.9f, 2.9f, 11.0f},
                                    {256, 128, 512, 1.6f, 1.65f, 7.0f},
-                                   {128, 128, 512, 1.0f, 0.92f, 5.0f},
+                                   {128, 128, 256, 1.0f, 0.92f, 5.0f},
                                    {64, 128, 256, 0.75f, 0.56f, 4.0f}};
 
 // Modelled time of tiles of one configuration in `splits` parts of K.

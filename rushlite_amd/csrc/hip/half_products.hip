@@ -1,5 +1,4 @@
-// Largest magnitudes of rows and columns, and a layer's two gradient products, on the fp16
-// matrix cores (gemm_half.hpp).
+// A layer's two gradient products on the fp16 matrix cores (gemm_half.hpp).
 #include "half_products.hpp"
 
 #include <hip/hip_runtime.h>
@@ -7,7 +6,7 @@
 #include <algorithm>
 
 #include "gemm_half.hpp"
-#include "strips.hpp"
+#include "half_panels.hpp"
 
 namespace lmp_hip {
 namespace {
@@ -23,78 +22,65 @@ __global__ __launch_bounds__(kThreads) void clear_rows(float* p, int64_t rows, i
     p[i / cols * ld + i % cols] = 0.0f;
 }
 
-// Bound by memory: 4 bytes a value.
-template <bool ROWS, bool COLS>
-__global__ __launch_bounds__(kStripThreads) void tops_kernel(const float* x, StripShape s, int64_t ld,
-                                                             uint32_t* row_top, uint32_t* col_top) {
-  const int col = strip_col();
-  uint32_t top[4] = {0, 0, 0, 0};
-  const int64_t end = strip_end(s);
-#pragma unroll 4
-  for (int64_t row = strip_begin(s); row < end; ++row) {
-    const hv4 v = load_four(x + row * ld, col, s.cols);
-    uint32_t most = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t bits = magnitude(v[e]);
-      top[e] = max(top[e], bits);
-      most = max(most, bits);
-    }
-    if constexpr (ROWS) raise_row(row_top + row, most);
-  }
-  if constexpr (COLS) raise_cols(col_top, col, s.cols, top);
-}
-
-// Where a product goes: C, or (splits > 1) the parts of each split, [split][m][n].
+// Where a product goes: C, or (splits > 1) the parts of each split, [split][m][n].  `hidden`: as
+// HalfBackward's, of C's columns.
 struct HalfOut {
   float* c;
   int64_t ldc;
-  int accumulate;
+  int accumulate, hidden;
   float* part;
 };
+// Where C holds column `col`, a multiple of 4, and where its run of columns ends.
+__device__ __forceinline__ int place_of(const HalfOut& o, int col, int n, int& end) {
+  end = n;
+  if (!o.hidden) return col;
+  const int second = col / 32 & 1;
+  end = (1 + second) * o.hidden;
+  return col / 64 * 32 + col % 32 + second * o.hidden;
+}
 
-template <class C, bool TA, bool TB>
+template <class C>
 __device__ __forceinline__ void half_plain(const HalfArgs& g, const HalfOut& o, int id, char* smem) {
   hv16 acc[C::TM][C::TN];
   const HalfItem at = half_item(g, id);
-  const int n0 = at.tile_n * C::BN;
-  const bool scaled = half_tile<C, TA, TB>(g, at, n0, [&](int c) { return min(c, g.n - 1 - n0); }, smem, acc);
-  const int wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % C::WN, col0 = n0 + wn * C::TN * 32;
-  const uint32_t* tops[C::TN];
-#pragma unroll
-  for (int j = 0; j < C::TN; ++j) tops[j] = g.b_top + col0 + 32 * j;
+  half_tile<C>(g, at, smem, acc);
+  const int wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % C::WN, col0 = at.tile_n * C::BN + wn * C::TN * 32;
   const bool partial = g.splits > 1;
-  float* out = partial ? o.part + int64_t(at.split) * g.m * g.n : o.c;
-  const int64_t ld = partial ? g.n : o.ldc;
   const bool add = !partial && o.accumulate;
-  half_epilogue<C>(g, at, scaled, smem, tops, acc, [&](int row, int c4, hv4 (&v)[C::TN]) {
+  half_epilogue<C>(g, at, smem, acc, [&](int row, int c4, hv4 (&v)[C::TN]) {
     if (row >= g.m) return;
-    float* p = out + row * ld;
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
       const int col = col0 + 32 * j + c4;
-      if (add) v[j] = load_four(p, col, g.n) + v[j];
-      store_four(p, col, g.n, v[j]);
+      if (partial) {
+        store_four(o.part + (int64_t(at.split) * g.m + row) * g.n, col, g.n, v[j]);
+        continue;
+      }
+      int end;
+      const int to = place_of(o, col, g.n, end);
+      float* p = o.c + row * o.ldc;
+      if (add) v[j] = load_four(p, to, end) + v[j];
+      store_four(p, to, end, v[j]);
     }
   });
 }
 
-template <int NT, int MINB, class C, bool TA, bool TB>
+template <int NT, int MINB, class C>
 __global__ __launch_bounds__(NT, MINB) void half_gemm(HalfArgs g, HalfOut o) {
   static_assert(NT == C::THREADS, "one lane per thread of the configuration");
   __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
-  half_plain<C, TA, TB>(g, o, int(blockIdx.x), smem);
+  half_plain<C>(g, o, int(blockIdx.x), smem);
 }
 
-// A layer's weight gradient (A transposed) and input gradient (B transposed) in one grid:
-// the CUs that the first frees start on the second.
+// A layer's weight gradient and input gradient in one grid: the CUs that the first frees
+// start on the second.
 template <int NT, int MINB, class CW, class CX>
 __global__ __launch_bounds__(NT, MINB) void half_gemm_pair(HalfArgs w, HalfOut wo, HalfArgs x, HalfOut xo) {
   static_assert(NT == CW::THREADS && NT == CX::THREADS, "one workgroup size for both");
   __shared__ __attribute__((aligned(1024))) char smem[CW::SMEM > CX::SMEM ? CW::SMEM : CX::SMEM];
   const int of_w = w.tiles_m * w.tiles_n * w.splits, id = int(blockIdx.x);
-  if (id < of_w) half_plain<CW, true, false>(w, wo, id, smem);
-  else half_plain<CX, false, true>(x, xo, id - of_w, smem);
+  if (id < of_w) half_plain<CW>(w, wo, id, smem);
+  else half_plain<CX>(x, xo, id - of_w, smem);
 }
 
 // C from the parts, added in their order; four values a lane.
@@ -113,9 +99,11 @@ __device__ __forceinline__ void fold_block(const HalfFold& f, int64_t block) {
   hv4 v = load_four(p, col, f.n);
 #pragma unroll 4
   for (int s = 1; s < f.splits; ++s) v = v + load_four(p + s * stride, col, f.n);
+  int end;
+  const int to = place_of(f.o, col, f.n, end);
   float* c = f.o.c + row * f.o.ldc;
-  if (f.o.accumulate) v = load_four(c, col, f.n) + v;
-  store_four(c, col, f.n, v);
+  if (f.o.accumulate) v = load_four(c, to, end) + v;
+  store_four(c, to, end, v);
 }
 __global__ __launch_bounds__(kThreads) void half_fold(HalfFold a, HalfFold b) {
   const int64_t block = blockIdx.x;
@@ -151,17 +139,6 @@ int clear_f32(Runtime* rt, float* p, size_t rows, size_t cols, size_t ld) {
   return LMP_OK;
 }
 
-int half_tops(Runtime* rt, const float* x, size_t rows, size_t cols, size_t ld, uint32_t* row_top,
-              uint32_t* col_top) {
-  const StripShape s = strips_of(rt, rows, cols);
-  const dim3 grid = strip_grid(s);
-  if (row_top && col_top) tops_kernel<true, true><<<grid, dim3(kStripThreads), 0, rt->stream>>>(x, s, int64_t(ld), row_top, col_top);
-  else if (row_top) tops_kernel<true, false><<<grid, dim3(kStripThreads), 0, rt->stream>>>(x, s, int64_t(ld), row_top, col_top);
-  else tops_kernel<false, true><<<grid, dim3(kStripThreads), 0, rt->stream>>>(x, s, int64_t(ld), row_top, col_top);
-  LMP_LAUNCH_CHECK("half_tops");
-  return LMP_OK;
-}
-
 int half_backward(Runtime* rt, const HalfBackward& b) {
   HalfJob w, x;
   const int64_t cus = rt->cu_count;
@@ -169,17 +146,17 @@ int half_backward(Runtime* rt, const HalfBackward& b) {
   if (b.dw) {
     w.wanted = true;
     w.plan = half_plan(cus, kHalfParts, in, width, rows, true);
-    w.o = {b.dw, int64_t(b.lddw), b.dw_accumulate ? 1 : 0, nullptr};
+    w.o = {b.dw, int64_t(b.lddw), b.dw_accumulate ? 1 : 0, int(b.hidden), nullptr};
   }
   if (b.dx) {
     x.wanted = true;
     x.plan = half_plan(cus, kHalfParts, rows, in, width, true);
-    x.o = {b.dx, int64_t(b.lddx), 0, nullptr};
+    x.o = {b.dx, int64_t(b.lddx), 0, 0, nullptr};
   }
   if ((w.wanted && w.plan.cfg < 0) || (x.wanted && x.plan.cfg < 0))
     return fail(LMP_ERR_UNSUPPORTED, "gradient products: more tiles than a grid holds");
-  if (w.wanted) w.g = half_args(b.x, int(b.ldx), b.d, int(b.ldd), in, width, rows, b.x_col, b.d_col, w.plan);
-  if (x.wanted) x.g = half_args(b.d, int(b.ldd), b.w, int(b.ldw), rows, in, width, b.d_row, b.w_row, x.plan);
+  if (w.wanted) w.g = half_args(b.x_cols, b.d_cols, in, width, rows, w.plan);
+  if (x.wanted) x.g = half_args(b.d_rows, b.w_rows, rows, in, width, x.plan);
   size_t parts = 0;
   for (HalfJob* j : {&w, &x})
     if (j->wanted && j->g.splits > 1) parts += (size_t(j->g.splits) * size_t(j->g.m) * size_t(j->g.n) + 3) / 4 * 4;
@@ -194,11 +171,10 @@ int half_backward(Runtime* rt, const HalfBackward& b) {
         p += (size_t(j->g.splits) * size_t(j->g.m) * size_t(j->g.n) + 3) / 4 * 4;
       }
   }
-  const auto alone = [&](const HalfJob& j, auto ta, auto tb) {
+  const auto alone = [&](const HalfJob& j) {
     return with_half_cfg(j.plan.cfg, [&](auto cfg) -> int {
       using C = decltype(cfg);
-      half_gemm<C::THREADS, C::MINB, C, decltype(ta)::value, decltype(tb)::value>
-          <<<dim3(half_items(j.g)), dim3(C::THREADS), 0, rt->stream>>>(j.g, j.o);
+      half_gemm<C::THREADS, C::MINB, C><<<dim3(half_items(j.g)), dim3(C::THREADS), 0, rt->stream>>>(j.g, j.o);
       LMP_LAUNCH_CHECK("half_gemm");
       return LMP_OK;
     });
@@ -226,12 +202,10 @@ int half_backward(Runtime* rt, const HalfBackward& b) {
       });
       if (rc) return rc;
     }
-    using std::false_type;
-    using std::true_type;
     if (!paired && w.wanted)
-      if (int s = alone(w, true_type{}, false_type{})) return s;
+      if (int s = alone(w)) return s;
     if (!paired && x.wanted)
-      if (int s = alone(x, false_type{}, true_type{})) return s;
+      if (int s = alone(x)) return s;
     const auto fold = [&](const HalfJob& j) {
       HalfFold f{j.o, j.g.m, j.g.n, j.g.splits, 0};
       if (j.wanted && j.g.splits > 1) f.blocks = (int64_t(f.m) * ((f.n + 3) / 4) + kThreads - 1) / kThreads;
