@@ -19,9 +19,11 @@
 namespace lmp_hip {
 namespace {
 
-// The larger of s(v) and s(-v) is 1 / (1 + e^-|v|), the smaller e^-|v| times that.
+// The larger of s(v) and s(-v) is 1 / (1 + e^-|v|), the smaller e^-|v| times that.  The
+// reciprocal, of a number from 1 to 2, is the hardware's with one step of Newton's: within a unit.
 __device__ __forceinline__ void logistic(float v, float& s, float& rest) {
-  const float e = expf(-fabsf(v)), big = 1.0f / (1.0f + e), small = e * big;
+  const float e = expf(-fabsf(v)), d = 1.0f + e, r = __builtin_amdgcn_rcpf(d);
+  const float big = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r), small = e * big;
   s = v < 0 ? small : big;
   rest = v < 0 ? big : small;
 }

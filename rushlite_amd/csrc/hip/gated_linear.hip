@@ -74,47 +74,46 @@ inline size_t turned_cols(size_t hidden) { return (hidden + 31) / 32 * 64; }
 __device__ __forceinline__ int second_half(int col) { return col / 32 & 1; }
 __device__ __forceinline__ int half_col(int col) { return col / 64 * 32 + col % 32; }
 
-struct GatedWeights {
+// A unit's eight columns: four of each half.
+struct Turned {
   int64_t rows;
-  int cols;
+  int cols, hidden;
+  __device__ __forceinline__ int column(int unit, int h) const { return unit / 8 * 64 + unit % 8 * 4 + 32 * h; }
+  __device__ __forceinline__ int within(int unit) const { return unit * 4; }  // the first one's place in its half
+  // Where a column is in the matrix itself, or -1.
+  __device__ __forceinline__ int place(int col) const {
+    const int c = half_col(col);
+    return c < hidden ? c + second_half(col) * hidden : -1;
+  }
+};
+struct GatedWeights : Turned {
   const float* w;
   int64_t ld;
-  int hidden;
-  __device__ __forceinline__ hv4 load(int64_t row, int col) const {
-    return load_four(w + row * ld + second_half(col) * hidden, half_col(col), hidden);
+  __device__ __forceinline__ void load(int64_t row, int unit, hv4 (&v)[2]) const {
+    const float* p = w + row * ld;
+    v[0] = load_four(p, within(unit), hidden);
+    v[1] = load_four(p + hidden, within(unit), hidden);
   }
-  __device__ __forceinline__ int place(int) const { return -1; }
 };
 
 // d, formed from pre and g.
 template <int GATE>
-struct GatedGradient {
-  int64_t rows;
-  int cols, hidden;
+struct GatedGradient : Turned {
   const float* pre;
   int64_t ldpre;
   const float* g;
   int64_t ldg;
-  __device__ __forceinline__ hv4 load(int64_t row, int col) const {
-    const int c = half_col(col);
-    const bool second = second_half(col);
+  __device__ __forceinline__ void load(int64_t row, int unit, hv4 (&v)[2]) const {
     const float* p = pre + row * ldpre;
-    const hv4 a = load_four(p, c, hidden), gr = load_four(g + row * ldg, c, hidden);
-    hv4 u = hv4(0.0f);
-    if (!second) u = load_four(p + hidden, c, hidden);
-    hv4 d;
+    const int c = within(unit);
+    const hv4 a = load_four(p, c, hidden), u = load_four(p + hidden, c, hidden), gr = load_four(g + row * ldg, c, hidden);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float act, slope;
       gate_at<GATE>(a[e], act, slope);
-      d[e] = second ? gr[e] * act : gr[e] * u[e] * slope;
+      v[0][e] = gr[e] * u[e] * slope;
+      v[1][e] = gr[e] * act;
     }
-    return d;
-  }
-  // Where d's column is in db, or -1.
-  __device__ __forceinline__ int place(int col) const {
-    const int c = half_col(col);
-    return c < hidden ? c + second_half(col) * hidden : -1;
   }
 };
 
@@ -178,7 +177,7 @@ HalfPanels panels_at(uint32_t* base, size_t panels, size_t k, size_t tops) {
 int gated_half(Runtime* rt, int gate, size_t rows, size_t in, size_t hidden, const float* x, size_t ldx,
                const float* w, size_t ldw, const float* bias, float* h, size_t ldh, float* pre, size_t ldpre) {
   const size_t cols = turned_cols(hidden);
-  const HalfPlan plan = half_plan(rt->cu_count, 0, int64_t(rows), int64_t(cols), int64_t(in), false);
+  const HalfPlan plan = half_plan(rt->cu_count, 0, {int64_t(rows), int64_t(cols), int64_t(in), false, 2.0f}, {});
   if (plan.cfg < 0) return fail(LMP_ERR_UNSUPPORTED, "gated_linear: more tiles than a grid holds");
   HalfRoom room;
   const size_t at_x = room.take(half_tops_words(rows)), at_w = room.take(half_tops_words(cols)), tops = room.words;
@@ -187,12 +186,12 @@ int gated_half(Runtime* rt, int gate, size_t rows, size_t in, size_t hidden, con
   if (!base) return LMP_ERR_OOM;
   const HalfPanels xr = panels_at(base, x_panels, in, at_x), wc = panels_at(base, w_panels, in, at_w), none{};
   const MatrixSource of_x{int64_t(rows), int(in), x, int64_t(ldx), nullptr};
-  const GatedWeights of_w{int64_t(in), int(cols), w, int64_t(ldw), int(hidden)};
+  const GatedWeights of_w{{int64_t(in), int(cols), int(hidden)}, w, int64_t(ldw)};
   const auto run = [&]() -> int {
     if (int s = clear_words(rt, base, tops)) return s;
     if (int s = run_panel_jobs(rt, tops_job(rt, of_w, nullptr, wc.tops), tops_job(rt, of_x, xr.tops, nullptr))) return s;
     if (int s = run_panel_jobs(rt, pack_job(of_w, none, wc), pack_job(of_x, xr, none))) return s;
-    const HalfArgs g = half_args(xr, wc, int(rows), int(cols), int(in), plan);
+    const HalfArgs g = half_args(xr, wc, int(rows), int(cols), int(in), plan.cfg, 1);
     const HalfGated o{gate, int(hidden), bias, h, int64_t(ldh), pre, int64_t(ldpre)};
     return with_half_cfg(plan.cfg, [&](auto cfg) -> int {
       using C = decltype(cfg);
@@ -226,19 +225,19 @@ int gated_half_backward(Runtime* rt, int gate, size_t rows, size_t in, size_t hi
   if (dw) dc = panels_at(base, d_cols, rows, at_dc), xc = panels_at(base, x_panels, rows, at_x);
   float* sums = db ? reinterpret_cast<float*>(base + at_sums) : nullptr;
   const MatrixSource of_x{dw ? int64_t(rows) : 0, int(in), x, int64_t(ldx), nullptr};
-  const GatedWeights of_w{dx ? int64_t(in) : 0, int(cols), w, int64_t(ldw), int(hidden)};
+  const GatedWeights of_w{{dx ? int64_t(in) : 0, int(cols), int(hidden)}, w, int64_t(ldw)};
   size_t strips = 0;
   const auto run = [&]() -> int {
     if (int s = clear_words(rt, base, tops)) return s;
     if (int s = run_panel_jobs(rt, tops_job(rt, of_w, wr.tops, nullptr), tops_job(rt, of_x, nullptr, xc.tops))) return s;
     if (int s = run_panel_jobs(rt, pack_job(of_w, wr, none), pack_job(of_x, none, xc))) return s;
     if (int s = with_gate(gate, [&](auto gt) -> int {
-          const GatedGradient<decltype(gt)::value> of_d{int64_t(rows), int(cols), int(hidden), pre, int64_t(ldpre), g, int64_t(ldg)};
+          const GatedGradient<decltype(gt)::value> of_d{{int64_t(rows), int(cols), int(hidden)}, pre, int64_t(ldpre), g, int64_t(ldg)};
           auto job = tops_job(rt, of_d, dr.tops, dc.tops, sums);
           job.sums_ld = int64_t(width);
           strips = size_t(job.blocks / job.col_blocks);
-          if (int e = run_panel_jobs(rt, job, NoJob{})) return e;
-          return dx || dw ? run_panel_jobs(rt, pack_job(of_d, dr, dc), NoJob{}) : LMP_OK;
+          if (int e = run_panel_job(rt, job)) return e;
+          return dx || dw ? run_panel_job(rt, pack_job(of_d, dr, dc)) : LMP_OK;
         }))
       return s;
     if (db)

@@ -323,9 +323,9 @@ __device__ __forceinline__ void store_four(float* row, int col, int n, hv4 v) {
   }
 }
 
-using HalfBig = HalfCfg<2, 4, 4, 2, 2>;    // 256 x 256, 8 waves of 128 x 64
+using HalfBig = HalfCfg<2, 4, 4, 2, 2>;   // 256 x 256, 8 waves of 128 x 64
 using HalfWide = HalfCfg<4, 2, 2, 2, 2>;  // 256 x 128, 8 waves of 64 x 64
-using HalfMid = HalfCfg<2, 2, 2, 2, 2>;   // 128 x 128, 4 waves of 64 x 64, two a CU
+using HalfMid = HalfCfg<4, 2, 1, 2, 4>;   // 128 x 128, 8 waves of 32 x 64, two a CU
 using HalfFlat = HalfCfg<2, 2, 1, 2, 2>;  // 64 x 128, 4 waves of 32 x 64, three a CU
 
 // kHalfTiles is what these types are.
@@ -347,10 +347,10 @@ int with_half_cfg(int cfg, F&& f) {
   }
 }
 
-// The launch arguments of a product under `plan`.
-inline HalfArgs half_args(const HalfPanels& a, const HalfPanels& b, int m, int n, int k, const HalfPlan& plan) {
-  const HalfTile& t = kHalfTiles[plan.cfg];
-  const int steps = (k + kHalfK - 1) / kHalfK, each = (steps + plan.splits - 1) / plan.splits;
+// The launch arguments of a product.
+inline HalfArgs half_args(const HalfPanels& a, const HalfPanels& b, int m, int n, int k, int cfg, int splits) {
+  const HalfTile& t = kHalfTiles[cfg];
+  const int steps = (k + kHalfK - 1) / kHalfK, each = (steps + splits - 1) / splits;
   return {a.panels, b.panels, a.stride, b.stride, m, n, steps, a.tops, b.tops, (m + t.bm - 1) / t.bm,
           (n + t.bn - 1) / t.bn, (steps + each - 1) / each, each};
 }

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <iterator>
 
@@ -166,48 +167,98 @@ inline bool bf3_pair_fits(uint64_t a, uint64_t b, int threads) {
 constexpr int kHalfK = 32;         // k values per step
 constexpr int kHalfStep = 8192;    // bytes of a panel's step: 64 rows, both parts
 
+struct HalfTile {
+  int bm, bn, threads, per_cu;
+  // Time in us of one 32-wide k step of a workgroup, `alone` on its CU and `shared` per
+  // workgroup where several take turns, and of its first loads and its tile's way out.
+  float alone, shared, ends;
+  float rate;  // TFLOP/s of long products on random operands, where the chip's power holds it back
+};
+constexpr HalfTile kHalfTiles[] = {{256, 256, 512, 1, 1.52f, 1.52f, 11.0f, 400},
+                                   {256, 128, 512, 1, 0.83f, 0.83f, 7.0f, 365},
+                                   {128, 128, 512, 2, 0.59f, 0.45f, 5.5f, 370},
+                                   {64, 128, 256, 3, 0.53f, 0.27f, 4.0f, 345}};
+
+// A product [m, n] over k, none if n is 0; `split`: its K may be.  `ends`: its way out's
+// weight against a plain product's.
+struct HalfSize {
+  int64_t m = 0, n = 0, k = 0;
+  bool split = false;
+  float ends = 1.0f;
+};
+// Tiles of one configuration, the splits of K, and which of the two products is launched first.
 struct HalfPlan {
   int cfg = -1;  // index into kHalfTiles; -1: no launch fits a grid
-  int splits = 1;
+  int splits[2] = {1, 1};
+  bool second_first = false;
 };
 
-// Time of one 32-wide k step of a workgroup, in us: `alone` on its CU, and `shared` per
-// workgroup where several take turns; `ends`: its first loads and its tile's way out.
-struct HalfTile {
-  int bm, bn, threads;
-  float alone, shared, ends;
-};
-constexpr HalfTile kHalfTiles[] = {{256, 256, 512, 2.9f, 2.9f, 11.0f},
-                                   {256, 128, 512, 1.6f, 1.65f, 7.0f},
-                                   {128, 128, 256, 1.0f, 0.92f, 5.0f},
-                                   {64, 128, 256, 0.75f, 0.56f, 4.0f}};
-
-// Modelled time of tiles of one configuration in `splits` parts of K.
-inline float half_time(const HalfTile& t, int64_t cus, int64_t items, int64_t steps) {
-  const float load = float((items + cus - 1) / cus);
-  return load * t.ends + float(steps) * std::max(t.alone, load * t.shared);
+// When the slots are done that take n0 items of t0 each and then n1 of t1 as they fall free.
+inline float half_makespan(int64_t slots, int64_t n0, float t0, int64_t n1, float t1) {
+  const int64_t whole = n0 / slots, late = n0 % slots;
+  const float begin = float(whole) * t0, last = late ? begin + t0 : begin;
+  if (n1 == 0) return last;
+  // Both kinds of slots take turns at t1: the least of the times at which one of them ends a turn
+  // that leaves nothing to do.
+  float best = 0.0f;
+  for (int64_t turns = std::max<int64_t>(n1 / slots, 1);; ++turns) {
+    const float ends[2] = {begin + float(turns) * t1, late ? last + float(turns) * t1 : begin + float(turns) * t1};
+    for (float end : ends) {
+      const int64_t early_turns = int64_t((end - begin) / t1 + 1e-3f), late_turns = int64_t((end - last) / t1 + 1e-3f);
+      if ((slots - late) * early_turns + late * std::max<int64_t>(late_turns, 0) >= n1 && (best == 0.0f || end < best)) best = end;
+    }
+    if (best != 0.0f) return std::max(best, last);
+  }
 }
 
-// Tiles (and, with `splits`, the split of K) with the least modelled time; partials stay
-// within `scratch` bytes and a split keeps at least 128 k.
-inline HalfPlan half_plan(int64_t cus, int64_t scratch, int64_t m, int64_t n, int64_t k, bool split) {
-  const int64_t steps = (k + kHalfK - 1) / kHalfK;
+// The configuration, splits and order with the least modelled time; partial sums stay within
+// `scratch` bytes and a split keeps at least 128 k.  The time at the rate that the chip's power
+// allows (operands of zeros run at 650 TFLOP/s in place of 400) and the makespan at that of a
+// chip that is not held back meet in a norm: 768 x 4096 over 12608 in 192 tiles
+// of 128 x 128 on 256 CUs takes 243 us, of 206 and 237.
+inline HalfPlan half_plan(int64_t cus, int64_t scratch, const HalfSize& a, const HalfSize& b) {
   HalfPlan plan;
   float best = 0.0f;
+  const HalfSize* size[2] = {&a, &b};
   for (int c = 0; c < int(std::size(kHalfTiles)); ++c) {
     const HalfTile& t = kHalfTiles[c];
-    const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
-    for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
-      if (s > 1 && (!split || steps / s < 4 || int64_t(s) * m * n > scratch / int64_t(sizeof(float)))) break;
-      if (uint64_t(tiles) * uint64_t(s) > kMaxGridThreads / uint64_t(t.threads)) break;
-      float us = half_time(t, cus, tiles * s, (steps + s - 1) / s);
-      if (s > 1) us += 3.0f + float(s + 1) * float(m) * float(n) * (4.0f / 5e6f);
-      if (plan.cfg < 0 || us < best) {
-        best = us;
-        plan.cfg = c;
-        plan.splits = s;
+    int64_t tiles[2], steps[2];
+    float power = 0.0f;
+    for (int i = 0; i < 2; ++i) {
+      tiles[i] = (size[i]->m + t.bm - 1) / t.bm * ((size[i]->n + t.bn - 1) / t.bn);
+      steps[i] = (size[i]->k + kHalfK - 1) / kHalfK;
+      power += float(tiles[i]) * float(steps[i]) * float(t.bm) * float(t.bn) * (2 * kHalfK / (1e6f * t.rate));
+    }
+    const auto fits = [&](int i, int s) {
+      return s == 1 || (size[i]->split && steps[i] / s >= 4 &&
+                        int64_t(s) * size[i]->m * size[i]->n <= scratch / int64_t(sizeof(float)));
+    };
+    constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+    for (int s0 : kSplits) {
+      if (!fits(0, s0)) break;
+      for (int s1 : kSplits) {
+        if (!fits(1, s1)) break;
+        const int64_t items[2] = {tiles[0] * s0, tiles[1] * s1};
+        if (uint64_t(items[0] + items[1]) > kMaxGridThreads / uint64_t(t.threads)) break;
+        const int64_t held = std::clamp<int64_t>((items[0] + items[1] + cus - 1) / cus, 1, t.per_cu);
+        float each[2], fold = 0.0f;
+        for (int i = 0; i < 2; ++i) {
+          const int s = i ? s1 : s0;
+          const float n = float((steps[i] + s - 1) / s);
+          each[i] = std::max(n * float(held) * t.shared, n * t.alone + t.ends * size[i]->ends);
+          if (s > 1) fold += 3.0f + float(s + 1) * float(size[i]->m) * float(size[i]->n) * (4.0f / 5e6f);
+        }
+        for (int order = 0; order < (items[1] ? 2 : 1); ++order) {
+          const float span = half_makespan(cus * held, items[order], each[order], items[1 - order], each[1 - order]);
+          const float us = std::cbrt(span * span * span + power * power * power) + fold;
+          if (plan.cfg < 0 || us < best) {
+            best = us;
+            plan = {c, {s0, s1}, order == 1};
+          }
+        }
+        if (items[1] > 4 * cus * t.per_cu) break;
       }
-      if (tiles * s > 8 * cus) break;
+      if (tiles[0] * s0 > 4 * cus * t.per_cu) break;
     }
   }
   return plan;

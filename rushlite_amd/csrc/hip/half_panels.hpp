@@ -4,8 +4,9 @@
 // Both passes take the matrix from a source, which reads it or forms it from what it is
 // made of:
 //   int64_t rows; int cols;
-//   hv4 load(int64_t row, int col)   columns col to col + 3 (col a multiple of 4), zeros past the last
-//   int place(int col)               where that column's sum goes, or -1
+//   void load(int64_t row, int unit, hv4 (&v)[2])   eight columns, zeros past the last
+//   int column(int unit, int h)                     the first column of v[h]; eight units are 64 columns in some order
+//   int place(int col)                              where that column's sum goes, or -1
 //
 // Bound by memory: a pass reads 4 bytes a value and the second writes 4 for each set of panels.
 #pragma once
@@ -42,10 +43,13 @@ struct MatrixSource {
   const float* x;
   int64_t ld;
   const int64_t* targets;
-  __device__ __forceinline__ hv4 load(int64_t row, int col) const {
-    if (targets && targets[row] < 0) return hv4(0.0f);
-    return load_four(x + row * ld, col, cols);
+  __device__ __forceinline__ void load(int64_t row, int unit, hv4 (&v)[2]) const {
+    v[0] = v[1] = hv4(0.0f);
+    if (targets && targets[row] < 0) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) v[h] = load_four(x + row * ld, column(unit, h), cols);
   }
+  __device__ __forceinline__ int column(int unit, int h) const { return 8 * unit + 4 * h; }
   __device__ __forceinline__ int place(int col) const { return col; }
 };
 
@@ -71,78 +75,97 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t x) {
   return x;
 }
 
-// A workgroup takes 256 columns, four a lane, down a strip of rows, each wave every fourth
-// row.  Maxima meet in atomics, which do not depend on their order; sums of the strip's
-// columns go to a row of their own.
+// A workgroup's sixteen waves, 2^`wide` of them side by side, take 512 columns each, eight a
+// lane, down a strip of rows.  Its rows' and columns' maxima meet in LDS, the workgroups' in
+// atomics, none of which depends on an order; the strip's sums go to a row of their own.
+constexpr int kTopsThreads = 1024, kTopsRows = 2048;  // a strip's rows at most
 template <class S>
 struct TopsJob {
   S s;
   uint32_t *row_top, *col_top;  // or null; zeros at first
   float* sums;                  // [strips, sums_ld], or null
   int64_t sums_ld;
-  int each, col_blocks;
+  int each, wide, col_blocks;
   int64_t blocks;
+  static constexpr int SMEM = (kTopsRows + 2048 + 16 * 512) * 4;
   __device__ __forceinline__ void run(int64_t block, char* smem) const {
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 4;
+    uint32_t* rows = reinterpret_cast<uint32_t*>(smem);
+    uint32_t* tops = rows + kTopsRows;
+    float* parts = reinterpret_cast<float*>(tops + 2048);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t strip = block / col_blocks;
-    const int col = int(block - strip * col_blocks) * 256 + lane * 4;
-    const int64_t begin = strip * each, end = min(s.rows, begin + each);
-    uint32_t top[4] = {0, 0, 0, 0};
-    hv4 sum = hv4(0.0f);
-    for (int64_t row = begin + wave; row < end; row += 4 * kAhead) {
-      hv4 v[kAhead];
+    const int across = wave & ((1 << wide) - 1), down = wave >> wide, step = 16 >> wide, width = 512 << wide;
+    const int64_t strip = block / col_blocks, begin = strip * each;
+    const int count = int(min(int64_t(each), s.rows - begin)), col0 = int(block - strip * col_blocks) * width;
+    const int unit = col0 / 8 + across * 64 + lane;
+    for (int i = threadIdx.x; i < kTopsRows + 2048; i += kTopsThreads) rows[i] = 0;
+    __syncthreads();
+    uint32_t top[2][4] = {};
+    hv4 sum[2] = {hv4(0.0f), hv4(0.0f)};
+    const bool inside = unit * 8 < (s.cols + 7) / 8 * 8;
+    for (int row = down; row < count; row += step * kAhead) {
+      hv4 v[kAhead][2];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        v[i] = hv4(0.0f);
-        if (row + 4 * i < end && col < s.cols) v[i] = s.load(row + 4 * i, col);
+        v[i][0] = v[i][1] = hv4(0.0f);
+        if (row + step * i < count && inside) s.load(begin + row + step * i, unit, v[i]);
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         uint32_t most = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t m = finite_magnitude(v[i][e]);
-          top[e] = max(top[e], m);
-          most = max(most, m);
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t m = finite_magnitude(v[i][h][e]);
+            top[h][e] = max(top[h][e], m);
+            most = max(most, m);
+          }
+          sum[h] = sum[h] + v[i][h];
         }
-        sum = sum + v[i];
-        if (row_top && row + 4 * i < end) {
+        if (row_top && row + step * i < count) {
           most = wave_most(most);
-          if (lane == 63) atomicMax(row_top + row + 4 * i, most);
+          if (lane == 63) atomicMax(rows + row + step * i, most);
         }
       }
     }
-    uint32_t* tops = reinterpret_cast<uint32_t*>(smem);
-    float* parts = reinterpret_cast<float*>(smem) + 1024;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      tops[wave * 256 + lane * 4 + e] = top[e];
-      if (sums) parts[wave * 256 + lane * 4 + e] = sum[e];
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = s.column(unit, h) + e - col0;
+        if (col_top) atomicMax(tops + at, top[h][e]);
+        if (sums) parts[down * width + at] = sum[h][e];
+      }
     __syncthreads();
-    const int i = threadIdx.x, mine = col - lane * 4 + i;
-    if (mine < s.cols) {
-      if (col_top) atomicMax(col_top + mine, max(max(tops[i], tops[256 + i]), max(tops[512 + i], tops[768 + i])));
-      const int to = sums ? s.place(mine) : -1;
-      if (to >= 0) sums[strip * sums_ld + to] = (parts[i] + parts[256 + i]) + (parts[512 + i] + parts[768 + i]);
+    if (row_top)
+      for (int i = threadIdx.x; i < count; i += kTopsThreads) atomicMax(row_top + begin + i, rows[i]);
+    for (int i = threadIdx.x; i < width && col0 + i < s.cols; i += kTopsThreads) {
+      if (col_top) atomicMax(col_top + col0 + i, tops[i]);
+      const int to = sums ? s.place(col0 + i) : -1;
+      if (to >= 0) {
+        float total = parts[i];
+        for (int d = 1; d < step; ++d) total += parts[d * width + i];
+        sums[strip * sums_ld + to] = total;
+      }
     }
   }
 };
 
-// Strips enough to fill the chip, of 16 rows at least, and 128 of them at most: a column's
-// maximum is an atomic a strip.
+// Strips enough to fill the chip, 256 of them at most: a column's maximum is an atomic a strip.
+inline int tops_wide(int64_t cols) { return cols > 1024 ? 2 : cols > 512 ? 1 : 0; }
 inline int64_t most_strips(Runtime* rt, int64_t rows, int64_t cols) {
-  const int64_t want = std::clamp<int64_t>(int64_t(rt->cu_count) * 4 / ((cols + 255) / 256), 1, 128);
-  return std::min(want, (rows + 15) / 16);
+  const int64_t width = 512 << tops_wide(cols);
+  const int64_t want = std::clamp<int64_t>(int64_t(rt->cu_count) * 2 / ((cols + width - 1) / width), 1, 256);
+  return std::max(want, (rows + kTopsRows - 1) / kTopsRows);
 }
 template <class S>
 TopsJob<S> tops_job(Runtime* rt, const S& s, uint32_t* row_top, uint32_t* col_top, float* sums = nullptr) {
-  const int col_blocks = (s.cols + 255) / 256;
-  const int64_t most = std::max<int64_t>(most_strips(rt, s.rows, s.cols), 1);
-  const int each = int(std::max<int64_t>((s.rows + most - 1) / most, 16));
-  return {s, row_top, col_top, sums, s.cols, each, col_blocks, (s.rows + each - 1) / each * col_blocks};
+  const int wide = tops_wide(s.cols), width = 512 << wide, col_blocks = (s.cols + width - 1) / width;
+  const int64_t most = most_strips(rt, s.rows, s.cols);
+  const int each = int(std::max<int64_t>((s.rows + most - 1) / most, 16 >> wide));
+  return {s, row_top, col_top, sums, s.cols, each, wide, col_blocks, (s.rows + each - 1) / each * col_blocks};
 }
 
 // ------------------------------------------------------------------------ panels
@@ -173,22 +196,25 @@ struct PackJob {
   S s;
   HalfPanels r, c;  // panels may be null
   int64_t tiles_c, blocks;
-  static constexpr int PITCH = 68;
+  static constexpr int PITCH = 68, SMEM = 64 * PITCH * 4;
   __device__ __forceinline__ void run(int64_t block, char* smem) const {
     float* t = reinterpret_cast<float*>(smem);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t tr = block / tiles_c, tc = block - tr * tiles_c;
-    hv4 v[4];
+    const int unit = int(tc) * 8 + threadIdx.x % 8;
+    hv4 v[2][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t row = tr * 64 + threadIdx.x / 16 + 16 * i, col = tc * 64 + threadIdx.x % 16 * 4;
-      v[i] = hv4(0.0f);
-      if (row < s.rows && col < s.cols) v[i] = s.load(row, int(col));
+    for (int i = 0; i < 2; ++i) {
+      const int64_t row = tr * 64 + threadIdx.x / 8 + 32 * i;
+      v[i][0] = v[i][1] = hv4(0.0f);
+      if (row < s.rows && unit * 8 < s.cols) s.load(row, unit, v[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<hv4*>(t + (threadIdx.x / 16 + 16 * i) * PITCH + threadIdx.x % 16 * 4) = v[i];
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<hv4*>(t + (threadIdx.x / 8 + 32 * i) * PITCH + s.column(unit, h) - int(tc) * 64) = v[i][h];
     __syncthreads();
     float o[8];
     if (r.panels) {
@@ -221,27 +247,39 @@ PackJob<S> pack_job(const S& s, const HalfPanels& r, const HalfPanels& c) {
   return {s, r, c, tiles_c, tiles_r * tiles_c};
 }
 
-// One launch for two jobs.
-struct NoJob {
-  int64_t blocks = 0;
-  __device__ __forceinline__ void run(int64_t, char*) const {}
-};
-template <class A, class B>
-__global__ __launch_bounds__(kPanelThreads) void panel_jobs(A a, B b) {
-  __shared__ __attribute__((aligned(16))) char smem[64 * 68 * 4];
+// One launch for two jobs of one kind.
+template <int NT, class A, class B>
+__global__ __launch_bounds__(NT) void panel_jobs(A a, B b) {
+  __shared__ __attribute__((aligned(16))) char smem[A::SMEM];
   const int64_t block = blockIdx.x;
   if (block < a.blocks) a.run(block, smem);
   else b.run(block - a.blocks, smem);
 }
-template <class A, class B>
-int run_panel_jobs(Runtime* rt, const A& a, const B& b) {
+template <int NT, class A, class B>
+int launch_panel_jobs(Runtime* rt, const A& a, const B& b) {
+  static_assert(A::SMEM == B::SMEM);
   const int64_t blocks = a.blocks + b.blocks;
   if (blocks == 0) return LMP_OK;
-  if (uint64_t(blocks) > kMaxGridThreads / kPanelThreads)
+  if (uint64_t(blocks) > kMaxGridThreads / NT)
     return fail(LMP_ERR_UNSUPPORTED, "split products: more tiles than a grid holds");
-  panel_jobs<<<dim3(uint32_t(blocks)), dim3(kPanelThreads), 0, rt->stream>>>(a, b);
+  panel_jobs<NT><<<dim3(uint32_t(blocks)), dim3(NT), 0, rt->stream>>>(a, b);
   LMP_LAUNCH_CHECK("panel_jobs");
   return LMP_OK;
+}
+template <class A, class B>
+int run_panel_jobs(Runtime* rt, const TopsJob<A>& a, const TopsJob<B>& b) {
+  return launch_panel_jobs<kTopsThreads>(rt, a, b);
+}
+template <class A, class B>
+int run_panel_jobs(Runtime* rt, const PackJob<A>& a, const PackJob<B>& b) {
+  return launch_panel_jobs<kPanelThreads>(rt, a, b);
+}
+// One job alone.
+template <class J>
+int run_panel_job(Runtime* rt, const J& a) {
+  J none = a;
+  none.blocks = 0;
+  return run_panel_jobs(rt, a, none);
 }
 
 }  // namespace

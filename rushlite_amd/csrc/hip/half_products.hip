@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "gemm_half.hpp"
 #include "half_panels.hpp"
@@ -65,22 +66,14 @@ __device__ __forceinline__ void half_plain(const HalfArgs& g, const HalfOut& o, 
   });
 }
 
+// Two products in one grid, or one: the CUs that the first frees start on the second.
 template <int NT, int MINB, class C>
-__global__ __launch_bounds__(NT, MINB) void half_gemm(HalfArgs g, HalfOut o) {
+__global__ __launch_bounds__(NT, MINB) void half_gemm(HalfArgs a, HalfOut ao, HalfArgs b, HalfOut bo) {
   static_assert(NT == C::THREADS, "one lane per thread of the configuration");
   __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
-  half_plain<C>(g, o, int(blockIdx.x), smem);
-}
-
-// A layer's weight gradient and input gradient in one grid: the CUs that the first frees
-// start on the second.
-template <int NT, int MINB, class CW, class CX>
-__global__ __launch_bounds__(NT, MINB) void half_gemm_pair(HalfArgs w, HalfOut wo, HalfArgs x, HalfOut xo) {
-  static_assert(NT == CW::THREADS && NT == CX::THREADS, "one workgroup size for both");
-  __shared__ __attribute__((aligned(1024))) char smem[CW::SMEM > CX::SMEM ? CW::SMEM : CX::SMEM];
-  const int of_w = w.tiles_m * w.tiles_n * w.splits, id = int(blockIdx.x);
-  if (id < of_w) half_plain<CW>(w, wo, id, smem);
-  else half_plain<CX>(x, xo, id - of_w, smem);
+  const int first = a.tiles_m * a.tiles_n * a.splits, id = int(blockIdx.x);
+  if (id < first) half_plain<C>(a, ao, id, smem);
+  else half_plain<C>(b, bo, id - first, smem);
 }
 
 // C from the parts, added in their order; four values a lane.
@@ -117,8 +110,6 @@ constexpr int64_t kHalfParts = int64_t(256) << 20;
 struct HalfJob {
   HalfArgs g{};
   HalfOut o{};
-  HalfPlan plan;
-  bool wanted = false;
 };
 
 }  // namespace
@@ -140,80 +131,54 @@ int clear_f32(Runtime* rt, float* p, size_t rows, size_t cols, size_t ld) {
 }
 
 int half_backward(Runtime* rt, const HalfBackward& b) {
-  HalfJob w, x;
-  const int64_t cus = rt->cu_count;
   const int rows = int(b.rows), in = int(b.in), width = int(b.width);
+  HalfSize sizes[2];
+  int jobs = 0;
+  if (b.dw) sizes[jobs++] = {in, width, rows, true};
+  if (b.dx) sizes[jobs++] = {rows, in, width, true};
+  if (jobs == 0) return LMP_OK;
+  const HalfPlan plan = half_plan(rt->cu_count, kHalfParts, sizes[0], sizes[1]);
+  if (plan.cfg < 0) return fail(LMP_ERR_UNSUPPORTED, "gradient products: more tiles than a grid holds");
+  HalfJob job[2];
+  jobs = 0;
   if (b.dw) {
-    w.wanted = true;
-    w.plan = half_plan(cus, kHalfParts, in, width, rows, true);
-    w.o = {b.dw, int64_t(b.lddw), b.dw_accumulate ? 1 : 0, int(b.hidden), nullptr};
+    job[jobs] = {half_args(b.x_cols, b.d_cols, in, width, rows, plan.cfg, plan.splits[jobs]),
+                 {b.dw, int64_t(b.lddw), b.dw_accumulate ? 1 : 0, int(b.hidden), nullptr}};
+    ++jobs;
   }
   if (b.dx) {
-    x.wanted = true;
-    x.plan = half_plan(cus, kHalfParts, rows, in, width, true);
-    x.o = {b.dx, int64_t(b.lddx), 0, 0, nullptr};
+    job[jobs] = {half_args(b.d_rows, b.w_rows, rows, in, width, plan.cfg, plan.splits[jobs]),
+                 {b.dx, int64_t(b.lddx), 0, 0, nullptr}};
+    ++jobs;
   }
-  if ((w.wanted && w.plan.cfg < 0) || (x.wanted && x.plan.cfg < 0))
-    return fail(LMP_ERR_UNSUPPORTED, "gradient products: more tiles than a grid holds");
-  if (w.wanted) w.g = half_args(b.x_cols, b.d_cols, in, width, rows, w.plan);
-  if (x.wanted) x.g = half_args(b.d_rows, b.w_rows, rows, in, width, x.plan);
-  size_t parts = 0;
-  for (HalfJob* j : {&w, &x})
-    if (j->wanted && j->g.splits > 1) parts += (size_t(j->g.splits) * size_t(j->g.m) * size_t(j->g.n) + 3) / 4 * 4;
+  if (plan.second_first) std::swap(job[0], job[1]);
+  HalfRoom room;
+  size_t at[2];
+  for (int i = 0; i < 2; ++i)
+    at[i] = room.take(job[i].g.splits > 1 ? size_t(job[i].g.splits) * size_t(job[i].g.m) * size_t(job[i].g.n) : 0);
   float* scratch = nullptr;
-  if (parts) {
-    scratch = static_cast<float*>(scratch_alloc(parts * sizeof(float)));
+  if (room.words) {
+    scratch = static_cast<float*>(scratch_alloc(room.words * sizeof(float)));
     if (!scratch) return LMP_ERR_OOM;
-    float* p = scratch;
-    for (HalfJob* j : {&w, &x})
-      if (j->wanted && j->g.splits > 1) {
-        j->o.part = p;
-        p += (size_t(j->g.splits) * size_t(j->g.m) * size_t(j->g.n) + 3) / 4 * 4;
-      }
+    for (int i = 0; i < 2; ++i) job[i].o.part = scratch + at[i];
   }
-  const auto alone = [&](const HalfJob& j) {
-    return with_half_cfg(j.plan.cfg, [&](auto cfg) -> int {
-      using C = decltype(cfg);
-      half_gemm<C::THREADS, C::MINB, C><<<dim3(half_items(j.g)), dim3(C::THREADS), 0, rt->stream>>>(j.g, j.o);
-      LMP_LAUNCH_CHECK("half_gemm");
-      return LMP_OK;
-    });
-  };
   const auto run = [&]() -> int {
-    bool paired = false;
-    if (w.wanted && x.wanted &&
-        kHalfTiles[w.plan.cfg].threads == kHalfTiles[x.plan.cfg].threads &&
-        bf3_pair_fits(half_items(w.g), half_items(x.g), kHalfTiles[w.plan.cfg].threads)) {
-      paired = true;
-      const int rc = with_half_cfg(w.plan.cfg, [&](auto cw) {
-        return with_half_cfg(x.plan.cfg, [&](auto cx) -> int {
-          using CW = decltype(cw);
-          using CX = decltype(cx);
-          if constexpr (CW::THREADS == CX::THREADS) {
-            constexpr int kMinB = CW::MINB < CX::MINB ? CW::MINB : CX::MINB;
-            half_gemm_pair<CW::THREADS, kMinB, CW, CX>
-                <<<dim3(half_items(w.g) + half_items(x.g)), dim3(CW::THREADS), 0, rt->stream>>>(w.g, w.o, x.g, x.o);
-            LMP_LAUNCH_CHECK("half_gemm_pair");
-            return LMP_OK;
-          } else {
-            return fail(LMP_ERR_RUNTIME, "gradient products: workgroup sizes differ");
-          }
-        });
-      });
-      if (rc) return rc;
-    }
-    if (!paired && w.wanted)
-      if (int s = alone(w)) return s;
-    if (!paired && x.wanted)
-      if (int s = alone(x)) return s;
+    if (int s = with_half_cfg(plan.cfg, [&](auto cfg) -> int {
+          using C = decltype(cfg);
+          half_gemm<C::THREADS, C::MINB, C><<<dim3(half_items(job[0].g) + half_items(job[1].g)), dim3(C::THREADS), 0,
+                                              rt->stream>>>(job[0].g, job[0].o, job[1].g, job[1].o);
+          LMP_LAUNCH_CHECK("half_gemm");
+          return LMP_OK;
+        }))
+      return s;
     const auto fold = [&](const HalfJob& j) {
       HalfFold f{j.o, j.g.m, j.g.n, j.g.splits, 0};
-      if (j.wanted && j.g.splits > 1) f.blocks = (int64_t(f.m) * ((f.n + 3) / 4) + kThreads - 1) / kThreads;
+      if (j.g.splits > 1) f.blocks = (int64_t(f.m) * ((f.n + 3) / 4) + kThreads - 1) / kThreads;
       return f;
     };
-    const HalfFold fw = fold(w), fx = fold(x);
-    if (fw.blocks + fx.blocks) {
-      half_fold<<<dim3(uint32_t(fw.blocks + fx.blocks)), dim3(kThreads), 0, rt->stream>>>(fw, fx);
+    const HalfFold f0 = fold(job[0]), f1 = fold(job[1]);
+    if (f0.blocks + f1.blocks) {
+      half_fold<<<dim3(uint32_t(f0.blocks + f1.blocks)), dim3(kThreads), 0, rt->stream>>>(f0, f1);
       LMP_LAUNCH_CHECK("half_fold");
     }
     return LMP_OK;
