@@ -205,7 +205,9 @@ int lmp_k_gated_linear_backward_f32(int gate, size_t rows, size_t in, size_t hid
  * bias vocab values or null (0), t = targets[i] (int64, on the device).  A row whose target
  * is negative is not counted: its loss is 0, whatever it holds.  A target of vocab or more
  * makes its row's loss NaN.  A logit of -inf has no share; a row of nothing else has the loss
- * NaN.  The logits are formed in pieces and never held whole.  in and vocab are positive. */
+ * NaN, and so has one with a logit of NaN or +inf.  The logits alone are not held at all, or
+ * are in pieces of 512 MB (256 rows, if they are more) with the gradients.  in and vocab are
+ * positive. */
 int lmp_k_linear_cross_entropy_f32(size_t rows, size_t in, size_t vocab, const float* x,
                                    size_t ldx, const float* w, size_t ldw, const float* bias,
                                    const int64_t* targets, float* loss);

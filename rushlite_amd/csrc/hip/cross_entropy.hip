@@ -48,29 +48,33 @@ __device__ __forceinline__ Softmax joined(Softmax a, Softmax b) {
   return {top, a.sum * fa + b.sum * fb};
 }
 
-// One workgroup per row: loss and, with GRAD, dz in the place of z.
-template <bool GRAD>
-__global__ __launch_bounds__(1024) void loss_rows(LossArgs a) {
+// Loss and, with GRAD, dz in the place of z: a row for each wave of a workgroup of four, or
+// (WAVES 16) one row for the workgroup.  32 rows of 10 take 3 us so, 8 with a workgroup each.
+template <bool GRAD, int WAVES>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 1024) void loss_rows(LossArgs a) {
   __shared__ Softmax parts[16];
+  constexpr int kLanes = 64 * WAVES, kRows = WAVES == 1 ? 4 : 1;
+  const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
   const float low = -__builtin_huge_valf();
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  for (int64_t row = int64_t(blockIdx.x) * kRows + (WAVES == 1 ? threadIdx.x >> 6 : 0); row < a.rows;
+       row += int64_t(gridDim.x) * kRows) {
     float* z = a.z + row * a.vocab;
     const int64_t t = a.targets[row];
     const bool counted = t >= 0, known = t < a.vocab;
     if (a.counted_x)
-      for (int i = threadIdx.x; i < a.in; i += 1024)
-        a.counted_x[row * a.in + i] = counted ? a.x[row * a.ldx + i] : 0.0f;
+      for (int i = lane; i < a.in; i += kLanes) a.counted_x[row * a.in + i] = counted ? a.x[row * a.ldx + i] : 0.0f;
     if (!counted) {
       if (GRAD)
-        for (int v = threadIdx.x; v < a.vocab; v += 1024) z[v] = 0.0f;
-      if (threadIdx.x == 0) a.loss[row] = 0.0f;
+        for (int v = lane; v < a.vocab; v += kLanes) z[v] = 0.0f;
+      if (lane == 0) a.loss[row] = 0.0f;
       continue;
     }
+    const float zt = known ? z[t] : __builtin_nanf("");
     Softmax s{low, 0.0f};
     bool nan = false;
-    for (int v = threadIdx.x; v < a.vocab; v += 1024) {
+    for (int v = lane; v < a.vocab; v += kLanes) {
       const float x = z[v];
-      nan |= x != x;
+      nan |= !(x < -low);  // +inf too: inf - inf
       if (x > s.top) {
         s.sum = s.sum * expf(s.top - x) + 1.0f;
         s.top = x;
@@ -79,26 +83,142 @@ __global__ __launch_bounds__(1024) void loss_rows(LossArgs a) {
       }
     }
     if (nan) s.sum = __builtin_nanf("");
-    for (int off = 1; off < 64; off *= 2) {
-      const Softmax o{__shfl_xor(s.top, off), __shfl_xor(s.sum, off)};
-      s = joined(s, o);
+    for (int off = 1; off < 64; off *= 2) s = joined(s, {__shfl_xor(s.top, off), __shfl_xor(s.sum, off)});
+    if constexpr (WAVES > 1) {
+      if ((lane & 63) == 0) parts[lane >> 6] = s;
+      __syncthreads();
+      s = parts[lane & 15];
+      for (int off = 1; off < 16; off *= 2) s = joined(s, {__shfl_xor(s.top, off), __shfl_xor(s.sum, off)});
+      __syncthreads();  // z[t] and parts are read before they are written again
     }
-    if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = s;
-    __syncthreads();
-    s = parts[0];
-    for (int i = 1; i < 16; ++i) s = joined(s, parts[i]);
-    const float zt = known ? z[t] : __builtin_nanf("");
-    __syncthreads();  // z[t] and parts are read before they are written again
-    if (threadIdx.x == 0) a.loss[row] = logf(s.sum) - (zt - s.top);
+    if (lane == 0) a.loss[row] = logf(s.sum) - (zt - s.top);
     if constexpr (GRAD) {
       const float w = a.weights ? a.weights[row] : 1.0f;
       const float f = known ? w / s.sum : __builtin_nanf("");
-      for (int v = threadIdx.x; v < a.vocab; v += 1024) {
+      for (int v = lane; v < a.vocab; v += kLanes) {
         const float p = expf(z[v] - s.top) * f;
         z[v] = v == t ? p - w : p;
       }
     }
   }
+}
+template <bool GRAD>
+int launch_loss_rows(Runtime* rt, const LossArgs& a) {
+  if (a.vocab <= 1024)
+    loss_rows<GRAD, 1><<<dim3(uint32_t(std::min<int64_t>((a.rows + 3) / 4, 65536))), dim3(256), 0, rt->stream>>>(a);
+  else
+    loss_rows<GRAD, 16><<<dim3(uint32_t(std::min<int64_t>(a.rows, 65536))), dim3(1024), 0, rt->stream>>>(a);
+  LMP_LAUNCH_CHECK("loss_rows");
+  return LMP_OK;
+}
+
+// --------------------------------------------------------------- one workgroup
+
+struct LossCall {
+  size_t rows, in, vocab;
+  const float* x;
+  size_t ldx;
+  const float* w;
+  size_t ldw;
+  const float* bias;
+  const int64_t* targets;
+  const float* weights;
+  float* loss;
+  float* dx;
+  size_t lddx;
+  float* dw;
+  size_t lddw;
+  float* db;
+};
+
+// A problem that one workgroup holds in LDS: bound by latency, so everything in one launch.
+// 32 x 64 over 10 words with the gradients takes 5 us, its four launches 12.
+constexpr size_t kTinyFloats = 15360, kTinyWork = size_t(1) << 17;
+bool tiny_fits(const LossCall& c) {
+  return c.rows <= kTinyFloats && c.in <= kTinyFloats && c.vocab <= kTinyFloats &&
+         c.rows * (c.in | 1) + (c.in + c.rows) * (c.vocab | 1) <= kTinyFloats && c.rows * c.in * c.vocab <= kTinyWork;
+}
+struct TinyLoss {
+  int rows, in, vocab;
+  const float* x;
+  int64_t ldx;
+  const float* w;
+  int64_t ldw;
+  const float* bias;
+  const int64_t* targets;
+  const float* weights;
+  float *loss, *dx;
+  int64_t lddx;
+  float* dw;
+  int64_t lddw;
+  float* db;
+};
+__global__ __launch_bounds__(1024) void tiny_loss(TinyLoss a) {
+  __shared__ float smem[kTinyFloats];
+  const int xp = a.in | 1, wp = a.vocab | 1, tid = threadIdx.x;
+  float *x = smem, *w = x + a.rows * xp, *z = w + a.in * wp;
+  for (int i = tid; i < a.rows * a.in; i += 1024) {
+    const int r = i / a.in, k = i % a.in;
+    x[r * xp + k] = a.targets[r] < 0 ? 0.0f : a.x[r * a.ldx + k];
+  }
+  for (int i = tid; i < a.in * a.vocab; i += 1024) w[i / a.vocab * wp + i % a.vocab] = a.w[i / a.vocab * a.ldw + i % a.vocab];
+  __syncthreads();
+  for (int i = tid; i < a.rows * a.vocab; i += 1024) {
+    const int r = i / a.vocab, v = i % a.vocab;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < a.in; ++k) sum = __builtin_fmaf(x[r * xp + k], w[k * wp + v], sum);
+    z[r * wp + v] = a.bias ? sum + a.bias[v] : sum;
+  }
+  __syncthreads();
+  const int lane = tid & 63;
+  for (int r = tid >> 6; r < a.rows; r += 16) {
+    const int64_t t = a.targets[r];
+    const bool counted = t >= 0, known = t < a.vocab;
+    const float low = -__builtin_huge_valf(), zt = counted && known ? z[r * wp + t] : __builtin_nanf("");
+    float top = low, sum = 0.0f;
+    for (int v = lane; v < a.vocab; v += 64) top = fmaxf(top, z[r * wp + v]);
+    for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
+    for (int v = lane; v < a.vocab; v += 64) sum += expf(z[r * wp + v] - top);
+    for (int off = 1; off < 64; off *= 2) sum += __shfl_xor(sum, off);
+    if (lane == 0) a.loss[r] = counted ? logf(sum) - (zt - top) : 0.0f;
+    if (!a.dx && !a.dw) continue;
+    const float weight = a.weights ? a.weights[r] : 1.0f, f = known ? weight / sum : __builtin_nanf("");
+    for (int v = lane; v < a.vocab; v += 64) {
+      const float p = expf(z[r * wp + v] - top) * f;
+      z[r * wp + v] = !counted ? 0.0f : v == t ? p - weight : p;
+    }
+  }
+  __syncthreads();
+  if (a.dx)
+    for (int i = tid; i < a.rows * a.in; i += 1024) {
+      const int r = i / a.in, k = i % a.in;
+      float sum = 0.0f;
+#pragma unroll 8
+      for (int v = 0; v < a.vocab; ++v) sum = __builtin_fmaf(z[r * wp + v], w[k * wp + v], sum);
+      a.dx[r * a.lddx + k] = sum;
+    }
+  if (a.dw)
+    for (int i = tid; i < a.in * a.vocab; i += 1024) {
+      const int k = i / a.vocab, v = i % a.vocab;
+      float sum = 0.0f;
+#pragma unroll 8
+      for (int r = 0; r < a.rows; ++r) sum = __builtin_fmaf(x[r * xp + k], z[r * wp + v], sum);
+      a.dw[k * a.lddw + v] = sum;
+    }
+  if (a.db)
+    for (int v = tid; v < a.vocab; v += 1024) {
+      float sum = 0.0f;
+      for (int r = 0; r < a.rows; ++r) sum += z[r * wp + v];
+      a.db[v] = sum;
+    }
+}
+int run_tiny_loss(Runtime* rt, const LossCall& c) {
+  tiny_loss<<<dim3(1), dim3(1024), 0, rt->stream>>>(
+      {int(c.rows), int(c.in), int(c.vocab), c.x, int64_t(c.ldx), c.w, int64_t(c.ldw), c.bias, c.targets, c.weights, c.loss,
+       c.dx, int64_t(c.lddx), c.dw, int64_t(c.lddw), c.db});
+  LMP_LAUNCH_CHECK("tiny_loss");
+  return LMP_OK;
 }
 
 // ------------------------------------------------------- on the fp16 matrix cores
@@ -234,22 +354,6 @@ struct LossGradient {
   __device__ __forceinline__ int place(int col) const { return col; }
 };
 
-struct LossCall {
-  size_t rows, in, vocab;
-  const float* x;
-  size_t ldx;
-  const float* w;
-  size_t ldw;
-  const float* bias;
-  const int64_t* targets;
-  const float* weights;
-  float* loss;
-  float* dx;
-  size_t lddx;
-  float* dw;
-  size_t lddw;
-  float* db;
-};
 
 int check_loss(const std::string& name, const LossCall& c) {
   if (c.in == 0 || c.vocab == 0) return fail(LMP_ERR_INVALID, name + "no inputs or no vocabulary");
@@ -262,9 +366,17 @@ int check_loss(const std::string& name, const LossCall& c) {
   return LMP_OK;
 }
 
-// From this many multiply-adds a product on, the fp16 matrix cores make up for the passes
-// that find the largest magnitudes.
-constexpr uint64_t kHalfWork = uint64_t(1) << 28;
+// Whether the split products pay for reading x and w twice, writing their panels (12 bytes a
+// value, 16 with the gradients) and their launches.  They save the pass over the logits
+// that the losses alone take, or cost 4 bytes a logit for the gradients' panels.  256 rows of
+// 1024 over 32768 words take 170 us without them and 135 with them (375 and 370 with the
+// gradients), 64 rows 81 and 114.
+bool half_pays(const LossCall& c) {
+  const double n = double(c.rows), d = double(c.in), v = double(c.vocab), work = n * d * v;
+  if (!half_fits(c.rows, c.in, c.vocab)) return false;
+  if (!c.dx && !c.dw) return half_saves_forward(work) + pass_time(8 * n * v) > 12 + pass_time(12 * (n * d + d * v));
+  return half_saves_forward(work) + half_saves_backward(work) > 25 + pass_time(16 * (n * d + d * v) + 4 * n * v);
+}
 
 int run_loss_half(Runtime* rt, const LossCall& c) {
   const bool grad = c.dx || c.dw;
@@ -357,9 +469,8 @@ int run_loss(Runtime* rt, const LossCall& c) {
     if (int s = clear_f32(rt, c.dw, c.in, c.vocab, c.lddw)) return s;
     return clear_f32(rt, c.db, 1, c.vocab, c.vocab);
   }
-  if (half_fits(c.rows, c.in, c.vocab) &&
-      uint64_t(c.rows) * c.in * c.vocab >= kHalfWork)
-    return run_loss_half(rt, c);
+  if (tiny_fits(c)) return run_tiny_loss(rt, c);
+  if (half_pays(c)) return run_loss_half(rt, c);
   const size_t fit = std::max<size_t>(256, kPieceBytes / (c.vocab * sizeof(float)));
   const size_t pieces = (c.rows + fit - 1) / fit, each = (c.rows + pieces - 1) / pieces;
   const size_t logits = (each * c.vocab + 3) / 4 * 4;
@@ -374,12 +485,12 @@ int run_loss(Runtime* rt, const LossCall& c) {
     const LossArgs a{int64_t(n), int(c.vocab), z, c.targets + at, c.weights ? c.weights + at : nullptr,
                      c.loss + at, x, int64_t(c.ldx), int(c.in), counted_x};
     const bool grad = c.dx || c.dw;
-    const dim3 grid(uint32_t(std::min<size_t>(n, 65536)));
-    if (grad) loss_rows<true><<<grid, dim3(1024), 0, rt->stream>>>(a);
-    else loss_rows<false><<<grid, dim3(1024), 0, rt->stream>>>(a);
-    LMP_LAUNCH_CHECK("loss_rows");
+    if (int s = grad ? launch_loss_rows<true>(rt, a) : launch_loss_rows<false>(rt, a)) return s;
     if (!grad) return LMP_OK;
     const int more = at > 0;
+    if (c.dx && c.db)
+      return lmp_k_linear_backward_f32(n, c.in, c.vocab, counted_x, c.in, c.w, c.ldw, z, c.vocab, c.dx + at * c.lddx, c.lddx,
+                                       0, c.dw, c.lddw, more, c.db, more);
     if (c.dw) {
       if (int s = c.db ? lmp_k_gemm_colsum_f32(1, 0, c.in, c.vocab, n, counted_x, c.in, z, c.vocab, c.dw, c.lddw, more, c.db, more)
                        : lmp_k_gemm_f32(1, 0, c.in, c.vocab, n, counted_x, c.in, z, c.vocab, c.dw, c.lddw, more))

@@ -161,12 +161,21 @@ __global__ __launch_bounds__(NT, MINB) void half_gated(HalfArgs g, HalfGated o) 
   });
 }
 
-// From this many multiply-adds a product on, the fp16 matrix cores make up for the passes
-// that find the largest magnitudes.
-constexpr uint64_t kHalfWork = uint64_t(1) << 28;
-
-bool use_half(size_t rows, size_t in, size_t hidden) {
-  return half_fits(rows, in, 2 * hidden) && hidden >= 32 && uint64_t(rows) * in * 2 * hidden >= kHalfWork;
+// Whether the split products pay for reading x and w twice and writing their panels (12 bytes a
+// value) and for their launches; forward they save a pass over pre besides (two where it is not
+// kept, but what is kept does not change the results).  128 rows of 4096 by 4096 x 16384 take 158 us without them and 264 with them, 512
+// of 768 by 768 x 4096 41 and 38, 16384 of 64 by 64 x 2048 95 and 51.
+bool half_forward_pays(size_t rows, size_t in, size_t hidden) {
+  const double n = double(rows), d = double(in), w = 2 * double(hidden);
+  return half_fits(rows, in, 2 * hidden) && hidden >= 32 &&
+         half_saves_forward(n * d * w) + pass_time(4 * n * w) > 12 + pass_time(12 * (n * d + d * w));
+}
+// Backward they form d twice from pre and g and write it in two sets of panels: 20 bytes a value
+// for 10.  16384 rows of 64 by 64 x 2048 take 164 us without them and 253 with them.
+bool half_backward_pays(size_t rows, size_t in, size_t hidden) {
+  const double n = double(rows), d = double(in), w = 2 * double(hidden);
+  return half_fits(rows, in, 2 * hidden) && hidden >= 32 &&
+         half_saves_backward(n * d * w) > 25 + pass_time(12 * (n * d + d * w) + 10 * n * w);
 }
 
 // The workspace as panels and their rows' magnitudes.
@@ -278,7 +287,7 @@ extern "C" int lmp_k_gated_linear_f32(int gate, size_t rows, size_t in, size_t h
   if (std::max({ldx, ldw, ldh, pre ? ldpre : 0}) >= kGemmMaxExtent)
     return fail(LMP_ERR_UNSUPPORTED, name + "dimension of 2^31 - 4096 or more");
   LMP_RUNTIME_OR_FAIL(rt);
-  if (use_half(rows, in, hidden))
+  if (half_forward_pays(rows, in, hidden))
     return gated_half(rt, gate, rows, in, hidden, x, ldx, w, ldw, bias, h, ldh, pre, ldpre);
   float* z = pre;
   if (!z) {
@@ -315,7 +324,7 @@ extern "C" int lmp_k_gated_linear_backward_f32(int gate, size_t rows, size_t in,
     if (int s = clear_f32(rt, dw, in, width, lddw)) return s;
     return clear_f32(rt, db, 1, width, width);
   }
-  if (use_half(rows, in, hidden))
+  if (half_backward_pays(rows, in, hidden))
     return gated_half_backward(rt, gate, rows, in, hidden, g, ldg, x, ldx, w, ldw, pre, ldpre, dx, lddx, dw, lddw, db);
   float* d = static_cast<float*>(scratch_alloc(rows * width * sizeof(float)));
   if (!d) return LMP_ERR_OOM;

@@ -155,8 +155,9 @@ def test_dropout_rates_and_what_is_dropped(hip):
 
 GATED = [(1, 1, 1), (1, 7, 3), (3, 5, 4), (2, 64, 33), (32, 64, 64), (5, 300, 70), (33, 40, 129), (31, 1000, 96), (32, 1024, 515),
          (64, 32, 200), (70, 129, 65), (129, 128, 128), (300, 77, 260), (200, 512, 300), (1000, 64, 31), (513, 256, 640),
-         # on the fp16 matrix cores
-         (700, 400, 600), (1031, 257, 521), (32, 2048, 2100), (4000, 33, 1037), (6007, 300, 97), (130, 4097, 300)]
+         (700, 400, 600), (1031, 257, 521), (32, 2048, 2100), (4000, 33, 1037), (6007, 300, 97), (130, 4097, 300),
+         # products split into fp16 parts: forward, and both ways
+         (9001, 33, 1037), (2100, 1031, 1100), (1031, 2050, 1001), (600, 2048, 2100), (5003, 600, 1201)]
 
 
 def gated(hip, gate, x, w, b, g, pads=(0, 0, 0, 0), want=(True, True, True), keep=True):
@@ -202,10 +203,14 @@ def test_gated_linear(hip, gate, rows, k, n):
         assert np.array_equal(gated(hip, gate, x, w, bias, g, pads, keep=False), got[0])
 
 
+def test_gated_linear_in_the_largest_tiles(hip):
+    test_gated_linear(hip, "silu", 8200, 1024, 2080)
+
+
 def test_gated_linear_relu_is_exact_on_integers(hip):
     """Small whole numbers: every product and sum is exact, so ReLU's two sides are too, at 0 as well."""
     rng = np.random.default_rng(4)
-    for rows, k, n in ((3, 5, 4), (40, 33, 70), (300, 64, 129), (301, 700, 701)):
+    for rows, k, n in ((3, 5, 4), (40, 33, 70), (300, 64, 129), (301, 700, 701), (1500, 1100, 1201)):
         x, w, g = (rng.integers(-3, 4, s).astype(np.float32) for s in ((rows, k), (k, 2 * n), (rows, n)))
         for got, want in zip(gated(hip, "relu", x, w, None, g), D.gated("relu", x, w, None, g)):
             assert np.array_equal(got, want)
@@ -213,7 +218,7 @@ def test_gated_linear_relu_is_exact_on_integers(hip):
 
 def test_gated_linear_parts_of_the_backward(hip):
     rng = np.random.default_rng(6)
-    for rows, k, n in ((5, 9, 6), (200, 70, 140), (300, 700, 701)):
+    for rows, k, n in ((5, 9, 6), (200, 70, 140), (300, 700, 701), (1500, 1100, 1201)):
         x, w, g = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (k, 2 * n), (rows, n)))
         want, bound = D.gated("silu", x, w, None, g), D.gated_bounds("silu", x, w, None, g)
         for parts in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (1, 0, 1), (0, 1, 1)):
@@ -235,7 +240,7 @@ def test_gated_linear_special_values(hip):
     """Infinities and NaN in one row touch no other; gates far out are 0, a or 1; operands far apart and past the split's
     range come out as float32's products give them."""
     rng = np.random.default_rng(8)
-    for rows, k, n in ((6, 40, 30), (150, 64, 130), (300, 700, 701)):
+    for rows, k, n in ((6, 40, 30), (150, 64, 130), (300, 700, 701), (1500, 1100, 1201)):
         x, w, g = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (k, 2 * n), (rows, n)))
         clean = gated(hip, "silu", x, w, None, g)
         x[2, 3], x[4, 0] = np.nan, np.inf
@@ -254,7 +259,7 @@ def test_gated_linear_special_values(hip):
         act = np.array([0, 1, 0, 1, 0.5]) if gate == "sigmoid" else np.maximum(x[:, 0].astype(np.float64), 0)
         close(h, act * u, 1e-5 * np.abs(act * u) + 1e-38, gate)
     # one row and one column far larger than the others, and far smaller
-    for rows, k, n, scale in [(*size, scale) for size in ((70, 96, 70), (400, 600, 700)) for scale in (1e-20, 1e-12, 1e12)]:
+    for rows, k, n, scale in [(*size, scale) for size in ((70, 96, 70), (400, 600, 700), (1500, 1100, 1201)) for scale in (1e-20, 1e-12, 1e12)]:
         x, w, g = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (k, 2 * n), (rows, n)))
         if k > 96:
             w *= np.float32(k ** -0.5)
@@ -270,8 +275,9 @@ def test_gated_linear_special_values(hip):
 
 LOSS = [(1, 1, 1), (1, 3, 2), (3, 5, 7), (32, 64, 10), (7, 33, 1000), (64, 16, 129), (40, 130, 515), (130, 64, 1024),
         (33, 100, 4099), (300, 40, 333), (65, 7, 20001), (129, 256, 640),
-        # on the fp16 matrix cores
-        (1031, 257, 1021), (40, 1000, 7001), (3000, 33, 2801), (32, 600, 14100), (9000, 520, 64), (777, 1111, 513)]
+        (1031, 257, 1021), (40, 1000, 7001), (3000, 33, 2801), (32, 600, 14100), (9000, 520, 64), (777, 1111, 513),
+        # products split into fp16 parts
+        (2300, 520, 10007), (9001, 97, 2801), (4099, 1031, 2001), (300, 1024, 30011), (5003, 600, 1009)]
 
 
 def loss(hip, x, w, b, targets, weights=None, pads=(0, 0), grads=True, want=(True, True, True)):
@@ -317,22 +323,39 @@ def test_cross_entropy(hip, rows, k, vocab):
     check_loss(hip, x, w, None, targets, None, (3, 1))
 
 
-def test_cross_entropy_in_several_pieces(hip):
-    """More logits than one piece of the workspace holds."""
+def test_cross_entropy_of_large_vocabularies(hip):
     rng = np.random.default_rng(1)
     for rows, k, vocab in ((2300, 12, 30011), (2300, 40, 30011), (1050, 64, 33000)):
-        several_pieces(hip, rng, rows, k, vocab)
+        x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
+        targets = rng.integers(-vocab // 4, vocab, rows)
+        check_loss(hip, x, w, rng.standard_normal(vocab).astype(np.float32), targets, rng.random(rows).astype(np.float32))
 
 
-def several_pieces(hip, rng, rows, k, vocab):
-    x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
-    targets = rng.integers(-vocab // 4, vocab, rows)
-    check_loss(hip, x, w, rng.standard_normal(vocab).astype(np.float32), targets, rng.random(rows).astype(np.float32))
+@pytest.mark.parametrize("k", [12, 64])  # as they are, and split into fp16 parts
+def test_cross_entropy_in_several_pieces(hip, k):
+    """More logits than one piece of the workspace holds.  The plain form by parts of the rows; a sum over all of them rounds
+    as often as three such parts' bounds allow."""
+    rng = np.random.default_rng(7)
+    rows, vocab = 4500, 30011
+    x, w = rng.standard_normal((rows, k)).astype(np.float32), (rng.standard_normal((k, vocab)) * k ** -0.5).astype(np.float32)
+    b, weights, targets = rng.standard_normal(vocab).astype(np.float32), rng.random(rows).astype(np.float32), \
+        rng.integers(-vocab // 4, vocab, rows)
+    got = loss(hip, x, w, b, targets, weights)
+    dw, db, ew, eb = 0, 0, 0, 0
+    for at in range(0, rows, 1500):
+        part = slice(at, at + 1500)
+        args = x[part], w, b, targets[part], weights[part]
+        want, bound = D.cross_entropy(*args), D.cross_entropy_bounds(*args)
+        close(got[0][part], want[0], bound[0], "loss")
+        close(got[1][part], want[1], bound[1], "dx")
+        dw, db, ew, eb = dw + want[2], db + want[3], ew + 3 * bound[2], eb + 3 * bound[3]
+    close(got[2], dw, ew, "dw")
+    close(got[3], db, eb, "db")
 
 
 def test_cross_entropy_rows_that_do_not_count_leave_no_trace(hip):
     rng = np.random.default_rng(2)
-    for rows, k, vocab in ((9, 20, 50), (140, 64, 700), (700, 500, 1009)):
+    for rows, k, vocab in ((9, 20, 50), (140, 64, 700), (700, 500, 1009), (2100, 900, 2003)):
         x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
         targets, weights = rng.integers(0, vocab, rows), rng.random(rows).astype(np.float32)
         targets[[1, 4]] = -1, -(1 << 40)
@@ -347,7 +370,7 @@ def test_cross_entropy_rows_that_do_not_count_leave_no_trace(hip):
 
 def test_cross_entropy_targets_past_the_vocabulary(hip):
     rng = np.random.default_rng(3)
-    for rows, k, vocab in ((6, 8, 33), (700, 500, 1009)):
+    for rows, k, vocab in ((6, 8, 33), (40, 130, 515), (700, 500, 1009), (2100, 900, 2003)):
         x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
         targets = rng.integers(0, vocab, rows)
         targets[[1, 3, 4]] = vocab, 1 << 40, vocab - 1
@@ -364,7 +387,7 @@ def test_cross_entropy_of_barred_and_extreme_logits(hip):
     """A bias of -inf, or of the lowest float, bars a word; a target so barred has an infinite loss; logits of 1e30 give
     weights of 0 and 1; one NaN logit makes its row NaN."""
     rng = np.random.default_rng(4)
-    for rows, k, vocab in ((5, 16, 300), (500, 600, 1001)):
+    for rows, k, vocab in ((5, 16, 300), (40, 130, 515), (9, 130, 2515), (500, 600, 1001), (2100, 900, 2003)):
         barred(hip, rng, rows, k, vocab)
     big = np.zeros((2, 1), np.float32) + 1e15
     wide = np.array([[1e15, -1e15, 0]], np.float32)
@@ -397,13 +420,15 @@ def barred(hip, rng, rows, k, vocab):
     assert value[1] == np.inf and np.isfinite(np.delete(value, 1)).all()
     assert np.isnan(loss(hip, x, w, np.full(vocab, -np.inf, np.float32), targets, grads=False)).all()
     b[:] = 0
-    b[9] = np.nan
-    assert np.isnan(loss(hip, x, w, b, targets, grads=False)).all()
+    for bad in (np.nan, np.inf):
+        b[9] = bad
+        assert np.isnan(loss(hip, x, w, b, targets, grads=False)).all()
+        assert np.isnan(loss(hip, x, w, b, targets)[0]).all()
 
 
 def test_cross_entropy_without_parts(hip):
     rng = np.random.default_rng(5)
-    for rows, k, vocab in ((70, 40, 90), (600, 500, 1003)):
+    for rows, k, vocab in ((3, 40, 90), (70, 40, 90), (600, 500, 1003), (2100, 900, 2003)):
         x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
         targets = rng.integers(0, vocab, rows)
         full = loss(hip, x, w, None, targets)
@@ -422,13 +447,13 @@ def test_cross_entropy_without_parts(hip):
 
 # ------------------------------------------------------------------ graphs
 
-def test_recorded_calls_equal_eager_ones(hip):
+@pytest.mark.parametrize("rows,k,n,vocab", [(96, 64, 80, 500), (1500, 1100, 1201, 3001)])
+def test_recorded_calls_equal_eager_ones(hip, rows, k, n, vocab):
     """Each operator recorded once and replayed, with eager calls and a second graph between the replays: every replay
     gives the eager bits, dropout those of the next call."""
     import ctypes as C
     rng = np.random.default_rng(11)
     lib = hip.lib()
-    rows, k, n, vocab = 96, 64, 80, 500
     f32 = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
     x, w, b, g, wv = f32(rows, k), f32(k, 2 * n), f32(2 * n), f32(rows, n), f32(k, vocab)
     dev = {name: up(hip, a) for name, a in dict(x=x, w=w, b=b, g=g, wv=wv, pos=np.arange(rows), fr=np.array([1.0, 0.1]),
