@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "common.hpp"
 #include "gemm_half.hpp"
@@ -48,68 +49,116 @@ __device__ __forceinline__ Softmax joined(Softmax a, Softmax b) {
   return {top, a.sum * fa + b.sum * fb};
 }
 
-// Loss and, with GRAD, dz in the place of z: a row for each wave of a workgroup of four, or
-// (WAVES 16) one row for the workgroup.  32 rows of 10 take 3 us so, 8 with a workgroup each.
-template <bool GRAD, int WAVES>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : 1024) void loss_rows(LossArgs a) {
+// e^x for x <= 0: 2^(x log2 e) with what rounding the product leaves out put back, so that
+// it errs by two units, not by |x| of them.
+__device__ __forceinline__ float exp_below(float x) {
+  constexpr float kHi = 1.44269504088896341f, kLo = 1.925963033500e-8f, kLn2 = 0.69314718055994531f;
+  const float t = x * kHi, e = __builtin_amdgcn_exp2f(t);
+  const float rest = __builtin_fmaf(x, kHi, -t) + x * kLo;
+  return t < -160.0f ? 0.0f : __builtin_fmaf(e, rest * kLn2, e);
+}
+
+// Loss and, with GRAD, dz in the place of z.  A row has the lanes of WAVES waves, which hold
+// it in registers, QUADS times four logits each, or (QUADS 0) read it again from memory.
+// Bound by memory there; short rows by the latency of their few loads and joins.
+template <bool GRAD, int WAVES, int QUADS>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void loss_rows(LossArgs a) {
   __shared__ Softmax parts[16];
   constexpr int kLanes = 64 * WAVES, kRows = WAVES == 1 ? 4 : 1;
-  const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
+  const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, n = a.vocab;
   const float low = -__builtin_huge_valf();
   for (int64_t row = int64_t(blockIdx.x) * kRows + (WAVES == 1 ? threadIdx.x >> 6 : 0); row < a.rows;
        row += int64_t(gridDim.x) * kRows) {
-    float* z = a.z + row * a.vocab;
+    float* z = a.z + row * n;
     const int64_t t = a.targets[row];
-    const bool counted = t >= 0, known = t < a.vocab;
+    const bool counted = t >= 0, known = t < n;
     if (a.counted_x)
-      for (int i = lane; i < a.in; i += kLanes) a.counted_x[row * a.in + i] = counted ? a.x[row * a.ldx + i] : 0.0f;
+      for (int i = lane * 4; i < a.in; i += kLanes * 4)
+        store_four(a.counted_x + row * a.in, i, a.in, counted ? load_four(a.x + row * a.ldx, i, a.in) : hv4(0.0f));
     if (!counted) {
       if (GRAD)
-        for (int v = lane; v < a.vocab; v += kLanes) z[v] = 0.0f;
+        for (int v = lane * 4; v < n; v += kLanes * 4) store_four(z, v, n, hv4(0.0f));
       if (lane == 0) a.loss[row] = 0.0f;
       continue;
     }
     const float zt = known ? z[t] : __builtin_nanf("");
+    hv4 held[QUADS ? QUADS : 1];
     Softmax s{low, 0.0f};
-    bool nan = false;
-    for (int v = lane; v < a.vocab; v += kLanes) {
-      const float x = z[v];
-      nan |= !(x < -low);  // +inf too: inf - inf
-      if (x > s.top) {
-        s.sum = s.sum * expf(s.top - x) + 1.0f;
-        s.top = x;
-      } else if (x > low) {
-        s.sum += expf(x - s.top);
+    if constexpr (QUADS > 0) {
+#pragma unroll
+      for (int q = 0; q < QUADS; ++q) {
+        const int v = (q * kLanes + lane) * 4;
+        held[q] = hv4(low);
+        if (v < n) held[q] = load_four(z, v, n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (v + e >= n) held[q][e] = low;
+          s.top = fmaxf(s.top, held[q][e]);
+        }
+      }
+      // Of a lane with nothing but -inf the sum is 0; of +inf and NaN it is NaN.
+      const float from = s.top > low ? s.top : 0.0f;
+#pragma unroll
+      for (int q = 0; q < QUADS; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s.sum += exp_below(held[q][e] - from);
+    } else {
+      for (int v = lane * 4; v < n; v += kLanes * 4) {
+        const hv4 x = load_four(z, v, n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (v + e >= n) continue;
+          const float top = fmaxf(s.top, x[e]), from = top > low ? top : 0.0f;
+          s.sum = s.sum * exp_below(s.top - from) + exp_below(x[e] - from);
+          s.top = top;
+        }
       }
     }
-    if (nan) s.sum = __builtin_nanf("");
     for (int off = 1; off < 64; off *= 2) s = joined(s, {__shfl_xor(s.top, off), __shfl_xor(s.sum, off)});
     if constexpr (WAVES > 1) {
       if ((lane & 63) == 0) parts[lane >> 6] = s;
       __syncthreads();
-      s = parts[lane & 15];
-      for (int off = 1; off < 16; off *= 2) s = joined(s, {__shfl_xor(s.top, off), __shfl_xor(s.sum, off)});
+      s = parts[lane & (WAVES - 1)];
+      for (int off = 1; off < WAVES; off *= 2) s = joined(s, {__shfl_xor(s.top, off), __shfl_xor(s.sum, off)});
       __syncthreads();  // z[t] and parts are read before they are written again
     }
     if (lane == 0) a.loss[row] = logf(s.sum) - (zt - s.top);
     if constexpr (GRAD) {
       const float w = a.weights ? a.weights[row] : 1.0f;
       const float f = known ? w / s.sum : __builtin_nanf("");
-      for (int v = lane; v < a.vocab; v += kLanes) {
-        const float p = expf(z[v] - s.top) * f;
-        z[v] = v == t ? p - w : p;
+      const auto put = [&](int v, hv4 x) {
+        if (v >= n) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = exp_below(x[e] - s.top) * f;
+          x[e] = v + e == t ? p - w : p;
+        }
+        store_four(z, v, n, x);
+      };
+      if constexpr (QUADS > 0) {
+#pragma unroll
+        for (int q = 0; q < QUADS; ++q) put((q * kLanes + lane) * 4, held[q]);
+      } else {
+        for (int v = lane * 4; v < n; v += kLanes * 4) put(v, load_four(z, v, n));
       }
     }
   }
 }
 template <bool GRAD>
 int launch_loss_rows(Runtime* rt, const LossArgs& a) {
-  if (a.vocab <= 1024)
-    loss_rows<GRAD, 1><<<dim3(uint32_t(std::min<int64_t>((a.rows + 3) / 4, 65536))), dim3(256), 0, rt->stream>>>(a);
-  else
-    loss_rows<GRAD, 16><<<dim3(uint32_t(std::min<int64_t>(a.rows, 65536))), dim3(1024), 0, rt->stream>>>(a);
-  LMP_LAUNCH_CHECK("loss_rows");
-  return LMP_OK;
+  const auto go = [&](auto waves, auto quads) -> int {
+    constexpr int W = decltype(waves)::value, each = W == 1 ? 4 : 1;
+    loss_rows<GRAD, W, decltype(quads)::value>
+        <<<dim3(uint32_t(std::min<int64_t>((a.rows + each - 1) / each, 65536))), dim3(W == 1 ? 256 : 64 * W), 0, rt->stream>>>(a);
+    LMP_LAUNCH_CHECK("loss_rows");
+    return LMP_OK;
+  };
+  using std::integral_constant;
+  if (a.vocab <= 512) return go(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+  if (a.vocab <= 4096) return go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+  if (a.vocab <= 8192) return go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+  if (a.vocab <= 32768) return go(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+  return go(integral_constant<int, 16>{}, integral_constant<int, 0>{});
 }
 
 // --------------------------------------------------------------- one workgroup
@@ -233,15 +282,6 @@ struct HalfLogits {
   const int64_t* targets;
   float* hit;  // [rows]: the target's logit
 };
-
-// e^x for x <= 0: 2^(x log2 e) with what rounding the product leaves out put back, so that
-// it errs by two units, not by |x| of them.
-__device__ __forceinline__ float exp_below(float x) {
-  constexpr float kHi = 1.44269504088896341f, kLo = 1.925963033500e-8f, kLn2 = 0.69314718055994531f;
-  const float t = x * kHi, e = __builtin_amdgcn_exp2f(t);
-  const float rest = __builtin_fmaf(x, kHi, -t) + x * kLo;
-  return t < -160.0f ? 0.0f : __builtin_fmaf(e, rest * kLn2, e);
-}
 
 __device__ __forceinline__ float over_eight(float x, bool most) {
 #define LMP_STEP(ctrl)                                                                                          \
@@ -470,12 +510,20 @@ int run_loss(Runtime* rt, const LossCall& c) {
     return clear_f32(rt, c.db, 1, c.vocab, c.vocab);
   }
   if (tiny_fits(c)) return run_tiny_loss(rt, c);
-  if (half_pays(c)) return run_loss_half(rt, c);
-  const size_t fit = std::max<size_t>(256, kPieceBytes / (c.vocab * sizeof(float)));
-  const size_t pieces = (c.rows + fit - 1) / fit, each = (c.rows + pieces - 1) / pieces;
-  const size_t logits = (each * c.vocab + 3) / 4 * 4;
-  float* z = static_cast<float*>(scratch_alloc((logits + (c.dw ? each * c.in : 0)) * sizeof(float)));
-  if (!z) return LMP_ERR_OOM;
+  // Where memory is short, products that need none besides the logits' take over, and then
+  // smaller pieces.
+  if (half_pays(c))
+    if (int s = run_loss_half(rt, c); s != LMP_ERR_OOM) return s;
+  size_t each = 0, logits = 0;
+  float* z = nullptr;
+  for (size_t bytes = kPieceBytes;; bytes /= 4) {
+    const size_t fit = std::max<size_t>(256, bytes / (c.vocab * sizeof(float))), pieces = (c.rows + fit - 1) / fit;
+    each = (c.rows + pieces - 1) / pieces;
+    logits = (each * c.vocab + 3) / 4 * 4;
+    z = static_cast<float*>(scratch_alloc((logits + (c.dw ? each * c.in : 0)) * sizeof(float)));
+    if (z) break;
+    if (fit == 256) return LMP_ERR_OOM;
+  }
   float* counted_x = c.dw ? z + logits : nullptr;
   const auto piece = [&](size_t at, size_t n) -> int {
     const float* x = c.x + at * c.ldx;

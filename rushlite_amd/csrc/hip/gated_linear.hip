@@ -27,7 +27,6 @@ namespace {
 constexpr int kThreads = 256;
 
 struct GateArgs {
-  int gate;
   int64_t rows;
   int hidden;
   const float* pre;
@@ -36,33 +35,45 @@ struct GateArgs {
   int64_t ldg;
   float* out;  // h [rows, hidden] or d [rows, 2 hidden]
   int64_t ldo;
+  int row_lanes;  // lanes of a row: a power of two
 };
 
-// h from pre, or (BACK) d from pre and g: columns over a workgroup's lanes, rows over the
-// grid's y.
-template <bool BACK>
+// h from pre, or (BACK) d from pre and g, four columns a lane.  Bound by memory: d of 5563 rows
+// of 4672 takes 101 us, 520 MB at 5.1 TB/s.
+template <int GATE, bool BACK>
 __global__ __launch_bounds__(kThreads) void gate_rows(GateArgs a) {
-  const int col = blockIdx.x * kThreads + threadIdx.x;
-  if (col >= a.hidden) return;
-  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    const float p = a.pre[row * a.ldpre + col], u = a.pre[row * a.ldpre + a.hidden + col];
-    float act, slope;
-    with_gate(a.gate, [&](auto gate) { gate_at<decltype(gate)::value>(p, act, slope); });
-    if constexpr (BACK) {
-      const float g = a.g[row * a.ldg + col];
-      a.out[row * a.ldo + col] = g * u * slope;
-      a.out[row * a.ldo + a.hidden + col] = g * act;
-    } else {
-      a.out[row * a.ldo + col] = act * u;
+  const int lane = threadIdx.x & (a.row_lanes - 1), each = kThreads / a.row_lanes, n = a.hidden;
+  for (int64_t row = int64_t(blockIdx.x) * each + threadIdx.x / a.row_lanes; row < a.rows; row += int64_t(gridDim.x) * each)
+    for (int col = (int(blockIdx.y) * a.row_lanes + lane) * 4; col < n; col += int(gridDim.y) * a.row_lanes * 4) {
+      const float* p = a.pre + row * a.ldpre;
+      const hv4 x = load_four(p, col, n), u = load_four(p + n, col, n);
+      hv4 act, slope;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float f, s;
+        gate_at<GATE>(x[e], f, s);
+        act[e] = f;
+        slope[e] = s;
+      }
+      float* out = a.out + row * a.ldo;
+      if constexpr (BACK) {
+        const hv4 g = load_four(a.g + row * a.ldg, col, n);
+        store_four(out, col, n, g * u * slope);
+        store_four(out + n, col, n, g * act);
+      } else {
+        store_four(out, col, n, act * u);
+      }
     }
-  }
 }
 
 template <bool BACK>
-int launch_gate(Runtime* rt, const GateArgs& a) {
-  const uint32_t cols = uint32_t((int64_t(a.hidden) + kThreads - 1) / kThreads);
-  const uint32_t rows = uint32_t(std::min<int64_t>(a.rows, 65535));
-  gate_rows<BACK><<<dim3(cols, rows), dim3(kThreads), 0, rt->stream>>>(a);
+int launch_gate(Runtime* rt, int gate, GateArgs a) {
+  a.row_lanes = 1;
+  while (a.row_lanes < kThreads && a.row_lanes * 4 < a.hidden) a.row_lanes *= 2;
+  const int64_t each = kThreads / a.row_lanes, groups = (a.rows + each - 1) / each;
+  const int64_t across = std::min<int64_t>((int64_t(a.hidden) + kThreads * 4 - 1) / (kThreads * 4), 1024);
+  const dim3 grid(uint32_t(std::min<int64_t>(groups, 65536)), uint32_t(across));
+  with_gate(gate, [&](auto g) { gate_rows<decltype(g)::value, BACK><<<grid, dim3(kThreads), 0, rt->stream>>>(a); });
   LMP_LAUNCH_CHECK("gate");
   return LMP_OK;
 }
@@ -287,8 +298,9 @@ extern "C" int lmp_k_gated_linear_f32(int gate, size_t rows, size_t in, size_t h
   if (std::max({ldx, ldw, ldh, pre ? ldpre : 0}) >= kGemmMaxExtent)
     return fail(LMP_ERR_UNSUPPORTED, name + "dimension of 2^31 - 4096 or more");
   LMP_RUNTIME_OR_FAIL(rt);
+  // Where memory for the panels is short, the fp32 products take over.
   if (half_forward_pays(rows, in, hidden))
-    return gated_half(rt, gate, rows, in, hidden, x, ldx, w, ldw, bias, h, ldh, pre, ldpre);
+    if (int s = gated_half(rt, gate, rows, in, hidden, x, ldx, w, ldw, bias, h, ldh, pre, ldpre); s != LMP_ERR_OOM) return s;
   float* z = pre;
   if (!z) {
     z = static_cast<float*>(scratch_alloc(rows * 2 * hidden * sizeof(float)));
@@ -298,7 +310,7 @@ extern "C" int lmp_k_gated_linear_f32(int gate, size_t rows, size_t in, size_t h
   int rc = bias ? lmp_k_linear_f32(0, 0, rows, 2 * hidden, in, x, ldx, w, ldw, bias, z, ldpre)
                 : lmp_k_gemm_f32(0, 0, rows, 2 * hidden, in, x, ldx, w, ldw, z, ldpre, 0);
   if (rc == LMP_OK)
-    rc = launch_gate<false>(rt, {gate, int64_t(rows), int(hidden), z, int64_t(ldpre), nullptr, 0, h, int64_t(ldh)});
+    rc = launch_gate<false>(rt, gate, {int64_t(rows), int(hidden), z, int64_t(ldpre), nullptr, 0, h, int64_t(ldh), 0});
   if (!pre) scratch_free(z);
   return rc;
 }
@@ -325,12 +337,14 @@ extern "C" int lmp_k_gated_linear_backward_f32(int gate, size_t rows, size_t in,
     return clear_f32(rt, db, 1, width, width);
   }
   if (half_backward_pays(rows, in, hidden))
-    return gated_half_backward(rt, gate, rows, in, hidden, g, ldg, x, ldx, w, ldw, pre, ldpre, dx, lddx, dw, lddw, db);
+    if (int s = gated_half_backward(rt, gate, rows, in, hidden, g, ldg, x, ldx, w, ldw, pre, ldpre, dx, lddx, dw, lddw, db);
+        s != LMP_ERR_OOM)
+      return s;
   float* d = static_cast<float*>(scratch_alloc(rows * width * sizeof(float)));
   if (!d) return LMP_ERR_OOM;
   const auto run = [&]() -> int {
-    if (int s = launch_gate<true>(rt, {gate, int64_t(rows), int(hidden), pre, int64_t(ldpre), g, int64_t(ldg), d,
-                                       int64_t(width)}))
+    if (int s = launch_gate<true>(rt, gate, {int64_t(rows), int(hidden), pre, int64_t(ldpre), g, int64_t(ldg), d,
+                                             int64_t(width), 0}))
       return s;
     if (dx && dw && db)
       return lmp_k_linear_backward_f32(rows, in, width, x, ldx, w, ldw, d, width, dx, lddx, 0, dw, lddw, 0, db, 0);

@@ -86,11 +86,15 @@ class Rotary(Module):
             raise ValueError("rotary_dim is above head_dim")
         self.interleaved = interleaved
         self.frequencies, self.scale = rotary_frequencies(self.rotary_dim, base, scaling)
-        self._held = None
+        # Sent before any recording, in which a copy from the host has no place.
+        self._held = self._on_device() if _C.hip.is_available() else None
+
+    def _on_device(self):
+        return _C._Tensor(self.frequencies, [len(self.frequencies)], _C.device.hip, _C.dtype.float64)
 
     def forward(self, x, positions, heads: int):
         if self._held is None:
-            self._held = _C._Tensor(self.frequencies, [len(self.frequencies)], _C.device.hip, _C.dtype.float64)
+            self._held = self._on_device()
         return _C.rotary(x, positions, self._held, heads=heads, head_dim=self.head_dim, interleaved=self.interleaved,
                          scale=self.scale)
 

@@ -330,6 +330,20 @@ def test_recorded_decoder_step_equals_the_eager_one(rsl):
 
 
 @gpu
+def test_rotary_first_called_in_a_recording(rsl):
+    from rushlite_amd.nets import layers
+    layer, positions = layers.Rotary(8), layers.packed_positions([5])
+    x = rsl.Variable(np.random.default_rng(2).standard_normal((5, 16)).astype(np.float32))
+    graph = rsl.hip.Graph()
+    with graph.capture(), rsl.no_grad():
+        y = layer(x, positions, 2)
+    for _ in range(3):
+        graph.replay()
+        with rsl.no_grad():
+            assert np.array_equal(y.numpy(), layer(x, positions, 2).numpy())
+
+
+@gpu
 def test_the_example_runs(rsl):
     sys.path.insert(0, str(ROOT / "examples"))
     import decoder
