@@ -474,7 +474,7 @@ int run_loss_half(Runtime* rt, const LossCall& c) {
     const LossGradient of_d{int64_t(n), int(c.vocab), z, info};
     if (c.dw) {
       const auto job = tops_job(rt, of_d, nullptr, dc.tops, c.db ? base + at_sums : nullptr);
-      if (int s = run_panel_job(rt, job)) return s;
+      if (int s = run_panel_jobs(rt, job)) return s;
       if (c.db) {
         float* to = at ? base + at_db : c.db;
         const size_t mine_strips = size_t(job.blocks / job.col_blocks);
@@ -483,7 +483,7 @@ int run_loss_half(Runtime* rt, const LossCall& c) {
           if (int s = lmp_k_add_inplace(LMP_FLOAT32, c.db, to, c.vocab)) return s;
       }
     }
-    if (int s = run_panel_job(rt, pack_job(of_d, dr, dc))) return s;
+    if (int s = run_panel_jobs(rt, pack_job(of_d, dr, dc))) return s;
     HalfPanels xp = xc;  // K of dw from this piece's first row on
     if (c.dw) xp.panels += int64_t(at / kHalfK) * kHalfStep;
     return half_backward(rt, {n, c.in, c.vocab, dr, dc, xp, wr, c.dx ? c.dx + at * c.lddx : nullptr, c.lddx, c.dw, c.lddw,

@@ -249,15 +249,14 @@ int gated_half_backward(Runtime* rt, int gate, size_t rows, size_t in, size_t hi
   size_t strips = 0;
   const auto run = [&]() -> int {
     if (int s = clear_words(rt, base, tops)) return s;
-    if (int s = run_panel_jobs(rt, tops_job(rt, of_w, wr.tops, nullptr), tops_job(rt, of_x, nullptr, xc.tops))) return s;
-    if (int s = run_panel_jobs(rt, pack_job(of_w, wr, none), pack_job(of_x, none, xc))) return s;
     if (int s = with_gate(gate, [&](auto gt) -> int {
           const GatedGradient<decltype(gt)::value> of_d{{int64_t(rows), int(cols), int(hidden)}, pre, int64_t(ldpre), g, int64_t(ldg)};
           auto job = tops_job(rt, of_d, dr.tops, dc.tops, sums);
           job.sums_ld = int64_t(width);
           strips = size_t(job.blocks / job.col_blocks);
-          if (int e = run_panel_job(rt, job)) return e;
-          return dx || dw ? run_panel_job(rt, pack_job(of_d, dr, dc)) : LMP_OK;
+          if (int e = run_panel_jobs(rt, job, tops_job(rt, of_w, wr.tops, nullptr), tops_job(rt, of_x, nullptr, xc.tops))) return e;
+          if (!dx && !dw) return LMP_OK;
+          return run_panel_jobs(rt, pack_job(of_d, dr, dc), pack_job(of_w, wr, none), pack_job(of_x, none, xc));
         }))
       return s;
     if (db)

@@ -99,7 +99,9 @@ struct TopsJob {
     const int64_t strip = block / col_blocks, begin = strip * each;
     const int count = int(min(int64_t(each), s.rows - begin)), col0 = int(block - strip * col_blocks) * width;
     const int unit = col0 / 8 + across * 64 + lane;
-    for (int i = threadIdx.x; i < kTopsRows + 2048; i += kTopsThreads) rows[i] = 0;
+    if (row_top)
+      for (int i = threadIdx.x; i < count; i += kTopsThreads) rows[i] = 0;
+    for (int i = threadIdx.x; i < width; i += kTopsThreads) tops[i] = 0;
     __syncthreads();
     uint32_t top[2][4] = {};
     hv4 sum[2] = {hv4(0.0f), hv4(0.0f)};
@@ -164,7 +166,7 @@ template <class S>
 TopsJob<S> tops_job(Runtime* rt, const S& s, uint32_t* row_top, uint32_t* col_top, float* sums = nullptr) {
   const int wide = tops_wide(s.cols), width = 512 << wide, col_blocks = (s.cols + width - 1) / width;
   const int64_t most = most_strips(rt, s.rows, s.cols);
-  const int each = int(std::max<int64_t>((s.rows + most - 1) / most, 16 >> wide));
+  const int each = int(std::max<int64_t>((s.rows + most - 1) / most, 64 >> wide));
   return {s, row_top, col_top, sums, s.cols, each, wide, col_blocks, (s.rows + each - 1) / each * col_blocks};
 }
 
@@ -247,39 +249,38 @@ PackJob<S> pack_job(const S& s, const HalfPanels& r, const HalfPanels& c) {
   return {s, r, c, tiles_c, tiles_r * tiles_c};
 }
 
-// One launch for two jobs of one kind.
-template <int NT, class A, class B>
-__global__ __launch_bounds__(NT) void panel_jobs(A a, B b) {
-  __shared__ __attribute__((aligned(16))) char smem[A::SMEM];
-  const int64_t block = blockIdx.x;
-  if (block < a.blocks) a.run(block, smem);
-  else b.run(block - a.blocks, smem);
+// One launch for jobs of one kind, one after another in the grid.
+template <int NT, int SMEM, class... Jobs>
+__global__ __launch_bounds__(NT) void panel_jobs(Jobs... jobs) {
+  __shared__ __attribute__((aligned(16))) char smem[SMEM];
+  int64_t block = blockIdx.x;
+  bool done = false;
+  const auto turn = [&](const auto& job) {
+    if (!done && block < job.blocks) {
+      job.run(block, smem);
+      done = true;
+    }
+    block -= job.blocks;
+  };
+  (turn(jobs), ...);
 }
-template <int NT, class A, class B>
-int launch_panel_jobs(Runtime* rt, const A& a, const B& b) {
-  static_assert(A::SMEM == B::SMEM);
-  const int64_t blocks = a.blocks + b.blocks;
+template <int NT, int SMEM, class... Jobs>
+int launch_panel_jobs(Runtime* rt, const Jobs&... jobs) {
+  const int64_t blocks = (jobs.blocks + ...);
   if (blocks == 0) return LMP_OK;
   if (uint64_t(blocks) > kMaxGridThreads / NT)
     return fail(LMP_ERR_UNSUPPORTED, "split products: more tiles than a grid holds");
-  panel_jobs<NT><<<dim3(uint32_t(blocks)), dim3(NT), 0, rt->stream>>>(a, b);
+  panel_jobs<NT, SMEM><<<dim3(uint32_t(blocks)), dim3(NT), 0, rt->stream>>>(jobs...);
   LMP_LAUNCH_CHECK("panel_jobs");
   return LMP_OK;
 }
-template <class A, class B>
-int run_panel_jobs(Runtime* rt, const TopsJob<A>& a, const TopsJob<B>& b) {
-  return launch_panel_jobs<kTopsThreads>(rt, a, b);
+template <class... S>
+int run_panel_jobs(Runtime* rt, const TopsJob<S>&... jobs) {
+  return launch_panel_jobs<kTopsThreads, TopsJob<MatrixSource>::SMEM>(rt, jobs...);
 }
-template <class A, class B>
-int run_panel_jobs(Runtime* rt, const PackJob<A>& a, const PackJob<B>& b) {
-  return launch_panel_jobs<kPanelThreads>(rt, a, b);
-}
-// One job alone.
-template <class J>
-int run_panel_job(Runtime* rt, const J& a) {
-  J none = a;
-  none.blocks = 0;
-  return run_panel_jobs(rt, a, none);
+template <class... S>
+int run_panel_jobs(Runtime* rt, const PackJob<S>&... jobs) {
+  return launch_panel_jobs<kPanelThreads, PackJob<MatrixSource>::SMEM>(rt, jobs...);
 }
 
 }  // namespace
