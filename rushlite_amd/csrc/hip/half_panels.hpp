@@ -9,6 +9,8 @@
 //   int place(int col)                              where that column's sum goes, or -1
 //
 // Bound by memory: a pass reads 4 bytes a value and the second writes 4 for each set of panels.
+// w of 1024 x 32768 and x of 4096 x 1024 take 42 us and, with both sets of panels, 76 (151 MB at
+// 3.6 TB/s, 453 at 5.9); dz of 4096 x 32768, formed from the logits in both, 165 and 300.
 #pragma once
 
 #include <hip/hip_runtime.h>
