@@ -24,7 +24,7 @@
 // advances 32 at a time through two LDS stages, each half's fragments read while the products
 // of the half before run.  One barrier a step, in its middle: the stage has been read by
 // then, the next one has arrived, and the loads of the one after it start, a whole step
-// ahead of their use.  Of a 256 x 256 step's 3072 cycles of MFMA the LDS takes 2048.
+// ahead of their use.  The LDS is busy for two thirds of a 256 x 256 step's MFMA cycles.
 //
 // Bound by the chip's power: random operands run at 397 TFLOP/s (8192 x 32768 over 1024,
 // 1.19 PFLOP/s of fp16, the clock at 1.7 of 2.4 GHz) to 422 (1024 x 32768 over 4096), zeros at
