@@ -198,17 +198,24 @@ inline float half_makespan(int64_t slots, int64_t n0, float t0, int64_t n1, floa
   const int64_t whole = n0 / slots, late = n0 % slots;
   const float begin = float(whole) * t0, last = late ? begin + t0 : begin;
   if (n1 == 0) return last;
-  // Both kinds of slots take turns at t1: the least of the times at which one of them ends a turn
-  // that leaves nothing to do.
-  float best = 0.0f;
-  for (int64_t turns = std::max<int64_t>(n1 / slots, 1);; ++turns) {
-    const float ends[2] = {begin + float(turns) * t1, late ? last + float(turns) * t1 : begin + float(turns) * t1};
-    for (float end : ends) {
-      const int64_t early_turns = int64_t((end - begin) / t1 + 1e-3f), late_turns = int64_t((end - last) / t1 + 1e-3f);
-      if ((slots - late) * early_turns + late * std::max<int64_t>(late_turns, 0) >= n1 && (best == 0.0f || end < best)) best = end;
+  // Both kinds of slots take turns at t1: the first end of a turn of one of them at which n1 are done.
+  const auto done = [&](float end) {
+    const int64_t early = int64_t((end - begin) / t1 + 1e-3f), after = std::max<int64_t>(int64_t((end - last) / t1 + 1e-3f), 0);
+    return (slots - late) * early + late * after >= n1;
+  };
+  const auto first = [&](float from, int64_t most) {  // of turns 1 to `most`, the last of which is enough
+    int64_t low = 1;
+    while (low < most) {
+      const int64_t mid = (low + most) / 2;
+      if (done(from + float(mid) * t1)) most = mid;
+      else low = mid + 1;
     }
-    if (best != 0.0f) return std::max(best, last);
-  }
+    return from + float(low) * t1;
+  };
+  float end = first(begin, (n1 + slots - late - 1) / (slots - late));
+  const int64_t turns = late ? int64_t((end - last) / t1) : 0;
+  if (turns >= 1 && done(last + float(turns) * t1)) end = std::min(end, first(last, turns));
+  return std::max(end, last);
 }
 
 // The configuration, splits and order with the least modelled time; partial sums stay within
