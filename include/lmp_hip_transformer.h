@@ -162,12 +162,12 @@ int lmp_k_rotary(int dtype, size_t rows, size_t cols, size_t heads, size_t head_
  * library's, 0 before the first call.  Keeping it on the device lets a recorded call draw
  * afresh at every replay.  `used` (one int64 on the device, or null where no backward pass
  * follows) takes the number of this call.  What is dropped, infinities and NaN too, leaves
- * no trace.  y may be x or residual. */
+ * no trace.  y may be x or residual; another overlap is refused. */
 int lmp_k_dropout(int dtype, size_t n, const void* x, const void* residual, double rate,
                   uint64_t seed, int64_t* state, int64_t* used, void* y);
 
 /* dx = kept ? g / (1 - rate) : 0 by what the call numbered *used kept (the residual's
- * gradient is g).  dx may be g. */
+ * gradient is g).  dx may be g; another overlap is refused. */
 int lmp_k_dropout_backward(int dtype, size_t n, const void* g, double rate, uint64_t seed,
                            const int64_t* used, void* dx);
 

@@ -144,6 +144,14 @@ int check_dropout(const std::string& name, int dtype, size_t n, double rate) {
   return LMP_OK;
 }
 
+// y is an operand or apart from it: workgroups have no order among them.
+int check_apart(const std::string& name, int dtype, size_t n, const void* operand, const void* y) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(operand), b = reinterpret_cast<uintptr_t>(y);
+  if (operand && a != b && (a < b ? b - a : a - b) < n * (dtype == LMP_FLOAT64 ? 8 : 4))
+    return fail(LMP_ERR_INVALID, name + "the output overlaps an operand without being it");
+  return LMP_OK;
+}
+
 template <typename T>
 DropoutArgs<T> dropout_args(size_t n, const void* x, const void* residual, double rate, uint64_t seed,
                             void* y) {
@@ -172,6 +180,8 @@ extern "C" int lmp_k_dropout(int dtype, size_t n, const void* x, const void* res
   if (!state || (n && (!x || !y))) return fail(LMP_ERR_INVALID, "lmp_k_dropout: null buffer");
   if (used && (used == state || used == state + 1))
     return fail(LMP_ERR_INVALID, "lmp_k_dropout: used is part of the state");
+  for (const void* operand : {x, residual})
+    if (int s = check_apart("lmp_k_dropout: ", dtype, n, operand, y)) return s;
   LMP_RUNTIME_OR_FAIL(rt);
   const auto go = [&](auto zero) {
     using T = decltype(zero);
@@ -188,6 +198,7 @@ extern "C" int lmp_k_dropout_backward(int dtype, size_t n, const void* g, double
   if (int s = check_dropout("lmp_k_dropout_backward: ", dtype, n, rate)) return s;
   if (n == 0) return LMP_OK;
   if (!g || !used || !dx) return fail(LMP_ERR_INVALID, "lmp_k_dropout_backward: null buffer");
+  if (int s = check_apart("lmp_k_dropout_backward: ", dtype, n, g, dx)) return s;
   LMP_RUNTIME_OR_FAIL(rt);
   const auto go = [&](auto zero) {
     using T = decltype(zero);

@@ -73,6 +73,21 @@ def test_dropout_backward_refusals(L, change, text):
     refused(L.lmp_k_dropout_backward(*{**DROP_BACK, **change}.values()), text)
 
 
+@pytest.mark.parametrize("change", [dict(y=P + 4), dict(y=P + 36), dict(x=P + 36, y=P), dict(residual=3 * P + 8),
+                                    dict(dtype=5, y=P + 76)], ids=str)
+def test_dropout_refuses_an_output_beside_itself(L, change):
+    refused(L.lmp_k_dropout(*{**DROP, **change}.values()), "overlaps")
+    if "residual" not in change:
+        y = change["y"]
+        refused(L.lmp_k_dropout_backward(*{**DROP_BACK, "dtype": change.get("dtype", 4), "g": change.get("x", P), "dx": y}.values()),
+                "overlaps")
+
+
+def test_dropout_takes_outputs_that_touch_an_operand(L):
+    for change in (dict(y=P + 40), dict(x=P + 40, y=P), dict(dtype=5, y=P + 80), dict(residual=3 * P)):
+        no_device(L.lmp_k_dropout(*{**DROP, **change}.values()))
+
+
 def test_dropout_edges(L):
     assert L.lmp_k_dropout_backward(*{**DROP_BACK, "n": 0, "g": None}.values()) == 0
     refused(L.lmp_k_dropout(*{**DROP, "n": 1 << 41}.values()), "too many", 4)
