@@ -19,6 +19,7 @@
 
 #include "common.hpp"
 #include "gemm_half.hpp"
+#include "half_backward.hpp"
 #include "half_panels.hpp"
 #include "half_products.hpp"
 #include "lmp_hip_transformer.h"
@@ -303,14 +304,12 @@ __device__ __forceinline__ float over_eight(float x, bool most) {
 }
 
 template <int NT, int MINB, class C>
-__global__ __launch_bounds__(NT, MINB) void half_logits(HalfArgs g, HalfLogits o) {
+__global__ __launch_bounds__(NT, MINB) void half_logits(HalfArgs g, HalfLogits o, RowsOf<MatrixSource> x, ColsOf<MatrixSource> w) {
   static_assert(NT == C::THREADS && C::TN == 2, "a wave has 64 columns");
   __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
-  hv16 acc[C::TM][C::TN];
   const HalfItem at = half_item(g, int(blockIdx.x));
-  half_tile<C>(g, at, smem, acc);
   const int wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % C::WN, col0 = at.tile_n * C::BN + wn * 64;
-  half_epilogue<C>(g, at, smem, acc, [&](int row, int c4, hv4 (&v)[2]) {
+  half_product<C>(g, at, smem, x, w, [&](int row, int c4, hv4 (&v)[2]) {
     const float low = -__builtin_huge_valf();
     const int64_t target = row < g.m ? o.targets[row] : -1;
     float top = low;
@@ -344,8 +343,7 @@ struct LossRow {
   int target;  // -1: not counted, or past the vocabulary (whose factor is NaN)
 };
 
-// The rows' losses from their parts, a wave a row; with `info` what the gradient needs, and
-// |weight|, which no |dz| passes, as the row's largest magnitude.
+// The rows' losses from their parts, a wave a row; with `info` what the gradient needs.
 struct HalfRows {
   int64_t rows;
   int parts, vocab;
@@ -355,7 +353,6 @@ struct HalfRows {
   const float* weights;
   float* loss;
   LossRow* info;
-  uint32_t* row_top;
 };
 __global__ __launch_bounds__(256) void half_loss_rows(HalfRows a) {
   const int lane = threadIdx.x & 63;
@@ -372,7 +369,6 @@ __global__ __launch_bounds__(256) void half_loss_rows(HalfRows a) {
     if (a.info) {
       const float w = !counted ? 0.0f : !known ? nan : a.weights ? a.weights[row] : 1.0f;
       a.info[row] = {s.top, w / s.sum, w, counted && known ? int(t) : counted ? -2 : -1};
-      a.row_top[row] = finite_magnitude(w);
     }
   }
 }
@@ -398,8 +394,12 @@ struct LossGradient {
   }
   __device__ __forceinline__ int column(int unit, int h) const { return 8 * unit + 4 * h; }
   __device__ __forceinline__ int place(int col) const { return col; }
+  __device__ __forceinline__ float value(int64_t row, int col) const {
+    const LossRow r = info[row];
+    const float p = exp_below(z[row * cols + col] - r.top) * r.factor;
+    return r.target == -1 ? 0.0f : col == r.target ? p - r.weight : p;
+  }
 };
-
 
 int check_loss(const std::string& name, const LossCall& c) {
   if (c.in == 0 || c.vocab == 0) return fail(LMP_ERR_INVALID, name + "no inputs or no vocabulary");
@@ -438,7 +438,7 @@ int run_loss_half(Runtime* rt, const LossCall& c) {
   const size_t of_xr = room.take(half_tops_words(c.rows)), of_wc = room.take(half_tops_words(c.vocab));
   const size_t of_xc = room.take(c.dw ? half_tops_words(c.in) : 0), of_wr = room.take(c.dx ? half_tops_words(c.in) : 0);
   const size_t of_dr = room.take(grad ? half_tops_words(each) : 0), of_dc = room.take(grad ? half_tops_words(c.vocab) : 0);
-  const size_t tops = room.words;
+  const size_t tops = room.words, of_marks = room.take(tops);
   const size_t at_part = room.take(each * size_t(parts) * 2), at_hit = room.take(each), at_info = room.take(grad ? each * 4 : 0);
   const size_t at_sums = room.take(strips * c.vocab), at_db = room.take(c.db ? c.vocab : 0);
   const size_t at_z = room.take(grad ? each * c.vocab : 0);
@@ -451,54 +451,55 @@ int run_loss_half(Runtime* rt, const LossCall& c) {
   if (!base) return LMP_ERR_OOM;
   uint32_t* words = reinterpret_cast<uint32_t*>(base);
   const auto panels = [&](size_t at, size_t k, size_t of) {
-    return HalfPanels{reinterpret_cast<char*>(words + at), int64_t(half_stride(k)), words + of};
+    return HalfPanels{reinterpret_cast<char*>(words + at), int64_t(half_stride(k)), words + of, words + of_marks + of};
   };
   const HalfPanels none{}, xr = panels(at_xr, c.in, of_xr), wc = panels(at_wc, c.in, of_wc);
   const HalfPanels xc = c.dw ? panels(at_xc, c.rows, of_xc) : none, wr = c.dx ? panels(at_wr, c.vocab, of_wr) : none;
+  const MatrixSource of_w{int64_t(c.in), int(c.vocab), c.w, int64_t(c.ldw), nullptr};
   const auto piece = [&](size_t at, size_t n) -> int {
-    const HalfPanels mine{xr.panels + int64_t(at / 64) * xr.stride, xr.stride, xr.tops + at};
+    const HalfPanels mine{xr.panels + int64_t(at / 64) * xr.stride, xr.stride, xr.tops + at, xr.marks + at};
     const HalfArgs g = half_args(mine, wc, int(n), int(c.vocab), int(c.in), plan.cfg, 1);
     float* z = grad ? base + at_z : nullptr;
     Softmax* part = reinterpret_cast<Softmax*>(base + at_part);
     LossRow* info = grad ? reinterpret_cast<LossRow*>(base + at_info) : nullptr;
     const HalfLogits o{c.bias, z, part, parts, c.targets + at, base + at_hit};
+    const MatrixSource x{int64_t(n), int(c.in), c.x + at * c.ldx, int64_t(c.ldx), c.targets + at};
     if (int s = with_half_cfg(plan.cfg, [&](auto cfg) -> int {
           using C = decltype(cfg);
-          half_logits<C::THREADS, C::MINB, C><<<dim3(half_items(g)), dim3(C::THREADS), 0, rt->stream>>>(g, o);
+          half_logits<C::THREADS, C::MINB, C><<<dim3(half_items(g)), dim3(C::THREADS), 0, rt->stream>>>(g, o, {x}, {of_w});
           LMP_LAUNCH_CHECK("half_logits");
           return LMP_OK;
         }))
       return s;
     const HalfRows r{int64_t(n), parts, int(c.vocab), part, base + at_hit, c.targets + at,
-                     c.weights ? c.weights + at : nullptr, c.loss + at, info, words + of_dr};
+                     c.weights ? c.weights + at : nullptr, c.loss + at, info};
     half_loss_rows<<<dim3(uint32_t(std::min<size_t>((n + 3) / 4, 65536))), dim3(256), 0, rt->stream>>>(r);
     LMP_LAUNCH_CHECK("half_loss_rows");
     if (!grad) return LMP_OK;
-    if (at)
-      if (int s = clear_words(rt, words + of_dc, half_tops_words(c.vocab))) return s;
+    if (at) {
+      if (int s = clear_words(rt, words + of_dr, tops - of_dr)) return s;
+      if (int s = clear_words(rt, words + of_marks + of_dr, tops - of_dr)) return s;
+    }
     const HalfPanels dr = c.dx ? panels(at_dr, c.vocab, of_dr) : none, dc = c.dw ? panels(at_dc, n, of_dc) : none;
     const LossGradient of_d{int64_t(n), int(c.vocab), z, info};
-    if (c.dw) {
-      const auto job = tops_job(rt, of_d, nullptr, dc.tops, c.db ? base + at_sums : nullptr);
-      if (int s = run_panel_jobs(rt, job)) return s;
-      if (c.db) {
-        float* to = at ? base + at_db : c.db;
-        const size_t mine_strips = size_t(job.blocks / job.col_blocks);
-        if (int s = lmp_k_reduce(LMP_RED_SUM, LMP_FLOAT32, to, base + at_sums, 1, mine_strips, c.vocab)) return s;
-        if (at)
-          if (int s = lmp_k_add_inplace(LMP_FLOAT32, c.db, to, c.vocab)) return s;
-      }
+    const auto job = tops_job(rt, of_d, dr.tops, dc.tops, c.db ? base + at_sums : nullptr);
+    if (int s = run_panel_jobs(rt, job)) return s;
+    if (c.db) {
+      float* to = at ? base + at_db : c.db;
+      const size_t mine_strips = size_t(job.blocks / job.col_blocks);
+      if (int s = lmp_k_reduce(LMP_RED_SUM, LMP_FLOAT32, to, base + at_sums, 1, mine_strips, c.vocab)) return s;
+      if (at)
+        if (int s = lmp_k_add_inplace(LMP_FLOAT32, c.db, to, c.vocab)) return s;
     }
     if (int s = run_panel_jobs(rt, pack_job(of_d, dr, dc))) return s;
     HalfPanels xp = xc;  // K of dw from this piece's first row on
     if (c.dw) xp.panels += int64_t(at / kHalfK) * kHalfStep;
-    return half_backward(rt, {n, c.in, c.vocab, dr, dc, xp, wr, c.dx ? c.dx + at * c.lddx : nullptr, c.lddx, c.dw, c.lddw,
-                              at > 0, 0});
+    return half_backward<LossGradient, MatrixSource>(
+        rt, {n, c.in, c.vocab, dr, dc, xp, wr, c.dx ? c.dx + at * c.lddx : nullptr, c.lddx, c.dw, c.lddw, at > 0, 0, x, of_d, of_w});
   };
   const auto run = [&]() -> int {
-    if (int s = clear_words(rt, words, tops)) return s;
+    if (int s = clear_words(rt, words, 2 * tops)) return s;
     const MatrixSource of_x{int64_t(c.rows), int(c.in), c.x, int64_t(c.ldx), c.targets};
-    const MatrixSource of_w{int64_t(c.in), int(c.vocab), c.w, int64_t(c.ldw), nullptr};
     if (int s = run_panel_jobs(rt, tops_job(rt, of_w, wr.tops, wc.tops), tops_job(rt, of_x, xr.tops, xc.tops))) return s;
     if (int s = run_panel_jobs(rt, pack_job(of_w, wr, wc), pack_job(of_x, xr, xc))) return s;
     for (size_t at = 0; at < c.rows; at += each)

@@ -18,6 +18,7 @@
 #include "common.hpp"
 #include "gate.hpp"
 #include "gemm_half.hpp"
+#include "half_backward.hpp"
 #include "half_panels.hpp"
 #include "half_products.hpp"
 #include "lmp_hip_transformer.h"
@@ -106,6 +107,10 @@ struct GatedWeights : Turned {
     v[0] = load_four(p, within(unit), hidden);
     v[1] = load_four(p + hidden, within(unit), hidden);
   }
+  __device__ __forceinline__ float value(int64_t row, int col) const {
+    const int at = place(col);
+    return at < 0 ? 0.0f : w[row * ld + at];
+  }
 };
 
 // d, formed from pre and g.
@@ -128,6 +133,27 @@ struct GatedGradient : Turned {
     }
   }
 };
+// The same of any gate, for what is formed again.
+struct AnyGatedGradient : Turned {
+  const float* pre;
+  int64_t ldpre;
+  const float* g;
+  int64_t ldg;
+  int gate;
+  __device__ __forceinline__ void load(int64_t row, int unit, hv4 (&v)[2]) const {
+    with_gate(gate, [&](auto gt) {
+      GatedGradient<decltype(gt)::value>{{rows, cols, hidden}, pre, ldpre, g, ldg}.load(row, unit, v);
+    });
+  }
+  __device__ __forceinline__ float value(int64_t row, int col) const {
+    const int c = half_col(col);
+    if (c >= hidden) return 0.0f;
+    const float a = pre[row * ldpre + c], u = pre[row * ldpre + hidden + c], gr = g[row * ldg + c];
+    float act, slope;
+    with_gate(gate, [&](auto gt) { gate_at<decltype(gt)::value>(a, act, slope); });
+    return second_half(col) ? gr * act : gr * u * slope;
+  }
+};
 
 struct HalfGated {
   int gate, hidden;
@@ -140,15 +166,13 @@ struct HalfGated {
 
 // h (and pre) of a tile: a lane ends with both halves of a hidden value.
 template <int NT, int MINB, class C>
-__global__ __launch_bounds__(NT, MINB) void half_gated(HalfArgs g, HalfGated o) {
+__global__ __launch_bounds__(NT, MINB) void half_gated(HalfArgs g, HalfGated o, RowsOf<MatrixSource> x, ColsOf<GatedWeights> w) {
   static_assert(NT == C::THREADS && C::TN == 2, "a wave has 32 columns of each half");
   __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
-  hv16 acc[C::TM][C::TN];
   const HalfItem at = half_item(g, int(blockIdx.x));
-  half_tile<C>(g, at, smem, acc);
   const int wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % C::WN;
   const int col0 = at.tile_n * (C::BN / 2) + wn * 32;
-  half_epilogue<C>(g, at, smem, acc, [&](int row, int c4, hv4 (&v)[2]) {
+  half_product<C>(g, at, smem, x, w, [&](int row, int c4, hv4 (&v)[2]) {
     const int col = col0 + c4;
     if (row >= g.m || col >= o.hidden) return;
     if (o.bias) {
@@ -190,9 +214,9 @@ bool half_backward_pays(size_t rows, size_t in, size_t hidden) {
          half_saves_backward(n * d * w) > 25 + pass_time(12 * (n * d + d * w) + 10 * n * w);
 }
 
-// The workspace as panels and their rows' magnitudes.
-HalfPanels panels_at(uint32_t* base, size_t panels, size_t k, size_t tops) {
-  return {reinterpret_cast<char*>(base + panels), int64_t(half_stride(k)), base + tops};
+// The workspace as panels, their rows' magnitudes and, `tops` words on, marks.
+HalfPanels panels_at(uint32_t* base, size_t panels, size_t k, size_t at, size_t tops) {
+  return {reinterpret_cast<char*>(base + panels), int64_t(half_stride(k)), base + at, base + at + tops};
 }
 
 int gated_half(Runtime* rt, int gate, size_t rows, size_t in, size_t hidden, const float* x, size_t ldx,
@@ -202,21 +226,22 @@ int gated_half(Runtime* rt, int gate, size_t rows, size_t in, size_t hidden, con
   if (plan.cfg < 0) return fail(LMP_ERR_UNSUPPORTED, "gated_linear: more tiles than a grid holds");
   HalfRoom room;
   const size_t at_x = room.take(half_tops_words(rows)), at_w = room.take(half_tops_words(cols)), tops = room.words;
+  room.take(tops);
   const size_t x_panels = room.take(half_panel_words(rows, in)), w_panels = room.take(half_panel_words(cols, in));
   uint32_t* base = static_cast<uint32_t*>(scratch_alloc(room.words * sizeof(uint32_t)));
   if (!base) return LMP_ERR_OOM;
-  const HalfPanels xr = panels_at(base, x_panels, in, at_x), wc = panels_at(base, w_panels, in, at_w), none{};
+  const HalfPanels xr = panels_at(base, x_panels, in, at_x, tops), wc = panels_at(base, w_panels, in, at_w, tops), none{};
   const MatrixSource of_x{int64_t(rows), int(in), x, int64_t(ldx), nullptr};
   const GatedWeights of_w{{int64_t(in), int(cols), int(hidden)}, w, int64_t(ldw)};
   const auto run = [&]() -> int {
-    if (int s = clear_words(rt, base, tops)) return s;
+    if (int s = clear_words(rt, base, 2 * tops)) return s;
     if (int s = run_panel_jobs(rt, tops_job(rt, of_w, nullptr, wc.tops), tops_job(rt, of_x, xr.tops, nullptr))) return s;
     if (int s = run_panel_jobs(rt, pack_job(of_w, none, wc), pack_job(of_x, xr, none))) return s;
     const HalfArgs g = half_args(xr, wc, int(rows), int(cols), int(in), plan.cfg, 1);
     const HalfGated o{gate, int(hidden), bias, h, int64_t(ldh), pre, int64_t(ldpre)};
     return with_half_cfg(plan.cfg, [&](auto cfg) -> int {
       using C = decltype(cfg);
-      half_gated<C::THREADS, C::MINB, C><<<dim3(half_items(g)), dim3(C::THREADS), 0, rt->stream>>>(g, o);
+      half_gated<C::THREADS, C::MINB, C><<<dim3(half_items(g)), dim3(C::THREADS), 0, rt->stream>>>(g, o, {of_x}, {of_w});
       LMP_LAUNCH_CHECK("half_gated");
       return LMP_OK;
     });
@@ -234,6 +259,7 @@ int gated_half_backward(Runtime* rt, int gate, size_t rows, size_t in, size_t hi
   HalfRoom room;
   const size_t at_dr = room.take(half_tops_words(rows)), at_dc = room.take(half_tops_words(cols));
   const size_t at_x = room.take(half_tops_words(in)), at_w = room.take(half_tops_words(in)), tops = room.words;
+  room.take(tops);
   const size_t d_rows = room.take(dx ? half_panel_words(rows, cols) : 0);
   const size_t d_cols = room.take(dw ? half_panel_words(cols, rows) : 0);
   const size_t x_panels = room.take(dw ? half_panel_words(in, rows) : 0);
@@ -242,14 +268,14 @@ int gated_half_backward(Runtime* rt, int gate, size_t rows, size_t in, size_t hi
   uint32_t* base = static_cast<uint32_t*>(scratch_alloc(room.words * sizeof(uint32_t)));
   if (!base) return LMP_ERR_OOM;
   HalfPanels none{}, dr = none, dc = none, xc = none, wr = none;
-  if (dx) dr = panels_at(base, d_rows, cols, at_dr), wr = panels_at(base, w_panels, cols, at_w);
-  if (dw) dc = panels_at(base, d_cols, rows, at_dc), xc = panels_at(base, x_panels, rows, at_x);
+  if (dx) dr = panels_at(base, d_rows, cols, at_dr, tops), wr = panels_at(base, w_panels, cols, at_w, tops);
+  if (dw) dc = panels_at(base, d_cols, rows, at_dc, tops), xc = panels_at(base, x_panels, rows, at_x, tops);
   float* sums = db ? reinterpret_cast<float*>(base + at_sums) : nullptr;
   const MatrixSource of_x{dw ? int64_t(rows) : 0, int(in), x, int64_t(ldx), nullptr};
   const GatedWeights of_w{{dx ? int64_t(in) : 0, int(cols), int(hidden)}, w, int64_t(ldw)};
   size_t strips = 0;
   const auto run = [&]() -> int {
-    if (int s = clear_words(rt, base, tops)) return s;
+    if (int s = clear_words(rt, base, 2 * tops)) return s;
     if (int s = with_gate(gate, [&](auto gt) -> int {
           const GatedGradient<decltype(gt)::value> of_d{{int64_t(rows), int(cols), int(hidden)}, pre, int64_t(ldpre), g, int64_t(ldg)};
           auto job = tops_job(rt, of_d, dr.tops, dc.tops, sums);
@@ -262,7 +288,9 @@ int gated_half_backward(Runtime* rt, int gate, size_t rows, size_t in, size_t hi
       return s;
     if (db)
       if (int s = lmp_k_reduce(LMP_RED_SUM, LMP_FLOAT32, db, sums, 1, strips, width)) return s;
-    return half_backward(rt, {rows, in, cols, dr, dc, xc, wr, dx, lddx, dw, lddw, false, hidden});
+    const AnyGatedGradient any{{int64_t(rows), int(cols), int(hidden)}, pre, int64_t(ldpre), g, int64_t(ldg), gate};
+    return half_backward<AnyGatedGradient, GatedWeights>(
+        rt, {rows, in, cols, dr, dc, xc, wr, dx, lddx, dw, lddw, false, hidden, of_x, any, of_w});
   };
   const int rc = run();
   scratch_free(base);

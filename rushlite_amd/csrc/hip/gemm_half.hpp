@@ -1,20 +1,28 @@
 // fp32 products on the fp16 matrix cores, each operand in two fp16 parts.
 //
-// Why.  A value scaled by a power of two is x = h + m + r with h = fp16(x), m =
-// fp16(x - h) and |r| <= 2^-22 |x|, so
-//   a b = ah bh + ah bm + am bh + (am bm and what the r leave out: 3 x 2^-22 at most)
+// Why.  A value scaled by a power of two is x = h + m / 64 + r with h = fp16(x), m =
+// fp16(64 (x - h)) and |r| <= 2^-22 |x|, so
+//   a b = ah bh + (ah / 64) bm + am (bh / 64) + (what both m make and what the r leave out: 3 x 2^-22 at most)
 // is three fp16 MFMAs with fp32 accumulation, half of what three bf16 parts cost
 // (gemm_bf3.hpp), with a product's error near that of rounding its operands: a sum's
-// error is its own roundings'.
+// error is its own roundings'.  The h / 64 are formed in registers.
 //
 // Range.  Each row of A and each column of B has a power of two that takes its largest
-// finite magnitude to [2^14, 2^15): values down to 2^-17 of the largest keep both parts
-// whole, smaller ones lose at most 2^-40 of it.  The two powers leave the sum at the end,
-// exactly.  An infinity keeps its sign in h and has m = 0; it leaves a sum that is not
-// finite, and a workgroup that finds one forms its tile again with the parts h that are not
-// finite left out of the two small products, where 0 x infinity would be NaN.
+// finite magnitude to [2^14, 2^15).  Values down to 2^-8, 2^-23 of the largest, keep both
+// parts whole.  Of a smaller one r, and what rounding h / 64 to fp16's smallest step costs its
+// product with the other operand's m, are 2^-31 and 2^-30 + 2^-36 of the other value at most:
+// 2^-19 of the product down to 2^-11.  The na and nb values of a sum's row and column that are
+// smaller still (kHalfSmall) put it off by (na + nb) 2^15 (2^-31 + 2^-30 + 2^-36) < (na + nb) 2^-14.  So
+// a sum of k products that is 2^8 (na + nb) / k or more errs by (4 k + 44) 2^-24 of its products'
+// magnitudes at most, and by far less where the roundings go both ways; one that is less,
+// where large values meet zeros, or that is not finite, is formed again in fp32 from the
+// operands themselves: up to kHalfList of a tile one by one, and all of the tile by fp32 MFMAs
+// where there are more.  The panels' kernel counts the small values.  One tile of 256 x 256 over
+// 1024 normal values in 35 has any and looks at its sums; the others know before the K loop that
+// they need not.  The second part's own power of two, which makes the small values 32 times
+// fewer, takes 1% of 8192 x 32768 over 1024 and 2% of 12608 x 4096 over 768.
 //
-// Operands are split once, by kernels of their own (half_products.hip), into panels of 64
+// Operands are split once, by kernels of their own (half_panels.hpp), into panels of 64
 // rows of A, or columns of B:
 //   [row / 64][k / 8][part][row % 64][k % 8], K filled up with zeros to a multiple of 32, rows to 256,
 // so that 64 rows of one octet are a kilobyte in a row, which one wave's load takes to LDS
@@ -51,12 +59,14 @@ typedef float hv4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef float hv16 __attribute__((ext_vector_type(16)));
 typedef uint32_t hu4 __attribute__((ext_vector_type(4)));
 typedef int hi4 __attribute__((ext_vector_type(4)));
-typedef uint16_t hw8 __attribute__((ext_vector_type(8)));
 
 // Kept out of the templates: a target builtin inside a kernel template keeps the host
 // pass from emitting the kernel's launch stub.
 __device__ __forceinline__ hv16 mfma_f16(hf8 a, hf8 b, hv16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ hv16 mfma_whole(float a, float b, hv16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
 }
 // 16 bytes a lane from memory to LDS: lane l's to lds + 16 l.
 __device__ __forceinline__ void panel_load(const char* src, char* lds) {
@@ -76,6 +86,21 @@ __device__ __forceinline__ float power_of(int e) {
   return __builtin_bit_cast(float, uint32_t(e + 127) << 23);
 }
 
+constexpr float kHalfSecond = 1.0f / 64;  // what m is a multiple of
+// Values, scaled, below kHalfSmall are counted.  Sums are formed again below kHalfLeast times the share of
+// such values, one by one up to kHalfList of a tile.
+constexpr float kHalfSmall = 1.0f / 2048, kHalfLeast = 256.0f;
+constexpr uint32_t kHalfInfinite = 1u << 31;  // the mark of a row that is not finite
+constexpr int kHalfList = 32;
+// What a tile has to form again, in LDS: whether any sum may be, whether any is, how many are, where
+// (row << 16 | column in the tile), and the values, scaled as the others are.
+struct HalfDoubt {
+  int any, again, count;
+  uint32_t at[kHalfList];
+  float value[kHalfList];
+  float shares[8];
+};
+
 template <int WM_, int WN_, int TM_, int TN_, int MINB_>
 struct HalfCfg {
   static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, MINB = MINB_;
@@ -84,20 +109,24 @@ struct HalfCfg {
   static constexpr int A_PANELS = BM / 64, PANELS = (BM + BN) / 64;
   static constexpr int STAGE = PANELS * kHalfStep;
   static constexpr int LOADS = PANELS * 8 / NW;  // of a wave, a step
-  static constexpr int SMEM = 2 * STAGE + 16;    // the stages and the flag of sums that are not finite
+  // The stages, what is formed again, and what rows' and columns' sums may not be below.
+  static constexpr int SMEM = 2 * STAGE + int(sizeof(HalfDoubt)) + (BM + BN) * 4;
   static_assert((TM == 1 || TM % 2 == 0) && TN % 2 == 0, "a wave's blocks are whole panels, or half of one");
   static_assert(2 * STAGE >= NW * 16 * (32 * TN + 4) * 4, "the epilogue's wave tiles fit");
+  static_assert(BM + BN <= THREADS, "a lane each loads their limits");
   static_assert(BM % 64 == 0 && BN % 64 == 0 && LOADS * NW == PANELS * 8, "whole panels, split evenly");
 };
 
 // A product op(A) [m, k] op(B) [k, n] of panels.  `a_top` and `b_top`: the bits of the
-// largest finite magnitude of each row of op(A) and column of op(B), rounded up to 256 of them.
+// largest finite magnitude of each row of op(A) and column of op(B), rounded up to 256 of them;
+// `a_marks` and `b_marks`: their marks (HalfPanels).
 struct HalfArgs {
   const char *a, *b;
   int64_t a_stride, b_stride;  // bytes from panel to panel
-  int m, n;
+  int m, n, k;
   int steps;  // 32-wide k steps
   const uint32_t *a_top, *b_top;
+  const uint32_t *a_marks, *b_marks;
   int tiles_m, tiles_n;
   int splits, steps_per_split;
 };
@@ -123,26 +152,147 @@ __device__ __forceinline__ HalfItem half_item(const HalfArgs& g, int id) {
   return {group * kGroup + in_group % gsize, in_group / gsize, split};
 }
 
-// The parts that are finite, zeros in place of the others.
-__device__ __forceinline__ hf8 finite_parts(hf8 x) {
-  const hw8 b = __builtin_bit_cast(hw8, x);
-  hw8 r;
+// An operand as the products' slow path reads it: rows of its source along K (RowsOf), or columns
+// (ColsOf).  A source is as half_panels.hpp's passes take it, and has besides
+//   float value(int64_t row, int col)   one value
+// stage() puts 64 of K from k0 on, of N rows of the operand from row0 on, into t[k][N], zeros
+// past the matrix; row0 and k0 are multiples of 64.
+template <class S>
+struct RowsOf {
+  static constexpr bool ROWS = true;
+  S s;
+  __device__ __forceinline__ int64_t extent() const { return s.cols; }
+  __device__ __forceinline__ float value(int64_t row, int64_t k) const { return s.value(row, int(k)); }
+  template <int N, int NT>
+  __device__ __forceinline__ void stage(float* t, int64_t row0, int64_t k0) const {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < N * 8; i += NT) {
+      const int r = i % N, unit = int(k0 / 8) + i / N;
+      hv4 v[2] = {hv4(0.0f), hv4(0.0f)};
+      if (row0 + r < s.rows && unit * 8 < s.cols) s.load(row0 + r, unit, v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = (b[i] & 0x7c00) == 0x7c00 ? uint16_t(0) : b[i];
-  return __builtin_bit_cast(hf8, r);
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[(s.column(unit, h) + e - int(k0)) * N + r] = v[h][e];
+    }
+  }
+};
+template <class S>
+struct ColsOf {
+  static constexpr bool ROWS = false;
+  S s;
+  __device__ __forceinline__ int64_t extent() const { return s.rows; }
+  __device__ __forceinline__ float value(int64_t row, int64_t k) const { return s.value(k, int(row)); }
+  template <int N, int NT>
+  __device__ __forceinline__ void stage(float* t, int64_t row0, int64_t k0) const {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < 64 * (N / 8); i += NT) {
+      const int k = i / (N / 8), unit = int(row0 / 8) + i % (N / 8);
+      hv4 v[2] = {hv4(0.0f), hv4(0.0f)};
+      if (k0 + k < s.rows && unit * 8 < s.cols) s.load(k0 + k, unit, v);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<hv4*>(t + k * N + s.column(unit, h) - int(row0)) = v[h];
+    }
+  }
+};
+
+// Sum (row, col) in fp32 by the whole workgroup.
+template <int NT, class A, class B>
+__device__ __forceinline__ float whole_sum(const A& a, const B& b, int64_t row, int64_t col, float* shares) {
+  float sum = 0.0f;
+  if constexpr (A::ROWS && B::ROWS) {
+#pragma unroll 2
+    for (int unit = threadIdx.x; unit * 8 < a.s.cols; unit += NT) {
+      hv4 x[2], y[2];
+      a.s.load(row, unit, x);
+      b.s.load(col, unit, y);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(x[h][e], y[h][e], sum);
+    }
+  } else {
+#pragma unroll 4
+    for (int64_t k = threadIdx.x; k < a.extent(); k += NT) sum = __builtin_fmaf(a.value(row, k), b.value(col, k), sum);
+  }
+  for (int off = 1; off < 64; off *= 2) sum += __shfl_xor(sum, off);
+  if ((threadIdx.x & 63) == 0) shares[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  sum = shares[0];
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) sum += shares[w];
+  __syncthreads();
+  return sum;
+}
+
+// The sums of the waves' blocks (i, j) of C's tile at (row0, col0) in fp32, by way of (BM + BN) 256
+// bytes of LDS.
+template <class C, class A, class B>
+__device__ __forceinline__ void whole_blocks(const A& a, const B& b, int64_t row0, int64_t col0, int i, char* smem,
+                                             hv16 (&acc)[C::TN]) {
+  float *ta = reinterpret_cast<float*>(smem), *tb = ta + 64 * C::BM;
+  const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float* ra = ta + lh * C::BM + (wave % (C::WM * C::WN) / C::WN * C::TM + i) * 32 + li;
+  const float* rb = tb + lh * C::BN + wave % C::WN * C::TN * 32 + li;
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j) acc[j] = hv16(0.0f);
+#pragma unroll 1
+  for (int64_t k0 = 0; k0 < a.extent(); k0 += 64) {
+    a.template stage<C::BM, C::THREADS>(ta, row0, k0);
+    b.template stage<C::BN, C::THREADS>(tb, col0, k0);
+    __syncthreads();
+#pragma unroll 8
+    for (int k = 0; k < 64; k += 2)
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) acc[j] = mfma_whole(ra[k * C::BM], rb[k * C::BN + 32 * j], acc[j]);
+    __syncthreads();
+  }
+}
+
+// A row's share of what a scaled sum may not be below, from its largest magnitude and its word of
+// marks.  Rows of zeros, and those past the matrix, make sums of zero; all of a row that is not
+// finite are formed again.
+__device__ __forceinline__ float half_limit(uint32_t top, uint32_t marks, float per_k) {
+  if (marks & kHalfInfinite) return 1e38f;
+  return top ? float(marks) * per_k : -1e37f;
+}
+
+// Whether a sum is to be formed again, by its row's and its column's limit.
+__device__ __forceinline__ bool half_doubtful(float sum, float row, float col) {
+  const float above = fabsf(sum) - col;
+  return !(above >= row && above < __builtin_huge_valf());
+}
+
+// Lists what a lane found: bit b of `found` is at + b / 4 four + b % 4 one, in the list's terms.
+__device__ __forceinline__ void note_doubts(HalfDoubt* d, uint32_t found, uint32_t at, uint32_t four, uint32_t one) {
+  if (!found) return;
+  int i = atomicAdd(&d->count, __popc(found));
+  for (; found && i < kHalfList; ++i, found &= found - 1) {
+    const uint32_t b = __ffs(int(found)) - 1;
+    d->at[i] = at + b / 4 * four + b % 4 * one;
+  }
+}
+
+template <class C>
+__device__ __forceinline__ HalfDoubt* half_doubt(char* smem) {
+  return reinterpret_cast<HalfDoubt*>(smem + 2 * C::STAGE);
+}
+// The tile's limits: its rows', then its columns'.
+template <class C>
+__device__ __forceinline__ float* half_limits(char* smem) {
+  return reinterpret_cast<float*>(smem + 2 * C::STAGE + sizeof(HalfDoubt));
 }
 
 // The tile's sums, scaled by the powers of two of rows and columns, into acc: block (i, j)
-// of the wave, register r: row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32.
-template <class C>
-__device__ __forceinline__ void half_tile(const HalfArgs& g, const HalfItem& at, char* smem,
+// of the wave, register r: row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32.  With LIMITS
+// also what its rows' and columns' sums may not be below, into LDS.
+template <class C, bool LIMITS>
+__device__ __forceinline__ void half_sums(const HalfArgs& g, const HalfItem& at, char* smem,
                                           hv16 (&acc)[C::TM][C::TN]) {
   constexpr int TM = C::TM, TN = C::TN;
   const int first = at.split * g.steps_per_split;
   const int steps = min(g.steps - first, g.steps_per_split);
-  int* flag = reinterpret_cast<int*>(smem + 2 * C::STAGE);
-  if (threadIdx.x == 0) *flag = 0;  // set after the K loop's barriers
-
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
@@ -177,9 +327,9 @@ __device__ __forceinline__ void half_tile(const HalfArgs& g, const HalfItem& at,
 #pragma unroll
     for (int i = 0; i < TM; ++i) f.ah[i] = *reinterpret_cast<const hf8*>(a + i / 2 * kHalfStep + i % 2 * 512);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) f.bm[j] = *reinterpret_cast<const hf8*>(b + 1024 + j / 2 * kHalfStep + j % 2 * 512);
-#pragma unroll
     for (int j = 0; j < TN; ++j) f.bh[j] = *reinterpret_cast<const hf8*>(b + j / 2 * kHalfStep + j % 2 * 512);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) f.bm[j] = *reinterpret_cast<const hf8*>(b + 1024 + j / 2 * kHalfStep + j % 2 * 512);
 #pragma unroll
     for (int i = 0; i < TM; ++i) f.am[i] = *reinterpret_cast<const hf8*>(a + 1024 + i / 2 * kHalfStep + i % 2 * 512);
   };
@@ -189,10 +339,14 @@ __device__ __forceinline__ void half_tile(const HalfArgs& g, const HalfItem& at,
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = mfma_f16(x[i], y[j], acc[i][j]);
   };
-  const auto products = [&](const Fragments& f) {
+  const auto products = [&](Fragments& f) {
+    product(f.ah, f.bh);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) f.ah[i] = f.ah[i] * _Float16(kHalfSecond);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) f.bh[j] = f.bh[j] * _Float16(kHalfSecond);
     product(f.ah, f.bm);
     product(f.am, f.bh);
-    product(f.ah, f.bh);
   };
   // A half's products with the next half's reads among them: 0x8 MFMA, 0x100 LDS read.
   const auto order = [&]() {
@@ -209,8 +363,22 @@ __device__ __forceinline__ void half_tile(const HalfArgs& g, const HalfItem& at,
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = hv16(0.0f);
+  const int mine = threadIdx.x;
+  const bool of_a = mine < C::BM, limited = LIMITS && mine < C::BM + C::BN;
+  uint32_t top = 0, marks = 0;
+  if (limited) {
+    const int64_t row = of_a ? int64_t(at.tile_m) * C::BM + mine : int64_t(at.tile_n) * C::BN + mine - C::BM;
+    top = (of_a ? g.a_top : g.b_top)[row];
+    marks = (of_a ? g.a_marks : g.b_marks)[row];
+  }
   issue(0);
   if (steps > 1) issue(1);
+  if (limited) {
+    const float limit = half_limit(top, marks, kHalfLeast / float(g.k));
+    half_limits<C>(smem)[mine] = limit;
+    if (limit > 0.0f) half_doubt<C>(smem)->any = 1;
+    if (marks & kHalfInfinite) half_doubt<C>(smem)->again = 1;
+  }
   panels_settled();
   Fragments f0, f1;
   read(f0, smem, 0);
@@ -232,88 +400,158 @@ __device__ __forceinline__ void half_tile(const HalfArgs& g, const HalfItem& at,
     step(std::integral_constant<int, 1>{}, t++);
   }
   if (t < steps) step(std::integral_constant<int, 0>{}, t);
-
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        top = max(top, __builtin_bit_cast(uint32_t, float(acc[i][j][r])) & 0x7fffffffu);
-  if (top >= 0x7f800000u) *flag = 1;
-  __syncthreads();
-  if (!*flag) return;
-
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = hv16(0.0f);
-  ahead = lane * 16;
-#pragma unroll 1
-  for (int u = 0; u < steps; ++u) {
-    issue(0);
-    panels_settled();
-#pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-      read(f0, smem, half);
-      product(f0.ah, f0.bh);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) f0.ah[i] = finite_parts(f0.ah[i]);
-#pragma unroll
-      for (int j = 0; j < TN; ++j) f0.bh[j] = finite_parts(f0.bh[j]);
-      product(f0.ah, f0.bm);
-      product(f0.am, f0.bh);
-    }
-    panels_settled();
-  }
 }
 
-// Calls f(row, column, values) for every four consecutive columns of the wave's rows: values
-// [j] are block column j's at columns column + 32 j of the tile (so a lane has the same place
-// of every block), unscaled.  Through a wave-private LDS tile of 16 rows (LDS requests
-// of one wave complete in order).
-template <class C, class F>
-__device__ __forceinline__ void half_epilogue(const HalfArgs& g, const HalfItem& at, char* smem, hv16 (&acc)[C::TM][C::TN], F&& f) {
+// The same, and how many of them are too small or not finite: up to kHalfList are formed again and
+// listed.
+template <class C, class A, class B>
+__device__ __forceinline__ int half_tile(const HalfArgs& g, const HalfItem& at, char* smem, hv16 (&acc)[C::TM][C::TN],
+                                         const A& a, const B& b) {
+  constexpr int TM = C::TM, TN = C::TN;
+  HalfDoubt* doubt = half_doubt<C>(smem);
+  if (threadIdx.x == 0) doubt->any = doubt->again = doubt->count = 0;
+  __syncthreads();
+  half_sums<C, true>(g, at, smem, acc);
+  if (!doubt->any) {  // as the K loop's first barrier left it
+    __syncthreads();  // the stages have been read
+    return 0;
+  }
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row_at = wave / C::WN * TM * 32 + 4 * (lane >> 5), col_at = wave % C::WN * TN * 32 + (lane & 31);
+  const float *row_limits = half_limits<C>(smem) + row_at, *col_limits = half_limits<C>(smem) + C::BM + col_at;
+  float col_limit[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) col_limit[j] = col_limits[32 * j];
+  bool again = false;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const hv4 limits = *reinterpret_cast<const hv4*>(row_limits + 32 * i + 8 * q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float above = fabsf(acc[i][0][4 * q + e]) - col_limit[0];
+#pragma unroll
+        for (int j = 1; j < TN; ++j) above = fminf(above, fabsf(acc[i][j][4 * q + e]) - col_limit[j]);
+        again |= above < limits[e];
+      }
+      __builtin_amdgcn_sched_barrier(0);  // the sums leave no registers for more limits at a time
+    }
+  if (again) doubt->again = 1;
+  __syncthreads();
+  if (!doubt->again) return 0;
+
+  // Seldom reached, so what matters of this code is that it stays out of the way.
+  const int64_t row0 = int64_t(at.tile_m) * C::BM, col0 = int64_t(at.tile_n) * C::BN;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int row = row_at + 32 * i, col = col_at + 32 * j;
+      uint32_t found = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const hv4 limits = *reinterpret_cast<const hv4*>(row_limits + 32 * i + 8 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (half_doubtful(acc[i][j][4 * q + e], limits[e], col_limits[32 * j])) found |= 1u << (4 * q + e);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (col0 + col >= g.n) found = 0;
+#pragma unroll 1
+      for (uint32_t f = found; f; f &= f - 1) {
+        const int bit = __ffs(int(f)) - 1;
+        if (row0 + row + bit / 4 * 8 + bit % 4 >= g.m) found &= ~(1u << bit);
+      }
+      note_doubts(doubt, found, uint32_t(row) << 16 | uint32_t(col), 8 << 16, 1 << 16);
+    }
+  __syncthreads();
+  const int count = doubt->count;
+  if (count > kHalfList) return count;
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    const uint32_t where = doubt->at[i];
+    const int64_t row = row0 + (where >> 16), col = col0 + (where & 0xffff);
+    const float sum = whole_sum<C::THREADS>(a, b, row, col, doubt->shares);
+    if (threadIdx.x == 0) doubt->value[i] = ldexpf(sum, half_exponent(g.a_top[row]) + half_exponent(g.b_top[col]));
+  }
+  __syncthreads();
+  return count;
+}
+
+// Calls f(row, column, values) for every four consecutive columns of rows of the wave's blocks
+// (i, j): values [j] are block column j's at columns column + 32 j of the tile (so a lane
+// has the same place of every block).  Of scaled sums the powers of two are taken out and the
+// first `patches` of the list put in their places.  Through a wave-private LDS tile of 16
+// rows (LDS requests of one wave complete in order).
+template <class C, bool SCALED, class F>
+__device__ __forceinline__ void half_out(const HalfArgs& g, const HalfItem& at, char* smem, const hv16 (&acc)[C::TN], int i,
+                                         const hi4 (&eb)[C::TN], int patches, F&& f) {
   constexpr int TM = C::TM, TN = C::TN, PITCH = 32 * TN + 4;
-  static_assert(2 * C::STAGE >= C::NW * 16 * PITCH * 4, "the wave tiles fit");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
-  const int li = lane & 31, lh = lane >> 5;
+  const int li = lane & 31, lh = lane >> 5, c4 = 4 * (lane & 7);
   float* w = reinterpret_cast<float*>(smem) + wave * (16 * PITCH);
-  const int c4 = 4 * (lane & 7);
-  hi4 eb[TN];
+  const HalfDoubt* doubt = half_doubt<C>(smem);
 #pragma unroll
-  for (int j = 0; j < TN; ++j)
+  for (int half = 0; half < 2; ++half) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) eb[j][e] = half_exponent(g.b_top[at.tile_n * C::BN + wn * TN * 32 + j * 32 + c4 + e]);
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+      for (int r = 0; r < 8; ++r) w[((r / 4) * 8 + lh * 4 + r % 4) * PITCH + j * 32 + li] = acc[j][8 * half + r];
+    if (SCALED && lane < patches) {
+      const int r = int(doubt->at[lane] >> 16) - (wm * TM + i) * 32 - half * 16, c = int(doubt->at[lane] & 0xffff) - wn * TN * 32;
+      if (r >= 0 && r < 16 && c >= 0 && c < TN * 32) w[r * PITCH + c] = doubt->value[lane];
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1  // the code that a tile passes through once has to leave the K loop's in the instruction cache
+    for (int q = 0; q < 2; ++q) {
+      const int rr = q * 8 + (lane >> 3);
+      const int row = at.tile_m * C::BM + (wm * TM + i) * 32 + half * 16 + rr;
+      const int ea = SCALED ? half_exponent(g.a_top[row]) : 0;
+      hv4 v[TN];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          w[((r / 4) * 8 + lh * 4 + r % 4) * PITCH + j * 32 + li] = acc[i][j][8 * half + r];
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int rr = q * 8 + (lane >> 3);
-        const int row = at.tile_m * C::BM + (wm * TM + i) * 32 + half * 16 + rr;
-        const int ea = half_exponent(g.a_top[row]);
-        hv4 v[TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          v[j] = *reinterpret_cast<const hv4*>(w + rr * PITCH + j * 32 + c4);
+      for (int j = 0; j < TN; ++j) {
+        v[j] = *reinterpret_cast<const hv4*>(w + rr * PITCH + j * 32 + c4);
+        if constexpr (SCALED)
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[j][e] = ldexpf(v[j][e], -(ea + eb[j][e]));
-        }
-        f(row, c4, v);
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      f(row, c4, v);
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+// A tile's product, f called with its sums as half_out does.
+template <class C, class A, class B, class F>
+__device__ __forceinline__ void half_product(const HalfArgs& g, const HalfItem& at, char* smem, const A& a, const B& b, F&& f) {
+  static_assert(2 * C::STAGE >= C::NW * 16 * (32 * C::TN + 4) * 4, "the wave tiles fit");
+  hi4 eb[C::TN];
+  {
+    hv16 acc[C::TM][C::TN];
+    const int again = half_tile<C>(g, at, smem, acc, a, b);
+    if (again <= kHalfList) {
+      const int col = at.tile_n * C::BN + (threadIdx.x >> 6) % C::WN * C::TN * 32 + 4 * (threadIdx.x & 7);
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) eb[j][e] = half_exponent(g.b_top[col + j * 32 + e]);
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) half_out<C, true>(g, at, smem, acc[i], i, eb, again, f);
+      return;
+    }
+  }
+#pragma unroll 1
+  for (int i = 0; i < C::TM; ++i) {
+    hv16 acc[C::TN];
+    whole_blocks<C>(a, b, int64_t(at.tile_m) * C::BM, int64_t(at.tile_n) * C::BN, i, smem, acc);
+    half_out<C, false>(g, at, smem, acc, i, eb, 0, f);
+    __syncthreads();
+  }
 }
 
 // Four values of a row from `col` on, as far as the row's n go.
@@ -355,8 +593,8 @@ int with_half_cfg(int cfg, F&& f) {
 inline HalfArgs half_args(const HalfPanels& a, const HalfPanels& b, int m, int n, int k, int cfg, int splits) {
   const HalfTile& t = kHalfTiles[cfg];
   const int steps = (k + kHalfK - 1) / kHalfK, each = (steps + splits - 1) / splits;
-  return {a.panels, b.panels, a.stride, b.stride, m, n, steps, a.tops, b.tops, (m + t.bm - 1) / t.bm,
-          (n + t.bn - 1) / t.bn, (steps + each - 1) / each, each};
+  return {a.panels, b.panels, a.stride, b.stride, m, n, k, steps, a.tops, b.tops, a.marks, b.marks,
+          (m + t.bm - 1) / t.bm, (n + t.bn - 1) / t.bn, (steps + each - 1) / each, each};
 }
 inline uint32_t half_items(const HalfArgs& g) { return uint32_t(int64_t(g.tiles_m) * g.tiles_n * g.splits); }
 

@@ -7,6 +7,7 @@
 //   void load(int64_t row, int unit, hv4 (&v)[2])   eight columns, zeros past the last
 //   int column(int unit, int h)                     the first column of v[h]; eight units are 64 columns in some order
 //   int place(int col)                              where that column's sum goes, or -1
+//   float value(int64_t row, int col)               one value, for sums that are formed again
 //
 // Bound by memory: a pass reads 4 bytes a value and the second writes 4 for each set of panels.
 // w of 1024 x 32768 and x of 4096 x 1024 take 42 us and, with both sets of panels, 76 (151 MB at
@@ -53,6 +54,9 @@ struct MatrixSource {
   }
   __device__ __forceinline__ int column(int unit, int h) const { return 8 * unit + 4 * h; }
   __device__ __forceinline__ int place(int col) const { return col; }
+  __device__ __forceinline__ float value(int64_t row, int col) const {
+    return targets && targets[row] < 0 ? 0.0f : x[row * ld + col];
+  }
 };
 
 // ------------------------------------------------------------ largest magnitudes
@@ -174,23 +178,35 @@ TopsJob<S> tops_job(Runtime* rt, const S& s, uint32_t* row_top, uint32_t* col_to
 
 // ------------------------------------------------------------------------ panels
 
-// Two values times s into the two parts, packed; an infinity has no second part.
+// Two values times s into the two parts, packed.  Of what is not finite the second part is NaN
+// at worst: such sums are formed again.
 __device__ __forceinline__ void half_pair(float x, float y, float s, uint32_t& h, uint32_t& m) {
   const hf2 a = __builtin_convertvector(hv2{x * s, y * s}, hf2);
   hf2 b;
-  b.x = _Float16(__builtin_fmaf(x, s, -float(a.x)));
-  b.y = _Float16(__builtin_fmaf(y, s, -float(a.y)));
+  b.x = _Float16(__builtin_fmaf(x, s, -float(a.x)) * (1 / kHalfSecond));
+  b.y = _Float16(__builtin_fmaf(y, s, -float(a.y)) * (1 / kHalfSecond));
   h = __builtin_bit_cast(uint32_t, a);
   m = __builtin_bit_cast(uint32_t, b);
-  if ((h & 0x7fff) == 0x7c00) m &= 0xffff0000u;
-  if ((h & 0x7fff0000) == 0x7c000000) m &= 0xffffu;
 }
-__device__ __forceinline__ void put_octet(char* to, const float (&v)[8], float s) {
+__device__ __forceinline__ void put_octet(char* to, const float (&v)[8], float s, uint32_t& marks) {
   uint32_t h[4], m[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) half_pair(v[2 * j], v[2 * j + 1], s, h[j], m[j]);
   *reinterpret_cast<hu4*>(to) = hu4{h[0], h[1], h[2], h[3]};
   *reinterpret_cast<hu4*>(to + 1024) = hu4{m[0], m[1], m[2], m[3]};
+  bool infinite = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = fabsf(v[j] * s);
+    infinite |= !(x < __builtin_huge_valf());
+    marks += x < kHalfSmall && v[j] != 0.0f;
+  }
+  if (infinite) marks |= kHalfInfinite;
+}
+// Counts add, the mark of a row that is not finite stays.
+__device__ __forceinline__ void put_marks(uint32_t* to, uint32_t marks) {
+  if (marks & ~kHalfInfinite) atomicAdd(to, marks & ~kHalfInfinite);
+  if (marks & kHalfInfinite) atomicOr(to, kHalfInfinite);
 }
 
 // Panels of the matrix (`r`: its rows are the panels', its columns K) and of its transpose
@@ -200,13 +216,15 @@ struct PackJob {
   S s;
   HalfPanels r, c;  // panels may be null
   int64_t tiles_c, blocks;
-  static constexpr int PITCH = 68, SMEM = 64 * PITCH * 4;
+  static constexpr int PITCH = 68, SMEM = (64 * PITCH + 128) * 4;
   __device__ __forceinline__ void run(int64_t block, char* smem) const {
     float* t = reinterpret_cast<float*>(smem);
+    uint32_t* found = reinterpret_cast<uint32_t*>(t + 64 * PITCH);  // marks of the tile's rows, then of its columns
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t tr = block / tiles_c, tc = block - tr * tiles_c;
     const int unit = int(tc) * 8 + threadIdx.x % 8;
+    if (threadIdx.x < 128) found[threadIdx.x] = 0;
     hv4 v[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -223,24 +241,31 @@ struct PackJob {
     float o[8];
     if (r.panels) {
       const float power = power_of(half_exponent(r.tops[tr * 64 + lane]));
+      uint32_t marks = 0;
 #pragma unroll
       for (int oct = wave; oct < 8; oct += 4) {
         if (tc * 64 + oct * 8 >= (int64_t(s.cols) + 31) / 32 * 32) break;
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = t[lane * PITCH + oct * 8 + j];
-        put_octet(r.panels + tr * r.stride + (tc * 8 + oct) * 2048 + lane * 16, o, power);
+        put_octet(r.panels + tr * r.stride + (tc * 8 + oct) * 2048 + lane * 16, o, power, marks);
       }
+      put_marks(found + lane, marks);
     }
     if (c.panels) {
       const float power = power_of(half_exponent(c.tops[tc * 64 + lane]));
+      uint32_t marks = 0;
 #pragma unroll
       for (int oct = wave; oct < 8; oct += 4) {
         if (tr * 64 + oct * 8 >= (s.rows + 31) / 32 * 32) break;
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = t[(oct * 8 + j) * PITCH + lane];
-        put_octet(c.panels + tc * c.stride + (tr * 8 + oct) * 2048 + lane * 16, o, power);
+        put_octet(c.panels + tc * c.stride + (tr * 8 + oct) * 2048 + lane * 16, o, power, marks);
       }
+      put_marks(found + 64 + lane, marks);
     }
+    __syncthreads();
+    if (r.panels && threadIdx.x < 64) put_marks(r.marks + tr * 64 + lane, found[lane]);
+    if (c.panels && threadIdx.x >= 64 && threadIdx.x < 128) put_marks(c.marks + tc * 64 + lane, found[64 + lane]);
   }
 };
 // Whole groups of four panels, the rows past the matrix zeros.

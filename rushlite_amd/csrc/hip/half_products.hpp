@@ -1,5 +1,5 @@
-// Products on the fp16 matrix cores shared by the operators that use them
-// (half_products.hip; the tiles are gemm_half.hpp's, the operands half_panels.hpp's).
+// What the operators on the fp16 matrix cores share on the host (the tiles are gemm_half.hpp's,
+// the operands half_panels.hpp's, the gradient products half_backward.hpp's).
 #pragma once
 
 #include <cstddef>
@@ -10,12 +10,12 @@
 
 namespace lmp_hip {
 
-// One operand: its panels of 64 rows, `stride` bytes apart, and the bits of its rows'
-// largest finite magnitudes.
+// One operand: its panels of 64 rows, `stride` bytes apart, the bits of its rows' largest finite
+// magnitudes, and their marks: how many small values a row has, and whether one is not finite.
 struct HalfPanels {
   char* panels;
   int64_t stride;
-  uint32_t* tops;
+  uint32_t *tops, *marks;
 };
 
 // Whether a layer's products x [rows, in] w [in, width] and their gradients may run there: each
@@ -41,7 +41,7 @@ struct HalfRoom {
     return at;
   }
 };
-// Words of `n` rows' largest magnitudes (tiles read whole groups of 256), of an operand's panels
+// Words of a number for each of `n` rows (tiles read whole groups of 256), of an operand's panels
 // [rows, k], and bytes from panel to panel.
 inline size_t half_tops_words(size_t n) { return (n + 255) / 256 * 256; }
 inline size_t half_stride(size_t k) { return (k + kHalfK - 1) / kHalfK * size_t(kHalfStep); }
@@ -51,22 +51,5 @@ inline size_t half_panel_words(size_t rows, size_t k) { return (rows + 255) / 25
 int clear_words(Runtime* rt, uint32_t* p, size_t n);
 // Zeros in `cols` columns of `rows` rows (the gradients of no rows).
 int clear_f32(Runtime* rt, float* p, size_t rows, size_t cols, size_t ld);
-
-// dx = d w^T and dw (+)= x^T d of a layer with x [rows, in] and w [in, width], each null
-// where it is not wanted: d_rows [rows, width], w_rows [in, width], x_cols [in, rows], d_cols
-// [width, rows].
-struct HalfBackward {
-  size_t rows, in, width;
-  HalfPanels d_rows, d_cols, x_cols, w_rows;
-  float* dx;
-  size_t lddx;
-  float* dw;
-  size_t lddw;
-  bool dw_accumulate;
-  // Not 0: the layer is gated, and its columns are 32 of the one half and 32 of the other by
-  // turns, each half `hidden` columns long in dw.
-  size_t hidden;
-};
-int half_backward(Runtime* rt, const HalfBackward& b);
 
 }  // namespace lmp_hip

@@ -1,0 +1,148 @@
+"""Products of operands that spread widely along K, in the sizes whose products run on split operands: gated linear layers and
+the vocabulary loss against 64-bit forms.
+
+The bounds are four times those of tests/_decoder.py, which count a rounding a term: a sum of k products errs by 4 k + 64
+units of its magnitudes, whatever else its operands hold."""
+import numpy as np
+import pytest
+
+import _decoder as D
+from test_gpu_decoder import close, gated, loss
+
+pytestmark = pytest.mark.gpu
+
+
+def gated_operands(rng, rows, k, n):
+    return (rng.standard_normal((rows, k)).astype(np.float32), (rng.standard_normal((k, 2 * n)) * k ** -0.5).astype(np.float32),
+            rng.standard_normal((rows, n)).astype(np.float32))
+
+
+def check_gated(hip, gate, x, w, g, what=()):
+    want, bound = D.gated(gate, x, w, None, g), D.gated_bounds(gate, x, w, None, g)
+    for a, v, e, part in zip(gated(hip, gate, x, w, None, g), want, bound, ("h", "dx", "dw", "db")):
+        # a product below float32's normal range, 2^-126, is off by up to itself
+        close(a, v, 4 * e + 2.0 ** -126, (*what, part))
+
+
+def check_loss(hip, x, w, b, targets, weights=None, what=()):
+    want, bound = D.cross_entropy(x, w, b, targets, weights), D.cross_entropy_bounds(x, w, b, targets, weights)
+    for a, v, e, part in zip(loss(hip, x, w, b, targets, weights), want, bound, ("loss", "dx", "dw", "db")):
+        close(a, v, 4 * e, (*what, part))
+    close(loss(hip, x, w, b, targets, grads=False), want[0], 4 * bound[0], (*what, "loss alone"))
+
+
+# Rows, inputs and outputs that take the tiles of 64 x 128 to 256 x 256, in one piece of K and in several.
+GATED = [(1500, 1100, 1201), (1031, 2050, 1001), (5003, 600, 1201)]
+LOSS = [(2100, 900, 2003), (5003, 600, 1009)]
+
+
+@pytest.mark.parametrize("rows,k,n", GATED)
+def test_gated_an_input_column_far_above_the_others(hip, rows, k, n):
+    """Its weights are zeros, or small enough to make up for it."""
+    rng = np.random.default_rng(1)
+    x, w, g = gated_operands(rng, rows, k, n)
+    for c in (1e5, 1e7, 1e9, 1e11, 1e13, 1e25):
+        for weight in (0.0, 1 / c):
+            x[:, 5], w[5] = c, weight
+            check_gated(hip, "sigmoid", x, w, g, (c, weight))
+
+
+@pytest.mark.parametrize("rows,k,n", GATED)
+def test_gated_rows_and_weights_that_meet_zeros(hip, rows, k, n):
+    """A row of huge inputs without a gradient, and a huge weight of an output without one."""
+    rng = np.random.default_rng(2)
+    for c in (1e8, 1e10, 1e12):
+        x, w, g = gated_operands(rng, rows, k, n)
+        x[5] *= np.float32(c)
+        g[5] = 0
+        check_gated(hip, "sigmoid", x, w, g, (c, "row"))
+        x, w, g = gated_operands(rng, rows, k, n)
+        w[3, 7], w[4, n + 9] = c, -c
+        x[:, 3:5] *= np.float32(1 / c)
+        g[:, [7, 9]] = 0
+        check_gated(hip, "sigmoid", x, w, g, (c, "weight"))
+
+
+def test_gated_few_sums_far_below_their_operands(hip):
+    """A column with one weight, met by a few inputs of almost nothing; rows and columns of zeros beside them."""
+    rng = np.random.default_rng(3)
+    for rows, k, n in GATED:
+        x, w, g = gated_operands(rng, rows, k, n)
+        for col in (17, n - 1, n + 17, 2 * n - 1):
+            w[:, col] = 0
+            w[70, col] = 0.7
+        few = [0, 63, 64, 200, rows - 1]
+        x[few, 70] = [1e-9, -3e-12, 1e-20, 2e-30, 5e-7]
+        x[300:340] = 0
+        x[:, 90], w[:, 40] = 0, 0
+        check_gated(hip, "silu", x, w, g)
+        # the same of both gradients: an output with a gradient in one row, whose inputs are almost nothing, and an input
+        # with one weight, for an output with gradients of almost nothing
+        x, w, g = gated_operands(rng, rows, k, n)
+        g[:, 7], g[9, 7] = 0, 1
+        x[9, [3, 40, k - 1]] = [1e-12, -1e-20, 1e-9]
+        w[5], w[5, 20] = 0, 0.3
+        g[[4, 70, rows - 1], 20] = [1e-11, -1e-18, 1e-25]
+        check_gated(hip, "sigmoid", x, w, g)
+
+
+def test_gated_infinities_and_weights_of_almost_nothing(hip):
+    """An infinity times a value far below the largest it is held beside is an infinity, as in float32."""
+    rng = np.random.default_rng(4)
+    for rows, k, n in GATED:
+        x, w, g = gated_operands(rng, rows, k, n)
+        x[2, 3], w[3] = np.inf, 1e-30
+        h = gated(hip, "sigmoid", x, w, None, g, keep=False)
+        assert (h[2] == np.inf).all() and np.isfinite(np.delete(h, 2, 0)).all()
+        x[2, 3] = 0
+        clean = gated(hip, "sigmoid", x, w, None, g, keep=False)
+        bound = D.gated_bounds("sigmoid", x, w, None, g)[0]
+        close(np.delete(h, 2, 0), np.delete(clean, 2, 0).astype(np.float64), np.delete(8 * bound, 2, 0))
+        # of the weights: one column of the second half
+        x[:, 8] = np.abs(x[:, 8]) + 1e-30
+        x[20:200, 8] = 1e-25
+        w[8, n + 13] = np.inf
+        h = gated(hip, "sigmoid", x, w, None, g, keep=False)
+        assert (h[:, 13] == np.inf).all() and np.isfinite(np.delete(h, 13, 1)).all()
+
+
+@pytest.mark.parametrize("rows,k,vocab", LOSS)
+def test_loss_of_inputs_far_above_the_others(hip, rows, k, vocab):
+    rng = np.random.default_rng(5)
+    targets, weights = rng.integers(0, vocab, rows), rng.random(rows).astype(np.float32)
+    w0 = (2 * rng.standard_normal((k, vocab)) * k ** -0.5).astype(np.float32)
+    for c in (1e7, 1e10, 1e13):
+        x, w = rng.standard_normal((rows, k)).astype(np.float32), w0.copy()
+        x[:, 5], w[5] = c, 0
+        check_loss(hip, x, w, None, targets, weights, (c, "column"))
+    for c in (1e8, 1e12):
+        # rows that count for nothing, and a word that a bias bars
+        x, w, b = rng.standard_normal((rows, k)).astype(np.float32), w0.copy(), np.zeros(vocab, np.float32)
+        x[5] *= np.float32(c)
+        weights[5] = 0
+        t = targets.copy()
+        t[t == 11] = 12
+        w[:, 11] *= np.float32(c)
+        b[11] = -np.inf
+        open_ = np.arange(vocab) != 11
+        got = loss(hip, x, w, b, t, weights)
+        args = x, w[:, open_], None, np.cumsum(open_)[t] - 1, weights
+        for a, v, e, part in zip((got[0], got[1], got[2][:, open_]), D.cross_entropy(*args), D.cross_entropy_bounds(*args),
+                                 ("loss", "dx", "dw")):
+            keep = np.arange(len(a)) != 5 if part != "dw" else slice(None)
+            close(a[keep], v[keep], 4 * e[keep], (c, part))
+
+
+@pytest.mark.parametrize("rows,k,vocab", LOSS)
+def test_loss_of_sparse_inputs_and_steep_logits(hip, rows, k, vocab):
+    """Half of the inputs are zeros and the shares of a row span twenty orders of magnitude: where a word's own row has a zero,
+    its gradient is what the small shares add up to."""
+    rng = np.random.default_rng(6)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    x[rng.random((rows, k)) < 0.5] = 0
+    w = (9 * rng.standard_normal((k, vocab)) * k ** -0.5).astype(np.float32)
+    targets, weights = rng.integers(-vocab // 4, vocab, rows), rng.random(rows).astype(np.float32)
+    check_loss(hip, x, w, None, targets, weights)
+    # rows that are sure of their target
+    z = x.astype(np.float64) @ w
+    check_loss(hip, x, w, None, np.where(targets < 0, -1, z.argmax(1)), weights, ("sure",))
