@@ -190,7 +190,7 @@ typedef enum {
  * Here and below a sum of k products errs by (4 k + 64) 2^-24 of their magnitudes' sum at
  * most, and what is not finite comes out as float32's products give it, also where a size's
  * products run on operands in two fp16 parts: sums that those do not hold well enough are
- * formed again in float32, a few at no cost, whole tiles of them five to ten times slower. */
+ * formed again in float32, a few at no cost, whole tiles of them four to eight times slower. */
 int lmp_k_gated_linear_f32(int gate, size_t rows, size_t in, size_t hidden, const float* x,
                            size_t ldx, const float* w, size_t ldw, const float* bias, float* h,
                            size_t ldh, float* pre, size_t ldpre);

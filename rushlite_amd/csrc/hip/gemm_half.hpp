@@ -566,7 +566,6 @@ __device__ __forceinline__ void store_four(float* row, int col, int n, hv4 v) {
 }
 
 using HalfBig = HalfCfg<2, 4, 4, 2, 2>;   // 256 x 256, 8 waves of 128 x 64
-using HalfWide = HalfCfg<4, 2, 2, 2, 2>;  // 256 x 128, 8 waves of 64 x 64
 using HalfMid = HalfCfg<4, 2, 1, 2, 4>;   // 128 x 128, 8 waves of 32 x 64, two a CU
 using HalfFlat = HalfCfg<2, 2, 1, 2, 2>;  // 64 x 128, 4 waves of 32 x 64, three a CU
 
@@ -575,16 +574,15 @@ template <class C>
 constexpr bool half_is(int cfg) {
   return kHalfTiles[cfg].bm == C::BM && kHalfTiles[cfg].bn == C::BN && kHalfTiles[cfg].threads == C::THREADS;
 }
-static_assert(half_is<HalfBig>(0) && half_is<HalfWide>(1) && half_is<HalfMid>(2) && half_is<HalfFlat>(3));
-static_assert(HalfBig::TN == 2 && HalfWide::TN == 2 && HalfMid::TN == 2 && HalfFlat::TN == 2);
+static_assert(half_is<HalfBig>(0) && half_is<HalfMid>(1) && half_is<HalfFlat>(2));
+static_assert(HalfBig::TN == 2 && HalfMid::TN == 2 && HalfFlat::TN == 2);
 
 // Calls f with the configuration's type.
 template <class F>
 int with_half_cfg(int cfg, F&& f) {
   switch (cfg) {
     case 0: return f(HalfBig{});
-    case 1: return f(HalfWide{});
-    case 2: return f(HalfMid{});
+    case 1: return f(HalfMid{});
     default: return f(HalfFlat{});
   }
 }

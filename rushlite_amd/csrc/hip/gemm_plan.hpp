@@ -175,7 +175,6 @@ struct HalfTile {
   float rate;  // TFLOP/s of long products on random operands, where the chip's power holds it back
 };
 constexpr HalfTile kHalfTiles[] = {{256, 256, 512, 1, 1.52f, 1.52f, 11.0f, 400},
-                                   {256, 128, 512, 1, 0.83f, 0.83f, 7.0f, 365},
                                    {128, 128, 512, 2, 0.59f, 0.45f, 5.5f, 370},
                                    {64, 128, 256, 3, 0.53f, 0.27f, 4.0f, 345}};
 
