@@ -31,7 +31,7 @@ def check_loss(hip, x, w, b, targets, weights=None, what=()):
     close(loss(hip, x, w, b, targets, grads=False), want[0], 4 * bound[0], (*what, "loss alone"))
 
 
-# Rows, inputs and outputs that take the tiles of 64 x 128 to 256 x 256, in one piece of K and in several.
+# Rows, inputs and outputs that take several tiles, with K in one piece and in more (tests/native/half_plan_cases.cpp).
 GATED = [(1500, 1100, 1201), (1031, 2050, 1001), (5003, 600, 1201)]
 LOSS = [(2100, 900, 2003), (5003, 600, 1009)]
 
@@ -146,3 +146,31 @@ def test_loss_of_sparse_inputs_and_steep_logits(hip, rows, k, vocab):
     # rows that are sure of their target
     z = x.astype(np.float64) @ w
     check_loss(hip, x, w, None, np.where(targets < 0, -1, z.argmax(1)), weights, ("sure",))
+
+
+@pytest.mark.parametrize("rows,k,n", [(423, 1000, 16001), (2300, 520, 5003), (1005, 2000, 1501), (8200, 1024, 2080)])
+def test_gated_in_every_tile(hip, rows, k, n):
+    """Forward in tiles of 256 x 256 and 128 x 128, the gradients in 256 x 256 with and without K in pieces: operands of one
+    size, and a column, a row and a weight far above the others."""
+    rng = np.random.default_rng(7)
+    x, w, g = gated_operands(rng, rows, k, n)
+    if rows < 8000:
+        check_gated(hip, "silu", x, w, g)
+    x[:, 5], w[5] = 1e9, 0
+    x[rows - 2] *= np.float32(1e10)
+    g[rows - 2] = 0
+    w[3, 7], w[4, n + 9] = 1e10, -1e10
+    x[:, 3:5] *= np.float32(1e-10)
+    g[:, [7, 9]] = 0
+    check_gated(hip, "sigmoid", x, w, g)
+
+
+@pytest.mark.parametrize("rows,k,vocab", [(423, 1000, 32003), (2300, 520, 10007)])
+def test_loss_in_every_tile(hip, rows, k, vocab):
+    rng = np.random.default_rng(8)
+    x, w = rng.standard_normal((rows, k)).astype(np.float32), (2 * rng.standard_normal((k, vocab)) * k ** -0.5).astype(np.float32)
+    targets, weights = rng.integers(-vocab // 4, vocab, rows), rng.random(rows).astype(np.float32)
+    check_loss(hip, x, w, rng.standard_normal(vocab).astype(np.float32), targets, weights)
+    x[:, 5], w[5] = 1e9, 0
+    x[:, 3], w[3, 7] = x[:, 3] * np.float32(1e-10), 1e10
+    check_loss(hip, x, w, None, targets, weights, ("spread",))
