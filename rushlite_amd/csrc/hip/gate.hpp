@@ -43,7 +43,9 @@ __device__ __forceinline__ void gate_at(float a, float& act, float& slope) {
   } else if constexpr (GATE == LMP_GATE_GELU_TANH) {
     logistic(a * kTwoC * (1.0f + kCube * a * a), s, rest);
     act = a * s;
-    slope = s + act * rest * (kTwoC * (1.0f + 3.0f * kCube * a * a));
+    // Past 64 act or rest is 0 (e^-19000): bounded, so that a * a stays finite beside it.
+    const float b = fminf(fabsf(a), 64.0f);
+    slope = s + act * rest * (kTwoC * (1.0f + 3.0f * kCube * b * b));
   } else if constexpr (GATE == LMP_GATE_RELU) {
     act = a < 0.0f ? 0.0f : a;
     slope = a > 0.0f ? 1.0f : 0.0f;
