@@ -105,14 +105,16 @@ void bind_transformer(py::module_& m) {
       "linear_cross_entropy",
       [](const Variable& x, const Variable& w, const Variable* b, const Variable& targets,
          const Variable* weights) {
+        if (weights && weights->requires_grad() && ag::is_grad_enabled())
+          throw py::value_error("linear_cross_entropy: the weights take no gradient");
         return ag::ops::linear_cross_entropy(x, w, b, targets.data(),
                                              weights ? weights->data() : Tensor());
       },
       py::arg("x"), py::arg("w"), py::arg("b").none(true), py::arg("targets"),
       py::arg("weights").none(true) = py::none(),
       "The softmax cross entropies of the rows of x @ w + b against targets (int64; a negative one "
-      "is not counted), summed with weights (finite) or averaged over what counts, of shape [1].  "
-      "The logits are never held whole, and the gradients are formed with the losses.");
+      "is not counted), summed with weights (finite, without a gradient) or averaged over what counts, "
+      "of shape [1].  The logits are never held whole, and the gradients are formed with the losses.");
   m.def(
       "linear_cross_entropy_rows",
       [](const Variable& x, const Variable& w, const Variable* b, const Variable& targets) {
