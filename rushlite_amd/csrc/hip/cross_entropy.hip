@@ -426,9 +426,10 @@ bool half_pays(const LossCall& c) {
 
 int run_loss_half(Runtime* rt, const LossCall& c) {
   const bool grad = c.dx || c.dw;
-  // Pieces of whole groups of panels.
-  const size_t fit = std::max<size_t>(256, kPieceBytes / (c.vocab * sizeof(float)) / 256 * 256);
-  const size_t pieces = grad ? (c.rows + fit - 1) / fit : 1;
+  // Pieces of whole groups of panels: of logits, or for the losses alone of what is kept of 64 of them.
+  const size_t row_bytes = grad ? c.vocab * sizeof(float) : (c.vocab + 63) / 64 * sizeof(Softmax);
+  const size_t fit = std::max<size_t>(256, kPieceBytes / row_bytes / 256 * 256);
+  const size_t pieces = (c.rows + fit - 1) / fit;
   const size_t each = pieces > 1 ? ((c.rows + pieces - 1) / pieces + 255) / 256 * 256 : c.rows;
   const HalfPlan plan = half_plan(rt->cu_count, 0, {int64_t(each), int64_t(c.vocab), int64_t(c.in), false, 2.0f}, {});
   if (plan.cfg < 0) return fail(LMP_ERR_UNSUPPORTED, "linear_cross_entropy: more tiles than a grid holds");

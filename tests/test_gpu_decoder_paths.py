@@ -62,6 +62,29 @@ def test_loss_in_several_pieces_of_some_gradients(hip, k):
             close(got[3], full[3].astype(np.float64), 2 * (rows + 16) * D.U32 * columns, want)
 
 
+def test_losses_alone_of_a_long_batch_keep_to_their_workspace(hip):
+    """40000 rows over 131072 words: 655 MB of maxima and sums, in pieces of 512 MB."""
+    lib = hip.lib()
+    rng = np.random.default_rng(11)
+    rows, k, vocab = 40000, 32, 131072
+    x, w = rng.standard_normal((rows, k)).astype(np.float32), (rng.standard_normal((k, vocab)) * k ** -0.5).astype(np.float32)
+    targets = rng.integers(-vocab // 4, vocab, rows)
+    dx, dw, dt, out = up(hip, x), up(hip, w), up(hip, targets.astype(np.int64)), up(hip, np.full(rows, 7, np.float32))
+    hip.check(lib.lmp_rt_empty_cache())
+    stats = hip.PoolStats()
+    hip.check(lib.lmp_rt_pool_stats_get(C.byref(stats)))
+    before = stats.reserved_bytes
+    hip.check(lib.lmp_k_linear_cross_entropy_f32(rows, k, vocab, dx.ptr, k, dw.ptr, vocab, None, dt.ptr, out.ptr))
+    got = out.numpy()
+    hip.check(lib.lmp_rt_pool_stats_get(C.byref(stats)))
+    assert stats.reserved_bytes - before < 600 << 20
+    some = np.r_[0:40, 32600:32900, rows - 40:rows]  # on both sides of where the second piece begins
+    args = x[some], w, None, targets[some]
+    close(got[some], D.cross_entropy(*args)[0], D.cross_entropy_bounds(*args)[0])
+    parts = [loss(hip, x[at:at + 8000], w, None, targets[at:at + 8000], grads=False) for at in range(0, rows, 8000)]
+    close(got, np.concatenate(parts).astype(np.float64), 2 * D.cross_entropy_bounds(*args)[0].max())
+
+
 def fill(hip, leave):
     """Takes all of the device's memory but `leave` bytes."""
     lib = hip.lib()
