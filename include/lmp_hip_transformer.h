@@ -210,9 +210,12 @@ int lmp_k_gated_linear_backward_f32(int gate, size_t rows, size_t in, size_t hid
  * bias vocab values or null (0), t = targets[i] (int64, on the device).  A row whose target
  * is negative is not counted: its loss is 0, whatever it holds.  A target of vocab or more
  * makes its row's loss NaN.  A logit of -inf has no share; a row of nothing else has the loss
- * NaN, and so has one with a logit of NaN or +inf.  The logits alone are not held at all, or
- * are in pieces of 512 MB (256 rows, if they are more) with the gradients.  in and vocab are
- * positive. */
+ * NaN, and so has one with a logit of NaN or +inf.  in and vocab are positive.
+ *
+ * Workspace: the losses alone of large problems hold a maximum and a sum for 64 logits; other
+ * sizes, and the gradients, hold logits.  Either comes in pieces of 512 MB (256 rows, if they
+ * are more), 128 MB and less where memory is short, beside the operands' parts (as large as
+ * x, w and, with the gradients, a piece's logits twice). */
 int lmp_k_linear_cross_entropy_f32(size_t rows, size_t in, size_t vocab, const float* x,
                                    size_t ldx, const float* w, size_t ldw, const float* bias,
                                    const int64_t* targets, float* loss);
@@ -220,7 +223,7 @@ int lmp_k_linear_cross_entropy_f32(size_t rows, size_t in, size_t vocab, const f
 /* The losses and, of sum_i weights[i] loss[i] (weights null: 1 each), the gradients dx
  * [rows, in], dw [in, vocab] and db (vocab values), each null where it is not wanted (db
  * only with dw).  A row that is not counted has no part in them, whatever it and its weight
- * hold. */
+ * hold; its own dx is 0 (times w: NaN where w is infinite). */
 int lmp_k_linear_cross_entropy_grad_f32(size_t rows, size_t in, size_t vocab, const float* x,
                                         size_t ldx, const float* w, size_t ldw,
                                         const float* bias, const int64_t* targets,

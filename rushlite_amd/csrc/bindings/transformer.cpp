@@ -114,7 +114,8 @@ void bind_transformer(py::module_& m) {
       py::arg("weights").none(true) = py::none(),
       "The softmax cross entropies of the rows of x @ w + b against targets (int64; a negative one "
       "is not counted), summed with weights (finite, without a gradient) or averaged over what counts, "
-      "of shape [1].  The logits are never held whole, and the gradients are formed with the losses.");
+      "of shape [1].  Logits are held in pieces of 512 MB at most, and the gradients are formed with the "
+      "losses.");
   m.def(
       "linear_cross_entropy_rows",
       [](const Variable& x, const Variable& w, const Variable* b, const Variable& targets) {

@@ -7,8 +7,8 @@
 // products are large enough they run on the fp16 matrix cores (gemm_half.hpp): the product's
 // epilogue leaves a maximum and a sum of exponents per row and 64 columns, and for the losses
 // alone no logits at all; with the gradients pieces of rows keep theirs, and dz is formed
-// from them where it is split.  4096 x 1024 over 32768 words takes 2.54 to 2.66 ms, of which
-// the three products would take 2.1 at the library's rate; scoring 8192 rows 1.48 to 1.57 ms of 1.4.
+// from them where it is split.  4096 x 1024 over 32768 words takes 2.63 to 2.71 ms, of which
+// the three products would take 2.1 at the library's rate; scoring 8192 rows 1.52 to 1.59 ms of 1.4.
 // Other sizes take the framework's fp32 products around a pass over the rows.
 #include <hip/hip_runtime.h>
 
@@ -27,8 +27,9 @@
 namespace lmp_hip {
 namespace {
 
-// Bytes of one piece's logits.  Each piece adds to dW once more: 4096 rows of 1024 over a
-// vocabulary of 32768 take 3.23 ms in pieces of 128 MB, 2.71 of 256, 2.57 of 512, 2.58 of 1024.
+// Bytes of one piece's logits, or of what the losses alone keep of them.  Each piece adds to dW
+// once more: 4096 rows of 1024 over a vocabulary of 32768, 512 MB of logits, took 3.23 ms in pieces
+// of 128 MB, 2.71 of 256, 2.57 of 512, 2.58 of 1024; a row more makes it two pieces, some 5%.
 constexpr size_t kPieceBytes = size_t(512) << 20;
 
 struct LossArgs {
@@ -414,9 +415,9 @@ int check_loss(const std::string& name, const LossCall& c) {
 
 // Whether the split products pay for reading x and w twice, writing their panels (12 bytes a
 // value, 16 with the gradients) and their launches.  They save the pass over the logits
-// that the losses alone take, or cost 4 bytes a logit for the gradients' panels.  256 rows of
-// 1024 over 32768 words take 170 us without them and 135 with them (375 and 370 with the
-// gradients), 64 rows 81 and 114.
+// that the losses alone take, or cost 4 bytes a logit for the gradients' panels.  384 rows of
+// 1024 over 32768 words take 265 us without them and 165 with them (586 and 463 with the
+// gradients), 256 rows 150 and 139 (352 and 376), 64 rows 65 and 111.
 bool half_pays(const LossCall& c) {
   const double n = double(c.rows), d = double(c.in), v = double(c.vocab), work = n * d * v;
   if (!half_fits(c.rows, c.in, c.vocab)) return false;

@@ -7,7 +7,7 @@
 // Large layers run on the fp16 matrix cores (gemm_half.hpp), their columns 32 of the one half
 // and 32 of the other by turns: forward the product's epilogue forms h; backward d is
 // formed where it is split, and never held whole.  Smaller ones take the framework's fp32
-// products.  12608 rows of 768 by 768 x 4096 take 0.93 to 0.97 ms forward and backward, of which the
+// products.  12608 rows of 768 by 768 x 4096 take 0.95 to 0.98 ms forward and backward, of which the
 // products would take 0.61 at the library's rate and the passes over pre, g and d 0.2.
 #include <hip/hip_runtime.h>
 
@@ -199,15 +199,15 @@ __global__ __launch_bounds__(NT, MINB) void half_gated(HalfArgs g, HalfGated o, 
 
 // Whether the split products pay for reading x and w twice and writing their panels (12 bytes a
 // value) and for their launches; forward they save a pass over pre besides (two where it is not
-// kept, but what is kept does not change the results).  128 rows of 4096 by 4096 x 16384 take 158 us without them and 264 with them, 512
-// of 768 by 768 x 4096 41 and 38, 16384 of 64 by 64 x 2048 95 and 51.
+// kept, but what is kept does not change the results).  128 rows of 4096 by 4096 x 16384 take 160 us
+// without them and 271 with them, 512 of 768 by 768 x 4096 39 and 36, 16384 of 64 by 64 x 2048 84 and 58.
 bool half_forward_pays(size_t rows, size_t in, size_t hidden) {
   const double n = double(rows), d = double(in), w = 2 * double(hidden);
   return half_fits(rows, in, 2 * hidden) && hidden >= 32 &&
          half_saves_forward(n * d * w) + pass_time(4 * n * w) > 12 + pass_time(12 * (n * d + d * w));
 }
 // Backward they form d twice from pre and g and write it in two sets of panels: 20 bytes a value
-// for 10.  16384 rows of 64 by 64 x 2048 take 164 us without them and 253 with them.
+// for 10.  16384 rows of 64 by 64 x 2048 take 143 us without them and 228 with them.
 bool half_backward_pays(size_t rows, size_t in, size_t hidden) {
   const double n = double(rows), d = double(in), w = 2 * double(hidden);
   return half_fits(rows, in, 2 * hidden) && hidden >= 32 &&

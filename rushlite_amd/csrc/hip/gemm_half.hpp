@@ -34,9 +34,9 @@
 // then, the next one has arrived, and the loads of the one after it start, a whole step
 // ahead of their use.  The LDS is busy for two thirds of a 256 x 256 step's MFMA cycles.
 //
-// Bound by the chip's power: random operands run at 397 TFLOP/s (8192 x 32768 over 1024,
-// 1.19 PFLOP/s of fp16, the clock at 1.7 of 2.4 GHz) to 422 (1024 x 32768 over 4096), zeros at
-// 654, and the library's fp16 product of the first at 1.18 PFLOP/s.  Splitting the operands in
+// Bound by the chip's power: random operands run at 385 TFLOP/s (8192 x 32768 over 1024,
+// 1.16 PFLOP/s of fp16, the clock at 1.7 of 2.4 GHz) to 410 (1024 x 32768 over 4096), zeros ran
+// at 654 before sums were looked after, and the library's fp16 product of the first at 1.18 PFLOP/s.  Splitting the operands in
 // registers on their way to LDS, in every tile that reads them, took it to 350.
 #pragma once
 

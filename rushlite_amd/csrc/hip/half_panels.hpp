@@ -10,8 +10,8 @@
 //   float value(int64_t row, int col)               one value, for sums that are formed again
 //
 // Bound by memory: a pass reads 4 bytes a value and the second writes 4 for each set of panels.
-// w of 1024 x 32768 and x of 4096 x 1024 take 42 us and, with both sets of panels, 76 (151 MB at
-// 3.6 TB/s, 453 at 5.9); dz of 4096 x 32768, formed from the logits in both, 165 and 300.
+// w of 1024 x 32768 and x of 4096 x 1024 take 42 us and, with both sets of panels, 79 (151 MB at
+// 3.6 TB/s, 453 at 5.7); dz of 4096 x 32768, formed from the logits in both, 167 and 310.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -161,7 +161,8 @@ struct TopsJob {
   }
 };
 
-// Strips enough to fill the chip, 256 of them at most: a column's maximum is an atomic a strip.
+// Strips enough to fill the chip: a column's maximum is an atomic a strip, so 256 of them at most unless
+// the rows are more than 256 strips hold.
 inline int tops_wide(int64_t cols) { return cols > 1024 ? 2 : cols > 512 ? 1 : 0; }
 inline int64_t most_strips(Runtime* rt, int64_t rows, int64_t cols) {
   const int64_t width = 512 << tops_wide(cols);

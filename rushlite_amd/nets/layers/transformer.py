@@ -39,7 +39,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling=None):
       {"kind": "by_parts", "factor": f, "original": n, "slow": 1, "fast": 32}
                                         pairs that turn less than `slow` times over the original context of n positions
                                         are f times slower, those that turn more than `fast` times are as before, linear
-                                        in their turns in between; the rotated values times 0.1 ln f + 1"""
+                                        in their turns in between; the rotated values times 0.1 ln f + 1 (Peng, Quesnelle,
+                                        Fan and Shippole, 2023)"""
     if rotary_dim < 0 or rotary_dim % 2:
         raise ValueError(f"rotary_frequencies: rotary_dim {rotary_dim} is not even")
     if not base > 0:
