@@ -174,3 +174,62 @@ def test_loss_in_every_tile(hip, rows, k, vocab):
     x[:, 5], w[5] = 1e9, 0
     x[:, 3], w[3, 7] = x[:, 3] * np.float32(1e-10), 1e10
     check_loss(hip, x, w, None, targets, weights, ("spread",))
+
+
+def test_the_same_bits_from_call_to_call(hip):
+    """In whatever order the sums that are formed again were found, one by one and tile by tile."""
+    rng = np.random.default_rng(9)
+    for rows, k, n in GATED:
+        x, w, g = gated_operands(rng, rows, k, n)
+        w[:, 17], w[70, 17] = 0, 0.7
+        x[:rows // 2:40, 70] = 1e-9
+        x[:, 5], w[5, n:] = 1e9, 0
+        g[rows // 2:] = 0
+        first = gated(hip, "silu", x, w, None, g)
+        for _ in range(3):
+            for a, b in zip(gated(hip, "silu", x, w, None, g), first):
+                assert np.array_equal(a, b)
+    for rows, k, vocab in LOSS:
+        x, w = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((k, vocab)).astype(np.float32)
+        x[rng.random((rows, k)) < 0.5] = 0
+        targets = rng.integers(-5, vocab, rows)
+        first = loss(hip, x, w, None, targets)
+        for _ in range(3):
+            for a, b in zip(loss(hip, x, w, None, targets), first):
+                assert np.array_equal(a, b)
+
+
+def test_a_recorded_call_looks_at_each_replays_operands(hip):
+    """Recorded on operands of one size, replayed on others that spread, and again on the first."""
+    import ctypes as C
+    from test_gpu_decoder import up
+    lib, rng = hip.lib(), np.random.default_rng(10)
+    rows, k, n = GATED[0]
+    plain = gated_operands(rng, rows, k, n)
+    spread = [a.copy() for a in plain]
+    spread[0][:, 5], spread[1][5] = 1e11, 0
+    spread[0][7] *= np.float32(1e12)
+    spread[2][7] = 0
+    dev = [up(hip, a) for a in plain]
+    outs = [up(hip, np.zeros(s, np.float32)) for s in ((rows, n), (rows, 2 * n), (rows, k), (k, 2 * n))]
+    x, w, g, h, pre, dx, dw = (t.ptr for t in dev + outs)
+
+    def calls():
+        hip.check(lib.lmp_k_gated_linear_f32(4, rows, k, n, x, k, w, 2 * n, None, h, n, pre, 2 * n))
+        hip.check(lib.lmp_k_gated_linear_backward_f32(4, rows, k, n, g, n, x, k, w, 2 * n, pre, 2 * n, dx, k, dw, 2 * n, None))
+
+    hip.check(lib.lmp_rt_graph_begin())
+    calls()
+    graph = C.c_void_p()
+    hip.check(lib.lmp_rt_graph_end(C.byref(graph)))
+    for operands in (plain, spread, plain, spread):
+        for t, a in zip(dev, operands):
+            hip.check(lib.lmp_rt_memcpy_h2d(t.ptr, a.ctypes.data, a.nbytes))
+        calls()
+        want = [t.numpy() for t in outs]
+        for t in outs:
+            hip.check(lib.lmp_rt_memcpy_h2d(t.ptr, np.full(t.shape, 7, np.float32).ctypes.data, t.nbytes))
+        hip.check(lib.lmp_rt_graph_launch(graph))
+        for t, a in zip(outs, want):
+            assert np.array_equal(t.numpy(), a)
+    hip.check(lib.lmp_rt_graph_destroy(graph))
